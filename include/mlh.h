@@ -26,6 +26,8 @@ extern "C" {
 
 #define MLH_DTYPE_F32 0
 #define MLH_DTYPE_BF16 1 /* matrices rounded to bf16 (RNE) at upload, fp32 accumulate */
+#define MLH_DTYPE_F16 2  /* IEEE half: operands of the entry points on device pointers only */
+#define MLH_CACHE_Q4 5   /* pages of 4-bit codes (mlh_kv_cache) */
 
 /* Runtime form of the compile-time macros of network_meta.h:3-20 (same names),
  * plus the fields the reference does not have. */
@@ -352,6 +354,90 @@ int mlh_selftest_gemm(int dtype, int M, int N, int K, const float* A, const floa
 int mlh_gemm_device_init(int device);
 int mlh_gemm_device(int dtype, int M, int N, int K, const void* dA, const void* dB, const float* dR, float* dC,
                     void* stream);
+
+/* Operators on a paged K/V cache in the caller's memory, for callers with a model loop of their own (the reference has no cache:
+ * inference.cu:376-751 recomputes every column).  All pointers in the structures are DEVICE pointers on the current device; a call
+ * enqueues one or two kernels on `stream` (a hipStream_t of that device; null: the default stream), allocates nothing, does not synchronise and can be recorded
+ * into a graph, whose replays read the tables, lengths and rows as they are then.  0, or -1 (arguments; nothing was enqueued) or -2 (launch), with the text in
+ * mlh_last_error(NULL).
+ *
+ * Cache.  Two pools of numPages pages of mlh_kv_page_size() = 64 positions, mlh_kv_page_bytes() each, 16-byte aligned.  Position p of sequence s is row
+ * p % 64 of page table[s * pagesPerSeq + p / 64].  Pages of MLH_DTYPE_F32, _BF16 and _F16 are [64, heads, headDim], as those of a context.  Pages
+ * of MLH_CACHE_Q4 are [heads] tiles of 64 * headDim / 2 bytes of codes, [64, headDim] with the even element of a pair in the low half of a byte, and behind
+ * them [64, headDim / 32] pairs of IEEE halves (minimum, scale), one for every 32 elements: 5 bits an element.  An element stands for
+ * minimum + code * scale (fp32, rounded once). */
+typedef struct {
+    void *k, *v;          /* pools */
+    const int32_t* table; /* [nseq, pagesPerSeq] */
+    int32_t type;         /* MLH_DTYPE_F32, _BF16, _F16 or MLH_CACHE_Q4 */
+    int32_t heads;        /* K/V heads */
+    int32_t headDim;      /* 64 or 128 */
+    int32_t numPages;
+    int32_t pagesPerSeq;
+    int32_t nseq;
+} mlh_kv_cache;
+/* Bytes of one page of one pool; 0 for a type, number of heads or head size that the operators do not take. */
+uint64_t mlh_kv_page_bytes(int type, int heads, int headDim);
+
+/* The rows of a call: sequence s brings rows start[s] .. start[s + 1] - 1 (none, one or many), the last of them at position len[s] - 1.
+ * start does not decrease and begins at 0.  Rows at and behind start[nseq] are neither read nor written.  A row is `heads` (q, out) or cache.heads (k, v) heads of
+ * headDim elements, rows `stride` elements apart; pointers and strides are multiples of 16 bytes. */
+typedef struct {
+    const int32_t* start; /* [nseq + 1] */
+    const int32_t* len;   /* [nseq] */
+    int32_t rows;         /* rows that the buffers hold, at least start[nseq] */
+    int32_t type;         /* element type of the rows: that of the cache's pages; any of the three with 4-bit pages */
+    int32_t heads;        /* query heads, a multiple of the cache's (at most 32 times as many): query head h reads K/V head h / (heads / cache.heads) */
+} mlh_kv_batch;
+
+/* Stores the rows' k and v at their positions, k rotated, and writes the rotated q.  Rotation: adjacent pairs (a, b) become
+ * (c a - s b, s a + c b) with the (c, s) pairs of row `position` of rope [ropeRows, headDim] (the table of mlh_upload_rope_table; inference.cu:113-134); rope null:
+ * none.  qGain, kGain [heads * headDim], [cache.heads * headDim]: per-head norm x -> gain * x / sqrt(mean(x^2) + 1e-8) in front of the rotation
+ * (inference.cu:52-81, 97-111); null: none.  Products and sums are in 64 bits, results are rounded to fp32 and then to the type that is stored.
+ * 4-bit pages: of every 32 elements x, minimum = half(min x), scale = half((max x - min x) / 15 in fp32), code = the nearest whole number to
+ * (x - minimum) / scale in 0 .. 15 (ties to even; scale 0: code 0); minima beyond the halves' range count as their largest, and a group with an infinity or NaN, or whose scale is
+ * beyond that range, reads back as NaN.
+ * q may be null (with qOut); qOut may be q with the same stride.  A row whose position is negative, beyond the page table or the rope table, or in a page outside
+ * the pool stores nothing, and its qOut is NaN.  Two rows of a call that share a place leave one of the two. */
+typedef struct {
+    const void *q, *k, *v;
+    void* qOut;
+    int64_t qStride, qOutStride, kStride, vStride;
+    const float* rope;
+    const float *qGain, *kGain;
+    int32_t ropeRows;
+} mlh_kv_append;
+int mlh_kv_append_device(const mlh_kv_cache* cache, const mlh_kv_batch* batch, const mlh_kv_append* args, void* stream);
+
+/* The other way round: k and v rows [rows, cache.heads, headDim] of the batch's positions as the cache holds them, in batch.type, which may be any of the three
+ * for any cache (batch.heads is not looked at).  NaN for a row whose position is negative, beyond the page table or in a page outside the pool. */
+typedef struct {
+    void *k, *v;
+    int64_t stride;
+} mlh_kv_read;
+int mlh_kv_read_device(const mlh_kv_cache* cache, const mlh_kv_batch* batch, const mlh_kv_read* args, void* stream);
+
+/* Attention of the batch's rows over what their sequences hold (their own k and v are in the cache by then).  Position p sees key position j when j <= p and,
+ * with window > 0, p - j < window or j < sinks.  out = sum over those of softmax(scale * q . k) v (inference.cu:136-239); zeros for a row that sees
+ * nothing.  Keys that a row does not see do not count for it, whatever they hold (infinities and NaN too); pages no row sees are not read, so their table entries may be
+ * stale.  A row that sees a position beyond the page table or in a page outside the pool is NaN.
+ * Scores, softmax statistics and sums are fp32; with rows of 16 bits the weights are rounded to the rows' type for the product with v, and values of 4-bit
+ * pages to halves (bf16 rows: to bf16) for both products, finite ones.
+ * maxLen, maxNew: what no len and no number of rows of a sequence exceeds (0: the page table's, rows).  They decide how the work is split and nothing else.
+ * work: mlh_attention_work_bytes() bytes (of the same structures; 0: none), 16-byte aligned, undefined before and after, not shared by calls that may overlap. */
+typedef struct {
+    const void* q;
+    void* out;      /* not q */
+    int64_t qStride, outStride;
+    int32_t window; /* 0: everything */
+    int32_t sinks;
+    int32_t maxLen, maxNew;
+    float scale;    /* 0: 1 / sqrt(headDim) */
+    void* work;
+    uint64_t workBytes;
+} mlh_attention;
+uint64_t mlh_attention_work_bytes(const mlh_kv_cache* cache, const mlh_kv_batch* batch, const mlh_attention* args);
+int mlh_attention_device(const mlh_kv_cache* cache, const mlh_kv_batch* batch, const mlh_attention* args, void* stream);
 
 #ifdef __cplusplus
 }

@@ -12,7 +12,7 @@ a valid Python identifier; load this package with :func:`importlib.util.spec_fro
 """
 import ctypes
 import os
-from ctypes import POINTER, byref, c_char_p, c_double, c_float, c_int, c_int32, c_uint64, c_void_p
+from ctypes import POINTER, byref, c_char_p, c_double, c_float, c_int, c_int32, c_int64, c_uint64, c_void_p
 
 import numpy as np
 
@@ -21,7 +21,8 @@ LIB_DIR = os.path.join(_HERE, "lib")
 MAX_LAYERS = 64
 
 KIND_ATTENTION, KIND_GDN = 0, 1
-DTYPE_F32, DTYPE_BF16 = 0, 1
+DTYPE_F32, DTYPE_BF16, DTYPE_F16 = 0, 1, 2
+CACHE_Q4 = 5  # pages of 4-bit codes (KvCache.type)
 PREFILL_BY_TOKEN, PREFILL_ROWS, PREFILL_HALVES, PREFILL_PAIRS, PREFILL_PLANES = range(5)  # Device.prefill_route
 
 DECODE_GEMV, DECODE_ROWS, DECODE_BARRIER, DECODE_XCD, DECODE_RANKS, DECODE_WIDE = range(6)  # Device.decode_route
@@ -65,6 +66,34 @@ def _load(name):
 
 dev = _load("libmlh.so")
 host = _load("libminillm.so")
+
+class KvCache(ctypes.Structure):
+    """mlh_kv_cache: a paged K/V cache in device memory of the caller's (pointers as integers)."""
+    _fields_ = [("k", c_void_p), ("v", c_void_p), ("table", c_void_p), ("type", c_int32), ("heads", c_int32), ("headDim", c_int32),
+                ("numPages", c_int32), ("pagesPerSeq", c_int32), ("nseq", c_int32)]
+
+
+class KvBatch(ctypes.Structure):
+    """mlh_kv_batch: which rows of a call belong to which sequence, and where they stand in it."""
+    _fields_ = [("start", c_void_p), ("len", c_void_p), ("rows", c_int32), ("type", c_int32), ("heads", c_int32)]
+
+
+class KvAppend(ctypes.Structure):
+    """mlh_kv_append: the rows that kv_append stores."""
+    _fields_ = [("q", c_void_p), ("k", c_void_p), ("v", c_void_p), ("qOut", c_void_p), ("qStride", c_int64), ("qOutStride", c_int64),
+                ("kStride", c_int64), ("vStride", c_int64), ("rope", c_void_p), ("qGain", c_void_p), ("kGain", c_void_p), ("ropeRows", c_int32)]
+
+
+class KvRead(ctypes.Structure):
+    """mlh_kv_read: where kv_read puts the rows."""
+    _fields_ = [("k", c_void_p), ("v", c_void_p), ("stride", c_int64)]
+
+
+class Attention(ctypes.Structure):
+    """mlh_attention: queries, output and mask of an attention call."""
+    _fields_ = [("q", c_void_p), ("out", c_void_p), ("qStride", c_int64), ("outStride", c_int64), ("window", c_int32), ("sinks", c_int32),
+                ("maxLen", c_int32), ("maxNew", c_int32), ("scale", c_float), ("work", c_void_p), ("workBytes", c_uint64)]
+
 
 _P = POINTER
 _sigs_dev = {
@@ -112,6 +141,11 @@ _sigs_dev = {
     "mlh_selftest_gemm": (c_int, [c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int, _P(c_double)]),
     "mlh_gemm_device_init": (c_int, [c_int]),
     "mlh_gemm_device": (c_int, [c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "mlh_kv_page_bytes": (c_uint64, [c_int, c_int, c_int]),
+    "mlh_kv_append_device": (c_int, [_P(KvCache), _P(KvBatch), _P(KvAppend), c_void_p]),
+    "mlh_kv_read_device": (c_int, [_P(KvCache), _P(KvBatch), _P(KvRead), c_void_p]),
+    "mlh_attention_work_bytes": (c_uint64, [_P(KvCache), _P(KvBatch), _P(Attention)]),
+    "mlh_attention_device": (c_int, [_P(KvCache), _P(KvBatch), _P(Attention), c_void_p]),
     "mlh_probe_hops": (c_int, [c_void_p, c_int, _P(c_double)]),
     "mlh_probe_mfma": (c_int, [c_void_p, c_int, c_int, c_int, _P(c_double)]),
     "mlh_probe_lds_loads": (c_int, [c_void_p, c_int, _P(c_double)]),
@@ -264,6 +298,36 @@ class Model:
             self.close()
         except Exception:
             pass
+
+
+def _checked(rc):
+    if rc != 0:
+        raise MlhError(f"device layer error {rc}: {dev.mlh_last_error(None).decode()}")
+
+
+def kv_page_bytes(type, heads, head_dim):
+    """Bytes of one page (64 positions) of one pool of a KvCache; 0 where there is no such cache."""
+    return dev.mlh_kv_page_bytes(type, heads, head_dim)
+
+
+def kv_append(cache, batch, args, stream=None):
+    """Stores a call's k and v rows, rotated, in a KvCache and writes the rotated q (mlh_kv_append_device).  stream: a raw stream handle."""
+    _checked(dev.mlh_kv_append_device(byref(cache), byref(batch), byref(args), stream))
+
+
+def kv_read(cache, batch, args, stream=None):
+    """The rows that a KvCache holds at a batch's positions (mlh_kv_read_device)."""
+    _checked(dev.mlh_kv_read_device(byref(cache), byref(batch), byref(args), stream))
+
+
+def attention_work_bytes(cache, batch, args):
+    """Bytes of Attention.work that such a call needs."""
+    return dev.mlh_attention_work_bytes(byref(cache), byref(batch), byref(args))
+
+
+def attention(cache, batch, args, stream=None):
+    """Attention of a batch's rows over a KvCache, with an optional window and first positions that stay visible (mlh_attention_device)."""
+    _checked(dev.mlh_attention_device(byref(cache), byref(batch), byref(args), stream))
 
 
 class Device:
