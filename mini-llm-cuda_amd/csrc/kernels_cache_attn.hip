@@ -1,92 +1,627 @@
 // Attention over a caller's paged K/V cache (mlh_attention_device): causal, with a sliding window and first positions that stay visible, over pages of 32, 16 or 4
-// bits.
+// bits.  Three kernels and one that joins:
+//   k_kvattn_f32   rows in fp32, 16 of them a workgroup, on the fp32 matrix cores
+//   k_kvattn_few   rows in 16 bits, few a sequence (single tokens): 16 a workgroup, its waves take key tiles in turn
+//   k_kvattn_many  rows in 16 bits, many a sequence (prompts): 32 a wave, key tiles through LDS
+//   k_kvattn_join  the shares of workgroups that split a sequence's keys
+//
+// A "row" here is a query head's query: the heads of one K/V head are rows of one workgroup, so that a key is fetched once for all of them.  Row r of a sequence is
+// head r % G of its query r / G, G = heads / kvHeads.
+//
+// All of them keep, per row, the running maximum m of the scores (times log2 e) and the sums l of 2^(s - m) and acc of 2^(s - m) v, in fp32.  What a row does not see
+// has weight zero whatever the memory holds: scores are replaced by a selection, and where a tile is hidden from some row, elements of v that are no numbers are taken out of
+// the product and added for the rows that see them alone (repair, below), as zero times infinity would be NaN.
 #include <math.h>
 
 #include <algorithm>
 
 #include "kv_cache.h"
 
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
 struct KvAttnArgs {
     const void *poolK, *poolV;
     const int32_t *table, *start, *len;
     const void* q;
     void* out;
+    float* part; // shares of split keys: acc [nsplit, rows * heads, HD], then (m, l) pairs [nsplit, rows * heads]
     long long qStride, outStride;
-    int nseq, rows, heads, kvHeads, pagesPerSeq, numPages, window, sinks;
-    float scale;
+    int nseq, rows, heads, kvHeads, group, pagesPerSeq, numPages, window, sinks, nsplit;
+    float scale2; // scale * log2 e
 };
 
-// One wave per row and head: lanes take a key each for the scores, then the output's elements.
-template <typename IT, typename CT, int HD>
-__global__ void __launch_bounds__(64) k_kv_attn(KvAttnArgs A) {
-    __shared__ float q[HD];
-    const int h = blockIdx.x % A.heads, row = blockIdx.x / A.heads, lane = threadIdx.x, kh = h / (A.heads / A.kvHeads);
-    const int s = kv_find(A.nseq, row, [&](int i) { return A.start[i]; });
-    const int b = A.start[s], e = A.start[s + 1];
-    if (row < b || row >= e) return;
-    const long long pos = (long long)A.len[s] - e + row;
-    if (lane < HD / 8) {
-        float x[8];
-        kv_load8((const IT*)A.q + (size_t)row * A.qStride + (size_t)h * HD + lane * 8, x);
-        for (int i = 0; i < 8; i++) q[lane * 8 + i] = x[i];
+#define KV_NAN __uint_as_float(0x7fc00000u)
+
+// The rows of a workgroup: nr of them from row r0 of sequence s.
+struct KvBlock {
+    int s, r0, nr, row0; // row0: the call's row of the sequence's first query
+    int pos0;            // its position
+    int minPos, maxPos;  // of the block's rows; maxPos inside the page table
+    int cap;             // positions that the page table has
+};
+
+// Blocks of QB rows: those of sequence s begin at number start[s] G / QB + s, which leaves every sequence enough of them.
+template <int QB> __device__ __forceinline__ bool kv_block(const KvAttnArgs& A, int blk, KvBlock& B) {
+    auto first = [&](int i) { return A.start[i] * A.group / QB + i; };
+    const int s = kv_find(A.nseq, blk, first);
+    const int b = A.start[s], e = A.start[s + 1], end = min(e, A.rows);
+    if (b < 0 || end <= b) return false;
+    const int r0 = (blk - first(s)) * QB, all = (end - b) * A.group;
+    if (r0 < 0 || r0 >= all) return false;
+    B.s = s; B.r0 = r0; B.nr = min(QB, all - r0); B.row0 = b;
+    B.pos0 = (int)((unsigned)A.len[s] - (unsigned)e + (unsigned)b);
+    B.cap = A.pagesPerSeq * MLH_KV_PAGE;
+    B.minPos = max(B.pos0 + r0 / A.group, -1);
+    B.maxPos = min(B.pos0 + (r0 + B.nr - 1) / A.group, B.cap - 1);
+    return true;
+}
+
+// The key tiles of TK positions that a block's rows see something of: the first positions' and the window's.
+template <int TK> struct KvTiles {
+    int firsts, skip, n;
+    __device__ __forceinline__ KvTiles(const KvAttnArgs& A, const KvBlock& B) {
+        const int low = A.window ? max(B.minPos + 1 - A.window, 0) / TK : 0;
+        firsts = A.window ? min(low, (min(A.sinks, B.maxPos + 1) + TK - 1) / TK) : 0;
+        firsts = max(firsts, 0);
+        skip = low - firsts;
+        n = B.maxPos < 0 ? 0 : max(B.maxPos / TK + 1 - skip, 0);
     }
-    __syncthreads();
-    float m = -INFINITY, l = 0.f, acc[HD / 64] = {};
-    auto row8 = [&](const void* pool, int page, int at, int d, float (&x)[8]) {
-        if constexpr (KvType<CT>::code != MLH_CACHE_Q4) {
-            kv_load8((const CT*)pool + (((size_t)page * MLH_KV_PAGE + at) * A.kvHeads + kh) * HD + d, x);
-        } else {
-            const uint8_t* tile = (const uint8_t*)pool + ((size_t)page * A.kvHeads + kh) * kv_tile_bytes(HD);
-            kv_values8(*reinterpret_cast<const uint32_t*>(tile + at * (HD / 2) + d / 2), *reinterpret_cast<const uint32_t*>(tile + kv_param_at(HD) + (at * (HD / KV_GROUP) + d / KV_GROUP) * 4), x);
-        }
-    };
-    const long long w0 = A.window ? std::max<long long>(0, pos + 1 - A.window) : 0;
-    for (long long j0 = 0; j0 <= pos; j0 += 64) {
-        if (A.window && j0 >= A.sinks && j0 + 64 <= w0) continue;
-        const int page = kv_page(A.table, A.pagesPerSeq, A.numPages, s, (int)(j0 >> 6));
-        const long long j = j0 + lane;
-        const bool seen = j <= pos && (j >= w0 || j < A.sinks);
-        float sc = -INFINITY;
-        if (seen && page < 0) sc = __uint_as_float(0x7fc00000u);
-        else if (seen) {
-            sc = 0.f;
-            for (int d = 0; d < HD; d += 8) {
-                float x[8];
-                row8(A.poolK, page, lane, d, x);
-                for (int i = 0; i < 8; i++) sc = fmaf(x[i], q[d + i], sc);
-            }
-            sc *= A.scale;
-        }
-        float mt = fmaxf(m, sc);
-        for (int o = 32; o > 0; o >>= 1) mt = fmaxf(mt, __shfl_xor(mt, o, 64));
-        const float ref = mt == -INFINITY ? 0.f : mt, corr = expf(m - ref), p = seen ? expf(sc - ref) : 0.f;
-        m = mt;
-        float ps = p;
-        for (int o = 32; o > 0; o >>= 1) ps += __shfl_xor(ps, o, 64);
-        l = l * corr + ps;
-        for (int i = 0; i < HD / 64; i++) acc[i] *= corr;
-        for (int k = 0; k < 64; k++) {
-            const float pk = __shfl(p, k, 64);
-            if (!((__ballot(seen) >> k) & 1)) continue;
-            float x[8];
-            for (int i = 0; i < HD / 64; i++) {
-                const int d = lane + 64 * i;
-                if (page >= 0) row8(A.poolV, page, k, d & ~7, x);
-                float v = 0.f;
-                for (int t = 0; t < 8; t++) v = page >= 0 && t == (d & 7) ? x[t] : v;
-                acc[i] = fmaf(pk, v, acc[i]);
-            }
-        }
-    }
-    for (int i = 0; i < HD / 64; i++) {
-        float o = l == 0.f ? 0.f : acc[i] / l;
-        IT* p = (IT*)A.out + (size_t)row * A.outStride + (size_t)h * HD + lane + 64 * i;
-        if constexpr (KvType<IT>::code == MLH_DTYPE_F32) *p = o;
-        else if constexpr (KvType<IT>::code == MLH_DTYPE_BF16) *p = (bf16_t)kv_to_bf16(o);
-        else p->bits = (uint16_t)kv_to_half(o);
+    __device__ __forceinline__ int at(int i) const { return i < firsts ? i : i + skip; }
+};
+
+// what a row sees: positions up to `pos`, above `below` or among the first `sinks`
+struct KvSight {
+    int pos, below, sinks;
+    __device__ __forceinline__ KvSight(const KvAttnArgs& A, int p) : pos(p), below(A.window ? max(p, -1) - A.window : -1), sinks(A.sinks) {}
+    __device__ __forceinline__ bool sees(int j) const { return j <= pos && (j > below || j < sinks); }
+};
+// do all rows of [minPos, maxPos] see all of a tile's n positions from j0?
+__device__ __forceinline__ bool kv_all_see(const KvAttnArgs& A, int minPos, int maxPos, int j0, int n) {
+    return j0 + n - 1 <= minPos && (!A.window || j0 > maxPos - A.window || j0 + n <= A.sinks);
+}
+
+__device__ __forceinline__ bool kv_finite(float v) { return (__float_as_uint(v) & 0x7f800000u) != 0x7f800000u; }
+__device__ __forceinline__ float kv_exp2(float v) { return __builtin_amdgcn_exp2f(v); }
+__device__ __forceinline__ float kv_quad_max(float v) { // over the four lanes that hold a column of a 16 x 16 product
+    v = fmaxf(v, __shfl_xor(v, 16, 64));
+    return fmaxf(v, __shfl_xor(v, 32, 64));
+}
+__device__ __forceinline__ float kv_quad_sum(float v) {
+    v += __shfl_xor(v, 16, 64);
+    return v + __shfl_xor(v, 32, 64);
+}
+
+__device__ __forceinline__ void kv_put(float* p, float v) { *p = v; }
+__device__ __forceinline__ void kv_put(bf16_t* p, float v) { *p = (bf16_t)kv_to_bf16(v); }
+__device__ __forceinline__ void kv_put(f16_t* p, float v) { p->bits = (uint16_t)kv_to_half(v); }
+
+template <typename T> __device__ __forceinline__ void kv_put4(T* p, const f32x4& v) {
+    if constexpr (sizeof(T) == 4) *reinterpret_cast<f32x4*>(p) = v;
+    else if constexpr (KvType<T>::code == MLH_DTYPE_BF16) *reinterpret_cast<uint2*>(p) = make_uint2(kv_to_bf16(v.x) | kv_to_bf16(v.y) << 16, kv_to_bf16(v.z) | kv_to_bf16(v.w) << 16);
+    else *reinterpret_cast<uint2*>(p) = make_uint2(kv_to_half(v.x) | kv_to_half(v.y) << 16, kv_to_half(v.z) | kv_to_half(v.w) << 16);
+}
+
+// one element of a page, as a float
+template <typename CT, int HD> __device__ __forceinline__ float kv_one(const void* pool, int page, int at, int kvHeads, int kh, int d) {
+    if constexpr (KvType<CT>::code == MLH_CACHE_Q4) {
+        const uint8_t* tile = (const uint8_t*)pool + ((size_t)page * kvHeads + kh) * kv_tile_bytes(HD);
+        const uint32_t code = (uint32_t)tile[at * (HD / 2) + d / 2] >> (4 * (d & 1)) & 15u;
+        const uint32_t par = *reinterpret_cast<const uint32_t*>(tile + kv_param_at(HD) + (at * (HD / KV_GROUP) + d / KV_GROUP) * 4);
+        return fmaf((float)code, kv_half(par >> 16), kv_half(par & 0xffffu));
+    } else {
+        const CT* p = (const CT*)pool + (((size_t)page * MLH_KV_PAGE + at) * kvHeads + kh) * HD + d;
+        if constexpr (sizeof(CT) == 4) return *p;
+        else if constexpr (KvType<CT>::code == MLH_DTYPE_BF16) return kv_bf16(*p);
+        else return kv_half(p->bits);
     }
 }
 
+// The end of the 16-row kernels: acc of every wave (block b, element i of lane 16 g + n: row n, element dim(b, 4 g + i)), its m and l (of row n), joined over the waves, and
+// written as the row's result or, with split keys, as this workgroup's share.  lds: NW * 16 * (HD + 4 + 2) floats.
+template <typename IT, int HD, int NW, typename F>
+__device__ __forceinline__ void kv_finish16(const KvAttnArgs& A, const KvBlock& B, int kh, int split, const f32x4 (&acc)[HD / 16], float m, float l, float* lds, F dim4) {
+    constexpr int LDO = HD + 4;
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, n = lane & 15, g = lane >> 4;
+    float (*part)[16][LDO] = reinterpret_cast<float (*)[16][LDO]>(lds);
+    float (*stat)[2][16] = reinterpret_cast<float (*)[2][16]>(lds + NW * 16 * LDO);
+    if (g == 0) { stat[wave][0][n] = m; stat[wave][1][n] = l; }
+    dim4([&](int d, const f32x4& v) { *reinterpret_cast<f32x4*>(&part[wave][n][d]) = v; });
+    __syncthreads();
+    for (int i = tid; i < B.nr * (HD / 4); i += NW * 64) {
+        const int r = i / (HD / 4), d = (i % (HD / 4)) * 4;
+        float M = -INFINITY, den = 0.f;
+#pragma unroll
+        for (int w = 0; w < NW; w++) M = fmaxf(M, stat[w][0][r]);
+        const float ref = M == -INFINITY ? 0.f : M;
+        f32x4 o = (f32x4)(0.f);
+#pragma unroll
+        for (int w = 0; w < NW; w++) {
+            const float f = kv_exp2(stat[w][0][r] - ref);
+            den = fmaf(stat[w][1][r], f, den);
+            o += *reinterpret_cast<const f32x4*>(&part[w][r][d]) * f;
+        }
+        const int qi = (B.r0 + r) / A.group, h = kh * A.group + (B.r0 + r) % A.group, row = B.row0 + qi;
+        if (B.pos0 + qi >= B.cap) { den = KV_NAN; M = 0.f; } // (its own position is behind the page table)
+        if (A.nsplit > 1) {
+            const size_t rh = (size_t)split * A.rows * A.heads + (size_t)row * A.heads + h;
+            *reinterpret_cast<f32x4*>(A.part + rh * HD + d) = o;
+            if (d == 0) *reinterpret_cast<float2*>(A.part + (size_t)A.nsplit * A.rows * A.heads * HD + rh * 2) = make_float2(M, den);
+        } else {
+            const float inv = den == 0.f ? 0.f : 1.0f / den;
+            if constexpr (sizeof(IT) == 4) { // (a division's rounding, not a product's with a rounded inverse)
+                o = den == 0.f ? (f32x4)(0.f) : f32x4{o.x / den, o.y / den, o.z / den, o.w / den};
+                kv_put4((IT*)A.out + (size_t)row * A.outStride + (size_t)h * HD + d, o);
+            } else {
+                kv_put4((IT*)A.out + (size_t)row * A.outStride + (size_t)h * HD + d, den == 0.f ? (f32x4)(0.f) : o * inv);
+            }
+        }
+    }
+}
+
+// ----------------------------------------------------------------------------
+// fp32 rows.  Products on v_mfma_f32_16x16x4_f32: S^T[key, row] = K . Q^T, then O^T += V^T . P^T, K and V from the pages straight into registers in 16-byte pieces:
+// lane 16 g + n holds elements [g HD/4, (g + 1) HD/4) of key n (the order of a contraction is free), the product leaves it the scores of keys 4 g .. 4 g + 3 of row n,
+// which is the second product's operand as it stands; row m of V's operand of block b is element m HD/16 + b.  The waves take tiles of 16 keys in turn, the next tile's loads
+// go out before this one's products.
+// ----------------------------------------------------------------------------
+template <typename CT, int HD> struct KvTile32 { // a lane's part of 16 keys
+    static constexpr int KC = HD / 4, VB = HD / 16;
+    f32x4 k[KC / 4], v[4][VB / 4];
+    __device__ __forceinline__ void fetch(const KvAttnArgs& A, int page, int at, int last, int kh, int n, int g) {
+        const size_t row = (size_t)A.kvHeads * HD, base = ((size_t)page * MLH_KV_PAGE + at) * row + (size_t)kh * HD;
+        const float* kr = (const float*)A.poolK + base + (size_t)min(n, last) * row + g * KC;
+#pragma unroll
+        for (int c = 0; c < KC / 4; c++) k[c] = *reinterpret_cast<const f32x4*>(kr + 4 * c);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float* vr = (const float*)A.poolV + base + (size_t)min(4 * g + i, last) * row + n * VB;
+#pragma unroll
+            for (int c = 0; c < VB / 4; c++) v[i][c] = *reinterpret_cast<const f32x4*>(vr + 4 * c);
+        }
+    }
+    __device__ __forceinline__ void values(f32x4 (&ko)[KC / 4], f32x4 (&vo)[4][VB / 4]) const {
+#pragma unroll
+        for (int c = 0; c < KC / 4; c++) ko[c] = k[c];
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+            for (int c = 0; c < VB / 4; c++) vo[i][c] = v[i][c];
+    }
+};
+template <int HD> struct KvTile32<q4_t, HD> {
+    static constexpr int KC = HD / 4, VB = HD / 16;
+    uint32_t k[KC / 8], kp, v[4], vp[4];
+    __device__ __forceinline__ void fetch(const KvAttnArgs& A, int page, int at, int last, int kh, int n, int g) {
+        const size_t base = ((size_t)page * A.kvHeads + kh) * kv_tile_bytes(HD);
+        const uint8_t *tk = (const uint8_t*)A.poolK + base, *tv = (const uint8_t*)A.poolV + base;
+        const int rk = at + min(n, last);
+#pragma unroll
+        for (int c = 0; c < KC / 8; c += 2) *reinterpret_cast<uint2*>(&k[c]) = *reinterpret_cast<const uint2*>(tk + rk * (HD / 2) + g * (KC / 2) + 4 * c);
+        kp = *reinterpret_cast<const uint32_t*>(tk + kv_param_at(HD) + (rk * (HD / KV_GROUP) + g * KC / KV_GROUP) * 4);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int rv = at + min(4 * g + i, last);
+            if constexpr (HD == 128) v[i] = *reinterpret_cast<const uint32_t*>(tv + rv * (HD / 2) + n * 4);
+            else v[i] = *reinterpret_cast<const uint16_t*>(tv + rv * (HD / 2) + n * 2);
+            vp[i] = *reinterpret_cast<const uint32_t*>(tv + kv_param_at(HD) + (rv * (HD / KV_GROUP) + n * VB / KV_GROUP) * 4);
+        }
+    }
+    __device__ __forceinline__ void values(f32x4 (&ko)[KC / 4], f32x4 (&vo)[4][VB / 4]) const {
+#pragma unroll
+        for (int c = 0; c < KC / 8; c++) {
+            float x[8];
+            kv_values8(k[c], kp, x);
+#pragma unroll
+            for (int i = 0; i < 8; i++) ko[2 * c + i / 4][i % 4] = x[i];
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            float x[8];
+            kv_values8(v[i], vp[i], x);
+#pragma unroll
+            for (int j = 0; j < VB; j++) vo[i][j / 4][j % 4] = x[j];
+        }
+    }
+};
+
+#define KV_W32 8 // waves of a workgroup
+template <typename CT, int HD>
+__global__ void __launch_bounds__(KV_W32 * 64) k_kvattn_f32(KvAttnArgs A) {
+    constexpr int NW = KV_W32, KC = HD / 4, VB = HD / 16;
+    __shared__ __attribute__((aligned(16))) float lds[NW * 16 * (HD + 4 + 2)];
+    const int kh = blockIdx.x % A.kvHeads, split = blockIdx.y, tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, n = lane & 15, g = lane >> 4;
+    KvBlock B;
+    if (!kv_block<16>(A, blockIdx.x / A.kvHeads, B)) return;
+    const int r = B.r0 + min(n, B.nr - 1), h = kh * A.group + r % A.group;
+    const KvSight sight(A, B.pos0 + r / A.group);
+    f32x4 q[KC / 4];
+    {
+        const float* qr = (const float*)A.q + (size_t)(B.row0 + r / A.group) * A.qStride + (size_t)h * HD + g * KC;
+#pragma unroll
+        for (int c = 0; c < KC / 4; c++) q[c] = *reinterpret_cast<const f32x4*>(qr + 4 * c);
+    }
+    f32x4 acc[VB];
+#pragma unroll
+    for (int b = 0; b < VB; b++) acc[b] = (f32x4)(0.f);
+    float m = -INFINITY, l = 0.f; // of row n; l: over this lane's keys
+    const KvTiles<16> tiles(A, B);
+    KvTile32<CT, HD> raw[2];
+    int page[2];
+    auto fetch = [&](int i, int set) __attribute__((always_inline)) {
+        const int j0 = tiles.at(i) * 16;
+        page[set] = kv_page(A.table, A.pagesPerSeq, A.numPages, B.s, j0 >> 6);
+        raw[set].fetch(A, max(page[set], 0), j0 & 63, min(B.maxPos - j0, 15), kh, n, g);
+    };
+    auto tile = [&](int i, int set) __attribute__((always_inline)) {
+        const int j0 = tiles.at(i) * 16, key = j0 + 4 * g;
+        f32x4 k[KC / 4], v[4][VB / 4];
+        raw[set].values(k, v);
+        f32x4 s0 = (f32x4)(0.f), s1 = (f32x4)(0.f); // two chains
+#pragma unroll
+        for (int c = 0; c < KC / 4; c++) {
+            s0 = __builtin_amdgcn_mfma_f32_16x16x4f32(k[c].x, q[c].x, s0, 0, 0, 0);
+            s1 = __builtin_amdgcn_mfma_f32_16x16x4f32(k[c].y, q[c].y, s1, 0, 0, 0);
+            s0 = __builtin_amdgcn_mfma_f32_16x16x4f32(k[c].z, q[c].z, s0, 0, 0, 0);
+            s1 = __builtin_amdgcn_mfma_f32_16x16x4f32(k[c].w, q[c].w, s1, 0, 0, 0);
+        }
+        const bool whole = kv_all_see(A, B.minPos, B.maxPos, j0, 16) && page[set] >= 0;
+        float p[4], mt = m;
+        bool see[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            see[e] = whole || sight.sees(key + e);
+            p[e] = (s0[e] + s1[e]) * A.scale2;
+            if (!whole) p[e] = !see[e] ? -INFINITY : page[set] < 0 ? KV_NAN : p[e];
+            mt = fmaxf(mt, p[e]);
+        }
+        mt = kv_quad_max(mt);
+        const float ref = mt == -INFINITY ? 0.f : mt, corr = kv_exp2(m - ref);
+        m = mt;
+        l *= corr;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            p[e] = see[e] ? kv_exp2(p[e] - ref) : 0.f;
+            l += p[e];
+        }
+#pragma unroll
+        for (int b = 0; b < VB; b++) acc[b] *= corr;
+        if (!whole) { // repair
+            bool odd = false;
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+#pragma unroll
+                for (int b = 0; b < VB; b++) odd = odd || !kv_finite(v[e][b / 4][b % 4]);
+            if (__ballot(odd)) {
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+#pragma unroll
+                    for (int b = 0; b < VB; b++) v[e][b / 4][b % 4] = kv_finite(v[e][b / 4][b % 4]) ? v[e][b / 4][b % 4] : 0.f;
+                    for (int gk = 0; gk < 4; gk++) {
+                        const int j = j0 + 4 * gk + e;
+                        if (j > B.maxPos) break;
+                        const float w = __shfl(p[e], 16 * gk + n, 64);
+                        for (int i4 = 0; i4 < 4; i4++)
+#pragma unroll
+                            for (int b = 0; b < VB; b++) {
+                                const float x = kv_one<CT, HD>(A.poolV, max(page[set], 0), j & 63, A.kvHeads, kh, (4 * g + i4) * VB + b);
+                                const float add = sight.sees(j) && !kv_finite(x) ? w * x : 0.f;
+                                acc[b].x += i4 == 0 ? add : 0.f; acc[b].y += i4 == 1 ? add : 0.f; acc[b].z += i4 == 2 ? add : 0.f; acc[b].w += i4 == 3 ? add : 0.f;
+                            }
+                    }
+                }
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+#pragma unroll
+            for (int b = 0; b < VB; b++) acc[b] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[e][b / 4][b % 4], p[e], acc[b], 0, 0, 0);
+    };
+    const int step = NW * A.nsplit;
+    int t = split * NW + wave;
+    if (t < tiles.n) fetch(t, 0);
+    while (t < tiles.n) { // (no further tile: the same loads again, dropped)
+        fetch(min(t + step, tiles.n - 1), 1);
+        __builtin_amdgcn_sched_barrier(0); // (the compiler would put the loads behind the products)
+        tile(t, 0);
+        t += step;
+        if (t >= tiles.n) break;
+        fetch(min(t + step, tiles.n - 1), 0);
+        __builtin_amdgcn_sched_barrier(0);
+        tile(t, 1);
+        t += step;
+    }
+    l = kv_quad_sum(l);
+    kv_finish16<float, HD, NW>(A, B, kh, split, acc, m, l, lds, [&](auto put) {
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+            for (int b = 0; b < VB; b += 4) put((4 * g + i) * VB + b, f32x4{acc[b][i], acc[b + 1][i], acc[b + 2][i], acc[b + 3][i]});
+    });
+}
+
+// ----------------------------------------------------------------------------
+// Few 16-bit rows of a sequence.  A wave takes 32 keys at a time: S^T[key, row] = K . Q^T on 16x16x32 products, K from the pages straight into registers; V's
+// rows go through the wave's own piece of LDS, which hands them back transposed (ds_read_b64_tr_b16: lane i of 16 gets column i of four rows), so that
+// O^T += V^T . P^T takes the weights from the registers that the first product left them in.  4-bit pages: codes become halves on the way (exact: the values
+// are minimum + code * scale in halves, one rounding), all products are in halves, and bf16 rows are scaled by a power of two first.
+// ----------------------------------------------------------------------------
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+template <bool BF> __device__ __forceinline__ f32x4 mfma16(const u32x4& a, const u32x4& b, const f32x4& c) {
+    if constexpr (BF) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+template <bool BF> __device__ __forceinline__ uint32_t kv_pack(float a, float b) {
+    if constexpr (BF) { typedef __bf16 bf16x2 __attribute__((ext_vector_type(2))); return __builtin_bit_cast(uint32_t, bf16x2{(__bf16)a, (__bf16)b}); }
+    else return pack_f16(a, b);
+}
+__device__ __forceinline__ u32x2 lds_transposed(const void* p) { // 4 rows x 16 columns of 16 bits from 16 lanes' addresses
+    return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p));
+}
+template <bool BF> __device__ __forceinline__ bool kv_odd(uint32_t w) { // is one of the two elements no number?
+    constexpr uint32_t E = BF ? 0x7f80u : 0x7c00u;
+    return (w & E) == E || (w >> 16 & E) == E;
+}
+template <bool BF> __device__ __forceinline__ uint32_t kv_without_odd(uint32_t w) {
+    constexpr uint32_t E = BF ? 0x7f80u : 0x7c00u;
+    return ((w & E) == E ? 0u : w & 0xffffu) | ((w >> 16 & E) == E ? 0u : w & 0xffff0000u);
+}
+// eight codes -> halves; pairs come out as elements (0, 4), (1, 5), (2, 6), (3, 7)
+__device__ __forceinline__ u32x4 kv_halves(uint32_t codes, uint32_t params) {
+    const _Float16 base = __builtin_bit_cast(_Float16, (uint16_t)(params & 0xffffu)), scale = __builtin_bit_cast(_Float16, (uint16_t)(params >> 16));
+    const f16x2 b = {base, base}, s = {scale, scale}, off = {(_Float16)-1024.f, (_Float16)-1024.f};
+    u32x4 o;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const f16x2 c = __builtin_bit_cast(f16x2, ((codes >> (4 * i)) & 0x000f000fu) | 0x64006400u) + off; // 1024 + code, less 1024: exact
+        o[i] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(c, s, b));
+    }
+    return o;
+}
+
+// A row's power of two: largest |q| into [1, 2), so that halves hold it.  (0: the row is zero, or holds an infinity or NaN, and stays as it is.)
+__device__ __forceinline__ int kv_row_exp(float most) {
+    const uint32_t e = __float_as_uint(most) >> 23 & 255u;
+    return e == 0 || e == 255 ? 0 : 127 - (int)e;
+}
+
+template <typename IT, typename CT, int HD> struct KvRaw16 { // a lane's part of 32 keys: key 16 b + n, elements 32 t + 8 g ..; of V the same
+    static constexpr int KS = HD / 32;
+    u32x4 k[2][KS], v[2][KS];
+    __device__ __forceinline__ void fetch(const KvAttnArgs& A, int page, int at, int last, int kh, int n, int g) {
+        const size_t row = (size_t)A.kvHeads * HD, base = ((size_t)page * MLH_KV_PAGE + at) * row + (size_t)kh * HD + g * 8;
+#pragma unroll
+        for (int b = 0; b < 2; b++) {
+            const size_t o = base + (size_t)min(16 * b + n, last) * row;
+#pragma unroll
+            for (int t = 0; t < KS; t++) k[b][t] = *reinterpret_cast<const u32x4*>((const uint16_t*)A.poolK + o + 32 * t);
+#pragma unroll
+            for (int t = 0; t < KS; t++) v[b][t] = *reinterpret_cast<const u32x4*>((const uint16_t*)A.poolV + o + 32 * t);
+        }
+    }
+    __device__ __forceinline__ u32x4 key(int b, int t) const { return k[b][t]; }
+    __device__ __forceinline__ u32x4 val(int b, int t) const { return v[b][t]; }
+};
+template <typename IT, int HD> struct KvRaw16<IT, q4_t, HD> { // the same, elements (HD / 4) g + 8 t .. (one group of 32, or half of one)
+    static constexpr int KS = HD / 32;
+    uint32_t k[2][KS], v[2][KS], kp[2], vp[2];
+    __device__ __forceinline__ void fetch(const KvAttnArgs& A, int page, int at, int last, int kh, int n, int g) {
+        const size_t base = ((size_t)page * A.kvHeads + kh) * kv_tile_bytes(HD);
+#pragma unroll
+        for (int b = 0; b < 2; b++) {
+            const int r = at + min(16 * b + n, last);
+            const size_t o = base + r * (HD / 2) + g * (HD / 8), p = base + kv_param_at(HD) + (r * (HD / KV_GROUP) + g * (HD / 4) / KV_GROUP) * 4;
+            kp[b] = *reinterpret_cast<const uint32_t*>((const uint8_t*)A.poolK + p);
+            vp[b] = *reinterpret_cast<const uint32_t*>((const uint8_t*)A.poolV + p);
+            if constexpr (HD == 128) {
+                *reinterpret_cast<u32x4*>(k[b]) = *reinterpret_cast<const u32x4*>((const uint8_t*)A.poolK + o);
+                *reinterpret_cast<u32x4*>(v[b]) = *reinterpret_cast<const u32x4*>((const uint8_t*)A.poolV + o);
+            } else {
+                *reinterpret_cast<u32x2*>(k[b]) = *reinterpret_cast<const u32x2*>((const uint8_t*)A.poolK + o);
+                *reinterpret_cast<u32x2*>(v[b]) = *reinterpret_cast<const u32x2*>((const uint8_t*)A.poolV + o);
+            }
+        }
+    }
+    __device__ __forceinline__ u32x4 key(int b, int t) const { return kv_halves(k[b][t], kp[b]); }
+    __device__ __forceinline__ u32x4 val(int b, int t) const { return kv_halves(v[b][t], vp[b]); }
+};
+
+#define KV_W16 8
+template <typename IT, typename CT, int HD>
+__global__ void __launch_bounds__(KV_W16 * 64) k_kvattn_few(KvAttnArgs A) {
+    constexpr bool FOUR = KvType<CT>::code == MLH_CACHE_Q4, BF = !FOUR && KvType<IT>::code == MLH_DTYPE_BF16; // products in bf16
+    constexpr int NW = KV_W16, KS = HD / 32, VB = HD / 16;
+    constexpr int VP = HD * 2 + 16; // bytes of a row of V in LDS: four rows start in different banks
+    constexpr int LV = NW * 32 * VP, LF = NW * 16 * (HD + 4 + 2) * 4;
+    __shared__ __attribute__((aligned(16))) unsigned char lds[LV > LF ? LV : LF];
+    const int kh = blockIdx.x % A.kvHeads, split = blockIdx.y, tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, n = lane & 15, g = lane >> 4;
+    KvBlock B;
+    if (!kv_block<16>(A, blockIdx.x / A.kvHeads, B)) return;
+    const int r = B.r0 + min(n, B.nr - 1), h = kh * A.group + r % A.group;
+    const KvSight sight(A, B.pos0 + r / A.group);
+    u32x4 q[KS];
+    float scale = A.scale2;
+    {
+        const IT* qr = (const IT*)A.q + (size_t)(B.row0 + r / A.group) * A.qStride + (size_t)h * HD;
+        if constexpr (!FOUR) {
+#pragma unroll
+            for (int t = 0; t < KS; t++) q[t] = *reinterpret_cast<const u32x4*>(qr + 32 * t + 8 * g);
+        } else {
+            float x[KS][8], most = 0.f;
+#pragma unroll
+            for (int t = 0; t < KS; t++) {
+                kv_load8(qr + (HD / 4) * g + 8 * t, x[t]);
+#pragma unroll
+                for (int i = 0; i < 8; i++) most = fmaxf(most, fabsf(x[t][i]));
+            }
+            const int e = KvType<IT>::code == MLH_DTYPE_BF16 ? kv_row_exp(kv_quad_max(most)) : 0;
+            scale = ldexpf(scale, -e);
+#pragma unroll
+            for (int t = 0; t < KS; t++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) q[t][i] = pack_f16(ldexpf(x[t][i], e), ldexpf(x[t][i + 4], e));
+        }
+    }
+    f32x4 acc[VB];
+#pragma unroll
+    for (int b = 0; b < VB; b++) acc[b] = (f32x4)(0.f);
+    float m = -INFINITY, l = 0.f;
+    unsigned char* const vt = lds + wave * 32 * VP;
+    const KvTiles<32> tiles(A, B);
+    KvRaw16<IT, CT, HD> raw[2];
+    int page[2];
+    auto fetch = [&](int i, int set) __attribute__((always_inline)) {
+        const int j0 = tiles.at(i) * 32;
+        page[set] = kv_page(A.table, A.pagesPerSeq, A.numPages, B.s, j0 >> 6);
+        raw[set].fetch(A, max(page[set], 0), j0 & 63, min(B.maxPos - j0, 31), kh, n, g);
+    };
+    auto tile = [&](int i, int set) __attribute__((always_inline)) {
+        const int j0 = tiles.at(i) * 32;
+        const bool whole = kv_all_see(A, B.minPos, B.maxPos, j0, 32) && page[set] >= 0;
+        f32x4 s[2];
+#pragma unroll
+        for (int b = 0; b < 2; b++) {
+            s[b] = (f32x4)(0.f);
+#pragma unroll
+            for (int t = 0; t < KS; t++) s[b] = mfma16<BF>(raw[set].key(b, t), q[t], s[b]);
+        }
+        // V's rows: columns in the order that the pieces come in (4-bit pages: (0, 4), (1, 5) ... of every eight)
+        bool odd[2] = {false, false};
+#pragma unroll
+        for (int b = 0; b < 2; b++)
+#pragma unroll
+            for (int t = 0; t < KS; t++) {
+                u32x4 x = raw[set].val(b, t);
+                if (!whole) {
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        odd[b] = odd[b] || kv_odd<BF>(x[i]);
+                        x[i] = kv_without_odd<BF>(x[i]);
+                    }
+                }
+                *reinterpret_cast<u32x4*>(vt + (16 * b + n) * VP + (FOUR ? (HD / 4) * g + 8 * t : 32 * t + 8 * g) * 2) = x;
+            }
+        float p[2][4], mt = m;
+        bool see[2][4];
+#pragma unroll
+        for (int b = 0; b < 2; b++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                see[b][e] = whole || sight.sees(j0 + 16 * b + 4 * g + e);
+                p[b][e] = s[b][e] * scale;
+                if (!whole) p[b][e] = !see[b][e] ? -INFINITY : page[set] < 0 ? KV_NAN : p[b][e];
+                mt = fmaxf(mt, p[b][e]);
+            }
+        mt = kv_quad_max(mt);
+        const float ref = mt == -INFINITY ? 0.f : mt, corr = kv_exp2(m - ref);
+        m = mt;
+        l *= corr;
+#pragma unroll
+        for (int b = 0; b < 2; b++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                p[b][e] = see[b][e] ? kv_exp2(p[b][e] - ref) : 0.f;
+                l += p[b][e];
+            }
+#pragma unroll
+        for (int b = 0; b < VB; b++) acc[b] *= corr;
+        if (!whole) { // repair
+#pragma unroll
+            for (int b = 0; b < 2; b++) {
+                unsigned long long hit = __ballot(odd[b]);
+                uint32_t keys = (uint32_t)((hit | hit >> 16 | hit >> 32 | hit >> 48) & 0xffffu);
+                while (keys) {
+                    const int k = __builtin_ctz(keys), j = j0 + 16 * b + k;
+                    keys &= keys - 1;
+                    if (j > B.maxPos) break;
+                    float w = p[b][0];
+                    if ((k & 3) == 1) w = p[b][1];
+                    if ((k & 3) == 2) w = p[b][2];
+                    if ((k & 3) == 3) w = p[b][3];
+                    w = __shfl(w, 16 * (k >> 2) + n, 64);
+#pragma unroll
+                    for (int c = 0; c < VB; c++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            const int at = 16 * c + 4 * g + e, d = FOUR ? (at & ~7) + (at & 7) / 2 + 4 * (at & 1) : at;
+                            float x = kv_one<CT, HD>(A.poolV, max(page[set], 0), j & 63, A.kvHeads, kh, d);
+                            if (FOUR) x = (float)(_Float16)x;
+                            acc[c][e] += sight.sees(j) && !kv_finite(x) ? w * x : 0.f;
+                        }
+                }
+            }
+        }
+        const u32x4 pw = {kv_pack<BF>(p[0][0], p[0][1]), kv_pack<BF>(p[0][2], p[0][3]), kv_pack<BF>(p[1][0], p[1][1]), kv_pack<BF>(p[1][2], p[1][3])};
+        // lane i of a group of 16 gives the address of row i / 4, columns 4 (i % 4) ..
+        const unsigned char* va = vt + (4 * g + (n >> 2)) * VP + (n & 3) * 8;
+#pragma unroll
+        for (int b = 0; b < VB; b++) {
+            const u32x2 lo = lds_transposed(va + 32 * b), hi = lds_transposed(va + 16 * VP + 32 * b);
+            acc[b] = mfma16<BF>(u32x4{lo.x, lo.y, hi.x, hi.y}, pw, acc[b]);
+        }
+    };
+    const int step = NW * A.nsplit;
+    int t = split * NW + wave;
+    if (t < tiles.n) fetch(t, 0);
+    while (t < tiles.n) { // (no further tile: the same loads again, dropped)
+        fetch(min(t + step, tiles.n - 1), 1);
+        __builtin_amdgcn_sched_barrier(0);
+        tile(t, 0);
+        t += step;
+        if (t >= tiles.n) break;
+        fetch(min(t + step, tiles.n - 1), 0);
+        __builtin_amdgcn_sched_barrier(0);
+        tile(t, 1);
+        t += step;
+    }
+    l = kv_quad_sum(l);
+    __syncthreads(); // the waves' V tiles become the place where they meet
+    kv_finish16<IT, HD, NW>(A, B, kh, split, acc, m, l, reinterpret_cast<float*>(lds), [&](auto put) {
+#pragma unroll
+        for (int b = 0; b < VB; b++) {
+            if constexpr (!FOUR) put(16 * b + 4 * g, acc[b]);
+            else { // columns (0, 4, 1, 5) or (2, 6, 3, 7) of every eight
+                float* f = reinterpret_cast<float*>(lds) + ((size_t)wave * 16 + n) * (HD + 4) + 16 * b + 8 * (g >> 1) + 2 * (g & 1);
+                f[0] = acc[b].x; f[4] = acc[b].y; f[1] = acc[b].z; f[5] = acc[b].w;
+            }
+        }
+    });
+}
+
+// ----------------------------------------------------------------------------
+// The shares of nsplit workgroups: one thread for four elements of a row.
+// ----------------------------------------------------------------------------
+template <typename IT, int HD>
+__global__ void __launch_bounds__(256) k_kvattn_join(KvAttnArgs A) {
+    const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x, n = (size_t)A.rows * A.heads;
+    const size_t rh = i / (HD / 4);
+    const int d = (int)(i % (HD / 4)) * 4;
+    if (rh >= n) return;
+    const int row = (int)(rh / A.heads), h = (int)(rh % A.heads);
+    if (row < A.start[0] || row >= A.start[A.nseq]) return;
+    const float2* stat = reinterpret_cast<const float2*>(A.part + (size_t)A.nsplit * n * HD);
+    float M = -INFINITY, den = 0.f;
+    for (int s = 0; s < A.nsplit; s++) M = fmaxf(M, stat[s * n + rh].x);
+    const float ref = M == -INFINITY ? 0.f : M;
+    f32x4 o = (f32x4)(0.f);
+    for (int s = 0; s < A.nsplit; s++) {
+        const float2 ml = stat[s * n + rh];
+        const float f = kv_exp2(ml.x - ref);
+        den = fmaf(ml.y, f, den);
+        o += *reinterpret_cast<const f32x4*>(A.part + (s * n + rh) * HD + d) * f;
+    }
+    o = den == 0.f ? (f32x4)(0.f) : f32x4{o.x / den, o.y / den, o.z / den, o.w / den};
+    kv_put4((IT*)A.out + (size_t)row * A.outStride + (size_t)h * HD + d, o);
+}
+
+// ----------------------------------------------------------------------------
+// host side
+// ----------------------------------------------------------------------------
 static std::string attn_check(const mlh_kv_cache* c, const mlh_kv_batch* b, const mlh_attention* a) {
     std::string bad = kv_check(c, b, false);
     if (!bad.empty()) return bad;
@@ -101,29 +636,70 @@ static std::string attn_check(const mlh_kv_cache* c, const mlh_kv_batch* b, cons
     return "";
 }
 
+struct AttnPlan { // how a call is split
+    int blocks, nsplit;
+    size_t bytes;
+};
+static AttnPlan attn_plan(const mlh_kv_cache* c, const mlh_kv_batch* b, const mlh_attention* a) {
+    AttnPlan P;
+    const int group = b->heads / c->heads;
+    const long long cap = (long long)c->pagesPerSeq * MLH_KV_PAGE;
+    const long long maxLen = a->maxLen ? std::min<long long>(a->maxLen, cap) : cap;
+    P.blocks = (int)((long long)b->rows * group / 16 + c->nseq);
+    // key tiles of the longest row: the window's and the first positions', in pieces of 32 keys a wave
+    const long long seen = a->window ? std::min<long long>(maxLen, (long long)a->window + std::min<long long>(a->sinks, maxLen) + 64) : maxLen;
+    const long long rounds = (seen + 8 * 32 - 1) / (8 * 32); // turns of a workgroup's eight waves
+    const long long wgs = (long long)std::min(P.blocks, (b->rows * group + 15) / 16 + std::min(c->nseq, b->rows)) * c->heads;
+    long long n = std::min<long long>((512 + wgs - 1) / wgs, (rounds + 1) / 2); // two workgroups a compute unit, two turns or more a workgroup
+    P.nsplit = (int)std::max<long long>(1, std::min<long long>(n, 64));
+    P.bytes = P.nsplit > 1 ? (size_t)P.nsplit * b->rows * b->heads * (c->headDim + 2) * 4 : 0;
+    return P;
+}
+
 extern "C" uint64_t mlh_attention_work_bytes(const mlh_kv_cache* c, const mlh_kv_batch* b, const mlh_attention* a) {
-    return attn_check(c, b, a).empty() ? 0 : 0;
+    return attn_check(c, b, a).empty() ? attn_plan(c, b, a).bytes : 0;
 }
 
 extern "C" int mlh_attention_device(const mlh_kv_cache* c, const mlh_kv_batch* b, const mlh_attention* a, void* stream) {
     const std::string bad = attn_check(c, b, a);
     if (!bad.empty()) return kv_fail(bad);
     if (b->rows == 0) return 0;
-    const KvAttnArgs A = {c->k, c->v, c->table, b->start, b->len, a->q, a->out, a->qStride, a->outStride, c->nseq, b->rows, b->heads, c->heads, c->pagesPerSeq, c->numPages, a->window, a->sinks,
-                          a->scale > 0.f ? a->scale : 1.0f / sqrtf((float)c->headDim)};
-    const dim3 grid((unsigned)b->rows * b->heads);
-#define GO(IT_, CT_) \
+    const AttnPlan P = attn_plan(c, b, a);
+    if (P.bytes > 0 && (!a->work || a->workBytes < P.bytes)) return kv_fail("work is smaller than mlh_attention_work_bytes() = " + std::to_string(P.bytes));
+    if (P.bytes > 0 && (uintptr_t)a->work % 16) return kv_fail("work must be 16-byte aligned");
+    if ((long long)P.blocks * c->heads * P.nsplit * 512 > 0xffffffffll) return kv_fail("too many rows or sequences for one call");
+    const int hd = c->headDim;
+    const KvAttnArgs A = {c->k, c->v, c->table, b->start, b->len, a->q, a->out, (float*)a->work, a->qStride, a->outStride, c->nseq, b->rows, b->heads, c->heads, b->heads / c->heads,
+                          c->pagesPerSeq, c->numPages, a->window, a->sinks, P.nsplit, (a->scale > 0.f ? a->scale : 1.0f / sqrtf((float)hd)) * 1.44269504088896341f};
+    const dim3 grid(c->heads * P.blocks, P.nsplit);
+    hipStream_t st = (hipStream_t)stream;
+#define GO(K_, ...) \
     do { \
-        if (c->headDim == 64) hipLaunchKernelGGL((k_kv_attn<IT_, CT_, 64>), grid, dim3(64), 0, (hipStream_t)stream, A); \
-        else hipLaunchKernelGGL((k_kv_attn<IT_, CT_, 128>), grid, dim3(64), 0, (hipStream_t)stream, A); \
+        if (hd == 64) hipLaunchKernelGGL((K_<__VA_ARGS__, 64>), grid, dim3(512), 0, st, A); \
+        else hipLaunchKernelGGL((K_<__VA_ARGS__, 128>), grid, dim3(512), 0, st, A); \
     } while (0)
-    if (c->type == MLH_CACHE_Q4) {
-        if (b->type == MLH_DTYPE_F32) GO(float, q4_t);
-        else if (b->type == MLH_DTYPE_BF16) GO(bf16_t, q4_t);
-        else GO(f16_t, q4_t);
-    } else if (b->type == MLH_DTYPE_F32) GO(float, float);
-    else if (b->type == MLH_DTYPE_BF16) GO(bf16_t, bf16_t);
-    else GO(f16_t, f16_t);
+    if (b->type == MLH_DTYPE_F32) {
+        if (c->type == MLH_CACHE_Q4) GO(k_kvattn_f32, q4_t);
+        else GO(k_kvattn_f32, float);
+    } else if (b->type == MLH_DTYPE_BF16) {
+        if (c->type == MLH_CACHE_Q4) GO(k_kvattn_few, bf16_t, q4_t);
+        else GO(k_kvattn_few, bf16_t, bf16_t);
+    } else {
+        if (c->type == MLH_CACHE_Q4) GO(k_kvattn_few, f16_t, q4_t);
+        else GO(k_kvattn_few, f16_t, f16_t);
+    }
 #undef GO
+    if (const int rc = kv_launched()) return rc;
+    if (P.nsplit == 1) return 0;
+    const unsigned jg = (unsigned)(((size_t)b->rows * b->heads * (hd / 4) + 255) / 256);
+#define JOIN(IT_) \
+    do { \
+        if (hd == 64) hipLaunchKernelGGL((k_kvattn_join<IT_, 64>), dim3(jg), dim3(256), 0, st, A); \
+        else hipLaunchKernelGGL((k_kvattn_join<IT_, 128>), dim3(jg), dim3(256), 0, st, A); \
+    } while (0)
+    if (b->type == MLH_DTYPE_F32) JOIN(float);
+    else if (b->type == MLH_DTYPE_BF16) JOIN(bf16_t);
+    else JOIN(f16_t);
+#undef JOIN
     return kv_launched();
 }
