@@ -594,6 +594,246 @@ __global__ void __launch_bounds__(KV_W16 * 64) k_kvattn_few(KvAttnArgs A) {
 }
 
 // ----------------------------------------------------------------------------
+// Many 16-bit rows of a sequence: 32 a wave, NW waves a workgroup, a page (64 keys) at a time through LDS, double-buffered.  S^T[key, row] = K . Q^T on 32x32x16
+// products: every lane owns one row (element i of lane l: key 8 (i / 4) + 4 (l / 32) + i % 4, row l % 32), so maximum and sum run down registers, with one
+// exchange between the lane halves; O^T += V^T . P^T takes the weights as they lie and V through the transposing LDS read.  Pages of 16 bits go straight to LDS
+// (the 16-byte pieces of a row in an order that keeps both readings free of bank conflicts), those of 4 bits through registers, where codes become halves.
+// ----------------------------------------------------------------------------
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+template <bool BF> __device__ __forceinline__ f32x16 mfma32(const u32x4& a, const u32x4& b, const f32x16& c) {
+    if constexpr (BF) return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+// place of 16-byte piece c of row r: K's operand takes the same piece of 32 rows at once, V's takes four pieces of four rows
+template <int HD> __device__ __forceinline__ int kv_place_k(int r, int c) { return r * (HD * 2) + 16 * (c ^ (HD == 128 ? r & 15 : (r >> 1) & 7)); }
+template <int HD> __device__ __forceinline__ int kv_place_v(int r, int c) { return r * (HD * 2) + 16 * (c ^ (HD == 128 ? 4 * (r & 3) : 4 * ((r >> 1) & 1))); }
+
+template <typename IT, typename CT, int HD, int NW>
+__global__ void __launch_bounds__(NW * 64, 2) k_kvattn_many(KvAttnArgs A) {
+    constexpr bool FOUR = KvType<CT>::code == MLH_CACHE_Q4, BF = !FOUR && KvType<IT>::code == MLH_DTYPE_BF16;
+    constexpr int KS = HD / 16, MB = HD / 32, TB = 64 * HD * 2, QB = NW * 32; // TB: bytes of a tile of K or V
+    extern __shared__ __attribute__((aligned(16))) unsigned char lds[]; // K, V of two tiles; keys to repair
+    uint32_t* const flags = reinterpret_cast<uint32_t*>(lds + 4 * TB);
+    const int kh = blockIdx.x % A.kvHeads, tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, n = lane & 31, half = lane >> 5;
+    KvBlock B;
+    if (!kv_block<QB>(A, (gridDim.x - 1 - blockIdx.x) / A.kvHeads, B)) return; // (the last rows of a sequence see most: first)
+    const bool active = wave * 32 < B.nr;
+    const int wr0 = B.r0 + min(wave * 32, B.nr - 1), wr1 = B.r0 + min(wave * 32 + 31, B.nr - 1); // this wave's rows
+    const int wMin = max(B.pos0 + wr0 / A.group, -1), wMax = min(B.pos0 + wr1 / A.group, B.cap - 1);
+    const int r = B.r0 + min(wave * 32 + n, B.nr - 1), h = kh * A.group + r % A.group;
+    const KvSight sight(A, B.pos0 + r / A.group);
+    u32x4 q[KS];
+    float scale = A.scale2;
+    {
+        const IT* qr = (const IT*)A.q + (size_t)(B.row0 + r / A.group) * A.qStride + (size_t)h * HD + 8 * half;
+        if constexpr (!FOUR) {
+#pragma unroll
+            for (int t = 0; t < KS; t++) q[t] = *reinterpret_cast<const u32x4*>(qr + 16 * t);
+        } else {
+            float most = 0.f;
+            if (KvType<IT>::code == MLH_DTYPE_BF16) {
+                for (int t = 0; t < KS; t++) {
+                    float x[8];
+                    kv_load8(qr + 16 * t, x);
+#pragma unroll
+                    for (int i = 0; i < 8; i++) most = fmaxf(most, fabsf(x[i]));
+                }
+                most = fmaxf(most, __shfl_xor(most, 32, 64));
+            }
+            const int e = kv_row_exp(most);
+            scale = ldexpf(scale, -e);
+#pragma unroll
+            for (int t = 0; t < KS; t++) {
+                float x[8];
+                kv_load8(qr + 16 * t, x);
+#pragma unroll
+                for (int i = 0; i < 4; i++) q[t][i] = pack_f16(ldexpf(x[i], e), ldexpf(x[i + 4], e));
+            }
+        }
+    }
+    f32x16 acc[MB];
+#pragma unroll
+    for (int b = 0; b < MB; b++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) acc[b][i] = 0.f;
+    float m = -INFINITY, l = 0.f; // (of the scores times scale)
+    const KvTiles<64> tiles(A, B);
+
+    // ---- a tile into LDS ----
+    constexpr int EPT = HD / NW; // 4-bit pages: elements a thread takes of K and of V
+    uint32_t kc[FOUR ? EPT / 8 : 1], vc[FOUR ? EPT / 8 : 1], kp = 0, vp = 0;
+    const int qRow = tid / NW, qAt = (tid % NW) * EPT;
+    auto fetch = [&](int i, int buf) __attribute__((always_inline)) {
+        const int page = max(kv_page(A.table, A.pagesPerSeq, A.numPages, B.s, tiles.at(i)), 0);
+        if constexpr (FOUR) {
+            const size_t base = ((size_t)page * A.kvHeads + kh) * kv_tile_bytes(HD);
+            const unsigned o = qRow * (HD / 2) + qAt / 2, p = kv_param_at(HD) + (qRow * (HD / KV_GROUP) + qAt / KV_GROUP) * 4;
+            const uint8_t *tk = (const uint8_t*)A.poolK + base, *tv = (const uint8_t*)A.poolV + base;
+            kp = *reinterpret_cast<const uint32_t*>(tk + p);
+            vp = *reinterpret_cast<const uint32_t*>(tv + p);
+            if constexpr (EPT == 32) { *reinterpret_cast<u32x4*>(kc) = *reinterpret_cast<const u32x4*>(tk + o); *reinterpret_cast<u32x4*>(vc) = *reinterpret_cast<const u32x4*>(tv + o); }
+            else if constexpr (EPT == 16) { *reinterpret_cast<u32x2*>(kc) = *reinterpret_cast<const u32x2*>(tk + o); *reinterpret_cast<u32x2*>(vc) = *reinterpret_cast<const u32x2*>(tv + o); }
+            else { kc[0] = *reinterpret_cast<const uint32_t*>(tk + o); vc[0] = *reinterpret_cast<const uint32_t*>(tv + o); }
+        } else { // 1 KiB an instruction: lane i's 16 bytes go to the i-th place of it
+            constexpr int RPI = 512 / HD, CPR = HD / 8; // rows an instruction, pieces a row
+            const size_t base = (((size_t)page * MLH_KV_PAGE) * A.kvHeads + kh) * HD * 2;
+            const int lr = lane / CPR, lc = lane % CPR;
+#pragma unroll
+            for (int j = 0; j < 64 / RPI / NW; j++) {
+                const int r0 = (j * NW + wave) * RPI, row = r0 + lr;
+                const unsigned ko = (unsigned)(row * A.kvHeads * HD * 2) + ((kv_place_k<HD>(row, lc) - row * (HD * 2)));
+                const unsigned vo = (unsigned)(row * A.kvHeads * HD * 2) + ((kv_place_v<HD>(row, lc) - row * (HD * 2)));
+                const unsigned to = (unsigned)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)lds + buf * 2 * TB + r0 * (HD * 2);
+                const unsigned char *sk = (const unsigned char*)A.poolK + base, *sv = (const unsigned char*)A.poolV + base;
+                asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(__builtin_amdgcn_readfirstlane(to)), "v"(ko), "s"(sk) : "memory", "m0");
+                asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(__builtin_amdgcn_readfirstlane(to + TB)), "v"(vo), "s"(sv) : "memory", "m0");
+            }
+        }
+    };
+    auto deposit = [&](int buf) __attribute__((always_inline)) { // 4-bit pages: what fetch left in registers
+        if constexpr (FOUR) {
+#pragma unroll
+            for (int i = 0; i < EPT / 8; i++) {
+                *reinterpret_cast<u32x4*>(lds + buf * 2 * TB + kv_place_k<HD>(qRow, qAt / 8 + i)) = kv_halves(kc[i], kp);
+                *reinterpret_cast<u32x4*>(lds + buf * 2 * TB + TB + kv_place_v<HD>(qRow, qAt / 8 + i)) = kv_halves(vc[i], vp);
+            }
+        }
+    };
+
+    auto tile = [&](int i, int buf) __attribute__((always_inline)) {
+        const int j0 = tiles.at(i) * 64;
+        const int page = kv_page(A.table, A.pagesPerSeq, A.numPages, B.s, j0 >> 6);
+        const unsigned char *kt = lds + buf * 2 * TB, *vt = kt + TB;
+        uint32_t odd[2] = {0, 0};
+        if (!kv_all_see(A, B.minPos, B.maxPos, j0, 64) || page < 0) { // repair: elements of V that are no numbers leave the tile
+            for (int c = tid; c < 64 * HD / 8; c += NW * 64) {
+                const int row = c / (HD / 8);
+                u32x4* p = reinterpret_cast<u32x4*>(const_cast<unsigned char*>(vt) + kv_place_v<HD>(row, c % (HD / 8)));
+                const u32x4 x = *p;
+                if (kv_odd<BF>(x.x) || kv_odd<BF>(x.y) || kv_odd<BF>(x.z) || kv_odd<BF>(x.w)) {
+                    *p = u32x4{kv_without_odd<BF>(x.x), kv_without_odd<BF>(x.y), kv_without_odd<BF>(x.z), kv_without_odd<BF>(x.w)};
+                    if (j0 + row <= B.maxPos && page >= 0) atomicOr(&flags[2 * buf + (row >> 5)], 1u << (row & 31));
+                }
+            }
+            __syncthreads();
+            odd[0] = __builtin_amdgcn_readfirstlane(flags[2 * buf]);
+            odd[1] = __builtin_amdgcn_readfirstlane(flags[2 * buf + 1]);
+        }
+        if (!active || j0 > wMax || (A.window && j0 + 63 <= wMin - A.window && j0 >= A.sinks)) return;
+        const bool whole = kv_all_see(A, wMin, wMax, j0, 64) && page >= 0;
+        f32x16 s[2];
+#pragma unroll
+        for (int b = 0; b < 2; b++) {
+#pragma unroll
+            for (int e = 0; e < 16; e++) s[b][e] = 0.f;
+#pragma unroll
+            for (int t = 0; t < KS; t++) s[b] = mfma32<BF>(*reinterpret_cast<const u32x4*>(kt + kv_place_k<HD>(32 * b + n, 2 * t + half)), q[t], s[b]);
+        }
+        float mx = -INFINITY;
+        if (!whole) {
+#pragma unroll
+            for (int b = 0; b < 2; b++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) s[b][e] = sight.sees(j0 + 32 * b + 8 * (e >> 2) + 4 * half + (e & 3)) ? page < 0 ? KV_NAN : s[b][e] : -INFINITY;
+        }
+#pragma unroll
+        for (int b = 0; b < 2; b++)
+#pragma unroll
+            for (int e = 0; e < 16; e += 2) mx = fmaxf(mx, fmaxf(s[b][e], s[b][e + 1]));
+        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+        const float mn = fmaxf(m, mx * scale);
+        if (__any(mn > m)) {
+            const float corr = m == -INFINITY ? 0.f : kv_exp2(m - mn);
+            l *= corr;
+#pragma unroll
+            for (int b = 0; b < MB; b++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) acc[b][e] *= corr;
+        }
+        m = mn;
+        const float ref = mn == -INFINITY ? 0.f : -mn;
+        if (whole) {
+#pragma unroll
+            for (int b = 0; b < 2; b++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) {
+                    s[b][e] = kv_exp2(fmaf(s[b][e], scale, ref));
+                    l += s[b][e];
+                }
+        } else { // (what is hidden carries -inf; times a scale that has underflowed that would be no number)
+#pragma unroll
+            for (int b = 0; b < 2; b++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) {
+                    s[b][e] = s[b][e] == -INFINITY ? 0.f : kv_exp2(fmaf(s[b][e], scale, ref));
+                    l += s[b][e];
+                }
+        }
+        if (odd[0] | odd[1]) {
+#pragma unroll
+            for (int b = 0; b < 2; b++)
+                for (uint32_t keys = odd[b]; keys; keys &= keys - 1) {
+                    const int k = __builtin_ctz(keys), j = j0 + 32 * b + k, at = 4 * (k >> 3) + (k & 3);
+                    float w = 0.f;
+#pragma unroll
+                    for (int e = 0; e < 16; e++) w = e == at ? s[b][e] : w;
+                    w = __shfl(w, n + 32 * ((k >> 2) & 1), 64);
+                    const bool see = sight.sees(j);
+#pragma unroll
+                    for (int c = 0; c < MB; c++)
+#pragma unroll
+                        for (int e = 0; e < 16; e++) {
+                            const int col = 32 * c + 8 * (e >> 2) + 4 * half + (e & 3), d = FOUR ? (col & ~7) + (col & 7) / 2 + 4 * (col & 1) : col;
+                            float x = kv_one<CT, HD>(A.poolV, page, j & 63, A.kvHeads, kh, d);
+                            if (FOUR) x = (float)(_Float16)x;
+                            acc[c][e] += see && !kv_finite(x) ? w * x : 0.f;
+                        }
+                }
+        }
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
+            const int b = t >> 1, e0 = 8 * (t & 1);
+            const u32x4 pw = {kv_pack<BF>(s[b][e0], s[b][e0 + 1]), kv_pack<BF>(s[b][e0 + 2], s[b][e0 + 3]), kv_pack<BF>(s[b][e0 + 4], s[b][e0 + 5]), kv_pack<BF>(s[b][e0 + 6], s[b][e0 + 7])};
+            const int row = 16 * t + 4 * half + ((lane & 15) >> 2), piece = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1), rest = 8 * (lane & 1);
+#pragma unroll
+            for (int c = 0; c < MB; c++) {
+                const u32x2 lo = lds_transposed(vt + kv_place_v<HD>(row, 4 * c + piece) + rest), hi = lds_transposed(vt + kv_place_v<HD>(row + 8, 4 * c + piece) + rest);
+                acc[c] = mfma32<BF>(u32x4{lo.x, lo.y, hi.x, hi.y}, pw, acc[c]);
+            }
+        }
+    };
+
+    if (tiles.n > 0) fetch(0, 0);
+    for (int i = 0; i < tiles.n; i++) {
+        const int buf = i & 1;
+        deposit(buf);
+        if (tid < 2) flags[2 * buf + tid] = 0; // (read last two tiles ago)
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); // tile i has landed ...
+        __syncthreads();                                  // ... for every wave, and every wave is done with tile i - 1
+        if (i + 1 < tiles.n) fetch(i + 1, buf ^ 1);
+        __builtin_amdgcn_sched_barrier(0);
+        tile(i, buf);
+    }
+    if (!active || wave * 32 + n >= B.nr) return;
+    l += __shfl_xor(l, 32, 64);
+    const int qi = r / A.group;
+    const float inv = B.pos0 + qi >= B.cap ? KV_NAN : l == 0.f ? 0.f : 1.0f / l;
+    IT* out = (IT*)A.out + (size_t)(B.row0 + qi) * A.outStride + (size_t)h * HD;
+#pragma unroll
+    for (int c = 0; c < MB; c++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            f32x4 o = f32x4{acc[c][4 * e], acc[c][4 * e + 1], acc[c][4 * e + 2], acc[c][4 * e + 3]} * inv;
+            if (l == 0.f && inv == 0.f) o = (f32x4)(0.f);
+            if (FOUR) { // columns (0, 4, 1, 5) here, (2, 6, 3, 7) in the other half: four neighbours each
+                const float a = __shfl_xor(half ? o.x : o.y, 32, 64), b = __shfl_xor(half ? o.z : o.w, 32, 64);
+                o = half ? f32x4{a, b, o.y, o.w} : f32x4{o.x, o.z, a, b};
+            }
+            kv_put4(out + 32 * c + 8 * e + 4 * half, o);
+        }
+}
+
+// ----------------------------------------------------------------------------
 // The shares of nsplit workgroups: one thread for four elements of a row.
 // ----------------------------------------------------------------------------
 template <typename IT, int HD>
@@ -636,7 +876,8 @@ static std::string attn_check(const mlh_kv_cache* c, const mlh_kv_batch* b, cons
     return "";
 }
 
-struct AttnPlan { // how a call is split
+struct AttnPlan { // which kernel, and how the keys are split
+    int many;         // waves of a workgroup of k_kvattn_many; 0: the kernels of 16 rows
     int blocks, nsplit;
     size_t bytes;
 };
@@ -645,15 +886,28 @@ static AttnPlan attn_plan(const mlh_kv_cache* c, const mlh_kv_batch* b, const ml
     const int group = b->heads / c->heads;
     const long long cap = (long long)c->pagesPerSeq * MLH_KV_PAGE;
     const long long maxLen = a->maxLen ? std::min<long long>(a->maxLen, cap) : cap;
-    P.blocks = (int)((long long)b->rows * group / 16 + c->nseq);
+    const long long maxNew = a->maxNew ? std::min(a->maxNew, b->rows) : b->rows;
+    P.many = b->type != MLH_DTYPE_F32 && maxNew * group > 64 ? 4 : 0;
+    const int qb = P.many ? P.many * 32 : 16;
+    P.blocks = (int)((long long)b->rows * group / qb + c->nseq);
     // key tiles of the longest row: the window's and the first positions', in pieces of 32 keys a wave
     const long long seen = a->window ? std::min<long long>(maxLen, (long long)a->window + std::min<long long>(a->sinks, maxLen) + 64) : maxLen;
     const long long rounds = (seen + 8 * 32 - 1) / (8 * 32); // turns of a workgroup's eight waves
     const long long wgs = (long long)std::min(P.blocks, (b->rows * group + 15) / 16 + std::min(c->nseq, b->rows)) * c->heads;
-    long long n = std::min<long long>((512 + wgs - 1) / wgs, (rounds + 1) / 2); // two workgroups a compute unit, two turns or more a workgroup
+    const long long n = P.many ? 1 : std::min<long long>((512 + wgs - 1) / wgs, (rounds + 1) / 2); // two workgroups a compute unit, two turns or more a workgroup
     P.nsplit = (int)std::max<long long>(1, std::min<long long>(n, 64));
     P.bytes = P.nsplit > 1 ? (size_t)P.nsplit * b->rows * b->heads * (c->headDim + 2) * 4 : 0;
     return P;
+}
+
+template <typename IT, typename CT, int HD, int NW> static hipError_t launch_many(dim3 grid, hipStream_t st, const KvAttnArgs& A) {
+    constexpr int bytes = 4 * 64 * HD * 2 + 16;
+    if (bytes > 65536) { // (asked for on every call: the attribute belongs to the device that is current)
+        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&k_kvattn_many<IT, CT, HD, NW>), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+        if (e != hipSuccess) return e;
+    }
+    hipLaunchKernelGGL((k_kvattn_many<IT, CT, HD, NW>), grid, dim3(NW * 64), bytes, st, A);
+    return hipSuccess;
 }
 
 extern "C" uint64_t mlh_attention_work_bytes(const mlh_kv_cache* c, const mlh_kv_batch* b, const mlh_attention* a) {
@@ -673,6 +927,15 @@ extern "C" int mlh_attention_device(const mlh_kv_cache* c, const mlh_kv_batch* b
                           c->pagesPerSeq, c->numPages, a->window, a->sinks, P.nsplit, (a->scale > 0.f ? a->scale : 1.0f / sqrtf((float)hd)) * 1.44269504088896341f};
     const dim3 grid(c->heads * P.blocks, P.nsplit);
     hipStream_t st = (hipStream_t)stream;
+    if (P.many) {
+        hipError_t e;
+#define MANY(IT_, CT_) (hd == 64 ? launch_many<IT_, CT_, 64, 4>(grid, st, A) : launch_many<IT_, CT_, 128, 4>(grid, st, A))
+        if (b->type == MLH_DTYPE_BF16) e = c->type == MLH_CACHE_Q4 ? MANY(bf16_t, q4_t) : MANY(bf16_t, bf16_t);
+        else e = c->type == MLH_CACHE_Q4 ? MANY(f16_t, q4_t) : MANY(f16_t, f16_t);
+#undef MANY
+        if (e != hipSuccess) { mlh_set_thread_error(std::string("launch failed: ") + hipGetErrorString(e)); return -2; }
+        return kv_launched();
+    }
 #define GO(K_, ...) \
     do { \
         if (hd == 64) hipLaunchKernelGGL((K_<__VA_ARGS__, 64>), grid, dim3(512), 0, st, A); \
