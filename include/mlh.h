@@ -249,6 +249,17 @@ int mlh_debug_inject_abort(mlh_ctx* ctx, int launches);
 int mlh_debug_inject_abort_at_step(mlh_ctx* ctx, int step);
 int mlh_debug_set_xcd_tag(mlh_ctx* ctx, unsigned tagsUsed);
 
+/* Attention layers that forget: with window > 0 a position sees the `window` positions up to its own and the first `sinks`
+ * positions of its sequence (mlh_attention_device); 0 (the default): everything before it.  From the next call on; what the pages hold stays, so a window can be widened
+ * again.  mlh_set_kv_type: what the pages of the attention layers are, MLH_DTYPE_F32 (the default) or MLH_CACHE_Q4 (mlh_kv_append_device: 5 bits an
+ * element instead of 32); all sequences must be empty, and the pools are allocated anew.  With either, decode runs as the kernel sequence (the single-launch modes know neither), and attention is that of
+ * mlh_kv_append_device and mlh_attention_device in fp32, in prefills too.  (No counterpart in the reference, whose attention recomputes every column, inference.cu:511-573.) */
+int mlh_set_attention_window(mlh_ctx* ctx, int window, int sinks);
+int mlh_set_kv_type(mlh_ctx* ctx, int type);
+/* K and V rows [n, dim] of positions pos .. pos + n - 1 of a sequence as an attention layer's pages hold them (layer: FILE block index; after per-head
+ * norm and rotation).  No counterpart in the reference. */
+int mlh_read_kv(mlh_ctx* ctx, int layer, int seq, int pos, int n, float* k, float* v);
+
 /* Next-token rule of the decode entry points.  temperature 0 (the default): greedy, the argmax fused into the
  * LM-head reduction, lowest index on ties (the reference's only mode: it keeps the top entry of a qsort of the
  * probabilities, inference_orchestrator.cu:120-165).  temperature > 0: the token is drawn on the device from

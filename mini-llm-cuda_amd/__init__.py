@@ -124,6 +124,9 @@ _sigs_dev = {
     "mlh_read_probs": (c_int, [c_void_p, c_int, c_void_p]),
     "mlh_set_graph": (c_int, [c_void_p, c_int]),
     "mlh_set_sampling": (c_int, [c_void_p, c_float, ctypes.c_ulonglong]),
+    "mlh_set_attention_window": (c_int, [c_void_p, c_int, c_int]),
+    "mlh_set_kv_type": (c_int, [c_void_p, c_int]),
+    "mlh_read_kv": (c_int, [c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_void_p]),
     "mlh_set_persistent": (c_int, [c_void_p, c_int]),
     "mlh_get_persistent": (c_int, [c_void_p]),
     "mlh_persistent_fallbacks": (c_int, [c_void_p]),
@@ -452,6 +455,20 @@ class Device:
     def set_sampling(self, temperature, seed=0):
         """temperature 0: greedy (default); > 0: tokens are drawn from softmax(logits / temperature)."""
         self._check(dev.mlh_set_sampling(self._h, float(temperature), int(seed)))
+
+    def set_attention_window(self, window, sinks=0):
+        """Attention layers see the last `window` positions and the first `sinks` (0: everything)."""
+        self._check(dev.mlh_set_attention_window(self._h, int(window), int(sinks)))
+
+    def set_kv_type(self, type):
+        """DTYPE_F32 (default) or CACHE_Q4: what the K/V pages hold.  All sequences must be empty."""
+        self._check(dev.mlh_set_kv_type(self._h, int(type)))
+
+    def read_kv(self, layer, seq, pos, n):
+        """K and V rows [n, dim] of positions pos .. pos + n - 1 as an attention layer's pages hold them."""
+        k, v = (np.empty((n, self.hp.dim), dtype=np.float32) for _ in range(2))
+        self._check(dev.mlh_read_kv(self._h, int(layer), int(seq), int(pos), int(n), k.ctypes.data, v.ctypes.data))
+        return k, v
 
     def set_persistent(self, enabled):
         self._check(dev.mlh_set_persistent(self._h, int(enabled)))

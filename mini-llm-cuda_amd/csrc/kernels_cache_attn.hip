@@ -876,6 +876,7 @@ static std::string attn_check(const mlh_kv_cache* c, const mlh_kv_batch* b, cons
     return "";
 }
 
+#define KV_SPLIT_WGS 512 // keys are split until a call has this many workgroups: two a compute unit
 struct AttnPlan { // which kernel, and how the keys are split
     int many;         // waves of a workgroup of k_kvattn_many; 0: the kernels of 16 rows
     int blocks, nsplit;
@@ -894,11 +895,14 @@ static AttnPlan attn_plan(const mlh_kv_cache* c, const mlh_kv_batch* b, const ml
     const long long seen = a->window ? std::min<long long>(maxLen, (long long)a->window + std::min<long long>(a->sinks, maxLen) + 64) : maxLen;
     const long long rounds = (seen + 8 * 32 - 1) / (8 * 32); // turns of a workgroup's eight waves
     const long long wgs = (long long)std::min(P.blocks, (b->rows * group + 15) / 16 + std::min(c->nseq, b->rows)) * c->heads;
-    const long long n = P.many ? 1 : std::min<long long>((512 + wgs - 1) / wgs, (rounds + 1) / 2); // two workgroups a compute unit, two turns or more a workgroup
+    const long long n = P.many ? 1 : std::min<long long>((KV_SPLIT_WGS + wgs - 1) / wgs, (rounds + 1) / 2); // two workgroups a compute unit, two turns or more a workgroup
     P.nsplit = (int)std::max<long long>(1, std::min<long long>(n, 64));
     P.bytes = P.nsplit > 1 ? (size_t)P.nsplit * b->rows * b->heads * (c->headDim + 2) * 4 : 0;
     return P;
 }
+
+// A workgroup has 16 rows at most, and nsplit times their number is below KV_SPLIT_WGS and once more their own, which is below that where keys are split.
+size_t mlh_attention_work_most(int headDim) { return (size_t)2 * KV_SPLIT_WGS * 16 * (headDim + 2) * 4; }
 
 template <typename IT, typename CT, int HD, int NW> static hipError_t launch_many(dim3 grid, hipStream_t st, const KvAttnArgs& A) {
     constexpr int bytes = 4 * 64 * HD * 2 + 16;

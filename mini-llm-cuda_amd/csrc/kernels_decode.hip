@@ -998,6 +998,7 @@ int mlh_init_kernels(mlh_ctx*) { return 0; }
 
 int mlh_launch_mix(mlh_ctx* c, const StepArgs& a, const LayerDev& L) {
     hipStream_t st = c->stream;
+    if (L.kind == MLH_KIND_ATTENTION && mlh_cache_ops(c)) return mlh_cache_step(c, a, L);
     if (L.kind == MLH_KIND_ATTENTION) {
         if (a.hd == 64) {
             size_t lds = attn_lds_bytes(64);
@@ -1043,6 +1044,7 @@ int mlh_launch_step(mlh_ctx* c, int nseq, const int* tokPtr, bool lmHead, bool e
     StepArgs a;
     mlh_fill_args(c, a, nseq, tokPtr);
     hipStream_t st = c->stream;
+    if (const int rc = mlh_cache_begin(c, nseq, nseq, c->d_sidx, nullptr, nullptr, nullptr)) return rc;
     if (c->hp.weightDtype == MLH_DTYPE_BF16)
         hipLaunchKernelGGL((k_embed<bf16_t>), dim3(ceil_div(a.dim, WG), nseq), dim3(WG), 0, st, a);
     else
@@ -1090,6 +1092,7 @@ int mlh_launch_one(mlh_ctx* c, int kernel, int layer, int nseq) {
             break;
         case MLH_K_ATTN:
             if (L.kind != MLH_KIND_ATTENTION) { c->err = "layer is not an attention layer"; return -1; }
+            if (mlh_cache_begin(c, nseq, nseq, c->d_sidx, nullptr, nullptr, nullptr) != 0) return -1;
             if (mlh_launch_mix(c, a, L) != 0) return -1;
             break;
         case MLH_K_GDN:
@@ -1142,8 +1145,12 @@ double mlh_kernel_bytes(mlh_ctx* c, int kernel, int layer, int nseq) {
         case MLH_K_FFN_DOWN: return wb * (double)hp.dim * hp.ffnDim;
         case MLH_K_LMHEAD: return wb * (double)hp.vocabSize * hp.dim;
         case MLH_K_ATTN: {
+            const double e = c->kvType == MLH_CACHE_Q4 ? 0.625 : 4.0; // bytes of an element in the pages
             double b = 0;
-            for (int s = 0; s < nseq; s++) b += 2.0 * 4.0 * hp.dim * (c->h_len[s] + 1) + 2.0 * 4.0 * hp.dim;
+            for (int s = 0; s < nseq; s++) {
+                const int n = c->h_len[s] + 1, seen = c->window && n > c->window ? c->window + std::min(c->sinks, n - c->window) : n;
+                b += 2.0 * e * hp.dim * seen + 2.0 * e * hp.dim;
+            }
             return b;
         }
         case MLH_K_GDN: return 2.0 * 4.0 * nseq * hp.gdnHeads * hp.gdnDk * hp.gdnDv;

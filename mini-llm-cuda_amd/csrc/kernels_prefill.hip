@@ -396,6 +396,22 @@ __global__ void __launch_bounds__(NW * 64) k_pf_attn(PfArgs P, LayerDev L) {
 }
 
 // ----------------------------------------------------------------------------
+// What the operators of a paged cache leave of an attention layer (kernels_cache_ctx.hip), gated, into the output projection's input.  Grid: pieces
+// of four columns a thread (and one for the PLE columns) x rows.
+// ----------------------------------------------------------------------------
+template <typename AT> __global__ void __launch_bounds__(PWG) k_pf_cache_put(PfArgs P, LayerDev L, const float* out) {
+    const int row = blockIdx.y, c4 = (blockIdx.x * PWG + threadIdx.x) * 4;
+    if ((int)blockIdx.x == (P.a.dim / 4 + PWG - 1) / PWG) { ple_columns<1>(P, L, row, 1, threadIdx.x, PWG); return; }
+    if (c4 >= P.a.dim) return;
+    f32x4 o = *reinterpret_cast<const f32x4*>(out + (size_t)row * P.a.dim + c4);
+    if (P.a.gating) {
+        const f32x4 z = *reinterpret_cast<const f32x4*>(P.QKV + (size_t)row * P.qkvLd + L.offG + c4);
+        o.x *= pf_sigmoid(z.x); o.y *= pf_sigmoid(z.y); o.z *= pf_sigmoid(z.z); o.w *= pf_sigmoid(z.w);
+    }
+    put_mix4<AT>(P, row, c4, o);
+}
+
+// ----------------------------------------------------------------------------
 // fp16 MFMA causal attention (bf16-weight models; their MFMA path computes in IEEE half, see the host section).  A workgroup owns one head and 128 consecutive
 // queries of one segment, a wave 32 of them.  Per 64-key page:
 //   S^T[key, query] = K . Q^T      (A = K tile from LDS, B = Q^T held in registers)
@@ -2157,6 +2173,7 @@ int mlh_run_prefill_gemm(mlh_ctx* c, int nseg, const int32_t* seqs, const int32_
         else if (dt == MLH_GEMM_P3) launch_rmsnorm<p3_t>(st, X_, gain_, P.Xn, nullptr, n, d_);                                \
         else launch_rmsnorm<h2_t>(st, X_, gain_, P.Xn, P.exps, n, d_);                                                        \
     } while (0)
+    if ((rc = mlh_cache_begin(c, nseg, n, P.segSeq, P.segStart, P.segLen, P.segPos0))) return rc;
     const int pleWgs = hp.pleDim > 0 && (P.half || rowsPath) ? 1 : 0; // a row's (segment's, chunk's) workgroup for the PLE columns
 
     if (rowsPath) mlh_rows_embed(c, P.ids, n, P.X, P.lay);
@@ -2172,7 +2189,12 @@ int mlh_run_prefill_gemm(mlh_ctx* c, int nseg, const int32_t* seqs, const int32_
             NORM(P.X, L.g1);
             GEMM(P.Xn, d_, P.exps, L.WaP, L.sWa, L.eWa, d_, P.QKV, P.qkvLd, nullptr, 0, n, L.rowsA, d_);
         }
-        if (L.kind == MLH_KIND_ATTENTION) {
+        if (L.kind == MLH_KIND_ATTENTION && mlh_cache_ops(c)) {
+            if ((rc = mlh_cache_layer(c, L, nseg, n, P.QKV, P.qkvLd, P.H1))) return rc; // (H1 is written by the output projection only)
+            const dim3 grid(cdiv(d_ / 4, PWG) + pleWgs, n);
+            if (P.half) hipLaunchKernelGGL((k_pf_cache_put<f16_t>), grid, dim3(PWG), 0, st, P, L, P.H1);
+            else hipLaunchKernelGGL((k_pf_cache_put<float>), grid, dim3(PWG), 0, st, P, L, P.H1);
+        } else if (L.kind == MLH_KIND_ATTENTION) {
 #define ATTN_ROWS(HD_, AT_)                                                                                                    \
     do {                                                                                                                     \
         if (hp.attnHeads * nblk <= c->numCUs) hipLaunchKernelGGL((k_pf_attn<HD_, 8, AT_>), dim3(hp.attnHeads, nblk), dim3(512), 0, st, P, L); \

@@ -494,8 +494,8 @@ int mlh_rows_step(mlh_ctx* c, int nseq, const int* tokPtr, bool lmHead, bool emb
     if (!embedded) mlh_mark(c, MLH_K_EMBED);
     RowsArgs base = {};
     base.M = nseq; base.lay = lay; base.normDim = d; base.sidx = c->d_sidx;
+    int rc = mlh_cache_begin(c, nseq, nseq, c->d_sidx, nullptr, nullptr, nullptr);
     int nparts = 1; // partial sums behind rowsX: one from the embedding, one per workgroup from a down projection
-    int rc = 0;
     for (int t = first; t >= 0 && rc == 0; t--) { // file block 0 is the top (inference.cu:384-385)
         const LayerDev& L = c->layers[t];
         RowsArgs P = base; // q | k | v | ... of the normalised rows (inference.cu:388-465, 487-507)
@@ -503,7 +503,7 @@ int mlh_rows_step(mlh_ctx* c, int nseq, const int* tokPtr, bool lmHead, bool emb
         mlh_rows_gemm(c, RW_PLAIN, L.WaR, L.rowsA, P);
         mlh_mark(c, MLH_K_QKV);
         rc = mlh_launch_mix(c, a, L);
-        if (L.kind == MLH_KIND_ATTENTION && c->nsplit > 1) hipLaunchKernelGGL(k_rows_mix, dim3(nseq, (L.ad + hp.pleDim + 255) / 256), dim3(256), 0, st, a, L);
+        if (L.kind == MLH_KIND_ATTENTION && c->nsplit > 1 && !mlh_cache_ops(c)) hipLaunchKernelGGL(k_rows_mix, dim3(nseq, (L.ad + hp.pleDim + 255) / 256), dim3(256), 0, st, a, L);
         mlh_mark(c, L.kind == MLH_KIND_ATTENTION ? MLH_K_ATTN : MLH_K_GDN); // (the combination of the partial results with it)
         mlh_rows_rest_of_layer(c, t, base, c->x, c->h1);
         nparts = d / RW_TILE;

@@ -685,7 +685,7 @@ static int ensure_graph(mlh_ctx* c, int slot, int nseq, int k) {
 // Several sequences, and one of a model that the XCD-rank kernel does not cover, in one launch of kernels_ranks.hip or kernels_wide.hip.  (A caller who
 // asked for graph replays gets those.)
 static bool for_ranks(const mlh_ctx* c, int nseq) {
-    if (c->usePersistent != 3 || c->temperature > 0.f || c->graphSteps > 0 || !mlh_ranks_applicable(c, nseq)) return false;
+    if (c->usePersistent != 3 || c->temperature > 0.f || c->graphSteps > 0 || mlh_cache_ops(c) || !mlh_ranks_applicable(c, nseq)) return false;
     return nseq > 1 || !mlh_xcd_supported(c);
 }
 static bool use_ranks(const mlh_ctx* c, int nseq) { return !c->ranksOff && for_ranks(c, nseq); }
@@ -693,7 +693,7 @@ static bool use_ranks(const mlh_ctx* c, int nseq) { return !c->ranksOff && for_r
 static bool use_persistent(const mlh_ctx* c, int nseq) {
     if (use_ranks(c, nseq)) return true;
     // (the single-launch kernels fuse the argmax only: sampling runs through the kernel sequence)
-    if (nseq != 1 || !c->usePersistent || c->temperature > 0.f) return false;
+    if (nseq != 1 || !c->usePersistent || c->temperature > 0.f || mlh_cache_ops(c)) return false; // (nor do they know windows and 4-bit pages)
     // mode 3 on a model the XCD-rank kernel does not cover: the row step where it applies (its launches cost less than the
     // barrier kernel's phases), else the barrier kernel
     if (c->usePersistent == 3) return mlh_xcd_supported(c) || (!mlh_rows_applicable(c, 1) && mlh_persistent_supported(c));
@@ -983,7 +983,7 @@ extern "C" int mlh_debug_set_xcd_tag(mlh_ctx* c, unsigned tagsUsed) {
 }
 
 extern "C" int mlh_single_launch_sequences(mlh_ctx* c) {
-    if (!c) return 0;
+    if (!c || mlh_cache_ops(c)) return 0;
     return std::max(c->ranksMax, mlh_xcd_supported(c) ? 1 : 0);
 }
 
@@ -994,7 +994,7 @@ extern "C" int mlh_decode_route(const mlh_ctx* c, int nseq) {
     return mlh_rows_applicable(c, nseq) ? MLH_DECODE_ROWS : MLH_DECODE_GEMV;
 }
 
-extern "C" int mlh_xcd_decode_supported(mlh_ctx* c) { return c && mlh_xcd_supported(c) ? 1 : 0; }
+extern "C" int mlh_xcd_decode_supported(mlh_ctx* c) { return c && !mlh_cache_ops(c) && mlh_xcd_supported(c) ? 1 : 0; }
 
 extern "C" int mlh_synchronize(mlh_ctx* c) {
     if (!c) return -1;

@@ -225,6 +225,12 @@ struct mlh_ctx {
     long f16Inexact = 0;       // bf16 weights that had no exact scaled-half representation (reported at finalize)
     void* gemmWs = nullptr;    // split-K workspace of the prefill's products
 
+    // attention layers on the operators of a paged cache (kernels_cache_ctx.hip)
+    int window = 0, sinks = 0;     // 0: every position is seen
+    int kvType = MLH_DTYPE_F32;    // of the pages: MLH_DTYPE_F32 or MLH_CACHE_Q4
+    int* cacheMeta = nullptr;      // rows, lengths and pages of the call at hand
+    void* cacheWork = nullptr;     // shares of split keys
+
     std::vector<int> h_len; // host mirror of d_pos
     std::vector<char> h_dirty;     // sequences that some launch may have given a length or GDN states since their last reset
     std::vector<char> h_nextKnown; // sequences whose next token h_next holds
@@ -318,6 +324,13 @@ int mlh_launch_ranks(mlh_ctx* c, int nseq, int steps);
 bool mlh_wide_model(const mlh_ctx* c);
 int mlh_wide_prepare(mlh_ctx* c);
 int mlh_launch_wide(mlh_ctx* c, int nseq, int steps, unsigned tagBase, int otherAt);
+
+// kernels_cache_ctx.hip: attention layers with a window or with pages of 4 bits; mlh_cache_begin once before the layers of a step or prefill
+bool mlh_cache_ops(const mlh_ctx* c);
+int mlh_cache_begin(mlh_ctx* c, int n, int rows, const int* seqs, const int* segStart, const int* segLen, const int* segPos0);
+int mlh_cache_layer(mlh_ctx* c, const LayerDev& L, int n, int rows, float* qkv, int ld, float* out);
+int mlh_cache_step(mlh_ctx* c, const StepArgs& a, const LayerDev& L);
+size_t mlh_attention_work_most(int headDim); // kernels_cache_attn.hip: what no call of fp32 rows needs more than
 
 // kernels_persistent.hip
 bool mlh_persistent_supported(const mlh_ctx* c);
