@@ -443,7 +443,7 @@ typedef struct {
     int32_t window; /* 0: everything */
     int32_t sinks;
     int32_t maxLen, maxNew;
-    float scale;    /* 0: 1 / sqrt(headDim) */
+    float scale;    /* 1e-30 to 1e30; 0: 1 / sqrt(headDim) */
     void* work;
     uint64_t workBytes;
 } mlh_attention;

@@ -6,8 +6,22 @@
 
 #include "kv_cache.h"
 
+#ifndef KV_WG
+#ifndef KV_WG
+#ifndef KV_WG
+#ifndef KV_WG
+#ifndef KV_WG
 #define KV_WG 256
-#define KV_MAX_GRID 1048576 // workgroups of a launch: beyond, they take several turns
+#endif
+#endif
+#endif
+#endif
+#endif
+#ifndef KV_RW
+#define KV_RW 4
+#endif
+// workgroups along the rows: with `pieces` of a row each below 2^32 threads, which is what a launch can have; beyond, they take several turns
+static unsigned kv_grid(int rows, int pieces) { return (unsigned)std::min(rows, std::max(1, (1 << 22) / pieces)); }
 
 struct KvRows { // what the kernels need of cache and batch
     const int32_t *start, *len, *table;
@@ -17,9 +31,9 @@ struct KvRows { // what the kernels need of cache and batch
 // sequence and position of a row; false: behind the last sequence
 __device__ __forceinline__ bool kv_row(const KvRows& R, int row, int& seq, int& pos) {
     const int s = kv_find(R.nseq, row, [&](int i) { return R.start[i]; });
-    const int b = R.start[s], e = R.start[s + 1];
+    const int b = kv_uniform(R.start, s), e = kv_uniform(R.start, s + 1);
     seq = s;
-    pos = (int)((unsigned)R.len[s] - (unsigned)e + (unsigned)row);
+    pos = (int)((unsigned)kv_uniform(R.len, s) - (unsigned)e + (unsigned)row);
     return row >= b && row < e;
 }
 
@@ -31,7 +45,6 @@ struct KvAppendArgs {
     long long qStride, qOutStride, kStride, vStride;
     const float *rope, *qGain, *kGain;
     int ropeRows;
-    int pieces; // workgroups a row
 };
 
 // The code of x: the nearest whole number to (x - base) / scale.  The fp32 quotient is off by less than 2^-20 (three roundings of values up to 15, and inv's): only
@@ -43,28 +56,29 @@ __device__ __forceinline__ uint32_t kv_code(float x, float base, float scale, fl
     return (uint32_t)fminf(fmaxf(c, 0.f), 15.f);
 }
 
-// One thread: eight elements of a head's row of q, k or v.  HD / 8 neighbouring threads hold the row (norm), four a group of 32 (4-bit codes).  Grid: rows
-// x pieces, a row's heads one after another over its pieces.
-template <typename IT, typename CT, int HD>
+// One thread: eight elements of a head's row of q, k or v.  HD / 8 neighbouring threads hold the row (norm), four a group of 32 (4-bit codes).  Grid: rows x pieces of the
+// heads.  Bound by memory: 17435 rows of 32 + 8 + 8 heads of 128 in bf16, 429 MB, 91 us (4.7 TB/s; a plain copy 5.2; 15 of them are the products in 64 bits).  Streaming
+// stores (NT) for calls that write more than the L2s hold: 112 us without.  Two, four and eight rows a workgroup, their loads together: 95, 107 and 149 us.
+template <typename IT, typename CT, int HD, bool NT>
 __global__ void __launch_bounds__(KV_WG) k_kv_append(KvAppendArgs A) {
     constexpr int T = HD / 8;
+    const int u = blockIdx.y * KV_WG + threadIdx.x;
     const int units = (A.R.heads + 2 * A.R.kvHeads) * T, qUnits = A.R.heads * T, kUnits = A.R.kvHeads * T;
-    const long long total = (long long)A.R.rows * A.pieces;
-    for (long long b = blockIdx.x; b < total; b += gridDim.x) {
-        const int row = (int)(b / A.pieces), u = (int)(b % A.pieces) * KV_WG + threadIdx.x;
+    const int kind = u < qUnits ? 0 : u < qUnits + kUnits ? 1 : 2; // q, k, v
+    const int w = u - (kind == 0 ? 0 : kind == 1 ? qUnits : qUnits + kUnits), h = w / T, d = (w % T) * 8;
+    const bool live = u < units && (kind != 0 || A.q); // (whole heads' threads: HD / 8 divides 64)
+    const IT* const src = (const IT*)(kind == 0 ? A.q : kind == 1 ? A.k : A.v) + (size_t)h * HD + d;
+    const long long stride = kind == 0 ? A.qStride : kind == 1 ? A.kStride : A.vStride;
+    const float* const gain = kind == 0 ? A.qGain : kind == 1 ? A.kGain : nullptr;
+    for (int row = blockIdx.x; row < A.R.rows; row += gridDim.x) {
+        float x[8], cs[8];
         int seq, pos;
-        if (!kv_row(A.R, row, seq, pos)) continue;
-        if (u >= units) continue; // (whole heads' threads: HD / 8 divides 64)
-        const int kind = u < qUnits ? 0 : u < qUnits + kUnits ? 1 : 2; // q, k, v
-        const int w = u - (kind == 0 ? 0 : kind == 1 ? qUnits : qUnits + kUnits), h = w / T, d = (w % T) * 8;
-        if (kind == 0 && !A.q) continue;
-        const int page = pos < 0 ? -1 : kv_page(A.R.table, A.R.pagesPerSeq, A.R.numPages, seq, pos >> 6);
-        const bool ok = page >= 0 && (!A.rope || pos < A.ropeRows);
-        if (!ok && kind != 0) continue;
-        const IT* src = kind == 0 ? (const IT*)A.q + (size_t)row * A.qStride : kind == 1 ? (const IT*)A.k + (size_t)row * A.kStride : (const IT*)A.v + (size_t)row * A.vStride;
-        float x[8];
-        kv_load8(src + (size_t)h * HD + d, x);
-        const float* gain = kind == 0 ? A.qGain : kind == 1 ? A.kGain : nullptr;
+        if (live) kv_load8(src + (size_t)row * stride, x); // (on its way while the row's sequence and page are looked up)
+        const bool mine = kv_row(A.R, row, seq, pos);
+        int page = pos < 0 ? -1 : kv_page(A.R.table, A.R.pagesPerSeq, A.R.numPages, seq, pos >> 6);
+        if (A.rope && pos >= A.ropeRows) page = -1;
+        if (!live || !mine || (page < 0 && kind != 0)) continue;
+        if (A.rope && kind != 2) kv_load8(A.rope + (size_t)(page < 0 ? 0 : pos) * HD + d, cs);
         if (gain) {
             double s = 0.0;
 #pragma unroll
@@ -75,9 +89,7 @@ __global__ void __launch_bounds__(KV_WG) k_kv_append(KvAppendArgs A) {
 #pragma unroll
             for (int i = 0; i < 8; i++) x[i] = (float)((double)gain[h * HD + d + i] * ((double)x[i] / r));
         }
-        if (A.rope && kind != 2 && ok) {
-            float cs[8];
-            kv_load8(A.rope + (size_t)pos * HD + d, cs);
+        if (A.rope && kind != 2) {
 #pragma unroll
             for (int i = 0; i < 8; i += 2) { // (products of two fp32 values are exact in 64 bits)
                 const double a = x[i], c = x[i + 1], co = cs[i], si = cs[i + 1];
@@ -86,16 +98,16 @@ __global__ void __launch_bounds__(KV_WG) k_kv_append(KvAppendArgs A) {
             }
         }
         if (kind == 0) {
-            if (!ok) {
+            if (page < 0) {
 #pragma unroll
                 for (int i = 0; i < 8; i++) x[i] = __uint_as_float(0x7fc00000u);
             }
-            kv_store8((IT*)A.qOut + (size_t)row * A.qOutStride + (size_t)h * HD + d, x);
+            kv_store8<NT>((IT*)A.qOut + (size_t)row * A.qOutStride + (size_t)h * HD + d, x);
             continue;
         }
         void* pool = kind == 1 ? A.poolK : A.poolV;
         if constexpr (KvType<CT>::code != MLH_CACHE_Q4) {
-            kv_store8((CT*)pool + (((size_t)page * MLH_KV_PAGE + (pos & 63)) * A.R.kvHeads + h) * HD + d, x);
+            kv_store8<NT>((CT*)pool + (((size_t)page * MLH_KV_PAGE + (pos & 63)) * A.R.kvHeads + h) * HD + d, x);
         } else {
             float lo = x[0], hi = x[0], bad = 0.f;
 #pragma unroll
@@ -123,16 +135,14 @@ struct KvReadArgs {
     const void *poolK, *poolV;
     void *k, *v;
     long long stride;
-    int pieces;
 };
 
 template <typename OT, typename CT, int HD>
 __global__ void __launch_bounds__(KV_WG) k_kv_read(KvReadArgs A) {
     constexpr int T = HD / 8;
     const int units = 2 * A.R.kvHeads * T, kUnits = A.R.kvHeads * T;
-    const long long total = (long long)A.R.rows * A.pieces;
-    for (long long b = blockIdx.x; b < total; b += gridDim.x) {
-        const int row = (int)(b / A.pieces), u = (int)(b % A.pieces) * KV_WG + threadIdx.x;
+    const int u = blockIdx.y * KV_WG + threadIdx.x;
+    for (int row = blockIdx.x; row < A.R.rows; row += gridDim.x) {
         int seq, pos;
         if (!kv_row(A.R, row, seq, pos)) continue;
         if (u >= units) continue;
@@ -151,7 +161,7 @@ __global__ void __launch_bounds__(KV_WG) k_kv_read(KvReadArgs A) {
             kv_values8(*reinterpret_cast<const uint32_t*>(tile + (pos & 63) * (HD / 2) + d / 2),
                        *reinterpret_cast<const uint32_t*>(tile + kv_param_at(HD) + ((pos & 63) * (HD / KV_GROUP) + d / KV_GROUP) * 4), x);
         }
-        kv_store8((OT*)(val ? A.v : A.k) + (size_t)row * A.stride + (size_t)h * HD + d, x);
+        kv_store8<false>((OT*)(val ? A.v : A.k) + (size_t)row * A.stride + (size_t)h * HD + d, x);
     }
 }
 
@@ -223,13 +233,16 @@ extern "C" int mlh_kv_append_device(const mlh_kv_cache* c, const mlh_kv_batch* b
     if (bad.empty() && ((uintptr_t)a->qGain | (uintptr_t)a->kGain) % 4) bad = "gains must be 4-byte aligned";
     if (!bad.empty()) return kv_fail(bad);
     if (b->rows == 0) return 0;
-    KvAppendArgs A = {kv_rows_of(c, b), c->k, c->v, a->q, a->k, a->v, a->qOut, a->qStride, a->qOutStride, a->kStride, a->vStride, a->rope, a->qGain, a->kGain, a->ropeRows, 0};
-    A.pieces = ((b->heads + 2 * c->heads) * (hd / 8) + KV_WG - 1) / KV_WG;
-    const unsigned grid = (unsigned)std::min<long long>((long long)b->rows * A.pieces, KV_MAX_GRID);
+    KvAppendArgs A = {kv_rows_of(c, b), c->k, c->v, a->q, a->k, a->v, a->qOut, a->qStride, a->qOutStride, a->kStride, a->vStride, a->rope, a->qGain, a->kGain, a->ropeRows};
+    const int pieces = ((b->heads + 2 * c->heads) * (hd / 8) + KV_WG - 1) / KV_WG;
+    const dim3 grid(kv_grid(b->rows, pieces), pieces);
+    const bool nt = (double)b->rows * (b->heads + 2 * c->heads) * hd * kv_elem_bytes(b->type) > 32e6; // eight L2s of 4 MB
 #define KV_GO(IT_, CT_) \
     do { \
-        if (hd == 64) hipLaunchKernelGGL((k_kv_append<IT_, CT_, 64>), dim3(grid), dim3(KV_WG), 0, (hipStream_t)stream, A); \
-        else hipLaunchKernelGGL((k_kv_append<IT_, CT_, 128>), dim3(grid), dim3(KV_WG), 0, (hipStream_t)stream, A); \
+        if (hd == 64 && nt) hipLaunchKernelGGL((k_kv_append<IT_, CT_, 64, true>), grid, dim3(KV_WG), 0, (hipStream_t)stream, A); \
+        else if (hd == 64) hipLaunchKernelGGL((k_kv_append<IT_, CT_, 64, false>), grid, dim3(KV_WG), 0, (hipStream_t)stream, A); \
+        else if (nt) hipLaunchKernelGGL((k_kv_append<IT_, CT_, 128, true>), grid, dim3(KV_WG), 0, (hipStream_t)stream, A); \
+        else hipLaunchKernelGGL((k_kv_append<IT_, CT_, 128, false>), grid, dim3(KV_WG), 0, (hipStream_t)stream, A); \
     } while (0)
     if (c->type == MLH_CACHE_Q4) {
         if (b->type == MLH_DTYPE_F32) KV_GO(float, q4_t);
@@ -251,13 +264,13 @@ extern "C" int mlh_kv_read_device(const mlh_kv_cache* c, const mlh_kv_batch* b, 
     if (bad.empty()) bad = kv_check_rows("v", a->v, a->stride, (long long)c->heads * hd, b->type);
     if (!bad.empty()) return kv_fail(bad);
     if (b->rows == 0) return 0;
-    KvReadArgs A = {kv_rows_of(c, b), c->k, c->v, a->k, a->v, a->stride, 0};
-    A.pieces = (2 * c->heads * (hd / 8) + KV_WG - 1) / KV_WG;
-    const unsigned grid = (unsigned)std::min<long long>((long long)b->rows * A.pieces, KV_MAX_GRID);
+    KvReadArgs A = {kv_rows_of(c, b), c->k, c->v, a->k, a->v, a->stride};
+    const int pieces = (2 * c->heads * (hd / 8) + KV_WG - 1) / KV_WG;
+    const dim3 grid(kv_grid(b->rows, pieces), pieces);
 #define KV_GO2(OT_, CT_) \
     do { \
-        if (hd == 64) hipLaunchKernelGGL((k_kv_read<OT_, CT_, 64>), dim3(grid), dim3(KV_WG), 0, (hipStream_t)stream, A); \
-        else hipLaunchKernelGGL((k_kv_read<OT_, CT_, 128>), dim3(grid), dim3(KV_WG), 0, (hipStream_t)stream, A); \
+        if (hd == 64) hipLaunchKernelGGL((k_kv_read<OT_, CT_, 64>), grid, dim3(KV_WG), 0, (hipStream_t)stream, A); \
+        else hipLaunchKernelGGL((k_kv_read<OT_, CT_, 128>), grid, dim3(KV_WG), 0, (hipStream_t)stream, A); \
     } while (0)
 #define KV_GO(CT_) \
     do { \

@@ -30,6 +30,13 @@ struct KvAttnArgs {
     float scale2; // scale * log2 e
 };
 
+#ifdef KV_MAP2
+#define KV_KH (blockIdx.x / (gridDim.x / A.kvHeads))
+#define KV_BLK (blockIdx.x % (gridDim.x / A.kvHeads))
+#else
+#define KV_KH (blockIdx.x % A.kvHeads)
+#define KV_BLK (blockIdx.x / A.kvHeads)
+#endif
 #define KV_NAN __uint_as_float(0x7fc00000u)
 
 // The rows of a workgroup: nr of them from row r0 of sequence s.
@@ -44,12 +51,12 @@ struct KvBlock {
 template <int QB> __device__ __forceinline__ bool kv_block(const KvAttnArgs& A, int blk, KvBlock& B) {
     auto first = [&](int i) { return A.start[i] * A.group / QB + i; };
     const int s = kv_find(A.nseq, blk, first);
-    const int b = A.start[s], e = A.start[s + 1], end = min(e, A.rows);
+    const int b = kv_uniform(A.start, s), e = kv_uniform(A.start, s + 1), end = min(e, A.rows);
     if (b < 0 || end <= b) return false;
-    const int r0 = (blk - first(s)) * QB, all = (end - b) * A.group;
+    const int r0 = (blk - (b * A.group / QB + s)) * QB, all = (end - b) * A.group;
     if (r0 < 0 || r0 >= all) return false;
     B.s = s; B.r0 = r0; B.nr = min(QB, all - r0); B.row0 = b;
-    B.pos0 = (int)((unsigned)A.len[s] - (unsigned)e + (unsigned)b);
+    B.pos0 = (int)((unsigned)kv_uniform(A.len, s) - (unsigned)e + (unsigned)b);
     B.cap = A.pagesPerSeq * MLH_KV_PAGE;
     B.minPos = max(B.pos0 + r0 / A.group, -1);
     B.maxPos = min(B.pos0 + (r0 + B.nr - 1) / A.group, B.cap - 1);
@@ -114,6 +121,18 @@ template <typename CT, int HD> __device__ __forceinline__ float kv_one(const voi
         else if constexpr (KvType<CT>::code == MLH_DTYPE_BF16) return kv_bf16(*p);
         else return kv_half(p->bits);
     }
+}
+
+// The elements of a row of V that are no numbers, zeros for the others, as floats into HD places of the wave's own: for the repair of a tile, by one key at a time.
+template <typename CT, int HD, bool HALVES> __device__ __forceinline__ void kv_odd_row(const KvAttnArgs& A, int page, int at, int kh, float* place) {
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll 1
+    for (int d = threadIdx.x & 63; d < HD; d += 64) {
+        float x = kv_one<CT, HD>(A.poolV, page, at, A.kvHeads, kh, d);
+        if (HALVES) x = (float)(_Float16)x;
+        place[d] = kv_finite(x) ? 0.f : x;
+    }
+    __builtin_amdgcn_wave_barrier(); // (LDS serves a wave's accesses in order)
 }
 
 // The end of the 16-row kernels: acc of every wave (block b, element i of lane 16 g + n: row n, element dim(b, 4 g + i)), its m and l (of row n), joined over the waves, and
@@ -229,9 +248,10 @@ template <typename CT, int HD>
 __global__ void __launch_bounds__(KV_W32 * 64) k_kvattn_f32(KvAttnArgs A) {
     constexpr int NW = KV_W32, KC = HD / 4, VB = HD / 16;
     __shared__ __attribute__((aligned(16))) float lds[NW * 16 * (HD + 4 + 2)];
-    const int kh = blockIdx.x % A.kvHeads, split = blockIdx.y, tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, n = lane & 15, g = lane >> 4;
+    __shared__ float odds[NW][HD];
+    const int kh = KV_KH, split = blockIdx.y, tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, n = lane & 15, g = lane >> 4;
     KvBlock B;
-    if (!kv_block<16>(A, blockIdx.x / A.kvHeads, B)) return;
+    if (!kv_block<16>(A, KV_BLK, B)) return;
     const int r = B.r0 + min(n, B.nr - 1), h = kh * A.group + r % A.group;
     const KvSight sight(A, B.pos0 + r / A.group);
     f32x4 q[KC / 4];
@@ -294,18 +314,27 @@ __global__ void __launch_bounds__(KV_W32 * 64) k_kvattn_f32(KvAttnArgs A) {
             if (__ballot(odd)) {
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
+                    bool odd_ = false;
 #pragma unroll
-                    for (int b = 0; b < VB; b++) v[e][b / 4][b % 4] = kv_finite(v[e][b / 4][b % 4]) ? v[e][b / 4][b % 4] : 0.f;
+                    for (int b = 0; b < VB; b++) {
+                        odd_ = odd_ || !kv_finite(v[e][b / 4][b % 4]);
+                        v[e][b / 4][b % 4] = kv_finite(v[e][b / 4][b % 4]) ? v[e][b / 4][b % 4] : 0.f;
+                    }
+                    const unsigned long long who = __ballot(odd_);
+#pragma unroll 1
                     for (int gk = 0; gk < 4; gk++) {
                         const int j = j0 + 4 * gk + e;
-                        if (j > B.maxPos) break;
+                        if (j > B.maxPos || page[set] < 0 || !(who >> (16 * gk) & 0xffffu)) continue;
+                        kv_odd_row<CT, HD, false>(A, page[set], j & 63, kh, odds[wave]);
                         const float w = __shfl(p[e], 16 * gk + n, 64);
-                        for (int i4 = 0; i4 < 4; i4++)
+                        const bool see_ = sight.sees(j);
 #pragma unroll
-                            for (int b = 0; b < VB; b++) {
-                                const float x = kv_one<CT, HD>(A.poolV, max(page[set], 0), j & 63, A.kvHeads, kh, (4 * g + i4) * VB + b);
-                                const float add = sight.sees(j) && !kv_finite(x) ? w * x : 0.f;
-                                acc[b].x += i4 == 0 ? add : 0.f; acc[b].y += i4 == 1 ? add : 0.f; acc[b].z += i4 == 2 ? add : 0.f; acc[b].w += i4 == 3 ? add : 0.f;
+                        for (int b = 0; b < VB; b++)
+#pragma unroll
+                            for (int i = 0; i < 4; i++) {
+                                if (i == 0) __builtin_amdgcn_sched_barrier(0); // (few registers for what hardly happens)
+                                const float x = odds[wave][(4 * g + i) * VB + b];
+                                acc[b][i] += see_ && x != 0.f ? w * x : 0.f;
                             }
                     }
                 }
@@ -384,10 +413,11 @@ __device__ __forceinline__ u32x4 kv_halves(uint32_t codes, uint32_t params) {
     return o;
 }
 
-// A row's power of two: largest |q| into [1, 2), so that halves hold it.  (0: the row is zero, or holds an infinity or NaN, and stays as it is.)
+// A row's power of two: largest |q| into [1, 2), so that halves hold it; 2^24 at most (what halves then lose of a row is 2^-49), so that the scale divided by it stays
+// a normal number.  (0: the row is zero, or holds an infinity or NaN, and stays as it is.)
 __device__ __forceinline__ int kv_row_exp(float most) {
     const uint32_t e = __float_as_uint(most) >> 23 & 255u;
-    return e == 0 || e == 255 ? 0 : 127 - (int)e;
+    return e == 0 || e == 255 ? 0 : min(127 - (int)e, 24);
 }
 
 template <typename IT, typename CT, int HD> struct KvRaw16 { // a lane's part of 32 keys: key 16 b + n, elements 32 t + 8 g ..; of V the same
@@ -431,17 +461,25 @@ template <typename IT, int HD> struct KvRaw16<IT, q4_t, HD> { // the same, eleme
     __device__ __forceinline__ u32x4 val(int b, int t) const { return kv_halves(v[b][t], vp[b]); }
 };
 
-#define KV_W16 8
+#ifndef KV_NWQ
+#define KV_NWQ 4
+#define KV_OCQ 3
+#endif
+#ifndef KV_NWB
+#define KV_NWB 8
+#endif
+template <typename CT> constexpr int kv_few_waves() { return KvType<CT>::code == MLH_CACHE_Q4 ? KV_NWQ : KV_NWB; }
 template <typename IT, typename CT, int HD>
-__global__ void __launch_bounds__(KV_W16 * 64) k_kvattn_few(KvAttnArgs A) {
+__global__ void __launch_bounds__(kv_few_waves<CT>() * 64, KvType<CT>::code == MLH_CACHE_Q4 ? KV_OCQ : 2) k_kvattn_few(KvAttnArgs A) {
     constexpr bool FOUR = KvType<CT>::code == MLH_CACHE_Q4, BF = !FOUR && KvType<IT>::code == MLH_DTYPE_BF16; // products in bf16
-    constexpr int NW = KV_W16, KS = HD / 32, VB = HD / 16;
+    constexpr int NW = kv_few_waves<CT>(), KS = HD / 32, VB = HD / 16;
     constexpr int VP = HD * 2 + 16; // bytes of a row of V in LDS: four rows start in different banks
     constexpr int LV = NW * 32 * VP, LF = NW * 16 * (HD + 4 + 2) * 4;
     __shared__ __attribute__((aligned(16))) unsigned char lds[LV > LF ? LV : LF];
-    const int kh = blockIdx.x % A.kvHeads, split = blockIdx.y, tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, n = lane & 15, g = lane >> 4;
+    __shared__ float odds[NW][HD];
+    const int kh = KV_KH, split = blockIdx.y, tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, n = lane & 15, g = lane >> 4;
     KvBlock B;
-    if (!kv_block<16>(A, blockIdx.x / A.kvHeads, B)) return;
+    if (!kv_block<16>(A, KV_BLK, B)) return;
     const int r = B.r0 + min(n, B.nr - 1), h = kh * A.group + r % A.group;
     const KvSight sight(A, B.pos0 + r / A.group);
     u32x4 q[KS];
@@ -539,19 +577,20 @@ __global__ void __launch_bounds__(KV_W16 * 64) k_kvattn_few(KvAttnArgs A) {
                     const int k = __builtin_ctz(keys), j = j0 + 16 * b + k;
                     keys &= keys - 1;
                     if (j > B.maxPos) break;
-                    float w = p[b][0];
-                    if ((k & 3) == 1) w = p[b][1];
-                    if ((k & 3) == 2) w = p[b][2];
-                    if ((k & 3) == 3) w = p[b][3];
+                    float w = 0.f;
+#pragma unroll
+                    for (int e = 0; e < 4; e++) w = fmaf(e == (k & 3) ? 1.f : 0.f, p[b][e], w); // (a selection would go through memory)
                     w = __shfl(w, 16 * (k >> 2) + n, 64);
+                    if (page[set] >= 0) kv_odd_row<CT, HD, FOUR>(A, page[set], j & 63, kh, odds[wave]);
+                    const bool see_ = page[set] >= 0 && sight.sees(j);
 #pragma unroll
                     for (int c = 0; c < VB; c++)
 #pragma unroll
                         for (int e = 0; e < 4; e++) {
+                            if (e == 0) __builtin_amdgcn_sched_barrier(0); // (few registers for what hardly happens)
                             const int at = 16 * c + 4 * g + e, d = FOUR ? (at & ~7) + (at & 7) / 2 + 4 * (at & 1) : at;
-                            float x = kv_one<CT, HD>(A.poolV, max(page[set], 0), j & 63, A.kvHeads, kh, d);
-                            if (FOUR) x = (float)(_Float16)x;
-                            acc[c][e] += sight.sees(j) && !kv_finite(x) ? w * x : 0.f;
+                            const float x = odds[wave][d];
+                            acc[c][e] += see_ && x != 0.f ? w * x : 0.f;
                         }
                 }
             }
@@ -612,8 +651,9 @@ template <typename IT, typename CT, int HD, int NW>
 __global__ void __launch_bounds__(NW * 64, 2) k_kvattn_many(KvAttnArgs A) {
     constexpr bool FOUR = KvType<CT>::code == MLH_CACHE_Q4, BF = !FOUR && KvType<IT>::code == MLH_DTYPE_BF16;
     constexpr int KS = HD / 16, MB = HD / 32, TB = 64 * HD * 2, QB = NW * 32; // TB: bytes of a tile of K or V
-    extern __shared__ __attribute__((aligned(16))) unsigned char lds[]; // K, V of two tiles; keys to repair
+    extern __shared__ __attribute__((aligned(16))) unsigned char lds[]; // K, V of two tiles; keys to repair; a row of V for each wave
     uint32_t* const flags = reinterpret_cast<uint32_t*>(lds + 4 * TB);
+    float (*const odds)[HD] = reinterpret_cast<float (*)[HD]>(lds + 4 * TB + 16);
     const int kh = blockIdx.x % A.kvHeads, tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, n = lane & 31, half = lane >> 5;
     KvBlock B;
     if (!kv_block<QB>(A, (gridDim.x - 1 - blockIdx.x) / A.kvHeads, B)) return; // (the last rows of a sequence see most: first)
@@ -752,23 +792,13 @@ __global__ void __launch_bounds__(NW * 64, 2) k_kvattn_many(KvAttnArgs A) {
         }
         m = mn;
         const float ref = mn == -INFINITY ? 0.f : -mn;
-        if (whole) {
 #pragma unroll
-            for (int b = 0; b < 2; b++)
+        for (int b = 0; b < 2; b++)
 #pragma unroll
-                for (int e = 0; e < 16; e++) {
-                    s[b][e] = kv_exp2(fmaf(s[b][e], scale, ref));
-                    l += s[b][e];
-                }
-        } else { // (what is hidden carries -inf; times a scale that has underflowed that would be no number)
-#pragma unroll
-            for (int b = 0; b < 2; b++)
-#pragma unroll
-                for (int e = 0; e < 16; e++) {
-                    s[b][e] = s[b][e] == -INFINITY ? 0.f : kv_exp2(fmaf(s[b][e], scale, ref));
-                    l += s[b][e];
-                }
-        }
+            for (int e = 0; e < 16; e++) { // (hidden: 2^-inf)
+                s[b][e] = kv_exp2(fmaf(s[b][e], scale, ref));
+                l += s[b][e];
+            }
         if (odd[0] | odd[1]) {
 #pragma unroll
             for (int b = 0; b < 2; b++)
@@ -779,14 +809,15 @@ __global__ void __launch_bounds__(NW * 64, 2) k_kvattn_many(KvAttnArgs A) {
                     for (int e = 0; e < 16; e++) w = e == at ? s[b][e] : w;
                     w = __shfl(w, n + 32 * ((k >> 2) & 1), 64);
                     const bool see = sight.sees(j);
+                    kv_odd_row<CT, HD, FOUR>(A, page, j & 63, kh, odds[wave]);
 #pragma unroll
                     for (int c = 0; c < MB; c++)
 #pragma unroll
                         for (int e = 0; e < 16; e++) {
+                            if (e % 4 == 0) __builtin_amdgcn_sched_barrier(0); // (few registers for what hardly happens)
                             const int col = 32 * c + 8 * (e >> 2) + 4 * half + (e & 3), d = FOUR ? (col & ~7) + (col & 7) / 2 + 4 * (col & 1) : col;
-                            float x = kv_one<CT, HD>(A.poolV, page, j & 63, A.kvHeads, kh, d);
-                            if (FOUR) x = (float)(_Float16)x;
-                            acc[c][e] += see && !kv_finite(x) ? w * x : 0.f;
+                            const float x = odds[wave][d];
+                            acc[c][e] += see && x != 0.f ? w * x : 0.f;
                         }
                 }
         }
@@ -834,29 +865,38 @@ __global__ void __launch_bounds__(NW * 64, 2) k_kvattn_many(KvAttnArgs A) {
 }
 
 // ----------------------------------------------------------------------------
-// The shares of nsplit workgroups: one thread for four elements of a row.
+// The shares of nsplit workgroups of a row and head: a lane a share for the factors, 256 / (HD / 4) groups of threads for the sums.
 // ----------------------------------------------------------------------------
+#define KV_MAX_SPLIT 64
 template <typename IT, int HD>
 __global__ void __launch_bounds__(256) k_kvattn_join(KvAttnArgs A) {
-    const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x, n = (size_t)A.rows * A.heads;
-    const size_t rh = i / (HD / 4);
-    const int d = (int)(i % (HD / 4)) * 4;
-    if (rh >= n) return;
-    const int row = (int)(rh / A.heads), h = (int)(rh % A.heads);
+    constexpr int T = HD / 4, G = 256 / T;
+    __shared__ f32x4 sum[G][T];
+    const size_t rh = blockIdx.x, n = (size_t)A.rows * A.heads;
+    const int row = (int)(rh / A.heads), h = (int)(rh % A.heads), lane = threadIdx.x & 63, t = threadIdx.x % T, g = threadIdx.x / T;
     if (row < A.start[0] || row >= A.start[A.nseq]) return;
     const float2* stat = reinterpret_cast<const float2*>(A.part + (size_t)A.nsplit * n * HD);
-    float M = -INFINITY, den = 0.f;
-    for (int s = 0; s < A.nsplit; s++) M = fmaxf(M, stat[s * n + rh].x);
-    const float ref = M == -INFINITY ? 0.f : M;
+    const float2 ml = lane < A.nsplit ? stat[lane * n + rh] : make_float2(-INFINITY, 0.f);
+    float M = ml.x;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
+    const float f = kv_exp2(ml.x - (M == -INFINITY ? 0.f : M));
+    float den = ml.y * f;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) den += __shfl_xor(den, o, 64);
     f32x4 o = (f32x4)(0.f);
-    for (int s = 0; s < A.nsplit; s++) {
-        const float2 ml = stat[s * n + rh];
-        const float f = kv_exp2(ml.x - ref);
-        den = fmaf(ml.y, f, den);
-        o += *reinterpret_cast<const f32x4*>(A.part + (s * n + rh) * HD + d) * f;
+    for (int s0 = 0; s0 < A.nsplit; s0 += G) { // (every lane of a wave takes the exchange)
+        const int s = s0 + g;
+        const float w = __shfl(f, min(s, KV_MAX_SPLIT - 1), 64);
+        if (s < A.nsplit) o += *reinterpret_cast<const f32x4*>(A.part + (s * n + rh) * HD + 4 * t) * w;
     }
+    sum[g][t] = o;
+    __syncthreads();
+    if (g > 0) return;
+#pragma unroll
+    for (int i = 1; i < G; i++) o += sum[i][t];
     o = den == 0.f ? (f32x4)(0.f) : f32x4{o.x / den, o.y / den, o.z / den, o.w / den};
-    kv_put4((IT*)A.out + (size_t)row * A.outStride + (size_t)h * HD + d, o);
+    kv_put4((IT*)A.out + (size_t)row * A.outStride + (size_t)h * HD + 4 * t, o);
 }
 
 // ----------------------------------------------------------------------------
@@ -872,11 +912,13 @@ static std::string attn_check(const mlh_kv_cache* c, const mlh_kv_batch* b, cons
     if (!bad.empty()) return bad;
     if (a->q == a->out) return "out must not be q";
     if (a->window < 0 || a->sinks < 0 || a->maxLen < 0 || a->maxNew < 0) return "window, sinks, maxLen and maxNew must not be negative";
-    if (!(a->scale >= 0.f) || !(a->scale <= 3.0e38f)) return "scale must be finite and not negative";
+    if (a->scale != 0.f && (!(a->scale >= 1.0e-30f) || !(a->scale <= 1.0e30f))) return "scale must be 0 or 1e-30 to 1e30";
     return "";
 }
 
-#define KV_SPLIT_WGS 512 // keys are split until a call has this many workgroups: two a compute unit
+#ifndef KV_SPLIT_WGS
+#define KV_SPLIT_WGS 2048 // keys are split until a call has this many workgroups: eight a compute unit
+#endif
 struct AttnPlan { // which kernel, and how the keys are split
     int many;         // waves of a workgroup of k_kvattn_many; 0: the kernels of 16 rows
     int blocks, nsplit;
@@ -896,7 +938,7 @@ static AttnPlan attn_plan(const mlh_kv_cache* c, const mlh_kv_batch* b, const ml
     const long long rounds = (seen + 8 * 32 - 1) / (8 * 32); // turns of a workgroup's eight waves
     const long long wgs = (long long)std::min(P.blocks, (b->rows * group + 15) / 16 + std::min(c->nseq, b->rows)) * c->heads;
     const long long n = P.many ? 1 : std::min<long long>((KV_SPLIT_WGS + wgs - 1) / wgs, (rounds + 1) / 2); // two workgroups a compute unit, two turns or more a workgroup
-    P.nsplit = (int)std::max<long long>(1, std::min<long long>(n, 64));
+    P.nsplit = (int)std::max<long long>(1, std::min<long long>(n, KV_MAX_SPLIT));
     P.bytes = P.nsplit > 1 ? (size_t)P.nsplit * b->rows * b->heads * (c->headDim + 2) * 4 : 0;
     return P;
 }
@@ -905,7 +947,7 @@ static AttnPlan attn_plan(const mlh_kv_cache* c, const mlh_kv_batch* b, const ml
 size_t mlh_attention_work_most(int headDim) { return (size_t)2 * KV_SPLIT_WGS * 16 * (headDim + 2) * 4; }
 
 template <typename IT, typename CT, int HD, int NW> static hipError_t launch_many(dim3 grid, hipStream_t st, const KvAttnArgs& A) {
-    constexpr int bytes = 4 * 64 * HD * 2 + 16;
+    constexpr int bytes = 4 * 64 * HD * 2 + 16 + NW * HD * 4;
     if (bytes > 65536) { // (asked for on every call: the attribute belongs to the device that is current)
         const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&k_kvattn_many<IT, CT, HD, NW>), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
         if (e != hipSuccess) return e;
@@ -940,25 +982,25 @@ extern "C" int mlh_attention_device(const mlh_kv_cache* c, const mlh_kv_batch* b
         if (e != hipSuccess) { mlh_set_thread_error(std::string("launch failed: ") + hipGetErrorString(e)); return -2; }
         return kv_launched();
     }
-#define GO(K_, ...) \
+#define GO(K_, NW_, ...) \
     do { \
-        if (hd == 64) hipLaunchKernelGGL((K_<__VA_ARGS__, 64>), grid, dim3(512), 0, st, A); \
-        else hipLaunchKernelGGL((K_<__VA_ARGS__, 128>), grid, dim3(512), 0, st, A); \
+        if (hd == 64) hipLaunchKernelGGL((K_<__VA_ARGS__, 64>), grid, dim3((NW_) * 64), 0, st, A); \
+        else hipLaunchKernelGGL((K_<__VA_ARGS__, 128>), grid, dim3((NW_) * 64), 0, st, A); \
     } while (0)
     if (b->type == MLH_DTYPE_F32) {
-        if (c->type == MLH_CACHE_Q4) GO(k_kvattn_f32, q4_t);
-        else GO(k_kvattn_f32, float);
+        if (c->type == MLH_CACHE_Q4) GO(k_kvattn_f32, KV_W32, q4_t);
+        else GO(k_kvattn_f32, KV_W32, float);
     } else if (b->type == MLH_DTYPE_BF16) {
-        if (c->type == MLH_CACHE_Q4) GO(k_kvattn_few, bf16_t, q4_t);
-        else GO(k_kvattn_few, bf16_t, bf16_t);
+        if (c->type == MLH_CACHE_Q4) GO(k_kvattn_few, kv_few_waves<q4_t>(), bf16_t, q4_t);
+        else GO(k_kvattn_few, kv_few_waves<bf16_t>(), bf16_t, bf16_t);
     } else {
-        if (c->type == MLH_CACHE_Q4) GO(k_kvattn_few, f16_t, q4_t);
-        else GO(k_kvattn_few, f16_t, f16_t);
+        if (c->type == MLH_CACHE_Q4) GO(k_kvattn_few, kv_few_waves<q4_t>(), f16_t, q4_t);
+        else GO(k_kvattn_few, kv_few_waves<f16_t>(), f16_t, f16_t);
     }
 #undef GO
     if (const int rc = kv_launched()) return rc;
     if (P.nsplit == 1) return 0;
-    const unsigned jg = (unsigned)(((size_t)b->rows * b->heads * (hd / 4) + 255) / 256);
+    const unsigned jg = (unsigned)(b->rows * b->heads); // (keys are split for few rows only)
 #define JOIN(IT_) \
     do { \
         if (hd == 64) hipLaunchKernelGGL((k_kvattn_join<IT_, 64>), dim3(jg), dim3(256), 0, st, A); \

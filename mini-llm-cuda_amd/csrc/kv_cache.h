@@ -40,38 +40,50 @@ __device__ __forceinline__ void kv_load8(const f16_t* p, float (&x)[8]) {
 #pragma unroll
     for (int i = 0; i < 4; i++) { x[2 * i] = kv_half(a[i] & 0xffffu); x[2 * i + 1] = kv_half(a[i] >> 16); }
 }
-__device__ __forceinline__ void kv_store8(float* p, const float (&x)[8]) {
-    *reinterpret_cast<kv_f32x4*>(p) = kv_f32x4{x[0], x[1], x[2], x[3]};
-    *reinterpret_cast<kv_f32x4*>(p + 4) = kv_f32x4{x[4], x[5], x[6], x[7]};
+template <bool NT, typename T> __device__ __forceinline__ void kv_store16(void* p, const T& v) { // NT: not to be kept in the caches
+    if constexpr (NT) __builtin_nontemporal_store(v, reinterpret_cast<T*>(p));
+    else *reinterpret_cast<T*>(p) = v;
 }
-__device__ __forceinline__ void kv_store8(bf16_t* p, const float (&x)[8]) {
+template <bool NT> __device__ __forceinline__ void kv_store8(float* p, const float (&x)[8]) {
+    kv_store16<NT>(p, kv_f32x4{x[0], x[1], x[2], x[3]});
+    kv_store16<NT>(p + 4, kv_f32x4{x[4], x[5], x[6], x[7]});
+}
+template <bool NT> __device__ __forceinline__ void kv_store8(bf16_t* p, const float (&x)[8]) {
     kv_u32x4 a;
 #pragma unroll
     for (int i = 0; i < 4; i++) a[i] = kv_to_bf16(x[2 * i]) | kv_to_bf16(x[2 * i + 1]) << 16;
-    *reinterpret_cast<kv_u32x4*>(p) = a;
+    kv_store16<NT>(p, a);
 }
-__device__ __forceinline__ void kv_store8(f16_t* p, const float (&x)[8]) {
+template <bool NT> __device__ __forceinline__ void kv_store8(f16_t* p, const float (&x)[8]) {
     kv_u32x4 a;
 #pragma unroll
     for (int i = 0; i < 4; i++) a[i] = kv_to_half(x[2 * i]) | kv_to_half(x[2 * i + 1]) << 16;
-    *reinterpret_cast<kv_u32x4*>(p) = a;
+    kv_store16<NT>(p, a);
 }
 
-// Largest s in [0, nseq) with key(s) <= b, for keys that do not decrease (0 if there is none).
+// Largest s in [0, nseq) with key(s) <= b, for keys that do not decrease (0 if there is none).  All lanes of a wave together, for one b: 64 places a load, since what a
+// search costs is a memory latency a step.
 template <typename F> __device__ __forceinline__ int kv_find(int nseq, int b, F key) {
+    const int lane = threadIdx.x & 63;
     int lo = 0, n = nseq;
     while (n > 1) {
-        const int h = n >> 1;
-        if (key(lo + h) <= b) { lo += h; n -= h; }
-        else n = h;
+        const int step = (n + 63) >> 6, i = lane * step;
+        const int below = __builtin_popcountll(__ballot(i < n && key(lo + min(i, n - 1)) <= b));
+        const int skip = max(below - 1, 0) * step;
+        lo += skip;
+        n = min(step, n - skip);
     }
     return lo;
 }
 
+// A word at an index that all lanes share, of memory that no kernel of the call writes: through the scalar cache.  (As a vector load, which the compiler takes where it
+// sees stores around, it waits for every load on its way before it.)
+__device__ __forceinline__ int kv_uniform(const int32_t* p, size_t i) { return *(const __attribute__((address_space(4))) int32_t*)(uintptr_t)(p + i); }
+
 // Pool page of page j of sequence s; -1: beyond the table, or not in the pool.
 __device__ __forceinline__ int kv_page(const int32_t* table, int pagesPerSeq, int numPages, int s, int j) {
     if (j < 0 || j >= pagesPerSeq) return -1;
-    const int p = table[(size_t)s * pagesPerSeq + j];
+    const int p = kv_uniform(table, (size_t)s * pagesPerSeq + j);
     return (unsigned)p < (unsigned)numPages ? p : -1;
 }
 
