@@ -30,13 +30,6 @@ struct KvAttnArgs {
     float scale2; // scale * log2 e
 };
 
-#ifdef KV_MAP2
-#define KV_KH (blockIdx.x / (gridDim.x / A.kvHeads))
-#define KV_BLK (blockIdx.x % (gridDim.x / A.kvHeads))
-#else
-#define KV_KH (blockIdx.x % A.kvHeads)
-#define KV_BLK (blockIdx.x / A.kvHeads)
-#endif
 #define KV_NAN __uint_as_float(0x7fc00000u)
 
 // The rows of a workgroup: nr of them from row r0 of sequence s.
@@ -80,7 +73,7 @@ template <int TK> struct KvTiles {
 struct KvSight {
     int pos, below, sinks;
     __device__ __forceinline__ KvSight(const KvAttnArgs& A, int p) : pos(p), below(A.window ? max(p, -1) - A.window : -1), sinks(A.sinks) {}
-    __device__ __forceinline__ bool sees(int j) const { return j <= pos && (j > below || j < sinks); }
+    __device__ __forceinline__ bool sees(int j) const { return (j <= pos) & ((j > below) | (j < sinks)); } // (without branches)
 };
 // do all rows of [minPos, maxPos] see all of a tile's n positions from j0?
 __device__ __forceinline__ bool kv_all_see(const KvAttnArgs& A, int minPos, int maxPos, int j0, int n) {
@@ -89,9 +82,15 @@ __device__ __forceinline__ bool kv_all_see(const KvAttnArgs& A, int minPos, int 
 
 __device__ __forceinline__ bool kv_finite(float v) { return (__float_as_uint(v) & 0x7f800000u) != 0x7f800000u; }
 __device__ __forceinline__ float kv_exp2(float v) { return __builtin_amdgcn_exp2f(v); }
+// The larger of two (as a median: fmaxf would first quiet both, an instruction each; where one is no number, either, and the row's sum is none then)
+__device__ __forceinline__ float kv_max(float a, float b) { return __builtin_amdgcn_fmed3f(a, b, INFINITY); }
+__device__ __forceinline__ float kv_halves_max(float v) { // of a lane and the one 32 further
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return kv_max(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
 __device__ __forceinline__ float kv_quad_max(float v) { // over the four lanes that hold a column of a 16 x 16 product
-    v = fmaxf(v, __shfl_xor(v, 16, 64));
-    return fmaxf(v, __shfl_xor(v, 32, 64));
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return kv_halves_max(kv_max(__uint_as_float(r[0]), __uint_as_float(r[1])));
 }
 __device__ __forceinline__ float kv_quad_sum(float v) {
     v += __shfl_xor(v, 16, 64);
@@ -243,15 +242,14 @@ template <int HD> struct KvTile32<q4_t, HD> {
     }
 };
 
-#define KV_W32 8 // waves of a workgroup
-template <typename CT, int HD>
-__global__ void __launch_bounds__(KV_W32 * 64) k_kvattn_f32(KvAttnArgs A) {
-    constexpr int NW = KV_W32, KC = HD / 4, VB = HD / 16;
+template <typename CT, int HD, int NW>
+__global__ void __launch_bounds__(NW * 64, 2) k_kvattn_f32(KvAttnArgs A) {
+    constexpr int KC = HD / 4, VB = HD / 16;
     __shared__ __attribute__((aligned(16))) float lds[NW * 16 * (HD + 4 + 2)];
     __shared__ float odds[NW][HD];
-    const int kh = KV_KH, split = blockIdx.y, tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, n = lane & 15, g = lane >> 4;
+    const int kh = blockIdx.x % A.kvHeads, split = blockIdx.y, tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, n = lane & 15, g = lane >> 4;
     KvBlock B;
-    if (!kv_block<16>(A, KV_BLK, B)) return;
+    if (!kv_block<16>(A, blockIdx.x / A.kvHeads, B)) return;
     const int r = B.r0 + min(n, B.nr - 1), h = kh * A.group + r % A.group;
     const KvSight sight(A, B.pos0 + r / A.group);
     f32x4 q[KC / 4];
@@ -292,7 +290,7 @@ __global__ void __launch_bounds__(KV_W32 * 64) k_kvattn_f32(KvAttnArgs A) {
             see[e] = whole || sight.sees(key + e);
             p[e] = (s0[e] + s1[e]) * A.scale2;
             if (!whole) p[e] = !see[e] ? -INFINITY : page[set] < 0 ? KV_NAN : p[e];
-            mt = fmaxf(mt, p[e]);
+            mt = kv_max(mt, p[e]);
         }
         mt = kv_quad_max(mt);
         const float ref = mt == -INFINITY ? 0.f : mt, corr = kv_exp2(m - ref);
@@ -461,25 +459,18 @@ template <typename IT, int HD> struct KvRaw16<IT, q4_t, HD> { // the same, eleme
     __device__ __forceinline__ u32x4 val(int b, int t) const { return kv_halves(v[b][t], vp[b]); }
 };
 
-#ifndef KV_NWQ
-#define KV_NWQ 4
-#define KV_OCQ 3
-#endif
-#ifndef KV_NWB
-#define KV_NWB 8
-#endif
-template <typename CT> constexpr int kv_few_waves() { return KvType<CT>::code == MLH_CACHE_Q4 ? KV_NWQ : KV_NWB; }
+template <typename CT> constexpr int kv_few_waves() { return KvType<CT>::code == MLH_CACHE_Q4 ? 4 : 8; }
 template <typename IT, typename CT, int HD>
-__global__ void __launch_bounds__(kv_few_waves<CT>() * 64, KvType<CT>::code == MLH_CACHE_Q4 ? KV_OCQ : 2) k_kvattn_few(KvAttnArgs A) {
+__global__ void __launch_bounds__(kv_few_waves<CT>() * 64, KvType<CT>::code == MLH_CACHE_Q4 ? 3 : 2) k_kvattn_few(KvAttnArgs A) {
     constexpr bool FOUR = KvType<CT>::code == MLH_CACHE_Q4, BF = !FOUR && KvType<IT>::code == MLH_DTYPE_BF16; // products in bf16
     constexpr int NW = kv_few_waves<CT>(), KS = HD / 32, VB = HD / 16;
     constexpr int VP = HD * 2 + 16; // bytes of a row of V in LDS: four rows start in different banks
     constexpr int LV = NW * 32 * VP, LF = NW * 16 * (HD + 4 + 2) * 4;
     __shared__ __attribute__((aligned(16))) unsigned char lds[LV > LF ? LV : LF];
     __shared__ float odds[NW][HD];
-    const int kh = KV_KH, split = blockIdx.y, tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, n = lane & 15, g = lane >> 4;
+    const int kh = blockIdx.x % A.kvHeads, split = blockIdx.y, tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, n = lane & 15, g = lane >> 4;
     KvBlock B;
-    if (!kv_block<16>(A, KV_BLK, B)) return;
+    if (!kv_block<16>(A, blockIdx.x / A.kvHeads, B)) return;
     const int r = B.r0 + min(n, B.nr - 1), h = kh * A.group + r % A.group;
     const KvSight sight(A, B.pos0 + r / A.group);
     u32x4 q[KS];
@@ -553,7 +544,7 @@ __global__ void __launch_bounds__(kv_few_waves<CT>() * 64, KvType<CT>::code == M
                 see[b][e] = whole || sight.sees(j0 + 16 * b + 4 * g + e);
                 p[b][e] = s[b][e] * scale;
                 if (!whole) p[b][e] = !see[b][e] ? -INFINITY : page[set] < 0 ? KV_NAN : p[b][e];
-                mt = fmaxf(mt, p[b][e]);
+                mt = kv_max(mt, p[b][e]);
             }
         mt = kv_quad_max(mt);
         const float ref = mt == -INFINITY ? 0.f : mt, corr = kv_exp2(m - ref);
@@ -639,6 +630,10 @@ __global__ void __launch_bounds__(kv_few_waves<CT>() * 64, KvType<CT>::code == M
 // (the 16-byte pieces of a row in an order that keeps both readings free of bank conflicts), those of 4 bits through registers, where codes become halves.
 // ----------------------------------------------------------------------------
 typedef float f32x16 __attribute__((ext_vector_type(16)));
+template <bool BF> __device__ __forceinline__ float kv_add2(uint32_t w, float sum) { // two 16-bit numbers onto a sum
+    if constexpr (BF) { typedef __bf16 bf16x2 __attribute__((ext_vector_type(2))); return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, w), bf16x2{(__bf16)1.f, (__bf16)1.f}, sum, false); }
+    else return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, w), f16x2{(_Float16)1.f, (_Float16)1.f}, sum, false);
+}
 template <bool BF> __device__ __forceinline__ f32x16 mfma32(const u32x4& a, const u32x4& b, const f32x16& c) {
     if constexpr (BF) return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
     else return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
@@ -698,6 +693,7 @@ __global__ void __launch_bounds__(NW * 64, 2) k_kvattn_many(KvAttnArgs A) {
         for (int i = 0; i < 16; i++) acc[b][i] = 0.f;
     float m = -INFINITY, l = 0.f; // (of the scores times scale)
     const KvTiles<64> tiles(A, B);
+    const int split = blockIdx.y, t0 = (int)((long long)tiles.n * split / A.nsplit), t1 = (int)((long long)tiles.n * (split + 1) / A.nsplit); // this workgroup's
 
     // ---- a tile into LDS ----
     constexpr int EPT = HD / NW; // 4-bit pages: elements a thread takes of K and of V
@@ -779,9 +775,8 @@ __global__ void __launch_bounds__(NW * 64, 2) k_kvattn_many(KvAttnArgs A) {
 #pragma unroll
         for (int b = 0; b < 2; b++)
 #pragma unroll
-            for (int e = 0; e < 16; e += 2) mx = fmaxf(mx, fmaxf(s[b][e], s[b][e + 1]));
-        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-        const float mn = fmaxf(m, mx * scale);
+            for (int e = 0; e < 16; e++) mx = kv_max(mx, s[b][e]);
+        const float mn = fmaxf(m, kv_halves_max(mx) * scale);
         if (__any(mn > m)) {
             const float corr = m == -INFINITY ? 0.f : kv_exp2(m - mn);
             l *= corr;
@@ -797,7 +792,6 @@ __global__ void __launch_bounds__(NW * 64, 2) k_kvattn_many(KvAttnArgs A) {
 #pragma unroll
             for (int e = 0; e < 16; e++) { // (hidden: 2^-inf)
                 s[b][e] = kv_exp2(fmaf(s[b][e], scale, ref));
-                l += s[b][e];
             }
         if (odd[0] | odd[1]) {
 #pragma unroll
@@ -825,6 +819,8 @@ __global__ void __launch_bounds__(NW * 64, 2) k_kvattn_many(KvAttnArgs A) {
         for (int t = 0; t < 4; t++) {
             const int b = t >> 1, e0 = 8 * (t & 1);
             const u32x4 pw = {kv_pack<BF>(s[b][e0], s[b][e0 + 1]), kv_pack<BF>(s[b][e0 + 2], s[b][e0 + 3]), kv_pack<BF>(s[b][e0 + 4], s[b][e0 + 5]), kv_pack<BF>(s[b][e0 + 6], s[b][e0 + 7])};
+#pragma unroll
+            for (int i = 0; i < 4; i++) l = kv_add2<BF>(pw[i], l); // (the weights as the product has them)
             const int row = 16 * t + 4 * half + ((lane & 15) >> 2), piece = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1), rest = 8 * (lane & 1);
 #pragma unroll
             for (int c = 0; c < MB; c++) {
@@ -834,33 +830,38 @@ __global__ void __launch_bounds__(NW * 64, 2) k_kvattn_many(KvAttnArgs A) {
         }
     };
 
-    if (tiles.n > 0) fetch(0, 0);
-    for (int i = 0; i < tiles.n; i++) {
-        const int buf = i & 1;
+    if (t0 < t1) fetch(t0, 0);
+    for (int i = t0; i < t1; i++) {
+        const int buf = (i - t0) & 1;
         deposit(buf);
         if (tid < 2) flags[2 * buf + tid] = 0; // (read last two tiles ago)
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); // tile i has landed ...
         __syncthreads();                                  // ... for every wave, and every wave is done with tile i - 1
-        if (i + 1 < tiles.n) fetch(i + 1, buf ^ 1);
+        if (i + 1 < t1) fetch(i + 1, buf ^ 1);
         __builtin_amdgcn_sched_barrier(0);
         tile(i, buf);
     }
     if (!active || wave * 32 + n >= B.nr) return;
     l += __shfl_xor(l, 32, 64);
     const int qi = r / A.group;
-    const float inv = B.pos0 + qi >= B.cap ? KV_NAN : l == 0.f ? 0.f : 1.0f / l;
+    const bool beyond = B.pos0 + qi >= B.cap; // (its own position is behind the page table)
+    const float inv = A.nsplit > 1 ? 1.f : beyond ? KV_NAN : l == 0.f ? 0.f : 1.0f / l;
     IT* out = (IT*)A.out + (size_t)(B.row0 + qi) * A.outStride + (size_t)h * HD;
+    const size_t shares = (size_t)A.rows * A.heads, rh = split * shares + (size_t)(B.row0 + qi) * A.heads + h;
+    float* part = A.part + rh * HD;
+    if (A.nsplit > 1 && half == 0) *reinterpret_cast<float2*>(A.part + A.nsplit * shares * HD + rh * 2) = beyond ? make_float2(0.f, KV_NAN) : make_float2(m, l);
 #pragma unroll
     for (int c = 0; c < MB; c++)
 #pragma unroll
         for (int e = 0; e < 4; e++) {
             f32x4 o = f32x4{acc[c][4 * e], acc[c][4 * e + 1], acc[c][4 * e + 2], acc[c][4 * e + 3]} * inv;
-            if (l == 0.f && inv == 0.f) o = (f32x4)(0.f);
+            if (inv == 0.f) o = (f32x4)(0.f);
             if (FOUR) { // columns (0, 4, 1, 5) here, (2, 6, 3, 7) in the other half: four neighbours each
                 const float a = __shfl_xor(half ? o.x : o.y, 32, 64), b = __shfl_xor(half ? o.z : o.w, 32, 64);
                 o = half ? f32x4{a, b, o.y, o.w} : f32x4{o.x, o.z, a, b};
             }
-            kv_put4(out + 32 * c + 8 * e + 4 * half, o);
+            if (A.nsplit > 1) *reinterpret_cast<f32x4*>(part + 32 * c + 8 * e + 4 * half) = o;
+            else kv_put4(out + 32 * c + 8 * e + 4 * half, o);
         }
 }
 
@@ -899,6 +900,38 @@ __global__ void __launch_bounds__(256) k_kvattn_join(KvAttnArgs A) {
     kv_put4((IT*)A.out + (size_t)row * A.outStride + (size_t)h * HD + 4 * t, o);
 }
 
+// The same of few shares (KV_JOIN_FEW at most): a thread for four elements.
+#define KV_JOIN_FEW 8
+template <typename IT, int HD>
+__global__ void __launch_bounds__(256) k_kvattn_join_few(KvAttnArgs A) {
+    constexpr int T = HD / 4;
+    const size_t rh = (size_t)blockIdx.x * (256 / T) + threadIdx.x / T, n = (size_t)A.rows * A.heads;
+    if (rh >= n) return;
+    const int row = (int)(rh / A.heads), h = (int)(rh % A.heads), d = threadIdx.x % T * 4;
+    if (row < A.start[0] || row >= A.start[A.nseq]) return;
+    const float2* stat = reinterpret_cast<const float2*>(A.part + (size_t)A.nsplit * n * HD);
+    float2 ml[KV_JOIN_FEW];
+    f32x4 v[KV_JOIN_FEW], o = (f32x4)(0.f);
+    float M = -INFINITY, den = 0.f;
+#pragma unroll
+    for (int s = 0; s < KV_JOIN_FEW; s++) {
+        const size_t i = (size_t)min(s, A.nsplit - 1) * n + rh;
+        ml[s] = stat[i];
+        v[s] = *reinterpret_cast<const f32x4*>(A.part + i * HD + d);
+        M = fmaxf(M, ml[s].x);
+    }
+    const float ref = M == -INFINITY ? 0.f : M;
+#pragma unroll
+    for (int s = 0; s < KV_JOIN_FEW; s++) {
+        if (s >= A.nsplit) continue;
+        const float f = kv_exp2(ml[s].x - ref);
+        den = fmaf(ml[s].y, f, den);
+        o += v[s] * f;
+    }
+    o = den == 0.f ? (f32x4)(0.f) : f32x4{o.x / den, o.y / den, o.z / den, o.w / den};
+    kv_put4((IT*)A.out + (size_t)row * A.outStride + (size_t)h * HD + d, o);
+}
+
 // ----------------------------------------------------------------------------
 // host side
 // ----------------------------------------------------------------------------
@@ -916,28 +949,34 @@ static std::string attn_check(const mlh_kv_cache* c, const mlh_kv_batch* b, cons
     return "";
 }
 
-#ifndef KV_SPLIT_WGS
-#define KV_SPLIT_WGS 2048 // keys are split until a call has this many workgroups: eight a compute unit
+#define KV_SPLIT_WGS 2048 // the kernels of 16 rows: keys are split until a call has this many workgroups, eight a compute unit
+#ifndef KV_SPLIT_MANY
+#define KV_SPLIT_MANY 1024 // k_kvattn_many: four
 #endif
-struct AttnPlan { // which kernel, and how the keys are split
-    int many;         // waves of a workgroup of k_kvattn_many; 0: the kernels of 16 rows
+#ifndef KV_WIDE_WGS
+#define KV_WIDE_WGS 256
+#endif
+struct AttnPlan {         // which kernel, and how the keys are split
+    int many;             // waves of a workgroup of k_kvattn_many; 0: the kernels of 16 rows
     int blocks, nsplit;
+    long long wgs;        // workgroups with rows, per split
     size_t bytes;
 };
 static AttnPlan attn_plan(const mlh_kv_cache* c, const mlh_kv_batch* b, const mlh_attention* a) {
     AttnPlan P;
     const int group = b->heads / c->heads;
-    const long long cap = (long long)c->pagesPerSeq * MLH_KV_PAGE;
+    const long long cap = (long long)c->pagesPerSeq * MLH_KV_PAGE, rows = (long long)b->rows * group;
     const long long maxLen = a->maxLen ? std::min<long long>(a->maxLen, cap) : cap;
     const long long maxNew = a->maxNew ? std::min(a->maxNew, b->rows) : b->rows;
     P.many = b->type != MLH_DTYPE_F32 && maxNew * group > 64 ? 4 : 0;
     const int qb = P.many ? P.many * 32 : 16;
-    P.blocks = (int)((long long)b->rows * group / qb + c->nseq);
-    // key tiles of the longest row: the window's and the first positions', in pieces of 32 keys a wave
+    P.blocks = (int)(rows / qb + c->nseq);
+    P.wgs = std::min<long long>(P.blocks, (rows + qb - 1) / qb + std::min(c->nseq, b->rows) - 1) * c->heads;
+    // positions that a row sees, in turns of a workgroup (eight waves of 32 keys, or a page)
     const long long seen = a->window ? std::min<long long>(maxLen, (long long)a->window + std::min<long long>(a->sinks, maxLen) + 64) : maxLen;
-    const long long rounds = (seen + 8 * 32 - 1) / (8 * 32); // turns of a workgroup's eight waves
-    const long long wgs = (long long)std::min(P.blocks, (b->rows * group + 15) / 16 + std::min(c->nseq, b->rows)) * c->heads;
-    const long long n = P.many ? 1 : std::min<long long>((KV_SPLIT_WGS + wgs - 1) / wgs, (rounds + 1) / 2); // two workgroups a compute unit, two turns or more a workgroup
+    const int turn = P.many ? 64 : 256;
+    const long long rounds = (seen + turn - 1) / turn;
+    const long long n = P.many ? std::min<long long>((KV_SPLIT_MANY + P.wgs - 1) / P.wgs, rounds / 8) : std::min<long long>((KV_SPLIT_WGS + P.wgs - 1) / P.wgs, (rounds + 1) / 2);
     P.nsplit = (int)std::max<long long>(1, std::min<long long>(n, KV_MAX_SPLIT));
     P.bytes = P.nsplit > 1 ? (size_t)P.nsplit * b->rows * b->heads * (c->headDim + 2) * 4 : 0;
     return P;
@@ -954,6 +993,21 @@ template <typename IT, typename CT, int HD, int NW> static hipError_t launch_man
     }
     hipLaunchKernelGGL((k_kvattn_many<IT, CT, HD, NW>), grid, dim3(NW * 64), bytes, st, A);
     return hipSuccess;
+}
+
+template <typename IT, int HD> static void launch_join(hipStream_t st, const KvAttnArgs& A) {
+    const unsigned n = (unsigned)(A.rows * A.heads), per = 256 / (HD / 4);
+    if (A.nsplit <= KV_JOIN_FEW) hipLaunchKernelGGL((k_kvattn_join_few<IT, HD>), dim3((n + per - 1) / per), dim3(256), 0, st, A);
+    else hipLaunchKernelGGL((k_kvattn_join<IT, HD>), dim3(n), dim3(256), 0, st, A);
+}
+static int launch_join(hipStream_t st, int type, int hd, const KvAttnArgs& A) {
+    if (A.nsplit == 1) return 0;
+#define JOIN(IT_) do { if (hd == 64) launch_join<IT_, 64>(st, A); else launch_join<IT_, 128>(st, A); } while (0)
+    if (type == MLH_DTYPE_F32) JOIN(float);
+    else if (type == MLH_DTYPE_BF16) JOIN(bf16_t);
+    else JOIN(f16_t);
+#undef JOIN
+    return kv_launched();
 }
 
 extern "C" uint64_t mlh_attention_work_bytes(const mlh_kv_cache* c, const mlh_kv_batch* b, const mlh_attention* a) {
@@ -980,35 +1034,26 @@ extern "C" int mlh_attention_device(const mlh_kv_cache* c, const mlh_kv_batch* b
         else e = c->type == MLH_CACHE_Q4 ? MANY(f16_t, q4_t) : MANY(f16_t, f16_t);
 #undef MANY
         if (e != hipSuccess) { mlh_set_thread_error(std::string("launch failed: ") + hipGetErrorString(e)); return -2; }
-        return kv_launched();
-    }
-#define GO(K_, NW_, ...) \
+    } else if (b->type == MLH_DTYPE_F32) {
+#define F32_ROWS(CT_, NW_) \
     do { \
-        if (hd == 64) hipLaunchKernelGGL((K_<__VA_ARGS__, 64>), grid, dim3((NW_) * 64), 0, st, A); \
-        else hipLaunchKernelGGL((K_<__VA_ARGS__, 128>), grid, dim3((NW_) * 64), 0, st, A); \
+        if (hd == 64) hipLaunchKernelGGL((k_kvattn_f32<CT_, 64, NW_>), grid, dim3(NW_ * 64), 0, st, A); \
+        else hipLaunchKernelGGL((k_kvattn_f32<CT_, 128, NW_>), grid, dim3(NW_ * 64), 0, st, A); \
     } while (0)
-    if (b->type == MLH_DTYPE_F32) {
-        if (c->type == MLH_CACHE_Q4) GO(k_kvattn_f32, KV_W32, q4_t);
-        else GO(k_kvattn_f32, KV_W32, float);
-    } else if (b->type == MLH_DTYPE_BF16) {
-        if (c->type == MLH_CACHE_Q4) GO(k_kvattn_few, kv_few_waves<q4_t>(), bf16_t, q4_t);
-        else GO(k_kvattn_few, kv_few_waves<bf16_t>(), bf16_t, bf16_t);
+        const bool wide = P.wgs * P.nsplit <= KV_WIDE_WGS; // eight waves a workgroup while that leaves a compute unit one of them
+        if (c->type == MLH_CACHE_Q4) { if (wide) F32_ROWS(q4_t, 8); else F32_ROWS(q4_t, 4); }
+        else { if (wide) F32_ROWS(float, 8); else F32_ROWS(float, 4); }
+#undef F32_ROWS
     } else {
-        if (c->type == MLH_CACHE_Q4) GO(k_kvattn_few, kv_few_waves<q4_t>(), f16_t, q4_t);
-        else GO(k_kvattn_few, kv_few_waves<f16_t>(), f16_t, f16_t);
-    }
-#undef GO
-    if (const int rc = kv_launched()) return rc;
-    if (P.nsplit == 1) return 0;
-    const unsigned jg = (unsigned)(b->rows * b->heads); // (keys are split for few rows only)
-#define JOIN(IT_) \
+#define FEW(IT_, CT_) \
     do { \
-        if (hd == 64) hipLaunchKernelGGL((k_kvattn_join<IT_, 64>), dim3(jg), dim3(256), 0, st, A); \
-        else hipLaunchKernelGGL((k_kvattn_join<IT_, 128>), dim3(jg), dim3(256), 0, st, A); \
+        if (hd == 64) hipLaunchKernelGGL((k_kvattn_few<IT_, CT_, 64>), grid, dim3(kv_few_waves<CT_>() * 64), 0, st, A); \
+        else hipLaunchKernelGGL((k_kvattn_few<IT_, CT_, 128>), grid, dim3(kv_few_waves<CT_>() * 64), 0, st, A); \
     } while (0)
-    if (b->type == MLH_DTYPE_F32) JOIN(float);
-    else if (b->type == MLH_DTYPE_BF16) JOIN(bf16_t);
-    else JOIN(f16_t);
-#undef JOIN
-    return kv_launched();
+        if (b->type == MLH_DTYPE_BF16) { if (c->type == MLH_CACHE_Q4) FEW(bf16_t, q4_t); else FEW(bf16_t, bf16_t); }
+        else { if (c->type == MLH_CACHE_Q4) FEW(f16_t, q4_t); else FEW(f16_t, f16_t); }
+#undef FEW
+    }
+    if (const int rc = kv_launched()) return rc;
+    return launch_join(st, b->type, hd, A);
 }
