@@ -72,7 +72,13 @@ template <int TK> struct KvTiles {
 // what a row sees: positions up to `pos`, above `below` or among the first `sinks`
 struct KvSight {
     int pos, below, sinks;
-    __device__ __forceinline__ KvSight(const KvAttnArgs& A, int p) : pos(p), below(A.window ? max(p, -1) - A.window : -1), sinks(A.sinks) {}
+    int low;       // without the first ones: positions low .. low + span
+    unsigned span;
+    __device__ __forceinline__ KvSight(const KvAttnArgs& A, int p) : pos(p), below(A.window ? max(p, -1) - A.window : -1), sinks(A.sinks) {
+        const int l = max(below + 1, 0);
+        low = p < l ? 0x7fffffff : l;
+        span = p < l ? 0u : (unsigned)(p - l);
+    }
     __device__ __forceinline__ bool sees(int j) const { return (j <= pos) & ((j > below) | (j < sinks)); } // (without branches)
 };
 // do all rows of [minPos, maxPos] see all of a tile's n positions from j0?
@@ -265,9 +271,11 @@ __global__ void __launch_bounds__(NW * 64, 2) k_kvattn_f32(KvAttnArgs A) {
     const KvTiles<16> tiles(A, B);
     KvTile32<CT, HD> raw[2];
     int page[2];
+    int next = 0; // page of the tile to be fetched next
+    auto look = [&](int i) { next = kv_page(A.table, A.pagesPerSeq, A.numPages, B.s, tiles.at(min(i, tiles.n - 1)) * 16 >> 6); };
     auto fetch = [&](int i, int set) __attribute__((always_inline)) {
         const int j0 = tiles.at(i) * 16;
-        page[set] = kv_page(A.table, A.pagesPerSeq, A.numPages, B.s, j0 >> 6);
+        page[set] = next;
         raw[set].fetch(A, max(page[set], 0), j0 & 63, min(B.maxPos - j0, 15), kh, n, g);
     };
     auto tile = [&](int i, int set) __attribute__((always_inline)) {
@@ -345,14 +353,20 @@ __global__ void __launch_bounds__(NW * 64, 2) k_kvattn_f32(KvAttnArgs A) {
     };
     const int step = NW * A.nsplit;
     int t = split * NW + wave;
-    if (t < tiles.n) fetch(t, 0);
+    if (t < tiles.n) {
+        look(t);
+        fetch(t, 0);
+        look(t + step);
+    }
     while (t < tiles.n) { // (no further tile: the same loads again, dropped)
         fetch(min(t + step, tiles.n - 1), 1);
+        look(t + 2 * step);
         __builtin_amdgcn_sched_barrier(0); // (the compiler would put the loads behind the products)
         tile(t, 0);
         t += step;
         if (t >= tiles.n) break;
         fetch(min(t + step, tiles.n - 1), 0);
+        look(t + 2 * step);
         __builtin_amdgcn_sched_barrier(0);
         tile(t, 1);
         t += step;
@@ -390,13 +404,18 @@ template <bool BF> __device__ __forceinline__ uint32_t kv_pack(float a, float b)
 __device__ __forceinline__ u32x2 lds_transposed(const void* p) { // 4 rows x 16 columns of 16 bits from 16 lanes' addresses
     return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p));
 }
-template <bool BF> __device__ __forceinline__ bool kv_odd(uint32_t w) { // is one of the two elements no number?
-    constexpr uint32_t E = BF ? 0x7f80u : 0x7c00u;
-    return (w & E) == E || (w >> 16 & E) == E;
+template <bool BF> __device__ __forceinline__ bool kv_odd(const u32x4& a) { // is one of eight elements no number?
+    typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+    u16x2 m = __builtin_bit_cast(u16x2, a.x & 0x7fff7fffu);
+#pragma unroll
+    for (int i = 1; i < 4; i++) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, a[i] & 0x7fff7fffu));
+    return __builtin_elementwise_max(m.x, m.y) >= (BF ? 0x7f80 : 0x7c00);
 }
-template <bool BF> __device__ __forceinline__ uint32_t kv_without_odd(uint32_t w) {
+template <bool BF> __device__ __forceinline__ u32x4 kv_without_odd(u32x4 a) { // zeros instead of those
     constexpr uint32_t E = BF ? 0x7f80u : 0x7c00u;
-    return ((w & E) == E ? 0u : w & 0xffffu) | ((w >> 16 & E) == E ? 0u : w & 0xffff0000u);
+#pragma unroll
+    for (int i = 0; i < 4; i++) a[i] = ((a[i] & E) == E ? 0u : a[i] & 0xffffu) | ((a[i] >> 16 & E) == E ? 0u : a[i] & 0xffff0000u);
+    return a;
 }
 // eight codes -> halves; pairs come out as elements (0, 4), (1, 5), (2, 6), (3, 7)
 __device__ __forceinline__ u32x4 kv_halves(uint32_t codes, uint32_t params) {
@@ -504,9 +523,11 @@ __global__ void __launch_bounds__(kv_few_waves<CT>() * 64, KvType<CT>::code == M
     const KvTiles<32> tiles(A, B);
     KvRaw16<IT, CT, HD> raw[2];
     int page[2];
+    int next = 0; // page of the tile to be fetched next
+    auto look = [&](int i) { next = kv_page(A.table, A.pagesPerSeq, A.numPages, B.s, tiles.at(min(i, tiles.n - 1)) * 32 >> 6); };
     auto fetch = [&](int i, int set) __attribute__((always_inline)) {
         const int j0 = tiles.at(i) * 32;
-        page[set] = kv_page(A.table, A.pagesPerSeq, A.numPages, B.s, j0 >> 6);
+        page[set] = next;
         raw[set].fetch(A, max(page[set], 0), j0 & 63, min(B.maxPos - j0, 31), kh, n, g);
     };
     auto tile = [&](int i, int set) __attribute__((always_inline)) {
@@ -526,12 +547,9 @@ __global__ void __launch_bounds__(kv_few_waves<CT>() * 64, KvType<CT>::code == M
 #pragma unroll
             for (int t = 0; t < KS; t++) {
                 u32x4 x = raw[set].val(b, t);
-                if (!whole) {
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        odd[b] = odd[b] || kv_odd<BF>(x[i]);
-                        x[i] = kv_without_odd<BF>(x[i]);
-                    }
+                if (!whole && kv_odd<BF>(x)) {
+                    odd[b] = true;
+                    x = kv_without_odd<BF>(x);
                 }
                 *reinterpret_cast<u32x4*>(vt + (16 * b + n) * VP + (FOUR ? (HD / 4) * g + 8 * t : 32 * t + 8 * g) * 2) = x;
             }
@@ -597,14 +615,20 @@ __global__ void __launch_bounds__(kv_few_waves<CT>() * 64, KvType<CT>::code == M
     };
     const int step = NW * A.nsplit;
     int t = split * NW + wave;
-    if (t < tiles.n) fetch(t, 0);
+    if (t < tiles.n) {
+        look(t);
+        fetch(t, 0);
+        look(t + step);
+    }
     while (t < tiles.n) { // (no further tile: the same loads again, dropped)
         fetch(min(t + step, tiles.n - 1), 1);
+        look(t + 2 * step);
         __builtin_amdgcn_sched_barrier(0);
         tile(t, 0);
         t += step;
         if (t >= tiles.n) break;
         fetch(min(t + step, tiles.n - 1), 0);
+        look(t + 2 * step);
         __builtin_amdgcn_sched_barrier(0);
         tile(t, 1);
         t += step;
@@ -643,12 +667,12 @@ template <int HD> __device__ __forceinline__ int kv_place_k(int r, int c) { retu
 template <int HD> __device__ __forceinline__ int kv_place_v(int r, int c) { return r * (HD * 2) + 16 * (c ^ (HD == 128 ? 4 * (r & 3) : 4 * ((r >> 1) & 1))); }
 
 template <typename IT, typename CT, int HD, int NW>
-__global__ void __launch_bounds__(NW * 64, 2) k_kvattn_many(KvAttnArgs A) {
+__global__ void __launch_bounds__(NW * 64, HD == 64 ? 3 : 2) k_kvattn_many(KvAttnArgs A) {
     constexpr bool FOUR = KvType<CT>::code == MLH_CACHE_Q4, BF = !FOUR && KvType<IT>::code == MLH_DTYPE_BF16;
     constexpr int KS = HD / 16, MB = HD / 32, TB = 64 * HD * 2, QB = NW * 32; // TB: bytes of a tile of K or V
     extern __shared__ __attribute__((aligned(16))) unsigned char lds[]; // K, V of two tiles; keys to repair; a row of V for each wave
     uint32_t* const flags = reinterpret_cast<uint32_t*>(lds + 4 * TB);
-    float (*const odds)[HD] = reinterpret_cast<float (*)[HD]>(lds + 4 * TB + 16);
+    float (*const odds)[HD] = reinterpret_cast<float (*)[HD]>(lds + 4 * TB + 32);
     const int kh = blockIdx.x % A.kvHeads, tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, n = lane & 31, half = lane >> 5;
     KvBlock B;
     if (!kv_block<QB>(A, (gridDim.x - 1 - blockIdx.x) / A.kvHeads, B)) return; // (the last rows of a sequence see most: first)
@@ -699,8 +723,10 @@ __global__ void __launch_bounds__(NW * 64, 2) k_kvattn_many(KvAttnArgs A) {
     constexpr int EPT = HD / NW; // 4-bit pages: elements a thread takes of K and of V
     uint32_t kc[FOUR ? EPT / 8 : 1], vc[FOUR ? EPT / 8 : 1], kp = 0, vp = 0;
     const int qRow = tid / NW, qAt = (tid % NW) * EPT;
-    auto fetch = [&](int i, int buf) __attribute__((always_inline)) {
-        const int page = max(kv_page(A.table, A.pagesPerSeq, A.numPages, B.s, tiles.at(i)), 0);
+    constexpr int RPI = 512 / HD, CPR = HD / 8; // 16-bit pages: rows an instruction, pieces a row
+    auto page_of = [&](int i) { return kv_page(A.table, A.pagesPerSeq, A.numPages, B.s, tiles.at(i)); };
+    auto fetch = [&](int found, int buf) __attribute__((always_inline)) { // the tile of that page
+        const int page = max(found, 0);
         if constexpr (FOUR) {
             const size_t base = ((size_t)page * A.kvHeads + kh) * kv_tile_bytes(HD);
             const unsigned o = qRow * (HD / 2) + qAt / 2, p = kv_param_at(HD) + (qRow * (HD / KV_GROUP) + qAt / KV_GROUP) * 4;
@@ -711,7 +737,6 @@ __global__ void __launch_bounds__(NW * 64, 2) k_kvattn_many(KvAttnArgs A) {
             else if constexpr (EPT == 16) { *reinterpret_cast<u32x2*>(kc) = *reinterpret_cast<const u32x2*>(tk + o); *reinterpret_cast<u32x2*>(vc) = *reinterpret_cast<const u32x2*>(tv + o); }
             else { kc[0] = *reinterpret_cast<const uint32_t*>(tk + o); vc[0] = *reinterpret_cast<const uint32_t*>(tv + o); }
         } else { // 1 KiB an instruction: lane i's 16 bytes go to the i-th place of it
-            constexpr int RPI = 512 / HD, CPR = HD / 8; // rows an instruction, pieces a row
             const size_t base = (((size_t)page * MLH_KV_PAGE) * A.kvHeads + kh) * HD * 2;
             const int lr = lane / CPR, lc = lane % CPR;
 #pragma unroll
@@ -726,36 +751,38 @@ __global__ void __launch_bounds__(NW * 64, 2) k_kvattn_many(KvAttnArgs A) {
             }
         }
     };
-    auto deposit = [&](int buf) __attribute__((always_inline)) { // 4-bit pages: what fetch left in registers
+    // Before tile i counts as landed: 4-bit pages are written from what fetch left in registers; and where some row does not see all of the tile, elements of V that are no
+    // numbers leave it, and their keys are noted (each wave: what it brought itself; a place to note three tiles long, so that it is cleared two barriers before).
+    auto land = [&](int i, int page, int buf, int slot) __attribute__((always_inline)) {
+        const int j0 = tiles.at(i) * 64;
+        const bool part = !kv_all_see(A, B.minPos, B.maxPos, j0, 64) || page < 0;
+        auto note = [&](int row) { if (j0 + row <= B.maxPos && page >= 0) atomicOr(&flags[2 * slot + (row >> 5)], 1u << (row & 31)); };
         if constexpr (FOUR) {
 #pragma unroll
-            for (int i = 0; i < EPT / 8; i++) {
-                *reinterpret_cast<u32x4*>(lds + buf * 2 * TB + kv_place_k<HD>(qRow, qAt / 8 + i)) = kv_halves(kc[i], kp);
-                *reinterpret_cast<u32x4*>(lds + buf * 2 * TB + TB + kv_place_v<HD>(qRow, qAt / 8 + i)) = kv_halves(vc[i], vp);
+            for (int e = 0; e < EPT / 8; e++) {
+                *reinterpret_cast<u32x4*>(lds + buf * 2 * TB + kv_place_k<HD>(qRow, qAt / 8 + e)) = kv_halves(kc[e], kp);
+                u32x4 x = kv_halves(vc[e], vp);
+                if (part && kv_odd<BF>(x)) { x = kv_without_odd<BF>(x); note(qRow); }
+                *reinterpret_cast<u32x4*>(lds + buf * 2 * TB + TB + kv_place_v<HD>(qRow, qAt / 8 + e)) = x;
+            }
+        } else {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            if (part) {
+#pragma unroll
+                for (int j = 0; j < 64 / RPI / NW; j++) {
+                    const int r0 = (j * NW + wave) * RPI;
+                    u32x4* p = reinterpret_cast<u32x4*>(lds + buf * 2 * TB + TB + r0 * (HD * 2)) + lane;
+                    const u32x4 x = *p;
+                    if (kv_odd<BF>(x)) { *p = kv_without_odd<BF>(x); note(r0 + lane / CPR); }
+                }
             }
         }
     };
 
-    auto tile = [&](int i, int buf) __attribute__((always_inline)) {
+    auto tile = [&](int i, int page, int buf, int slot) __attribute__((always_inline)) {
         const int j0 = tiles.at(i) * 64;
-        const int page = kv_page(A.table, A.pagesPerSeq, A.numPages, B.s, j0 >> 6);
-        const unsigned char *kt = lds + buf * 2 * TB, *vt = kt + TB;
-        uint32_t odd[2] = {0, 0};
-        if (!kv_all_see(A, B.minPos, B.maxPos, j0, 64) || page < 0) { // repair: elements of V that are no numbers leave the tile
-            for (int c = tid; c < 64 * HD / 8; c += NW * 64) {
-                const int row = c / (HD / 8);
-                u32x4* p = reinterpret_cast<u32x4*>(const_cast<unsigned char*>(vt) + kv_place_v<HD>(row, c % (HD / 8)));
-                const u32x4 x = *p;
-                if (kv_odd<BF>(x.x) || kv_odd<BF>(x.y) || kv_odd<BF>(x.z) || kv_odd<BF>(x.w)) {
-                    *p = u32x4{kv_without_odd<BF>(x.x), kv_without_odd<BF>(x.y), kv_without_odd<BF>(x.z), kv_without_odd<BF>(x.w)};
-                    if (j0 + row <= B.maxPos && page >= 0) atomicOr(&flags[2 * buf + (row >> 5)], 1u << (row & 31));
-                }
-            }
-            __syncthreads();
-            odd[0] = __builtin_amdgcn_readfirstlane(flags[2 * buf]);
-            odd[1] = __builtin_amdgcn_readfirstlane(flags[2 * buf + 1]);
-        }
         if (!active || j0 > wMax || (A.window && j0 + 63 <= wMin - A.window && j0 >= A.sinks)) return;
+        const unsigned char *kt = lds + buf * 2 * TB, *vt = kt + TB;
         const bool whole = kv_all_see(A, wMin, wMax, j0, 64) && page >= 0;
         f32x16 s[2];
 #pragma unroll
@@ -767,10 +794,25 @@ __global__ void __launch_bounds__(NW * 64, 2) k_kvattn_many(KvAttnArgs A) {
         }
         float mx = -INFINITY;
         if (!whole) {
+            if (page < 0) {
 #pragma unroll
-            for (int b = 0; b < 2; b++)
+                for (int b = 0; b < 2; b++)
 #pragma unroll
-                for (int e = 0; e < 16; e++) s[b][e] = sight.sees(j0 + 32 * b + 8 * (e >> 2) + 4 * half + (e & 3)) ? page < 0 ? KV_NAN : s[b][e] : -INFINITY;
+                    for (int e = 0; e < 16; e++) s[b][e] = KV_NAN;
+            }
+            const int j = j0 + 4 * half;
+            if (A.window && j0 < A.sinks) {
+#pragma unroll
+                for (int b = 0; b < 2; b++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++) s[b][e] = sight.sees(j + 32 * b + 8 * (e >> 2) + (e & 3)) ? s[b][e] : -INFINITY;
+            } else {
+                const unsigned from = j - sight.low;
+#pragma unroll
+                for (int b = 0; b < 2; b++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++) s[b][e] = from + (32 * b + 8 * (e >> 2) + (e & 3)) <= sight.span ? s[b][e] : -INFINITY;
+            }
         }
 #pragma unroll
         for (int b = 0; b < 2; b++)
@@ -793,7 +835,9 @@ __global__ void __launch_bounds__(NW * 64, 2) k_kvattn_many(KvAttnArgs A) {
             for (int e = 0; e < 16; e++) { // (hidden: 2^-inf)
                 s[b][e] = kv_exp2(fmaf(s[b][e], scale, ref));
             }
-        if (odd[0] | odd[1]) {
+        uint32_t odd[2] = {0, 0};
+        if (!kv_all_see(A, B.minPos, B.maxPos, j0, 64)) { odd[0] = __builtin_amdgcn_readfirstlane(flags[2 * slot]); odd[1] = __builtin_amdgcn_readfirstlane(flags[2 * slot + 1]); }
+        if (odd[0] | odd[1]) { // repair
 #pragma unroll
             for (int b = 0; b < 2; b++)
                 for (uint32_t keys = odd[b]; keys; keys &= keys - 1) {
@@ -830,16 +874,26 @@ __global__ void __launch_bounds__(NW * 64, 2) k_kvattn_many(KvAttnArgs A) {
         }
     };
 
-    if (t0 < t1) fetch(t0, 0);
-    for (int i = t0; i < t1; i++) {
+    if (tid < 6) flags[tid] = 0;
+    int page = 0, next = 0; // of tiles i and i + 1; looked up two tiles ahead
+    if (t0 < t1) {
+        page = page_of(t0);
+        next = page_of(min(t0 + 1, t1 - 1));
+        fetch(page, 0);
+    }
+    __syncthreads();
+    for (int i = t0, slot = 0; i < t1; i++) {
         const int buf = (i - t0) & 1;
-        deposit(buf);
-        if (tid < 2) flags[2 * buf + tid] = 0; // (read last two tiles ago)
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); // tile i has landed ...
-        __syncthreads();                                  // ... for every wave, and every wave is done with tile i - 1
-        if (i + 1 < t1) fetch(i + 1, buf ^ 1);
+        land(i, page, buf, slot);
+        __syncthreads(); // for every wave, and every wave is done with tile i - 1
+        if (i + 1 < t1) fetch(next, buf ^ 1);
+        const int later = page_of(min(i + 2, t1 - 1));
         __builtin_amdgcn_sched_barrier(0);
-        tile(i, buf);
+        if (tid < 2) flags[2 * (slot == 0 ? 2 : slot - 1) + tid] = 0; // tile i - 1's, and i + 2's
+        tile(i, page, buf, slot);
+        slot = slot == 2 ? 0 : slot + 1;
+        page = next;
+        next = later;
     }
     if (!active || wave * 32 + n >= B.nr) return;
     l += __shfl_xor(l, 32, 64);
@@ -986,7 +1040,7 @@ static AttnPlan attn_plan(const mlh_kv_cache* c, const mlh_kv_batch* b, const ml
 size_t mlh_attention_work_most(int headDim) { return (size_t)2 * KV_SPLIT_WGS * 16 * (headDim + 2) * 4; }
 
 template <typename IT, typename CT, int HD, int NW> static hipError_t launch_many(dim3 grid, hipStream_t st, const KvAttnArgs& A) {
-    constexpr int bytes = 4 * 64 * HD * 2 + 16 + NW * HD * 4;
+    constexpr int bytes = 4 * 64 * HD * 2 + 32 + NW * HD * 4;
     if (bytes > 65536) { // (asked for on every call: the attribute belongs to the device that is current)
         const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&k_kvattn_many<IT, CT, HD, NW>), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
         if (e != hipSuccess) return e;
