@@ -188,20 +188,28 @@ __device__ __forceinline__ void kv_finish16(const KvAttnArgs& A, const KvBlock& 
 // which is the second product's operand as it stands; row m of V's operand of block b is element m HD/16 + b.  The waves take tiles of 16 keys in turn, the next tile's loads
 // go out before this one's products.
 // ----------------------------------------------------------------------------
+// Keeps a lane's 32-bit offset one: widened outside of the loop, it would be added to each page's base in vector registers, and these wait for the loads that use them.
+__device__ __forceinline__ void kv_offset(unsigned& o) { asm volatile("" : "+v"(o)); }
 template <typename CT, int HD> struct KvTile32 { // a lane's part of 16 keys
     static constexpr int KC = HD / 4, VB = HD / 16;
     f32x4 k[KC / 4], v[4][VB / 4];
-    __device__ __forceinline__ void fetch(const KvAttnArgs& A, int page, int at, int last, int kh, int n, int g) {
-        const size_t row = (size_t)A.kvHeads * HD, base = ((size_t)page * MLH_KV_PAGE + at) * row + (size_t)kh * HD;
-        const float* kr = (const float*)A.poolK + base + (size_t)min(n, last) * row + g * KC;
+    struct Lane {
+        unsigned ko, vo;
+        __device__ __forceinline__ Lane(const KvAttnArgs& A, int n, int g) : ko(n * (unsigned)A.kvHeads * HD * 4 + g * KC * 4), vo(4 * g * (unsigned)A.kvHeads * HD * 4 + n * VB * 4) {}
+    };
+    // (a page's base is the same for all lanes and a lane's offset the same for all tiles: no address arithmetic in vector registers.  Rows behind the last position
+    // are read as they are, a page being whole, and weigh nothing.)
+    __device__ __forceinline__ void fetch(const KvAttnArgs& A, int page, int at, int kh, Lane& lane) {
+        const unsigned row = (unsigned)A.kvHeads * HD * 4;
+        kv_offset(lane.ko); kv_offset(lane.vo);
+        const size_t base = ((size_t)page * MLH_KV_PAGE + at) * row + (size_t)kh * HD * 4;
+        const char *bk = (const char*)A.poolK + base, *bv = (const char*)A.poolV + base;
 #pragma unroll
-        for (int c = 0; c < KC / 4; c++) k[c] = *reinterpret_cast<const f32x4*>(kr + 4 * c);
+        for (int c = 0; c < KC / 4; c++) k[c] = *reinterpret_cast<const f32x4*>(bk + lane.ko + 16 * c);
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const float* vr = (const float*)A.poolV + base + (size_t)min(4 * g + i, last) * row + n * VB;
+        for (int i = 0; i < 4; i++)
 #pragma unroll
-            for (int c = 0; c < VB / 4; c++) v[i][c] = *reinterpret_cast<const f32x4*>(vr + 4 * c);
-        }
+            for (int c = 0; c < VB / 4; c++) v[i][c] = *reinterpret_cast<const f32x4*>(bv + (size_t)i * row + lane.vo + 16 * c);
     }
     __device__ __forceinline__ void values(f32x4 (&ko)[KC / 4], f32x4 (&vo)[4][VB / 4]) const {
 #pragma unroll
@@ -215,19 +223,24 @@ template <typename CT, int HD> struct KvTile32 { // a lane's part of 16 keys
 template <int HD> struct KvTile32<q4_t, HD> {
     static constexpr int KC = HD / 4, VB = HD / 16;
     uint32_t k[KC / 8], kp, v[4], vp[4];
-    __device__ __forceinline__ void fetch(const KvAttnArgs& A, int page, int at, int last, int kh, int n, int g) {
+    struct Lane {
+        unsigned ko, kpo, vo, vpo;
+        __device__ __forceinline__ Lane(const KvAttnArgs&, int n, int g)
+            : ko(n * (HD / 2) + g * (KC / 2)), kpo((n * (HD / KV_GROUP) + g * KC / KV_GROUP) * 4), vo(4 * g * (HD / 2) + n * (VB / 2)), vpo((4 * g * (HD / KV_GROUP) + n * VB / KV_GROUP) * 4) {}
+    };
+    __device__ __forceinline__ void fetch(const KvAttnArgs& A, int page, int at, int kh, Lane& lane) {
         const size_t base = ((size_t)page * A.kvHeads + kh) * kv_tile_bytes(HD);
-        const uint8_t *tk = (const uint8_t*)A.poolK + base, *tv = (const uint8_t*)A.poolV + base;
-        const int rk = at + min(n, last);
+        const uint8_t *tk = (const uint8_t*)A.poolK + base + at * (HD / 2), *tv = (const uint8_t*)A.poolV + base + at * (HD / 2);
+        const uint8_t *pk = (const uint8_t*)A.poolK + base + kv_param_at(HD) + at * (HD / KV_GROUP) * 4, *pv = (const uint8_t*)A.poolV + base + kv_param_at(HD) + at * (HD / KV_GROUP) * 4;
+        kv_offset(lane.ko); kv_offset(lane.kpo); kv_offset(lane.vo); kv_offset(lane.vpo);
 #pragma unroll
-        for (int c = 0; c < KC / 8; c += 2) *reinterpret_cast<uint2*>(&k[c]) = *reinterpret_cast<const uint2*>(tk + rk * (HD / 2) + g * (KC / 2) + 4 * c);
-        kp = *reinterpret_cast<const uint32_t*>(tk + kv_param_at(HD) + (rk * (HD / KV_GROUP) + g * KC / KV_GROUP) * 4);
+        for (int c = 0; c < KC / 8; c += 2) *reinterpret_cast<uint2*>(&k[c]) = *reinterpret_cast<const uint2*>(tk + lane.ko + 4 * c);
+        kp = *reinterpret_cast<const uint32_t*>(pk + lane.kpo);
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            const int rv = at + min(4 * g + i, last);
-            if constexpr (HD == 128) v[i] = *reinterpret_cast<const uint32_t*>(tv + rv * (HD / 2) + n * 4);
-            else v[i] = *reinterpret_cast<const uint16_t*>(tv + rv * (HD / 2) + n * 2);
-            vp[i] = *reinterpret_cast<const uint32_t*>(tv + kv_param_at(HD) + (rv * (HD / KV_GROUP) + n * VB / KV_GROUP) * 4);
+            if constexpr (HD == 128) v[i] = *reinterpret_cast<const uint32_t*>(tv + lane.vo + i * (HD / 2));
+            else v[i] = *reinterpret_cast<const uint16_t*>(tv + lane.vo + i * (HD / 2));
+            vp[i] = *reinterpret_cast<const uint32_t*>(pv + lane.vpo + i * (HD / KV_GROUP) * 4);
         }
     }
     __device__ __forceinline__ void values(f32x4 (&ko)[KC / 4], f32x4 (&vo)[4][VB / 4]) const {
@@ -270,13 +283,14 @@ __global__ void __launch_bounds__(NW * 64, 2) k_kvattn_f32(KvAttnArgs A) {
     float m = -INFINITY, l = 0.f; // of row n; l: over this lane's keys
     const KvTiles<16> tiles(A, B);
     KvTile32<CT, HD> raw[2];
+    typename KvTile32<CT, HD>::Lane offsets(A, n, g);
     int page[2];
     int next = 0; // page of the tile to be fetched next
     auto look = [&](int i) { next = kv_page(A.table, A.pagesPerSeq, A.numPages, B.s, tiles.at(min(i, tiles.n - 1)) * 16 >> 6); };
     auto fetch = [&](int i, int set) __attribute__((always_inline)) {
         const int j0 = tiles.at(i) * 16;
         page[set] = next;
-        raw[set].fetch(A, max(page[set], 0), j0 & 63, min(B.maxPos - j0, 15), kh, n, g);
+        raw[set].fetch(A, max(page[set], 0), j0 & 63, kh, offsets);
     };
     auto tile = [&](int i, int set) __attribute__((always_inline)) {
         const int j0 = tiles.at(i) * 16, key = j0 + 4 * g;
@@ -440,16 +454,23 @@ __device__ __forceinline__ int kv_row_exp(float most) {
 template <typename IT, typename CT, int HD> struct KvRaw16 { // a lane's part of 32 keys: key 16 b + n, elements 32 t + 8 g ..; of V the same
     static constexpr int KS = HD / 32;
     u32x4 k[2][KS], v[2][KS];
-    __device__ __forceinline__ void fetch(const KvAttnArgs& A, int page, int at, int last, int kh, int n, int g) {
-        const size_t row = (size_t)A.kvHeads * HD, base = ((size_t)page * MLH_KV_PAGE + at) * row + (size_t)kh * HD + g * 8;
+    struct Lane {
+        unsigned o;
+        __device__ __forceinline__ Lane(const KvAttnArgs& A, int n, int g) : o(n * (unsigned)A.kvHeads * HD * 2 + g * 16) {}
+    };
+    __device__ __forceinline__ void fetch(const KvAttnArgs& A, int page, int at, int kh, Lane& lane) { // (addresses: as in KvTile32)
+        const unsigned row = (unsigned)A.kvHeads * HD * 2;
+        kv_offset(lane.o);
+        const size_t base = ((size_t)page * MLH_KV_PAGE + at) * row + (size_t)kh * HD * 2;
+        const char *bk = (const char*)A.poolK + base, *bv = (const char*)A.poolV + base;
 #pragma unroll
-        for (int b = 0; b < 2; b++) {
-            const size_t o = base + (size_t)min(16 * b + n, last) * row;
+        for (int b = 0; b < 2; b++)
 #pragma unroll
-            for (int t = 0; t < KS; t++) k[b][t] = *reinterpret_cast<const u32x4*>((const uint16_t*)A.poolK + o + 32 * t);
+            for (int t = 0; t < KS; t++) k[b][t] = *reinterpret_cast<const u32x4*>(bk + (size_t)(16 * b) * row + lane.o + 64 * t);
 #pragma unroll
-            for (int t = 0; t < KS; t++) v[b][t] = *reinterpret_cast<const u32x4*>((const uint16_t*)A.poolV + o + 32 * t);
-        }
+        for (int b = 0; b < 2; b++)
+#pragma unroll
+            for (int t = 0; t < KS; t++) v[b][t] = *reinterpret_cast<const u32x4*>(bv + (size_t)(16 * b) * row + lane.o + 64 * t);
     }
     __device__ __forceinline__ u32x4 key(int b, int t) const { return k[b][t]; }
     __device__ __forceinline__ u32x4 val(int b, int t) const { return v[b][t]; }
@@ -457,20 +478,25 @@ template <typename IT, typename CT, int HD> struct KvRaw16 { // a lane's part of
 template <typename IT, int HD> struct KvRaw16<IT, q4_t, HD> { // the same, elements (HD / 4) g + 8 t .. (one group of 32, or half of one)
     static constexpr int KS = HD / 32;
     uint32_t k[2][KS], v[2][KS], kp[2], vp[2];
-    __device__ __forceinline__ void fetch(const KvAttnArgs& A, int page, int at, int last, int kh, int n, int g) {
+    struct Lane {
+        unsigned o, p;
+        __device__ __forceinline__ Lane(const KvAttnArgs&, int n, int g) : o(n * (HD / 2) + g * (HD / 8)), p((n * (HD / KV_GROUP) + g * (HD / 4) / KV_GROUP) * 4) {}
+    };
+    __device__ __forceinline__ void fetch(const KvAttnArgs& A, int page, int at, int kh, Lane& lane) {
         const size_t base = ((size_t)page * A.kvHeads + kh) * kv_tile_bytes(HD);
+        kv_offset(lane.o); kv_offset(lane.p);
 #pragma unroll
         for (int b = 0; b < 2; b++) {
-            const int r = at + min(16 * b + n, last);
-            const size_t o = base + r * (HD / 2) + g * (HD / 8), p = base + kv_param_at(HD) + (r * (HD / KV_GROUP) + g * (HD / 4) / KV_GROUP) * 4;
-            kp[b] = *reinterpret_cast<const uint32_t*>((const uint8_t*)A.poolK + p);
-            vp[b] = *reinterpret_cast<const uint32_t*>((const uint8_t*)A.poolV + p);
+            const uint8_t *tk = (const uint8_t*)A.poolK + base + (at + 16 * b) * (HD / 2), *tv = (const uint8_t*)A.poolV + base + (at + 16 * b) * (HD / 2);
+            const uint8_t *pk = (const uint8_t*)A.poolK + base + kv_param_at(HD) + (at + 16 * b) * (HD / KV_GROUP) * 4, *pv = (const uint8_t*)A.poolV + base + kv_param_at(HD) + (at + 16 * b) * (HD / KV_GROUP) * 4;
+            kp[b] = *reinterpret_cast<const uint32_t*>(pk + lane.p);
+            vp[b] = *reinterpret_cast<const uint32_t*>(pv + lane.p);
             if constexpr (HD == 128) {
-                *reinterpret_cast<u32x4*>(k[b]) = *reinterpret_cast<const u32x4*>((const uint8_t*)A.poolK + o);
-                *reinterpret_cast<u32x4*>(v[b]) = *reinterpret_cast<const u32x4*>((const uint8_t*)A.poolV + o);
+                *reinterpret_cast<u32x4*>(k[b]) = *reinterpret_cast<const u32x4*>(tk + lane.o);
+                *reinterpret_cast<u32x4*>(v[b]) = *reinterpret_cast<const u32x4*>(tv + lane.o);
             } else {
-                *reinterpret_cast<u32x2*>(k[b]) = *reinterpret_cast<const u32x2*>((const uint8_t*)A.poolK + o);
-                *reinterpret_cast<u32x2*>(v[b]) = *reinterpret_cast<const u32x2*>((const uint8_t*)A.poolV + o);
+                *reinterpret_cast<u32x2*>(k[b]) = *reinterpret_cast<const u32x2*>(tk + lane.o);
+                *reinterpret_cast<u32x2*>(v[b]) = *reinterpret_cast<const u32x2*>(tv + lane.o);
             }
         }
     }
@@ -522,13 +548,14 @@ __global__ void __launch_bounds__(kv_few_waves<CT>() * 64, KvType<CT>::code == M
     unsigned char* const vt = lds + wave * 32 * VP;
     const KvTiles<32> tiles(A, B);
     KvRaw16<IT, CT, HD> raw[2];
+    typename KvRaw16<IT, CT, HD>::Lane offsets(A, n, g);
     int page[2];
     int next = 0; // page of the tile to be fetched next
     auto look = [&](int i) { next = kv_page(A.table, A.pagesPerSeq, A.numPages, B.s, tiles.at(min(i, tiles.n - 1)) * 32 >> 6); };
     auto fetch = [&](int i, int set) __attribute__((always_inline)) {
         const int j0 = tiles.at(i) * 32;
         page[set] = next;
-        raw[set].fetch(A, max(page[set], 0), j0 & 63, min(B.maxPos - j0, 31), kh, n, g);
+        raw[set].fetch(A, max(page[set], 0), j0 & 63, kh, offsets);
     };
     auto tile = [&](int i, int set) __attribute__((always_inline)) {
         const int j0 = tiles.at(i) * 32;
@@ -540,18 +567,23 @@ __global__ void __launch_bounds__(kv_few_waves<CT>() * 64, KvType<CT>::code == M
 #pragma unroll
             for (int t = 0; t < KS; t++) s[b] = mfma16<BF>(raw[set].key(b, t), q[t], s[b]);
         }
+        bool odd[2] = {false, false}; // does this lane hold an element of V that is no number?
+        if (!whole) {
+#pragma unroll
+            for (int b = 0; b < 2; b++)
+#pragma unroll
+                for (int t = 0; t < KS; t++) odd[b] |= kv_odd<BF>(raw[set].val(b, t));
+        }
+        const bool repair = __any(odd[0] | odd[1]);
         // V's rows: columns in the order that the pieces come in (4-bit pages: (0, 4), (1, 5) ... of every eight)
-        bool odd[2] = {false, false};
+        unsigned char* const place = vt + n * VP + (FOUR ? (HD / 4) * g : 8 * g) * 2;
 #pragma unroll
         for (int b = 0; b < 2; b++)
 #pragma unroll
             for (int t = 0; t < KS; t++) {
                 u32x4 x = raw[set].val(b, t);
-                if (!whole && kv_odd<BF>(x)) {
-                    odd[b] = true;
-                    x = kv_without_odd<BF>(x);
-                }
-                *reinterpret_cast<u32x4*>(vt + (16 * b + n) * VP + (FOUR ? (HD / 4) * g + 8 * t : 32 * t + 8 * g) * 2) = x;
+                if (repair) x = kv_without_odd<BF>(x);
+                *reinterpret_cast<u32x4*>(place + 16 * b * VP + (FOUR ? 8 * t : 32 * t) * 2) = x;
             }
         float p[2][4], mt = m;
         bool see[2][4];
@@ -577,7 +609,7 @@ __global__ void __launch_bounds__(kv_few_waves<CT>() * 64, KvType<CT>::code == M
             }
 #pragma unroll
         for (int b = 0; b < VB; b++) acc[b] *= corr;
-        if (!whole) { // repair
+        if (repair) {
 #pragma unroll
             for (int b = 0; b < 2; b++) {
                 unsigned long long hit = __ballot(odd[b]);
