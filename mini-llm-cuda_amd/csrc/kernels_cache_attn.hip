@@ -323,8 +323,10 @@ __global__ void __launch_bounds__(NW * 64, 2) k_kvattn_f32(KvAttnArgs A) {
             p[e] = see[e] ? kv_exp2(p[e] - ref) : 0.f;
             l += p[e];
         }
+        if (__any(corr != 1.f)) { // (a maximum that moves gets rare)
 #pragma unroll
-        for (int b = 0; b < VB; b++) acc[b] *= corr;
+            for (int b = 0; b < VB; b++) acc[b] *= corr;
+        }
         if (!whole) { // repair
             bool odd = false;
 #pragma unroll
@@ -518,27 +520,15 @@ __global__ void __launch_bounds__(kv_few_waves<CT>() * 64, KvType<CT>::code == M
     if (!kv_block<16>(A, blockIdx.x / A.kvHeads, B)) return;
     const int r = B.r0 + min(n, B.nr - 1), h = kh * A.group + r % A.group;
     const KvSight sight(A, B.pos0 + r / A.group);
+    // the row, on its way before the first tile and looked at behind it
     u32x4 q[KS];
-    float scale = A.scale2;
+    float scale = A.scale2, x[FOUR ? KS : 1][8];
     {
         const IT* qr = (const IT*)A.q + (size_t)(B.row0 + r / A.group) * A.qStride + (size_t)h * HD;
-        if constexpr (!FOUR) {
 #pragma unroll
-            for (int t = 0; t < KS; t++) q[t] = *reinterpret_cast<const u32x4*>(qr + 32 * t + 8 * g);
-        } else {
-            float x[KS][8], most = 0.f;
-#pragma unroll
-            for (int t = 0; t < KS; t++) {
-                kv_load8(qr + (HD / 4) * g + 8 * t, x[t]);
-#pragma unroll
-                for (int i = 0; i < 8; i++) most = fmaxf(most, fabsf(x[t][i]));
-            }
-            const int e = KvType<IT>::code == MLH_DTYPE_BF16 ? kv_row_exp(kv_quad_max(most)) : 0;
-            scale = ldexpf(scale, -e);
-#pragma unroll
-            for (int t = 0; t < KS; t++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) q[t][i] = pack_f16(ldexpf(x[t][i], e), ldexpf(x[t][i + 4], e));
+        for (int t = 0; t < KS; t++) {
+            if constexpr (FOUR) kv_load8(qr + (HD / 4) * g + 8 * t, x[t]);
+            else q[t] = *reinterpret_cast<const u32x4*>(qr + 32 * t + 8 * g);
         }
     }
     f32x4 acc[VB];
@@ -607,8 +597,10 @@ __global__ void __launch_bounds__(kv_few_waves<CT>() * 64, KvType<CT>::code == M
                 p[b][e] = see[b][e] ? kv_exp2(p[b][e] - ref) : 0.f;
                 l += p[b][e];
             }
+        if (__any(corr != 1.f)) { // (a maximum that moves gets rare)
 #pragma unroll
-        for (int b = 0; b < VB; b++) acc[b] *= corr;
+            for (int b = 0; b < VB; b++) acc[b] *= corr;
+        }
         if (repair) {
 #pragma unroll
             for (int b = 0; b < 2; b++) {
@@ -651,6 +643,19 @@ __global__ void __launch_bounds__(kv_few_waves<CT>() * 64, KvType<CT>::code == M
         look(t);
         fetch(t, 0);
         look(t + step);
+    }
+    if constexpr (FOUR) {
+        float most = 0.f;
+#pragma unroll
+        for (int t = 0; t < KS; t++)
+#pragma unroll
+            for (int i = 0; i < 8; i++) most = fmaxf(most, fabsf(x[t][i]));
+        const int e = KvType<IT>::code == MLH_DTYPE_BF16 ? kv_row_exp(kv_quad_max(most)) : 0;
+        scale = ldexpf(scale, -e);
+#pragma unroll
+        for (int t = 0; t < KS; t++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) q[t][i] = pack_f16(ldexpf(x[t][i], e), ldexpf(x[t][i + 4], e));
     }
     while (t < tiles.n) { // (no further tile: the same loads again, dropped)
         fetch(min(t + step, tiles.n - 1), 1);
@@ -961,9 +966,12 @@ __global__ void __launch_bounds__(256) k_kvattn_join(KvAttnArgs A) {
     __shared__ f32x4 sum[G][T];
     const size_t rh = blockIdx.x, n = (size_t)A.rows * A.heads;
     const int row = (int)(rh / A.heads), h = (int)(rh % A.heads), lane = threadIdx.x & 63, t = threadIdx.x % T, g = threadIdx.x / T;
-    if (row < A.start[0] || row >= A.start[A.nseq]) return;
     const float2* stat = reinterpret_cast<const float2*>(A.part + (size_t)A.nsplit * n * HD);
     const float2 ml = lane < A.nsplit ? stat[lane * n + rh] : make_float2(-INFINITY, 0.f);
+    f32x4 v[KV_MAX_SPLIT / G]; // (everything on its way before anything is waited for)
+#pragma unroll
+    for (int i = 0; i < KV_MAX_SPLIT / G; i++) v[i] = *reinterpret_cast<const f32x4*>(A.part + (min(i * G + g, A.nsplit - 1) * n + rh) * HD + 4 * t);
+    if (row < A.start[0] || row >= A.start[A.nseq]) return;
     float M = ml.x;
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
@@ -972,10 +980,10 @@ __global__ void __launch_bounds__(256) k_kvattn_join(KvAttnArgs A) {
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) den += __shfl_xor(den, o, 64);
     f32x4 o = (f32x4)(0.f);
-    for (int s0 = 0; s0 < A.nsplit; s0 += G) { // (every lane of a wave takes the exchange)
-        const int s = s0 + g;
-        const float w = __shfl(f, min(s, KV_MAX_SPLIT - 1), 64);
-        if (s < A.nsplit) o += *reinterpret_cast<const f32x4*>(A.part + (s * n + rh) * HD + 4 * t) * w;
+#pragma unroll
+    for (int i = 0; i < KV_MAX_SPLIT / G; i++) {
+        const float w = __shfl(f, i * G + g, 64); // (of a share that is not there: 2^-inf)
+        if (i * G + g < A.nsplit) o += v[i] * w;
     }
     sum[g][t] = o;
     __syncthreads();
@@ -994,7 +1002,6 @@ __global__ void __launch_bounds__(256) k_kvattn_join_few(KvAttnArgs A) {
     const size_t rh = (size_t)blockIdx.x * (256 / T) + threadIdx.x / T, n = (size_t)A.rows * A.heads;
     if (rh >= n) return;
     const int row = (int)(rh / A.heads), h = (int)(rh % A.heads), d = threadIdx.x % T * 4;
-    if (row < A.start[0] || row >= A.start[A.nseq]) return;
     const float2* stat = reinterpret_cast<const float2*>(A.part + (size_t)A.nsplit * n * HD);
     float2 ml[KV_JOIN_FEW];
     f32x4 v[KV_JOIN_FEW], o = (f32x4)(0.f);
@@ -1006,6 +1013,7 @@ __global__ void __launch_bounds__(256) k_kvattn_join_few(KvAttnArgs A) {
         v[s] = *reinterpret_cast<const f32x4*>(A.part + i * HD + d);
         M = fmaxf(M, ml[s].x);
     }
+    if (row < A.start[0] || row >= A.start[A.nseq]) return;
     const float ref = M == -INFINITY ? 0.f : M;
 #pragma unroll
     for (int s = 0; s < KV_JOIN_FEW; s++) {
