@@ -405,7 +405,7 @@ typedef struct {
  * (c a - s b, s a + c b) with the (c, s) pairs of row `position` of rope [ropeRows, headDim] (the table of mlh_upload_rope_table; inference.cu:113-134); rope null:
  * none.  qGain, kGain [heads * headDim], [cache.heads * headDim]: per-head norm x -> gain * x / sqrt(mean(x^2) + 1e-8) in front of the rotation
  * (inference.cu:52-81, 97-111); null: none.  Products and sums are in 64 bits, results are rounded to fp32 and then to the type that is stored.
- * 4-bit pages: of every 32 elements x, minimum = half(min x), scale = half((max x - min x) / 15 in fp32), code = the nearest whole number to
+ * 4-bit pages: of every 32 elements x, minimum = half(min x), scale = half((max x - min x) * (1 / 15), 1 / 15 and the product in fp32), code = the nearest whole number to
  * (x - minimum) / scale in 0 .. 15 (ties to even; scale 0: code 0); minima beyond the halves' range count as their largest, and a group with an infinity or NaN, or whose scale is
  * beyond that range, reads back as NaN.
  * q may be null (with qOut); qOut may be q with the same stride.  A row whose position is negative, beyond the page table or the rope table, or in a page outside

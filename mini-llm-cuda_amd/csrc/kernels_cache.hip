@@ -114,7 +114,9 @@ __global__ void __launch_bounds__(KV_WG) k_kv_append(KvAppendArgs A) {
             for (int i = 0; i < 8; i++) { lo = fminf(lo, x[i]); hi = fmaxf(hi, x[i]); bad += x[i] * 0.f; } // (bad: NaN with an infinity or NaN among them)
 #pragma unroll
             for (int o = 1; o < 4; o <<= 1) { lo = fminf(lo, __shfl_xor(lo, o, 64)); hi = fmaxf(hi, __shfl_xor(hi, o, 64)); bad += __shfl_xor(bad, o, 64); }
-            uint32_t minBits = kv_to_half(__builtin_amdgcn_fmed3f(lo, -65504.f, 65504.f)), scaleBits = kv_to_half((hi - lo) / 15.0f);
+            float step = (hi - lo) * (1.0f / 15.0f);
+            asm volatile("" : "+v"(step)); // (rounded to fp32 first; in one instruction with the conversion the product is not)
+            uint32_t minBits = kv_to_half(__builtin_amdgcn_fmed3f(lo, -65504.f, 65504.f)), scaleBits = kv_to_half(step);
             const float base = kv_half(minBits), scale = kv_half(scaleBits);
             uint32_t codes = 0;
             if (!(bad == 0.f) || scaleBits == 0x7c00u) { minBits = 0x7e00u; scaleBits = 0; }

@@ -234,7 +234,10 @@ template <int HD> struct KvTile32<q4_t, HD> {
         const uint8_t *pk = (const uint8_t*)A.poolK + base + kv_param_at(HD) + at * (HD / KV_GROUP) * 4, *pv = (const uint8_t*)A.poolV + base + kv_param_at(HD) + at * (HD / KV_GROUP) * 4;
         kv_offset(lane.ko); kv_offset(lane.kpo); kv_offset(lane.vo); kv_offset(lane.vpo);
 #pragma unroll
-        for (int c = 0; c < KC / 8; c += 2) *reinterpret_cast<uint2*>(&k[c]) = *reinterpret_cast<const uint2*>(tk + lane.ko + 4 * c);
+        for (int c = 0; c < KC / 8; c += 2) {
+            const uint2 w = *reinterpret_cast<const uint2*>(tk + lane.ko + 4 * c);
+            k[c] = w.x; k[c + 1] = w.y;
+        }
         kp = *reinterpret_cast<const uint32_t*>(pk + lane.kpo);
 #pragma unroll
         for (int i = 0; i < 4; i++) {
@@ -433,17 +436,44 @@ template <bool BF> __device__ __forceinline__ u32x4 kv_without_odd(u32x4 a) { //
     for (int i = 0; i < 4; i++) a[i] = ((a[i] & E) == E ? 0u : a[i] & 0xffffu) | ((a[i] >> 16 & E) == E ? 0u : a[i] & 0xffff0000u);
     return a;
 }
-// eight codes -> halves; pairs come out as elements (0, 4), (1, 5), (2, 6), (3, 7)
-__device__ __forceinline__ u32x4 kv_halves(uint32_t codes, uint32_t params) {
-    const _Float16 base = __builtin_bit_cast(_Float16, (uint16_t)(params & 0xffffu)), scale = __builtin_bit_cast(_Float16, (uint16_t)(params >> 16));
-    const f16x2 b = {base, base}, s = {scale, scale}, off = {(_Float16)-1024.f, (_Float16)-1024.f};
+// eight codes -> halves that are whole numbers, or the values; pairs come out as elements (0, 4), (1, 5), (2, 6), (3, 7)
+// (code | 1024 with the code in the lowest bits, code | 64 with it four bits higher, where a unit is sixteen of the last place: both exact, and so is taking 1024 and 64 off; the
+// constants in vector registers, as one instruction masks and joins then)
+__device__ __forceinline__ u32x4 kv_codes(uint32_t codes) {
+    uint32_t k = 0x64006400u, j = 0x54005400u;
+    asm("" : "+v"(k), "+v"(j));
+    const uint32_t up = codes >> 8;
+    const uint32_t w[4] = {(codes & 0x000f000fu) | k, (codes & 0x00f000f0u) | j, (up & 0x000f000fu) | k, (up & 0x00f000f0u) | j};
     u32x4 o;
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        const f16x2 c = __builtin_bit_cast(f16x2, ((codes >> (4 * i)) & 0x000f000fu) | 0x64006400u) + off; // 1024 + code, less 1024: exact
-        o[i] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(c, s, b));
+        const _Float16 off = i & 1 ? (_Float16)-64.f : (_Float16)-1024.f;
+        o[i] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, w[i]) + f16x2{off, off});
     }
     return o;
+}
+__device__ __forceinline__ u32x4 kv_halves(uint32_t codes, uint32_t params) {
+    const _Float16 base = __builtin_bit_cast(_Float16, (uint16_t)(params & 0xffffu)), scale = __builtin_bit_cast(_Float16, (uint16_t)(params >> 16));
+    const f16x2 b = {base, base}, s = {scale, scale};
+    u32x4 o = kv_codes(codes);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const uint32_t w = o[i]; // (a bit cast of an element of a vector reads the first)
+        o[i] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(__builtin_bit_cast(f16x2, w), s, b));
+    }
+    return o;
+}
+
+// one, two or four words
+__device__ __forceinline__ void kv_words(const uint8_t* p, uint32_t (&w)[1]) { w[0] = *reinterpret_cast<const uint32_t*>(p); }
+__device__ __forceinline__ void kv_words(const uint8_t* p, uint32_t (&w)[2]) {
+    const u32x2 x = *reinterpret_cast<const u32x2*>(p);
+    w[0] = x.x; w[1] = x.y;
+}
+__device__ __forceinline__ void kv_words(const uint8_t* p, uint32_t (&w)[4]) {
+    const u32x4 x = *reinterpret_cast<const u32x4*>(p);
+#pragma unroll
+    for (int i = 0; i < 4; i++) w[i] = x[i];
 }
 
 // A row's power of two: largest |q| into [1, 2), so that halves hold it; 2^24 at most (what halves then lose of a row is 2^-49), so that the scale divided by it stays
@@ -477,6 +507,21 @@ template <typename IT, typename CT, int HD> struct KvRaw16 { // a lane's part of
     __device__ __forceinline__ u32x4 key(int b, int t) const { return k[b][t]; }
     __device__ __forceinline__ u32x4 val(int b, int t) const { return v[b][t]; }
 };
+// Rows in halves over 4-bit pages: rounding K's values to halves costs such rows more than all else together, so that they are multiplied as what they are, minimum +
+// (high + low part of the scale) * code: parts of six and five bits times a code of four are exact in halves, two products instead of one, and the minima meet the sum of
+// the row's elements (as two halves) in one product more.  The weights are two halves as well.  (Error of a result, normal values, 4000 keys, against its norm: 4.4e-4 with
+// K, V and weights each rounded to halves, 2.8e-4 so, 2.1e-4 the rounding of the result alone.)  Rows in bf16 round their results eight times as far.
+template <typename IT, typename CT> constexpr bool kv_in_parts() { return KvType<CT>::code == MLH_CACHE_Q4 && KvType<IT>::code == MLH_DTYPE_F16; }
+__device__ __forceinline__ u32x4 kv_times(const u32x4& codes, uint32_t scaleBits) {
+    const _Float16 f = __builtin_bit_cast(_Float16, (uint16_t)scaleBits);
+    u32x4 o;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const uint32_t w = codes[i]; // (a bit cast of an element of a vector reads the first)
+        o[i] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, w) * f16x2{f, f});
+    }
+    return o;
+}
 template <typename IT, int HD> struct KvRaw16<IT, q4_t, HD> { // the same, elements (HD / 4) g + 8 t .. (one group of 32, or half of one)
     static constexpr int KS = HD / 32;
     uint32_t k[2][KS], v[2][KS], kp[2], vp[2];
@@ -493,13 +538,8 @@ template <typename IT, int HD> struct KvRaw16<IT, q4_t, HD> { // the same, eleme
             const uint8_t *pk = (const uint8_t*)A.poolK + base + kv_param_at(HD) + (at + 16 * b) * (HD / KV_GROUP) * 4, *pv = (const uint8_t*)A.poolV + base + kv_param_at(HD) + (at + 16 * b) * (HD / KV_GROUP) * 4;
             kp[b] = *reinterpret_cast<const uint32_t*>(pk + lane.p);
             vp[b] = *reinterpret_cast<const uint32_t*>(pv + lane.p);
-            if constexpr (HD == 128) {
-                *reinterpret_cast<u32x4*>(k[b]) = *reinterpret_cast<const u32x4*>(tk + lane.o);
-                *reinterpret_cast<u32x4*>(v[b]) = *reinterpret_cast<const u32x4*>(tv + lane.o);
-            } else {
-                *reinterpret_cast<u32x2*>(k[b]) = *reinterpret_cast<const u32x2*>(tk + lane.o);
-                *reinterpret_cast<u32x2*>(v[b]) = *reinterpret_cast<const u32x2*>(tv + lane.o);
-            }
+            kv_words(tk + lane.o, k[b]);
+            kv_words(tv + lane.o, v[b]);
         }
     }
     __device__ __forceinline__ u32x4 key(int b, int t) const { return kv_halves(k[b][t], kp[b]); }
@@ -510,6 +550,7 @@ template <typename CT> constexpr int kv_few_waves() { return KvType<CT>::code ==
 template <typename IT, typename CT, int HD>
 __global__ void __launch_bounds__(kv_few_waves<CT>() * 64, KvType<CT>::code == MLH_CACHE_Q4 ? 3 : 2) k_kvattn_few(KvAttnArgs A) {
     constexpr bool FOUR = KvType<CT>::code == MLH_CACHE_Q4, BF = !FOUR && KvType<IT>::code == MLH_DTYPE_BF16; // products in bf16
+    constexpr bool PARTS = kv_in_parts<IT, CT>();
     constexpr int NW = kv_few_waves<CT>(), KS = HD / 32, VB = HD / 16;
     constexpr int VP = HD * 2 + 16; // bytes of a row of V in LDS: four rows start in different banks
     constexpr int LV = NW * 32 * VP, LF = NW * 16 * (HD + 4 + 2) * 4;
@@ -521,7 +562,7 @@ __global__ void __launch_bounds__(kv_few_waves<CT>() * 64, KvType<CT>::code == M
     const int r = B.r0 + min(n, B.nr - 1), h = kh * A.group + r % A.group;
     const KvSight sight(A, B.pos0 + r / A.group);
     // the row, on its way before the first tile and looked at behind it
-    u32x4 q[KS];
+    u32x4 q[KS], qsum = (u32x4)(0u);
     float scale = A.scale2, x[FOUR ? KS : 1][8];
     {
         const IT* qr = (const IT*)A.q + (size_t)(B.row0 + r / A.group) * A.qStride + (size_t)h * HD;
@@ -554,8 +595,20 @@ __global__ void __launch_bounds__(kv_few_waves<CT>() * 64, KvType<CT>::code == M
 #pragma unroll
         for (int b = 0; b < 2; b++) {
             s[b] = (f32x4)(0.f);
+            if constexpr (PARTS) {
+                const uint32_t par = raw[set].kp[b], high = par >> 16 & 0xffe0u;
+                const _Float16 low = __builtin_bit_cast(_Float16, (uint16_t)(par >> 16)) - __builtin_bit_cast(_Float16, (uint16_t)high);
+                s[b] = mfma16<false>(u32x4{(par & 0xffffu) | par << 16, 0u, 0u, 0u}, qsum, s[b]);
 #pragma unroll
-            for (int t = 0; t < KS; t++) s[b] = mfma16<BF>(raw[set].key(b, t), q[t], s[b]);
+                for (int t = 0; t < KS; t++) {
+                    const u32x4 codes = kv_codes(raw[set].k[b][t]);
+                    s[b] = mfma16<false>(kv_times(codes, high), q[t], s[b]);
+                    s[b] = mfma16<false>(kv_times(codes, __builtin_bit_cast(uint16_t, low)), q[t], s[b]);
+                }
+            } else {
+#pragma unroll
+                for (int t = 0; t < KS; t++) s[b] = mfma16<BF>(raw[set].key(b, t), q[t], s[b]);
+            }
         }
         bool odd[2] = {false, false}; // does this lane hold an element of V that is no number?
         if (!whole) {
@@ -629,12 +682,18 @@ __global__ void __launch_bounds__(kv_few_waves<CT>() * 64, KvType<CT>::code == M
             }
         }
         const u32x4 pw = {kv_pack<BF>(p[0][0], p[0][1]), kv_pack<BF>(p[0][2], p[0][3]), kv_pack<BF>(p[1][0], p[1][1]), kv_pack<BF>(p[1][2], p[1][3])};
+        u32x4 rest = (u32x4)(0u); // what the halves leave of the weights
+        if constexpr (PARTS) {
+            auto left = [&](uint32_t w, float a, float b) { return pack_f16(a - kv_half(w & 0xffffu), b - kv_half(w >> 16)); };
+            rest = u32x4{left(pw.x, p[0][0], p[0][1]), left(pw.y, p[0][2], p[0][3]), left(pw.z, p[1][0], p[1][1]), left(pw.w, p[1][2], p[1][3])};
+        }
         // lane i of a group of 16 gives the address of row i / 4, columns 4 (i % 4) ..
         const unsigned char* va = vt + (4 * g + (n >> 2)) * VP + (n & 3) * 8;
 #pragma unroll
         for (int b = 0; b < VB; b++) {
             const u32x2 lo = lds_transposed(va + 32 * b), hi = lds_transposed(va + 16 * VP + 32 * b);
             acc[b] = mfma16<BF>(u32x4{lo.x, lo.y, hi.x, hi.y}, pw, acc[b]);
+            if constexpr (PARTS) acc[b] = mfma16<BF>(u32x4{lo.x, lo.y, hi.x, hi.y}, rest, acc[b]);
         }
     };
     const int step = NW * A.nsplit;
@@ -650,12 +709,20 @@ __global__ void __launch_bounds__(kv_few_waves<CT>() * 64, KvType<CT>::code == M
         for (int t = 0; t < KS; t++)
 #pragma unroll
             for (int i = 0; i < 8; i++) most = fmaxf(most, fabsf(x[t][i]));
-        const int e = KvType<IT>::code == MLH_DTYPE_BF16 ? kv_row_exp(kv_quad_max(most)) : 0;
+        const int e = kv_row_exp(kv_quad_max(most));
         scale = ldexpf(scale, -e);
 #pragma unroll
         for (int t = 0; t < KS; t++)
 #pragma unroll
             for (int i = 0; i < 4; i++) q[t][i] = pack_f16(ldexpf(x[t][i], e), ldexpf(x[t][i + 4], e));
+        if constexpr (PARTS) {
+            float sum = 0.f;
+#pragma unroll
+            for (int t = 0; t < KS; t++) sum += ((x[t][0] + x[t][1]) + (x[t][2] + x[t][3])) + ((x[t][4] + x[t][5]) + (x[t][6] + x[t][7]));
+            sum = ldexpf(sum, e);
+            const uint32_t first = kv_to_half(sum);
+            qsum.x = first | kv_to_half(sum - kv_half(first)) << 16;
+        }
     }
     while (t < tiles.n) { // (no further tile: the same loads again, dropped)
         fetch(min(t + step, tiles.n - 1), 1);
@@ -770,9 +837,8 @@ __global__ void __launch_bounds__(NW * 64, HD == 64 ? 3 : 2) k_kvattn_many(KvAtt
             const uint8_t *tk = (const uint8_t*)A.poolK + base, *tv = (const uint8_t*)A.poolV + base;
             kp = *reinterpret_cast<const uint32_t*>(tk + p);
             vp = *reinterpret_cast<const uint32_t*>(tv + p);
-            if constexpr (EPT == 32) { *reinterpret_cast<u32x4*>(kc) = *reinterpret_cast<const u32x4*>(tk + o); *reinterpret_cast<u32x4*>(vc) = *reinterpret_cast<const u32x4*>(tv + o); }
-            else if constexpr (EPT == 16) { *reinterpret_cast<u32x2*>(kc) = *reinterpret_cast<const u32x2*>(tk + o); *reinterpret_cast<u32x2*>(vc) = *reinterpret_cast<const u32x2*>(tv + o); }
-            else { kc[0] = *reinterpret_cast<const uint32_t*>(tk + o); vc[0] = *reinterpret_cast<const uint32_t*>(tv + o); }
+            kv_words(tk + o, kc);
+            kv_words(tv + o, vc);
         } else { // 1 KiB an instruction: lane i's 16 bytes go to the i-th place of it
             const size_t base = (((size_t)page * MLH_KV_PAGE) * A.kvHeads + kh) * HD * 2;
             const int lr = lane / CPR, lc = lane % CPR;

@@ -21,7 +21,7 @@ def quantise(x):
     g = x.unflatten(-1, (-1, GROUP))
     bad = ~torch.isfinite(g).all(-1, keepdim=True)
     low, high = g.amin(-1, keepdim=True), g.amax(-1, keepdim=True)
-    base, scale = low.clamp(-65504, 65504).half(), ((high - low) / 15.0).half()
+    base, scale = low.clamp(-65504, 65504).half(), ((high - low) * torch.tensor(1.0 / 15.0, dtype=torch.float32)).half()
     bad |= torch.isinf(scale)
     step = scale.double()
     c = ((g.double() - base.double()) / torch.where(step > 0, step, torch.ones_like(step))).round().clamp(0, 15)
