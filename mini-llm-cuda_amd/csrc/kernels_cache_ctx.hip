@@ -5,10 +5,9 @@
 
 #include "kv_cache.h"
 
-bool mlh_cache_ops(const mlh_ctx* c) { return c->window > 0 || c->kvType != MLH_DTYPE_F32; }
-
-static bool any_attention(const mlh_ctx* c) {
-    for (const LayerDev& L : c->layers)
+bool mlh_cache_ops(const mlh_ctx* c) {
+    if (c->window == 0 && c->kvType == MLH_DTYPE_F32) return false;
+    for (const LayerDev& L : c->layers) // (a model of gated-delta-net layers alone has neither)
         if (L.kind == MLH_KIND_ATTENTION) return true;
     return false;
 }
@@ -43,7 +42,7 @@ static int prepare(mlh_ctx* c) {
 
 // (no allocation, no synchronisation: can be captured)
 int mlh_cache_begin(mlh_ctx* c, int n, int rows, const int* seqs, const int* segStart, const int* segLen, const int* segPos0) {
-    if (!mlh_cache_ops(c) || !any_attention(c)) return 0;
+    if (!mlh_cache_ops(c)) return 0;
     hipLaunchKernelGGL(k_cache_begin, dim3(n), dim3(256), 0, c->stream, c->d_pageTable, c->pagesPerSeq, n, rows, seqs, c->d_pos, segStart, segLen, segPos0, cache_start(c), cache_len(c), cache_table(c));
     MLH_CHECK(c, hipGetLastError());
     return 0;

@@ -234,8 +234,87 @@ def test_graph_replays(pkg):
             torch.cuda.synchronize()
             g.replay()
             torch.cuda.synchronize()
-            assert torch.equal(c.out.cpu(), eager[name]), name
+            assert _same_bits(c.out.cpu(), eager[name]), name  # ("c" sees a position that holds NaN)
             torch.randn(1000, device="cuda").sum().item()
+
+
+def test_graph_of_prompts(pkg):
+    """The kernel of many rows in a graph: replays with other lengths, rows and hints than at the capture."""
+    for kind, cache in (("bf16", "bf16"), ("f16", "q4"), ("f32", "f32")):
+        c = Call(pkg, kind, cache, 4, 2, 128, [130, 90], [200, 90], 64, 2, seed=12)
+        lens, starts = {"a": [200, 90], "b": [150, 64], "c": [129, 91]}, {"a": [0, 130, 220], "b": [0, 100, 101], "c": [0, 1, 200]}
+        eager = {}
+        for name in lens:
+            c.rows.dlen.copy_(torch.tensor(lens[name], dtype=torch.int32))
+            c.rows.dstart.copy_(torch.tensor(starts[name], dtype=torch.int32))
+            c.out.fill_(5.0)
+            eager[name] = c.run().clone()
+            assert (eager[name][starts[name][-1]:] == 5.0).all()
+        side = torch.cuda.Stream()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.stream(side):
+            with torch.cuda.graph(g, stream=side):
+                pkg.attention(c.cache, c.batch, c.args, torch.cuda.current_stream().cuda_stream)
+        for name in ("b", "a", "c", "b"):
+            c.rows.dlen.copy_(torch.tensor(lens[name], dtype=torch.int32))
+            c.rows.dstart.copy_(torch.tensor(starts[name], dtype=torch.int32))
+            c.out.fill_(5.0)
+            torch.cuda.synchronize()
+            g.replay()
+            torch.cuda.synchronize()
+            assert _same_bits(c.out.cpu(), eager[name]), name  # ("c" sees a position that holds NaN)
+            torch.randn(1000, device="cuda").sum().item()
+
+
+@pytest.mark.parametrize("kind,cache", KINDS)
+def test_hints_decide_nothing_else(pkg, kind, cache):
+    """maxLen and maxNew that are too small, too large or missing: other kernels and splits, results within the bounds."""
+    for max_len, max_new in ((1, 1), (0, 0), (100000, 5), (7, 1000)):
+        for new, lens, window in (([1, 1], [1500, 3], 0), ([90, 40], [400, 40], 70)):
+            c = Call(pkg, kind, cache, 4, 2, 64, new, lens, window, 3, seed=31)
+            c.args.maxLen, c.args.maxNew = max_len, max_new
+            c.work_for(c.args)
+            c.check()
+
+
+@pytest.mark.parametrize("kind,cache", KINDS)
+@pytest.mark.parametrize("new,lens", [([3, 1], [90, 200]), ([150], [200])])
+def test_nonfinite_rows(pkg, kind, cache, new, lens):
+    """A row of q with NaN or infinities is none of its neighbours' business."""
+    c = Call(pkg, kind, cache, 2, 1, 64, new, lens, 60, 2, seed=14)
+    clean = c.run().clone()
+    bad = [0, new[0] - 1]
+    c.dq[bad[0], 5] = math.nan
+    c.dq[bad[1], 70] = math.inf
+    got = c.run()
+    for i in range(sum(new)):
+        for h in range(2):
+            hit = (i == bad[0] and h == 0) or (i == bad[1] and h == 1)
+            a, b = got[i, 64 * h:64 * h + 64], clean[i, 64 * h:64 * h + 64]
+            assert torch.isnan(a).any() if hit else torch.equal(a, b), (i, h)
+
+
+def test_many_sequences(pkg):
+    """More sequences than a search step has places; some without rows."""
+    new = [(7 * i) % 3 for i in range(150)]
+    lens = [n + (11 * i) % 70 for i, n in enumerate(new)]
+    for kind, cache in (("bf16", "bf16"), ("f32", "f32"), ("f16", "q4")):
+        Call(pkg, kind, cache, 2, 1, 64, new, lens, 20, 1, seed=3, pad=4).check()
+    a = Append(pkg, "bf16", "q4", 2, 1, 64, new, lens, seed=3, pad=4)
+    a.run()
+    a.expect()
+    assert _same_bits(a.pools.dk.cpu(), a.pools.k) and _same_bits(a.pools.dv.cpu(), a.pools.v)
+
+
+def test_small_work_is_refused(pkg):
+    c = Call(pkg, "bf16", "bf16", 2, 1, 64, [1], [9000], seed=1)
+    assert c.args.workBytes > 0
+    for change in (dict(workBytes=c.args.workBytes - 1), dict(work=None), dict(work=c.args.work + 8)):
+        c.work_for(c.args)
+        for k, v in change.items():
+            setattr(c.args, k, v)
+        with pytest.raises(pkg.MlhError, match="work"):
+            c.run()
 
 
 def test_two_streams(pkg):

@@ -269,3 +269,64 @@ def test_kv_type_rules(pkg):
     dev.prefill(0, tokens)
     assert np.array_equal(dev.logits(0), before)
     dev.close()
+
+
+def test_measurement_and_sampling(pkg):
+    """Timing of the attention part, a profile of steps and sampled tokens with a window and 4-bit pages."""
+    hp = _hp(pkg, 3, 64, 2, 0, 0, 0, seqs=3, maxL=120)
+    dev = pkg.Device(hp, 0)
+    dev.upload(_model(pkg, hp))
+    dev.set_kv_type(pkg.CACHE_Q4)
+    dev.set_attention_window(30, 2)
+    prompts = [np.arange(20 + s, dtype=np.int32) for s in range(3)]
+    dev.prefill_batch(range(3), prompts)
+    us, nbytes = dev.time_kernel(pkg.K_ATTN, 0, 3, 5)
+    assert us > 0 and nbytes == sum(2 * 0.625 * hp.dim * n + 2 * 0.625 * hp.dim for n in (21, 22, 23))
+    dev.reset()
+    runs = []
+    for k in (0, 2, 0):
+        dev.set_graph(k)
+        dev.reset()
+        dev.prefill_batch(range(3), prompts)
+        dev.set_sampling(0.8, 7)
+        runs.append(dev.decode_loop([1, 2, 3], 20))
+        dev.set_sampling(0.0)
+    assert np.array_equal(runs[0], runs[1]) and np.array_equal(runs[0], runs[2])
+    dev.close()
+
+
+def test_single_launch_shapes(pkg):
+    """A model that the single-launch kernels cover leaves them for a window or other pages, and comes back with neither."""
+    hp = _hp(pkg, 2, 64, 8, seqs=2, maxL=120)
+    dev = pkg.Device(hp, 0)
+    dev.upload(_model(pkg, hp))
+    n, route = dev.single_launch_sequences(), dev.decode_route(1)
+    assert n > 0 and route in (pkg.DECODE_XCD, pkg.DECODE_RANKS)
+    dev.set_kv_type(pkg.CACHE_Q4)
+    assert dev.single_launch_sequences() == 0 and dev.decode_route(1) == pkg.DECODE_ROWS
+    dev.set_attention_window(40)
+    dev.set_kv_type(pkg.DTYPE_F32)
+    assert dev.single_launch_sequences() == 0 and dev.decode_route(1) == pkg.DECODE_ROWS
+    dev.set_attention_window(0)
+    assert dev.single_launch_sequences() == n and dev.decode_route(1) == route
+    dev.close()
+
+
+def test_model_without_attention(pkg):
+    """Gated-delta-net layers have no window: nothing changes."""
+    hp = _hp(pkg, 2, 64, 2, 0, 0, 1, seqs=1, maxL=60)
+    for l in range(2):
+        hp.layerKinds[l] = pkg.KIND_GDN
+    dev = pkg.Device(hp, 0)
+    dev.upload(_model(pkg, hp, std=0.05))
+    tokens = np.arange(40, dtype=np.int32)
+    dev.prefill(0, tokens)
+    before, route = dev.logits(0), dev.decode_route(1)
+    dev.set_attention_window(5, 1)
+    dev.reset()
+    dev.set_kv_type(pkg.CACHE_Q4)
+    dev.prefill(0, tokens)
+    assert np.array_equal(dev.logits(0), before) and dev.decode_route(1) == route
+    with pytest.raises(pkg.MlhError, match="not an attention layer"):
+        dev.read_kv(0, 0, 0, 1)
+    dev.close()
