@@ -141,15 +141,15 @@ template <typename CT, int HD, bool HALVES> __device__ __forceinline__ void kv_o
 }
 
 // The end of the 16-row kernels: acc of every wave (block b, element i of lane 16 g + n: row n, element dim(b, 4 g + i)), its m and l (of row n), joined over the waves, and
-// written as the row's result or, with split keys, as this workgroup's share.  lds: NW * 16 * (HD + 4 + 2) floats.
-template <typename IT, int HD, int NW, typename F>
+// written as the row's result or, with split keys, as this workgroup's share.  lds: NW * 16 * (HD + 4 + 2) floats.  SP: columns of a row, all alike.
+template <typename IT, int HD, int NW, int SP, typename F>
 __device__ __forceinline__ void kv_finish16(const KvAttnArgs& A, const KvBlock& B, int kh, int split, const f32x4 (&acc)[HD / 16], float m, float l, float* lds, F dim4) {
     constexpr int LDO = HD + 4;
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, n = lane & 15, g = lane >> 4;
     float (*part)[16][LDO] = reinterpret_cast<float (*)[16][LDO]>(lds);
     float (*stat)[2][16] = reinterpret_cast<float (*)[2][16]>(lds + NW * 16 * LDO);
-    if (g == 0) { stat[wave][0][n] = m; stat[wave][1][n] = l; }
-    dim4([&](int d, const f32x4& v) { *reinterpret_cast<f32x4*>(&part[wave][n][d]) = v; });
+    if (g == 0 && n % SP == 0) { stat[wave][0][n / SP] = m; stat[wave][1][n / SP] = l; }
+    dim4([&](int d, const f32x4& v) { *reinterpret_cast<f32x4*>(&part[wave][n / SP][d]) = v; });
     __syncthreads();
     for (int i = tid; i < B.nr * (HD / 4); i += NW * 64) {
         const int r = i / (HD / 4), d = (i % (HD / 4)) * 4;
@@ -269,9 +269,10 @@ __global__ void __launch_bounds__(NW * 64, 2) k_kvattn_f32(KvAttnArgs A) {
     constexpr int KC = HD / 4, VB = HD / 16;
     __shared__ __attribute__((aligned(16))) float lds[NW * 16 * (HD + 4 + 2)];
     __shared__ float odds[NW][HD];
-    const int kh = blockIdx.x % A.kvHeads, split = blockIdx.y, tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, n = lane & 15, g = lane >> 4;
+    const int kh = blockIdx.x % A.kvHeads, block = blockIdx.x / A.kvHeads / A.nsplit, split = blockIdx.x / A.kvHeads % A.nsplit;
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, n = lane & 15, g = lane >> 4;
     KvBlock B;
-    if (!kv_block<16>(A, blockIdx.x / A.kvHeads, B)) return;
+    if (!kv_block<16>(A, block, B)) return;
     const int r = B.r0 + min(n, B.nr - 1), h = kh * A.group + r % A.group;
     const KvSight sight(A, B.pos0 + r / A.group);
     f32x4 q[KC / 4];
@@ -391,7 +392,7 @@ __global__ void __launch_bounds__(NW * 64, 2) k_kvattn_f32(KvAttnArgs A) {
         t += step;
     }
     l = kv_quad_sum(l);
-    kv_finish16<float, HD, NW>(A, B, kh, split, acc, m, l, lds, [&](auto put) {
+    kv_finish16<float, HD, NW, 1>(A, B, kh, split, acc, m, l, lds, [&](auto put) {
 #pragma unroll
         for (int i = 0; i < 4; i++)
 #pragma unroll
@@ -436,6 +437,9 @@ template <bool BF> __device__ __forceinline__ u32x4 kv_without_odd(u32x4 a) { //
     for (int i = 0; i < 4; i++) a[i] = ((a[i] & E) == E ? 0u : a[i] & 0xffffu) | ((a[i] >> 16 & E) == E ? 0u : a[i] & 0xffff0000u);
     return a;
 }
+template <int PERM> __device__ __forceinline__ float kv_neighbour(float v) { // among four lanes
+    return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), PERM, 0xf, 0xf, true));
+}
 // eight codes -> halves that are whole numbers, or the values; pairs come out as elements (0, 4), (1, 5), (2, 6), (3, 7)
 // (code | 1024 with the code in the lowest bits, code | 64 with it four bits higher, where a unit is sixteen of the last place: both exact, and so is taking 1024 and 64 off; the
 // constants in vector registers, as one instruction masks and joins then)
@@ -451,6 +455,11 @@ __device__ __forceinline__ u32x4 kv_codes(uint32_t codes) {
         o[i] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, w[i]) + f16x2{off, off});
     }
     return o;
+}
+// The same without taking anything off: halves below the normal ones, code * 2^-24, -20, -24, -20, which the matrix cores take as what they are.
+__device__ __forceinline__ u32x4 kv_tiny(uint32_t codes) {
+    const uint32_t up = codes >> 8;
+    return u32x4{codes & 0x000f000fu, codes & 0x00f000f0u, up & 0x000f000fu, up & 0x00f000f0u};
 }
 __device__ __forceinline__ u32x4 kv_halves(uint32_t codes, uint32_t params) {
     const _Float16 base = __builtin_bit_cast(_Float16, (uint16_t)(params & 0xffffu)), scale = __builtin_bit_cast(_Float16, (uint16_t)(params >> 16));
@@ -476,11 +485,11 @@ __device__ __forceinline__ void kv_words(const uint8_t* p, uint32_t (&w)[4]) {
     for (int i = 0; i < 4; i++) w[i] = x[i];
 }
 
-// A row's power of two: largest |q| into [1, 2), so that halves hold it; 2^24 at most (what halves then lose of a row is 2^-49), so that the scale divided by it stays
-// a normal number.  (0: the row is zero, or holds an infinity or NaN, and stays as it is.)
-__device__ __forceinline__ int kv_row_exp(float most) {
-    const uint32_t e = __float_as_uint(most) >> 23 & 255u;
-    return e == 0 || e == 255 ? 0 : min(127 - (int)e, 24);
+// A row's power of two: largest |q| into [1, 2), so that halves hold it, as long as the scale divided by it stays above 2^-100 (what halves then lose of a row moves no
+// score by 2^-70).  (0: the row holds an infinity or NaN and stays as it is.)
+__device__ __forceinline__ int kv_row_exp(float most, float scale) {
+    const int e = __float_as_uint(most) >> 23 & 255u;
+    return e == 255 ? 0 : min(127 - max(e, 1), (int)(__float_as_uint(scale) >> 23) - 27);
 }
 
 template <typename IT, typename CT, int HD> struct KvRaw16 { // a lane's part of 32 keys: key 16 b + n, elements 32 t + 8 g ..; of V the same
@@ -547,23 +556,28 @@ template <typename IT, int HD> struct KvRaw16<IT, q4_t, HD> { // the same, eleme
 };
 
 template <typename CT> constexpr int kv_few_waves() { return KvType<CT>::code == MLH_CACHE_Q4 ? 4 : 8; }
-template <typename IT, typename CT, int HD>
+template <typename IT, typename CT, int HD, int SP>
 __global__ void __launch_bounds__(kv_few_waves<CT>() * 64, KvType<CT>::code == MLH_CACHE_Q4 ? 3 : 2) k_kvattn_few(KvAttnArgs A) {
     constexpr bool FOUR = KvType<CT>::code == MLH_CACHE_Q4, BF = !FOUR && KvType<IT>::code == MLH_DTYPE_BF16; // products in bf16
     constexpr bool PARTS = kv_in_parts<IT, CT>();
     constexpr int NW = kv_few_waves<CT>(), KS = HD / 32, VB = HD / 16;
+    static_assert(SP == 1 || (FOUR && SP == HD / KV_GROUP), "a column for each group of a row");
     constexpr int VP = HD * 2 + 16; // bytes of a row of V in LDS: four rows start in different banks
     constexpr int LV = NW * 32 * VP, LF = NW * 16 * (HD + 4 + 2) * 4;
     __shared__ __attribute__((aligned(16))) unsigned char lds[LV > LF ? LV : LF];
     __shared__ float odds[NW][HD];
-    const int kh = blockIdx.x % A.kvHeads, split = blockIdx.y, tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, n = lane & 15, g = lane >> 4;
+    __shared__ __attribute__((aligned(16))) uint32_t params[SP > 1 ? NW : 1][SP][36]; // of 32 keys (four more words, so that the groups' rows start in different banks)
+    const int kh = blockIdx.x % A.kvHeads, block = blockIdx.x / A.kvHeads / A.nsplit, split = blockIdx.x / A.kvHeads % A.nsplit;
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, n = lane & 15, g = lane >> 4;
     KvBlock B;
-    if (!kv_block<16>(A, blockIdx.x / A.kvHeads, B)) return;
-    const int r = B.r0 + min(n, B.nr - 1), h = kh * A.group + r % A.group;
+    if (!kv_block<16 / SP>(A, block, B)) return;
+    const int r = B.r0 + min(n / SP, B.nr - 1), h = kh * A.group + r % A.group;
     const KvSight sight(A, B.pos0 + r / A.group);
     // the row, on its way before the first tile and looked at behind it
     u32x4 q[KS], qsum = (u32x4)(0u);
     float scale = A.scale2, x[FOUR ? KS : 1][8];
+    float zero = 0.f;
+    asm volatile("" : "+v"(zero)); // (a product with a half on it is one instruction)
     {
         const IT* qr = (const IT*)A.q + (size_t)(B.row0 + r / A.group) * A.qStride + (size_t)h * HD;
 #pragma unroll
@@ -595,7 +609,22 @@ __global__ void __launch_bounds__(kv_few_waves<CT>() * 64, KvType<CT>::code == M
 #pragma unroll
         for (int b = 0; b < 2; b++) {
             s[b] = (f32x4)(0.f);
-            if constexpr (PARTS) {
+            if constexpr (SP > 1) {
+                const uint32_t own = raw[set].kp[b];
+                params[wave][g * (HD / 4) / KV_GROUP][16 * b + n] = own;
+#pragma unroll
+                for (int t = 0; t < KS; t++) s[b] = mfma16<false>(kv_tiny(raw[set].k[b][t]), q[t], s[b]);
+                const f32x4 base = mfma16<false>(u32x4{(own & 0xffffu) | own << 16, 0u, 0u, 0u}, qsum, (f32x4)(0.f));
+                const u32x4 par = *reinterpret_cast<const u32x4*>(&params[wave][n % SP][16 * b + 4 * g]);
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const uint32_t w = par[e]; // (a bit cast of an element of a vector reads the first)
+                    float v = fmaf(kv_half(w >> 16), s[b][e], zero);
+                    v += kv_neighbour<0xb1>(v);
+                    if constexpr (SP == 4) v += kv_neighbour<0x4e>(v);
+                    s[b][e] = fmaf(v, 1024.f, base[e]);
+                }
+            } else if constexpr (PARTS) {
                 const uint32_t par = raw[set].kp[b], high = par >> 16 & 0xffe0u;
                 const _Float16 low = __builtin_bit_cast(_Float16, (uint16_t)(par >> 16)) - __builtin_bit_cast(_Float16, (uint16_t)high);
                 s[b] = mfma16<false>(u32x4{(par & 0xffffu) | par << 16, 0u, 0u, 0u}, qsum, s[b]);
@@ -628,26 +657,25 @@ __global__ void __launch_bounds__(kv_few_waves<CT>() * 64, KvType<CT>::code == M
                 if (repair) x = kv_without_odd<BF>(x);
                 *reinterpret_cast<u32x4*>(place + 16 * b * VP + (FOUR ? 8 * t : 32 * t) * 2) = x;
             }
-        float p[2][4], mt = m;
-        bool see[2][4];
+        if (!whole) {
+#pragma unroll
+            for (int b = 0; b < 2; b++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) s[b][e] = !sight.sees(j0 + 16 * b + 4 * g + e) ? -INFINITY : page[set] < 0 ? KV_NAN : s[b][e];
+        }
+        float mx = -INFINITY, p[2][4];
 #pragma unroll
         for (int b = 0; b < 2; b++)
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                see[b][e] = whole || sight.sees(j0 + 16 * b + 4 * g + e);
-                p[b][e] = s[b][e] * scale;
-                if (!whole) p[b][e] = !see[b][e] ? -INFINITY : page[set] < 0 ? KV_NAN : p[b][e];
-                mt = kv_max(mt, p[b][e]);
-            }
-        mt = kv_quad_max(mt);
-        const float ref = mt == -INFINITY ? 0.f : mt, corr = kv_exp2(m - ref);
+            for (int e = 0; e < 4; e++) mx = kv_max(mx, s[b][e]);
+        const float mt = fmaxf(m, kv_quad_max(mx) * scale), ref = mt == -INFINITY ? 0.f : mt, corr = kv_exp2(m - ref);
         m = mt;
         l *= corr;
 #pragma unroll
         for (int b = 0; b < 2; b++)
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                p[b][e] = see[b][e] ? kv_exp2(p[b][e] - ref) : 0.f;
+            for (int e = 0; e < 4; e++) { // (hidden: 2^-inf)
+                p[b][e] = kv_exp2(fmaf(s[b][e], scale, -ref));
                 l += p[b][e];
             }
         if (__any(corr != 1.f)) { // (a maximum that moves gets rare)
@@ -709,17 +737,26 @@ __global__ void __launch_bounds__(kv_few_waves<CT>() * 64, KvType<CT>::code == M
         for (int t = 0; t < KS; t++)
 #pragma unroll
             for (int i = 0; i < 8; i++) most = fmaxf(most, fabsf(x[t][i]));
-        const int e = kv_row_exp(kv_quad_max(most));
+        const int e = kv_row_exp(kv_quad_max(most), A.scale2);
+        float sum = 0.f;
+#pragma unroll
+        for (int t = 0; t < KS; t++) sum += ((x[t][0] + x[t][1]) + (x[t][2] + x[t][3])) + ((x[t][4] + x[t][5]) + (x[t][6] + x[t][7]));
+        sum = ldexpf(sum, e);
         scale = ldexpf(scale, -e);
+        if constexpr (SP > 1) {
+            // column n: this row's elements of group n % SP, zeros elsewhere; largest into [2^14, 2^15), that of the odd words 2^-4 of it; the product is 2^-10 of the sum then
+            const bool own = g * (HD / 4) / KV_GROUP == n % SP;
 #pragma unroll
-        for (int t = 0; t < KS; t++)
+            for (int t = 0; t < KS; t++)
 #pragma unroll
-            for (int i = 0; i < 4; i++) q[t][i] = pack_f16(ldexpf(x[t][i], e), ldexpf(x[t][i + 4], e));
-        if constexpr (PARTS) {
-            float sum = 0.f;
+                for (int i = 0; i < 4; i++) q[t][i] = own ? pack_f16(ldexpf(x[t][i], e + (i & 1 ? 10 : 14)), ldexpf(x[t][i + 4], e + (i & 1 ? 10 : 14))) : 0u;
+        } else {
 #pragma unroll
-            for (int t = 0; t < KS; t++) sum += ((x[t][0] + x[t][1]) + (x[t][2] + x[t][3])) + ((x[t][4] + x[t][5]) + (x[t][6] + x[t][7]));
-            sum = ldexpf(sum, e);
+            for (int t = 0; t < KS; t++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) q[t][i] = pack_f16(ldexpf(x[t][i], e), ldexpf(x[t][i + 4], e));
+        }
+        if constexpr (SP > 1 || PARTS) {
             const uint32_t first = kv_to_half(sum);
             qsum.x = first | kv_to_half(sum - kv_half(first)) << 16;
         }
@@ -739,12 +776,13 @@ __global__ void __launch_bounds__(kv_few_waves<CT>() * 64, KvType<CT>::code == M
     }
     l = kv_quad_sum(l);
     __syncthreads(); // the waves' V tiles become the place where they meet
-    kv_finish16<IT, HD, NW>(A, B, kh, split, acc, m, l, reinterpret_cast<float*>(lds), [&](auto put) {
+    kv_finish16<IT, HD, NW, SP>(A, B, kh, split, acc, m, l, reinterpret_cast<float*>(lds), [&](auto put) {
+        if (n % SP != 0) return;
 #pragma unroll
         for (int b = 0; b < VB; b++) {
             if constexpr (!FOUR) put(16 * b + 4 * g, acc[b]);
             else { // columns (0, 4, 1, 5) or (2, 6, 3, 7) of every eight
-                float* f = reinterpret_cast<float*>(lds) + ((size_t)wave * 16 + n) * (HD + 4) + 16 * b + 8 * (g >> 1) + 2 * (g & 1);
+                float* f = reinterpret_cast<float*>(lds) + ((size_t)wave * 16 + n / SP) * (HD + 4) + 16 * b + 8 * (g >> 1) + 2 * (g & 1);
                 f[0] = acc[b].x; f[4] = acc[b].y; f[1] = acc[b].z; f[5] = acc[b].w;
             }
         }
@@ -803,7 +841,7 @@ __global__ void __launch_bounds__(NW * 64, HD == 64 ? 3 : 2) k_kvattn_many(KvAtt
                 }
                 most = fmaxf(most, __shfl_xor(most, 32, 64));
             }
-            const int e = kv_row_exp(most);
+            const int e = KvType<IT>::code == MLH_DTYPE_BF16 ? kv_row_exp(most, A.scale2) : 0;
             scale = ldexpf(scale, -e);
 #pragma unroll
             for (int t = 0; t < KS; t++) {
@@ -1118,6 +1156,7 @@ static std::string attn_check(const mlh_kv_cache* c, const mlh_kv_batch* b, cons
 #endif
 struct AttnPlan {         // which kernel, and how the keys are split
     int many;             // waves of a workgroup of k_kvattn_many; 0: the kernels of 16 rows
+    int rowsPer;          // rows of a workgroup
     int blocks, nsplit;
     long long wgs;        // workgroups with rows, per split
     size_t bytes;
@@ -1129,9 +1168,11 @@ static AttnPlan attn_plan(const mlh_kv_cache* c, const mlh_kv_batch* b, const ml
     const long long maxLen = a->maxLen ? std::min<long long>(a->maxLen, cap) : cap;
     const long long maxNew = a->maxNew ? std::min(a->maxNew, b->rows) : b->rows;
     P.many = b->type != MLH_DTYPE_F32 && maxNew * group > 64 ? 4 : 0;
-    const int qb = P.many ? P.many * 32 : 16;
-    P.blocks = (int)(rows / qb + c->nseq);
-    P.wgs = std::min<long long>(P.blocks, (rows + qb - 1) / qb + std::min(c->nseq, b->rows) - 1) * c->heads;
+    const int spread = 16 * KV_GROUP / c->headDim; // rows that leave a column for each of their groups
+    P.rowsPer = P.many ? P.many * 32 : c->type == MLH_CACHE_Q4 && b->type != MLH_DTYPE_F32 && maxNew * group <= spread ? spread : 16;
+    const int qb = P.rowsPer;
+    P.blocks = (int)((rows + qb - 1) / qb + c->nseq - 1); // (floor(a) + ceil(b) <= ceil(a + b))
+    P.wgs = ((rows + qb - 1) / qb + std::min(c->nseq, b->rows) - 1) * c->heads;
     // positions that a row sees, in turns of a workgroup (eight waves of 32 keys, or a page)
     const long long seen = a->window ? std::min<long long>(maxLen, (long long)a->window + std::min<long long>(a->sinks, maxLen) + 64) : maxLen;
     const int turn = P.many ? 64 : 256;
@@ -1185,7 +1226,7 @@ extern "C" int mlh_attention_device(const mlh_kv_cache* c, const mlh_kv_batch* b
     const int hd = c->headDim;
     const KvAttnArgs A = {c->k, c->v, c->table, b->start, b->len, a->q, a->out, (float*)a->work, a->qStride, a->outStride, c->nseq, b->rows, b->heads, c->heads, b->heads / c->heads,
                           c->pagesPerSeq, c->numPages, a->window, a->sinks, P.nsplit, (a->scale > 0.f ? a->scale : 1.0f / sqrtf((float)hd)) * 1.44269504088896341f};
-    const dim3 grid(c->heads * P.blocks, P.nsplit);
+    const dim3 grid = P.many ? dim3(c->heads * P.blocks, P.nsplit) : dim3(c->heads * P.blocks * P.nsplit);
     hipStream_t st = (hipStream_t)stream;
     if (P.many) {
         hipError_t e;
@@ -1207,11 +1248,17 @@ extern "C" int mlh_attention_device(const mlh_kv_cache* c, const mlh_kv_batch* b
     } else {
 #define FEW(IT_, CT_) \
     do { \
-        if (hd == 64) hipLaunchKernelGGL((k_kvattn_few<IT_, CT_, 64>), grid, dim3(kv_few_waves<CT_>() * 64), 0, st, A); \
-        else hipLaunchKernelGGL((k_kvattn_few<IT_, CT_, 128>), grid, dim3(kv_few_waves<CT_>() * 64), 0, st, A); \
+        if (hd == 64) hipLaunchKernelGGL((k_kvattn_few<IT_, CT_, 64, SP64>), grid, dim3(kv_few_waves<CT_>() * 64), 0, st, A); \
+        else hipLaunchKernelGGL((k_kvattn_few<IT_, CT_, 128, SP64 * SP64>), grid, dim3(kv_few_waves<CT_>() * 64), 0, st, A); \
     } while (0)
-        if (b->type == MLH_DTYPE_BF16) { if (c->type == MLH_CACHE_Q4) FEW(bf16_t, q4_t); else FEW(bf16_t, bf16_t); }
-        else { if (c->type == MLH_CACHE_Q4) FEW(f16_t, q4_t); else FEW(f16_t, f16_t); }
+        if (c->type == MLH_CACHE_Q4 && P.rowsPer < 16) {
+            constexpr int SP64 = 2; // (4 for heads of 128)
+            if (b->type == MLH_DTYPE_BF16) FEW(bf16_t, q4_t); else FEW(f16_t, q4_t);
+        } else {
+            constexpr int SP64 = 1;
+            if (b->type == MLH_DTYPE_BF16) { if (c->type == MLH_CACHE_Q4) FEW(bf16_t, q4_t); else FEW(bf16_t, bf16_t); }
+            else { if (c->type == MLH_CACHE_Q4) FEW(f16_t, q4_t); else FEW(f16_t, f16_t); }
+        }
 #undef FEW
     }
     if (const int rc = kv_launched()) return rc;

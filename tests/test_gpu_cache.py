@@ -277,6 +277,14 @@ def test_hints_decide_nothing_else(pkg, kind, cache):
             c.check()
 
 
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("kind,spread,scale", [("bf16", 1e30, 1e-30), ("bf16", 1e-25, 1e24), ("bf16", 3e4, 1e-5), ("f16", 1.2e4, 1e-5), ("f16", 1e-5, 1e4)])
+def test_sizes_of_rows(pkg, kind, spread, scale, hd):
+    """4-bit pages: rows far from one, large and small, with a scale that brings the scores back (they leave for powers of two and return)."""
+    for new, lens in (([1, 1], [300, 65]), ([5], [200]), ([70], [100])):
+        Call(pkg, kind, "q4", 2, 1, hd, new, lens, seed=23, spread=spread, scale=scale).check()
+
+
 @pytest.mark.parametrize("kind,cache", KINDS)
 @pytest.mark.parametrize("new,lens", [([3, 1], [90, 200]), ([150], [200])])
 def test_nonfinite_rows(pkg, kind, cache, new, lens):
