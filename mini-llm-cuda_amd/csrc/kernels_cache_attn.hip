@@ -264,9 +264,10 @@ template <int HD> struct KvTile32<q4_t, HD> {
     }
 };
 
-template <typename CT, int HD, int NW>
-__global__ void __launch_bounds__(NW * 64, 2) k_kvattn_f32(KvAttnArgs A) {
-    constexpr int KC = HD / 4, VB = HD / 16;
+#define KV_F32_WAVES 4
+template <typename CT, int HD>
+__global__ void __launch_bounds__(KV_F32_WAVES * 64, 2) k_kvattn_f32(KvAttnArgs A) {
+    constexpr int NW = KV_F32_WAVES, KC = HD / 4, VB = HD / 16;
     __shared__ __attribute__((aligned(16))) float lds[NW * 16 * (HD + 4 + 2)];
     __shared__ float odds[NW][HD];
     const int kh = blockIdx.x % A.kvHeads, block = blockIdx.x / A.kvHeads / A.nsplit, split = blockIdx.x / A.kvHeads % A.nsplit;
@@ -555,13 +556,13 @@ template <typename IT, int HD> struct KvRaw16<IT, q4_t, HD> { // the same, eleme
     __device__ __forceinline__ u32x4 val(int b, int t) const { return kv_halves(v[b][t], vp[b]); }
 };
 
-template <typename CT> constexpr int kv_few_waves() { return KvType<CT>::code == MLH_CACHE_Q4 ? 4 : 8; }
+#define KV_FEW_WAVES 4
 template <typename IT, typename CT, int HD, int SP>
-__global__ void __launch_bounds__(kv_few_waves<CT>() * 64, KvType<CT>::code == MLH_CACHE_Q4 ? 3 : 2) k_kvattn_few(KvAttnArgs A) {
+__global__ void __launch_bounds__(KV_FEW_WAVES * 64, KvType<CT>::code == MLH_CACHE_Q4 ? 3 : 2) k_kvattn_few(KvAttnArgs A) {
     constexpr bool FOUR = KvType<CT>::code == MLH_CACHE_Q4, BF = !FOUR && KvType<IT>::code == MLH_DTYPE_BF16; // products in bf16
     constexpr bool PARTS = kv_in_parts<IT, CT>();
-    constexpr int NW = kv_few_waves<CT>(), KS = HD / 32, VB = HD / 16;
-    static_assert(SP == 1 || (FOUR && SP == HD / KV_GROUP), "a column for each group of a row");
+    constexpr int NW = KV_FEW_WAVES, KS = HD / 32, VB = HD / 16;
+    static_assert(SP == 1 || (PARTS && SP == HD / KV_GROUP), "a column for each group of a row");
     constexpr int VP = HD * 2 + 16; // bytes of a row of V in LDS: four rows start in different banks
     constexpr int LV = NW * 32 * VP, LF = NW * 16 * (HD + 4 + 2) * 4;
     __shared__ __attribute__((aligned(16))) unsigned char lds[LV > LF ? LV : LF];
@@ -1147,13 +1148,15 @@ static std::string attn_check(const mlh_kv_cache* c, const mlh_kv_batch* b, cons
     return "";
 }
 
-#define KV_SPLIT_WGS 2048 // the kernels of 16 rows: keys are split until a call has this many workgroups, eight a compute unit
-#ifndef KV_SPLIT_MANY
-#define KV_SPLIT_MANY 1024 // k_kvattn_many: four
-#endif
-#ifndef KV_WIDE_WGS
-#define KV_WIDE_WGS 256
-#endif
+// Which kernel (32 query heads on 8, heads of 128, 4000 positions; "rows" are a sequence's, over heads of one K/V head):
+//   16-bit pages, from 17 rows on k_kvattn_many: 16 sequences of 16, 32, 64 rows 53, 57, 73 us, k_kvattn_few 67, 111, 174; of one sequence 15, 16, 17 and 18, 19, 19.
+//     Single tokens (16 rows at most): k_kvattn_few, @FEW1@
+//   4-bit pages, from 65 on: 16 sequences of 32, 64, 96 rows 53, 69, 77 us, k_kvattn_few 44, 68, 95 (it makes halves of codes in the registers that use them).
+//   4-bit pages, fp16 rows that leave a column for each of their groups: k_kvattn_few spread over columns (4000 positions of 48 sequences, 16 heads: 112 us, 125 without).
+// How keys are split, a second kernel joining the shares:
+#define KV_SPLIT_WGS 2048 // the kernels of 16 rows: until a call has this many workgroups (64 tokens over up to 12000 positions: 307 us; 768: 320, 1280: 312, 3072: 314, 4096: 329)
+#define KV_SPLIT_MANY 1024 // k_kvattn_many: the same (512 to 3000: no difference within 3 of 118 us) ...
+#define KV_SPLIT_LEAST 8   // ... of at least eight tiles each, four until each compute unit has a workgroup (one sequence, 32 rows: 16 us, 21 with eight; two: 14, but 512 rows 44 for 32)
 struct AttnPlan {         // which kernel, and how the keys are split
     int many;             // waves of a workgroup of k_kvattn_many; 0: the kernels of 16 rows
     int rowsPer;          // rows of a workgroup
@@ -1167,17 +1170,18 @@ static AttnPlan attn_plan(const mlh_kv_cache* c, const mlh_kv_batch* b, const ml
     const long long cap = (long long)c->pagesPerSeq * MLH_KV_PAGE, rows = (long long)b->rows * group;
     const long long maxLen = a->maxLen ? std::min<long long>(a->maxLen, cap) : cap;
     const long long maxNew = a->maxNew ? std::min(a->maxNew, b->rows) : b->rows;
-    P.many = b->type != MLH_DTYPE_F32 && maxNew * group > 64 ? 4 : 0;
+    P.many = b->type != MLH_DTYPE_F32 && maxNew * group > (c->type == MLH_CACHE_Q4 ? 64 : 16) ? 4 : 0;
     const int spread = 16 * KV_GROUP / c->headDim; // rows that leave a column for each of their groups
-    P.rowsPer = P.many ? P.many * 32 : c->type == MLH_CACHE_Q4 && b->type != MLH_DTYPE_F32 && maxNew * group <= spread ? spread : 16;
+    P.rowsPer = P.many ? P.many * 32 : c->type == MLH_CACHE_Q4 && b->type == MLH_DTYPE_F16 && maxNew * group <= spread ? spread : 16;
     const int qb = P.rowsPer;
     P.blocks = (int)((rows + qb - 1) / qb + c->nseq - 1); // (floor(a) + ceil(b) <= ceil(a + b))
     P.wgs = ((rows + qb - 1) / qb + std::min(c->nseq, b->rows) - 1) * c->heads;
-    // positions that a row sees, in turns of a workgroup (eight waves of 32 keys, or a page)
+    // positions that a row sees, in turns of a workgroup (four waves of 32 keys, or a page)
     const long long seen = a->window ? std::min<long long>(maxLen, (long long)a->window + std::min<long long>(a->sinks, maxLen) + 64) : maxLen;
-    const int turn = P.many ? 64 : 256;
+    const int turn = P.many ? 64 : 128;
     const long long rounds = (seen + turn - 1) / turn;
-    const long long n = P.many ? std::min<long long>((KV_SPLIT_MANY + P.wgs - 1) / P.wgs, rounds / 8) : std::min<long long>((KV_SPLIT_WGS + P.wgs - 1) / P.wgs, (rounds + 1) / 2);
+    auto each = [&](long long most) { return (most + P.wgs - 1) / P.wgs; };
+    const long long n = P.many ? std::min(each(KV_SPLIT_MANY), std::max(rounds / KV_SPLIT_LEAST, std::min(rounds / (KV_SPLIT_LEAST / 2), each(256)))) : std::min(each(KV_SPLIT_WGS), std::max(rounds / 4, std::min(rounds / 2, each(256))));
     P.nsplit = (int)std::max<long long>(1, std::min<long long>(n, KV_MAX_SPLIT));
     P.bytes = P.nsplit > 1 ? (size_t)P.nsplit * b->rows * b->heads * (c->headDim + 2) * 4 : 0;
     return P;
@@ -1236,24 +1240,19 @@ extern "C" int mlh_attention_device(const mlh_kv_cache* c, const mlh_kv_batch* b
 #undef MANY
         if (e != hipSuccess) { mlh_set_thread_error(std::string("launch failed: ") + hipGetErrorString(e)); return -2; }
     } else if (b->type == MLH_DTYPE_F32) {
-#define F32_ROWS(CT_, NW_) \
-    do { \
-        if (hd == 64) hipLaunchKernelGGL((k_kvattn_f32<CT_, 64, NW_>), grid, dim3(NW_ * 64), 0, st, A); \
-        else hipLaunchKernelGGL((k_kvattn_f32<CT_, 128, NW_>), grid, dim3(NW_ * 64), 0, st, A); \
-    } while (0)
-        const bool wide = P.wgs * P.nsplit <= KV_WIDE_WGS; // eight waves a workgroup while that leaves a compute unit one of them
-        if (c->type == MLH_CACHE_Q4) { if (wide) F32_ROWS(q4_t, 8); else F32_ROWS(q4_t, 4); }
-        else { if (wide) F32_ROWS(float, 8); else F32_ROWS(float, 4); }
+#define F32_ROWS(CT_, HD_) hipLaunchKernelGGL((k_kvattn_f32<CT_, HD_>), grid, dim3(KV_F32_WAVES * 64), 0, st, A)
+        if (c->type == MLH_CACHE_Q4) { if (hd == 64) F32_ROWS(q4_t, 64); else F32_ROWS(q4_t, 128); }
+        else { if (hd == 64) F32_ROWS(float, 64); else F32_ROWS(float, 128); }
 #undef F32_ROWS
     } else {
 #define FEW(IT_, CT_) \
     do { \
-        if (hd == 64) hipLaunchKernelGGL((k_kvattn_few<IT_, CT_, 64, SP64>), grid, dim3(kv_few_waves<CT_>() * 64), 0, st, A); \
-        else hipLaunchKernelGGL((k_kvattn_few<IT_, CT_, 128, SP64 * SP64>), grid, dim3(kv_few_waves<CT_>() * 64), 0, st, A); \
+        if (hd == 64) hipLaunchKernelGGL((k_kvattn_few<IT_, CT_, 64, SP64>), grid, dim3(KV_FEW_WAVES * 64), 0, st, A); \
+        else hipLaunchKernelGGL((k_kvattn_few<IT_, CT_, 128, SP64 * SP64>), grid, dim3(KV_FEW_WAVES * 64), 0, st, A); \
     } while (0)
-        if (c->type == MLH_CACHE_Q4 && P.rowsPer < 16) {
+        if (P.rowsPer < 16) {
             constexpr int SP64 = 2; // (4 for heads of 128)
-            if (b->type == MLH_DTYPE_BF16) FEW(bf16_t, q4_t); else FEW(f16_t, q4_t);
+            FEW(f16_t, q4_t);
         } else {
             constexpr int SP64 = 1;
             if (b->type == MLH_DTYPE_BF16) { if (c->type == MLH_CACHE_Q4) FEW(bf16_t, q4_t); else FEW(bf16_t, bf16_t); }
