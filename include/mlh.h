@@ -391,7 +391,7 @@ typedef struct {
 uint64_t mlh_kv_page_bytes(int type, int heads, int headDim);
 
 /* The rows of a call: sequence s brings rows start[s] .. start[s + 1] - 1 (none, one or many), the last of them at position len[s] - 1.
- * start does not decrease and begins at 0.  Rows at and behind start[nseq] are neither read nor written.  A row is `heads` (q, out) or cache.heads (k, v) heads of
+ * start does not decrease and begins at 0.  Rows at and behind start[nseq] are left as they are.  A row is `heads` (q, out) or cache.heads (k, v) heads of
  * headDim elements, rows `stride` elements apart; pointers and strides are multiples of 16 bytes. */
 typedef struct {
     const int32_t* start; /* [nseq + 1] */
@@ -432,9 +432,12 @@ int mlh_kv_read_device(const mlh_kv_cache* cache, const mlh_kv_batch* batch, con
  * with window > 0, p - j < window or j < sinks.  out = sum over those of softmax(scale * q . k) v (inference.cu:136-239); zeros for a row that sees
  * nothing.  Keys that a row does not see do not count for it, whatever they hold (infinities and NaN too); pages no row sees are not read, so their table entries may be
  * stale.  A row that sees a position beyond the page table or in a page outside the pool is NaN.
- * Scores, softmax statistics and sums are fp32; with rows of 16 bits the weights are rounded to the rows' type for the product with v, and values of 4-bit
- * pages to halves (bf16 rows: to bf16) for both products, finite ones.
- * maxLen, maxNew: what no len and no number of rows of a sequence exceeds (0: the page table's, rows).  They decide how the work is split and nothing else.
+ * Scores, softmax statistics and sums are fp32, and with fp32 rows everything is.  With rows of 16 bits over pages of the same type the weights are rounded to it for the product
+ * with v.  Over 4-bit pages both products are of halves: v's values and the weights are rounded to them, q times a power of two (exactly, but for what is 2^-24 of its row's
+ * largest), and k's values, except in calls of fp16 rows whose maxNew * heads / cache.heads is at most 64: these take k as it is and the weights to 22 bits.
+ * Values of 4-bit pages beyond the halves' range count as infinite with rows of 16 bits; a group whose scale is an infinity or NaN counts as NaN or infinite.
+ * maxLen, maxNew: what no len and no number of rows of a sequence exceeds (0: the page table's, rows).  They decide which kernel runs and how the work is split; a call that
+ * exceeds them is right, and slower.
  * work: mlh_attention_work_bytes() bytes (of the same structures; 0: none), 16-byte aligned, undefined before and after, not shared by calls that may overlap. */
 typedef struct {
     const void* q;

@@ -1,7 +1,7 @@
 // Attention over a caller's paged K/V cache (mlh_attention_device): causal, with a sliding window and first positions that stay visible, over pages of 32, 16 or 4
 // bits.  Three kernels and one that joins:
 //   k_kvattn_f32   rows in fp32, 16 of them a workgroup, on the fp32 matrix cores
-//   k_kvattn_few   rows in 16 bits, few a sequence (single tokens): 16 a workgroup, its waves take key tiles in turn
+//   k_kvattn_few   rows in 16 bits, few a sequence (single tokens): 16 a workgroup (4 or 8 over 4-bit pages, a column for each group), its waves take key tiles in turn
 //   k_kvattn_many  rows in 16 bits, many a sequence (prompts): 32 a wave, key tiles through LDS
 //   k_kvattn_join  the shares of workgroups that split a sequence's keys
 //
@@ -187,6 +187,8 @@ __device__ __forceinline__ void kv_finish16(const KvAttnArgs& A, const KvBlock& 
 // lane 16 g + n holds elements [g HD/4, (g + 1) HD/4) of key n (the order of a contraction is free), the product leaves it the scores of keys 4 g .. 4 g + 3 of row n,
 // which is the second product's operand as it stands; row m of V's operand of block b is element m HD/16 + b.  The waves take tiles of 16 keys in turn, the next tile's loads
 // go out before this one's products.
+// Three sequences of 100, 308 and 517 rows, 6 heads of 128, window 200: 19 us, of which 4 are products (348 workgroups on 256 compute units: what a workgroup waits for,
+// start, page, first tile, bounds it).  One token over 256 positions of 12 heads of 64: 8 us, the same latencies.  Eight waves a workgroup: 24 and 8 us.
 // ----------------------------------------------------------------------------
 // Keeps a lane's 32-bit offset one: widened outside of the loop, it would be added to each page's base in vector registers, and these wait for the loads that use them.
 __device__ __forceinline__ void kv_offset(unsigned& o) { asm volatile("" : "+v"(o)); }
@@ -404,8 +406,11 @@ __global__ void __launch_bounds__(KV_F32_WAVES * 64, 2) k_kvattn_f32(KvAttnArgs 
 // ----------------------------------------------------------------------------
 // Few 16-bit rows of a sequence.  A wave takes 32 keys at a time: S^T[key, row] = K . Q^T on 16x16x32 products, K from the pages straight into registers; V's
 // rows go through the wave's own piece of LDS, which hands them back transposed (ds_read_b64_tr_b16: lane i of 16 gets column i of four rows), so that
-// O^T += V^T . P^T takes the weights from the registers that the first product left them in.  4-bit pages: codes become halves on the way (exact: the values
-// are minimum + code * scale in halves, one rounding), all products are in halves, and bf16 rows are scaled by a power of two first.
+// O^T += V^T . P^T takes the weights from the registers that the first product left them in.  4-bit pages: codes become halves on the way (the values
+// are minimum + code * scale in halves, one rounding), all products are in halves, and rows are scaled by a power of two first.
+// 16-bit pages are bound by memory: 64 tokens over 100 to 12000 positions, 32 heads on 8 of 128 in bf16, 1.59 GB, 316 us (5.0 TB/s; reads alone reach 6.1); 64 over 3000
+// each 156 us.  Eight waves a workgroup: 307 and 170, one token over 4000 17 for 12.  4-bit pages by the instructions that unpack them: one token over 65000 positions, bf16,
+// 21 us (83 MB, 3.9 TB/s); eight waves a workgroup: 146 us for 116 (48 tokens, before the spread below).
 // ----------------------------------------------------------------------------
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
@@ -517,7 +522,7 @@ template <typename IT, typename CT, int HD> struct KvRaw16 { // a lane's part of
     __device__ __forceinline__ u32x4 key(int b, int t) const { return k[b][t]; }
     __device__ __forceinline__ u32x4 val(int b, int t) const { return v[b][t]; }
 };
-// Rows in halves over 4-bit pages: rounding K's values to halves costs such rows more than all else together, so that they are multiplied as what they are, minimum +
+// Rows in halves over 4-bit pages (16 rows a workgroup): rounding K's values to halves costs such rows more than all else together, so that they are multiplied as what they are, minimum +
 // (high + low part of the scale) * code: parts of six and five bits times a code of four are exact in halves, two products instead of one, and the minima meet the sum of
 // the row's elements (as two halves) in one product more.  The weights are two halves as well.  (Error of a result, normal values, 4000 keys, against its norm: 4.4e-4 with
 // K, V and weights each rounded to halves, 2.8e-4 so, 2.1e-4 the rounding of the result alone.)  Rows in bf16 round their results eight times as far.
@@ -556,6 +561,10 @@ template <typename IT, int HD> struct KvRaw16<IT, q4_t, HD> { // the same, eleme
     __device__ __forceinline__ u32x4 val(int b, int t) const { return kv_halves(v[b][t], vp[b]); }
 };
 
+// SP > 1 (fp16 rows over 4-bit pages, at most 16 / SP of them a sequence): column n of the first product is row n / SP with the elements of group n % SP alone.  A sum's codes
+// then share minimum and scale: codes go in as they are (kv_tiny), the scale is one multiplication a key and group in fp32 behind them, exact where the 16-row form
+// needs two products, and the groups' sums meet in the neighbouring columns.  The minima meet the row's sums of elements in one product more.
+// 48 tokens over up to 9000 positions, window 4096, 16 heads of 128, 389 MB: 87 us (4.5 TB/s), 104 in the 16-row form (bf16 rows, whose 16-row form has one product: 108 us spread, 104 not).
 #define KV_FEW_WAVES 4
 template <typename IT, typename CT, int HD, int SP>
 __global__ void __launch_bounds__(KV_FEW_WAVES * 64, KvType<CT>::code == MLH_CACHE_Q4 ? 3 : 2) k_kvattn_few(KvAttnArgs A) {
@@ -794,7 +803,12 @@ __global__ void __launch_bounds__(KV_FEW_WAVES * 64, KvType<CT>::code == MLH_CAC
 // Many 16-bit rows of a sequence: 32 a wave, NW waves a workgroup, a page (64 keys) at a time through LDS, double-buffered.  S^T[key, row] = K . Q^T on 32x32x16
 // products: every lane owns one row (element i of lane l: key 8 (i / 4) + 4 (l / 32) + i % 4, row l % 32), so maximum and sum run down registers, with one
 // exchange between the lane halves; O^T += V^T . P^T takes the weights as they lie and V through the transposing LDS read.  Pages of 16 bits go straight to LDS
-// (the 16-byte pieces of a row in an order that keeps both readings free of bank conflicts), those of 4 bits through registers, where codes become halves.
+// (the 16-byte pieces of a row in an order that keeps both readings free of bank conflicts), those of 4 bits through registers, where codes become halves; fp16 rows too
+// meet K and V rounded to halves here (error against the result's norm 4.4e-4, 2.1e-4 the rounding of the result).
+// Bound by the matrix cores at the clock that their power leaves (1.8 GHz) and the vector ALU's exponentials between them: 16384 rows, 32 heads of 128 in fp16, window 4096
+// 1.10 ms, 0.89 PFLOP/s of what is seen (a library product of 8192 cubed: 1.05).  Eight prompts of 2048, window 1024: 0.17 ms, 0.61 PFLOP/s: of 19 tiles that a
+// workgroup's rows touch 16 are seen whole, and every workgroup starts with a lookup and a tile that nothing hides.  1289 rows behind 3000 to 7000 positions in 4 bits, heads
+// of 64: 108 us, 0.48 PFLOP/s (an exponential and its conversion for every 256 operations of the products).
 // ----------------------------------------------------------------------------
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 template <bool BF> __device__ __forceinline__ float kv_add2(uint32_t w, float sum) { // two 16-bit numbers onto a sum
@@ -1064,6 +1078,7 @@ __global__ void __launch_bounds__(NW * 64, HD == 64 ? 3 : 2) k_kvattn_many(KvAtt
 // ----------------------------------------------------------------------------
 // The shares of nsplit workgroups of a row and head: a lane a share for the factors, 256 / (HD / 4) groups of threads for the sums.
 // ----------------------------------------------------------------------------
+// (2048 rows of 16 shares: 4.8 us, latency)
 #define KV_MAX_SPLIT 64
 template <typename IT, int HD>
 __global__ void __launch_bounds__(256) k_kvattn_join(KvAttnArgs A) {
@@ -1099,7 +1114,7 @@ __global__ void __launch_bounds__(256) k_kvattn_join(KvAttnArgs A) {
     kv_put4((IT*)A.out + (size_t)row * A.outStride + (size_t)h * HD + 4 * t, o);
 }
 
-// The same of few shares (KV_JOIN_FEW at most): a thread for four elements.
+// The same of few shares (KV_JOIN_FEW at most): a thread for four elements.  (41248 rows of 4 shares of 64: 9 us, 4.6 TB/s; k_kvattn_join 43.)
 #define KV_JOIN_FEW 8
 template <typename IT, int HD>
 __global__ void __launch_bounds__(256) k_kvattn_join_few(KvAttnArgs A) {
@@ -1148,13 +1163,15 @@ static std::string attn_check(const mlh_kv_cache* c, const mlh_kv_batch* b, cons
     return "";
 }
 
-// Which kernel (32 query heads on 8, heads of 128, 4000 positions; "rows" are a sequence's, over heads of one K/V head):
-//   16-bit pages, from 17 rows on k_kvattn_many: 16 sequences of 16, 32, 64 rows 53, 57, 73 us, k_kvattn_few 67, 111, 174; of one sequence 15, 16, 17 and 18, 19, 19.
-//     Single tokens (16 rows at most): k_kvattn_few, @FEW1@
-//   4-bit pages, from 65 on: 16 sequences of 32, 64, 96 rows 53, 69, 77 us, k_kvattn_few 44, 68, 95 (it makes halves of codes in the registers that use them).
-//   4-bit pages, fp16 rows that leave a column for each of their groups: k_kvattn_few spread over columns (4000 positions of 48 sequences, 16 heads: 112 us, 125 without).
+// Which kernel (32 query heads on 8, heads of 128, bf16, 4000 positions; "rows" are a sequence's, over the heads of one K/V head):
+//   16-bit pages: k_kvattn_many from 17 rows on.  16 sequences of 4, 16, 32, 64 rows: k_kvattn_few 49, 59, 111, 174 us, k_kvattn_many 50, 53, 57, 73; one sequence: 12, 12, 19, 19
+//     and 15, 15, 16, 18; 64 of 4 rows over 100 to 12000 positions: 316 and 377 (it splits less).
+//   4-bit pages: from 65 on.  16 sequences of 32, 64, 96 rows: k_kvattn_few 44, 68, 95 us, k_kvattn_many 53, 69, 77 (its tiles pass through LDS as halves).
+//   fp16 rows over 4-bit pages that leave a column for each of their groups: spread (above).
 // How keys are split, a second kernel joining the shares:
-#define KV_SPLIT_WGS 2048 // the kernels of 16 rows: until a call has this many workgroups (64 tokens over up to 12000 positions: 307 us; 768: 320, 1280: 312, 3072: 314, 4096: 329)
+#define KV_SPLIT_WGS 2048 // k_kvattn_few, k_kvattn_f32: until a call has this many workgroups of at least four turns each, or two until each compute unit has one
+                          // (64 tokens over 100 to 12000, 64 over 3000 positions: 316, 156 us; 1024: 332, 151; 3072: 314, 160; 4096: 312, 164; four turns always: one token
+                          // over 4000 15 us for 12; two always: 64 over 300 30 for 17)
 #define KV_SPLIT_MANY 1024 // k_kvattn_many: the same (512 to 3000: no difference within 3 of 118 us) ...
 #define KV_SPLIT_LEAST 8   // ... of at least eight tiles each, four until each compute unit has a workgroup (one sequence, 32 rows: 16 us, 21 with eight; two: 14, but 512 rows 44 for 32)
 struct AttnPlan {         // which kernel, and how the keys are split
@@ -1176,7 +1193,7 @@ static AttnPlan attn_plan(const mlh_kv_cache* c, const mlh_kv_batch* b, const ml
     const int qb = P.rowsPer;
     P.blocks = (int)((rows + qb - 1) / qb + c->nseq - 1); // (floor(a) + ceil(b) <= ceil(a + b))
     P.wgs = ((rows + qb - 1) / qb + std::min(c->nseq, b->rows) - 1) * c->heads;
-    // positions that a row sees, in turns of a workgroup (four waves of 32 keys, or a page)
+    // positions that a row sees, in turns of a workgroup: four waves of 32 keys, or a page
     const long long seen = a->window ? std::min<long long>(maxLen, (long long)a->window + std::min<long long>(a->sinks, maxLen) + 64) : maxLen;
     const int turn = P.many ? 64 : 128;
     const long long rounds = (seen + turn - 1) / turn;

@@ -309,6 +309,18 @@ def test_single_launch_shapes(pkg):
     assert dev.single_launch_sequences() == 0 and dev.decode_route(1) == pkg.DECODE_ROWS
     dev.set_attention_window(0)
     assert dev.single_launch_sequences() == n and dev.decode_route(1) == route
+    other = pkg.Device(hp, 0)  # the pages are new ones: every route finds them
+    other.upload(_model(pkg, hp))
+    tokens = np.arange(50, dtype=np.int32)
+    for mode in (3, 0):
+        got = []
+        for d in (dev, other):
+            d.set_persistent(mode)
+            d.reset()
+            d.prefill_batch([0, 1], [tokens, tokens[:9]])
+            got.append((d.decode_loop([3, 4], 12), d.decode_loop([3], 12), d.logits(0)))
+        assert all(np.array_equal(a, b) for a, b in zip(*got)), mode
+    other.close()
     dev.close()
 
 
