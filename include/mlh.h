@@ -409,7 +409,7 @@ typedef struct {
  * (x - minimum) / scale in 0 .. 15 (ties to even; scale 0: code 0); minima beyond the halves' range count as their largest, and a group with an infinity or NaN, or whose scale is
  * beyond that range, reads back as NaN.
  * q may be null (with qOut); qOut may be q with the same stride.  A row whose position is negative, beyond the page table or the rope table, or in a page outside
- * the pool stores nothing, and its qOut is NaN.  Two rows of a call that share a place leave one of the two. */
+ * the pool stores nothing, and its qOut is NaN.  Two rows of a call that share a place leave parts of either. */
 typedef struct {
     const void *q, *k, *v;
     void* qOut;
