@@ -56,6 +56,45 @@ template <int QB> __device__ __forceinline__ bool kv_block(const KvAttnArgs& A, 
     return true;
 }
 
+// The same for calls of at most 64 sequences, the longest ones' blocks first: what starts last is short then, and the numbers without rows come behind all others
+// (64 tokens over 100 to 12000 positions 316 -> 292 us, 60 chunks of up to 120 rows behind up to 2000 139 -> 108).  LAST: of a sequence the last rows first, which see
+// most.  A lane a sequence: the blocks of longer ones are before its own.  From nine on, each of the four waves looks at a quarter of them (64 tokens over 300
+// each: 20 us where every wave looks at all, 17).  For workgroups of four waves, all together.
+template <int QB, bool LAST = false> __device__ __forceinline__ bool kv_block_longest_first(const KvAttnArgs& A, int blk, KvBlock& B) {
+    __shared__ int parts[4][64];
+    if (A.nseq > 64) return kv_block<QB>(A, LAST ? (gridDim.x - 1) / A.kvHeads - blk : blk, B);
+    const int lane = threadIdx.x & 63, own = min(lane, A.nseq - 1);
+    const int b = A.start[own], e = A.start[own + 1], len = A.len[own];
+    const int all = b < 0 || lane >= A.nseq ? 0 : max(min(e, A.rows) - b, 0) * A.group, blocks = (all + QB - 1) / QB;
+    const int key = min(max(len, 0), (1 << 25) - 1) << 6 | (63 - lane); // (each another)
+    const bool shared = A.nseq > 8;
+    int before = 0;
+    auto look = [&](int t) {
+        const int k = __builtin_amdgcn_readlane(key, t), n = __builtin_amdgcn_readlane(blocks, t);
+        before += k > key ? n : 0;
+    };
+    if (!shared) {
+        for (int t = 0; t < A.nseq; t++) look(t);
+    } else {
+        const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+#pragma unroll
+        for (int i = 0; i < 16; i++) look(16 * wave + i); // (lanes without a sequence have no blocks)
+        parts[wave][lane] = before;
+        __syncthreads();
+        before = parts[0][lane] + parts[1][lane] + parts[2][lane] + parts[3][lane];
+    }
+    const unsigned long long who = __ballot(blk >= before && blk < before + blocks);
+    if (!who) return false;
+    const int s = __builtin_ctzll(who);
+    const int nth = blk - __builtin_amdgcn_readlane(before, s), r0 = (LAST ? __builtin_amdgcn_readlane(blocks, s) - 1 - nth : nth) * QB;
+    B.s = s; B.r0 = r0; B.nr = min(QB, __builtin_amdgcn_readlane(all, s) - r0); B.row0 = __builtin_amdgcn_readlane(b, s);
+    B.pos0 = (int)((unsigned)__builtin_amdgcn_readlane(len, s) - (unsigned)__builtin_amdgcn_readlane(e, s) + (unsigned)B.row0);
+    B.cap = A.pagesPerSeq * MLH_KV_PAGE;
+    B.minPos = max(B.pos0 + r0 / A.group, -1);
+    B.maxPos = min(B.pos0 + (r0 + B.nr - 1) / A.group, B.cap - 1);
+    return true;
+}
+
 // The key tiles of TK positions that a block's rows see something of: the first positions' and the window's.
 template <int TK> struct KvTiles {
     int firsts, skip, n;
@@ -275,7 +314,7 @@ __global__ void __launch_bounds__(KV_F32_WAVES * 64, 2) k_kvattn_f32(KvAttnArgs 
     const int kh = blockIdx.x % A.kvHeads, block = blockIdx.x / A.kvHeads / A.nsplit, split = blockIdx.x / A.kvHeads % A.nsplit;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, n = lane & 15, g = lane >> 4;
     KvBlock B;
-    if (!kv_block<16>(A, block, B)) return;
+    if (!kv_block_longest_first<16>(A, block, B)) return;
     const int r = B.r0 + min(n, B.nr - 1), h = kh * A.group + r % A.group;
     const KvSight sight(A, B.pos0 + r / A.group);
     f32x4 q[KC / 4];
@@ -580,7 +619,7 @@ __global__ void __launch_bounds__(KV_FEW_WAVES * 64, KvType<CT>::code == MLH_CAC
     const int kh = blockIdx.x % A.kvHeads, block = blockIdx.x / A.kvHeads / A.nsplit, split = blockIdx.x / A.kvHeads % A.nsplit;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, n = lane & 15, g = lane >> 4;
     KvBlock B;
-    if (!kv_block<16 / SP>(A, block, B)) return;
+    if (!kv_block_longest_first<16 / SP>(A, block, B)) return;
     const int r = B.r0 + min(n / SP, B.nr - 1), h = kh * A.group + r % A.group;
     const KvSight sight(A, B.pos0 + r / A.group);
     // the row, on its way before the first tile and looked at behind it
@@ -832,7 +871,7 @@ __global__ void __launch_bounds__(NW * 64, HD == 64 ? 3 : 2) k_kvattn_many(KvAtt
     float (*const odds)[HD] = reinterpret_cast<float (*)[HD]>(lds + 4 * TB + 32);
     const int kh = blockIdx.x % A.kvHeads, tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, n = lane & 31, half = lane >> 5;
     KvBlock B;
-    if (!kv_block<QB>(A, (gridDim.x - 1 - blockIdx.x) / A.kvHeads, B)) return; // (the last rows of a sequence see most: first)
+    if (!kv_block_longest_first<QB, true>(A, blockIdx.x / A.kvHeads, B)) return;
     const bool active = wave * 32 < B.nr;
     const int wr0 = B.r0 + min(wave * 32, B.nr - 1), wr1 = B.r0 + min(wave * 32 + 31, B.nr - 1); // this wave's rows
     const int wMin = max(B.pos0 + wr0 / A.group, -1), wMax = min(B.pos0 + wr1 / A.group, B.cap - 1);
@@ -1169,9 +1208,9 @@ static std::string attn_check(const mlh_kv_cache* c, const mlh_kv_batch* b, cons
 //   4-bit pages: from 65 on.  16 sequences of 32, 64, 96 rows: k_kvattn_few 44, 68, 95 us, k_kvattn_many 53, 69, 77 (its tiles pass through LDS as halves).
 //   fp16 rows over 4-bit pages that leave a column for each of their groups: spread (above).
 // How keys are split, a second kernel joining the shares:
-#define KV_SPLIT_WGS 2048 // k_kvattn_few, k_kvattn_f32: until a call has this many workgroups of at least four turns each, or two until each compute unit has one
-                          // (64 tokens over 100 to 12000, 64 over 3000 positions: 316, 156 us; 1024: 332, 151; 3072: 314, 160; 4096: 312, 164; four turns always: one token
-                          // over 4000 15 us for 12; two always: 64 over 300 30 for 17)
+#define KV_SPLIT_WGS 768 // k_kvattn_few, k_kvattn_f32: until a call has this many workgroups of at least four turns each, or two until each compute unit has one
+                         // (64 tokens over 100 to 12000, 64 over 3000 positions, 48 over up to 9000 in 4 bits: 291, 150, 87 us; 512: 339, 141, 87; 1536: 293, 152, 90; 3072: 303, 162, 98;
+                         // four turns always: one token over 4000 15 us for 12; two always: 64 over 300 30 for 17)
 #define KV_SPLIT_MANY 1024 // k_kvattn_many: the same (512 to 3000: no difference within 3 of 118 us) ...
 #define KV_SPLIT_LEAST 8   // ... of at least eight tiles each, four until each compute unit has a workgroup (one sequence, 32 rows: 16 us, 21 with eight; two: 14, but 512 rows 44 for 32)
 struct AttnPlan {         // which kernel, and how the keys are split
