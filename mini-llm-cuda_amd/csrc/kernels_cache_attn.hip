@@ -447,9 +447,10 @@ __global__ void __launch_bounds__(KV_F32_WAVES * 64, 2) k_kvattn_f32(KvAttnArgs 
 // rows go through the wave's own piece of LDS, which hands them back transposed (ds_read_b64_tr_b16: lane i of 16 gets column i of four rows), so that
 // O^T += V^T . P^T takes the weights from the registers that the first product left them in.  4-bit pages: codes become halves on the way (the values
 // are minimum + code * scale in halves, one rounding), all products are in halves, and rows are scaled by a power of two first.
-// 16-bit pages are bound by memory: 64 tokens over 100 to 12000 positions, 32 heads on 8 of 128 in bf16, 1.59 GB, 316 us (5.0 TB/s; reads alone reach 6.1); 64 over 3000
-// each 156 us.  Eight waves a workgroup: 307 and 170, one token over 4000 17 for 12.  4-bit pages by the instructions that unpack them: one token over 65000 positions, bf16,
-// 21 us (83 MB, 3.9 TB/s); eight waves a workgroup: 146 us for 116 (48 tokens, before the spread below).
+// 16-bit pages are bound by memory: 64 tokens over 100 to 12000 positions, 32 heads on 8 of 128 in bf16, 1.59 GB, 288 us (5.5 TB/s; reads alone reach 6.1); 64 over 3000
+// each 150 us.  Eight waves a workgroup, one of them a compute unit then, before the longest came first: 307 and 170 us for 316 and 156, one token over 4000 17 for 12.  4-bit
+// pages by the instructions that unpack them: one token over 65000 positions, bf16, 21 us (83 MB, 3.9 TB/s); eight waves a workgroup 146 us for 116 (48 tokens, before the
+// spread below).
 // ----------------------------------------------------------------------------
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
@@ -603,7 +604,8 @@ template <typename IT, int HD> struct KvRaw16<IT, q4_t, HD> { // the same, eleme
 // SP > 1 (fp16 rows over 4-bit pages, at most 16 / SP of them a sequence): column n of the first product is row n / SP with the elements of group n % SP alone.  A sum's codes
 // then share minimum and scale: codes go in as they are (kv_tiny), the scale is one multiplication a key and group in fp32 behind them, exact where the 16-row form
 // needs two products, and the groups' sums meet in the neighbouring columns.  The minima meet the row's sums of elements in one product more.
-// 48 tokens over up to 9000 positions, window 4096, 16 heads of 128, 389 MB: 87 us (4.5 TB/s), 104 in the 16-row form (bf16 rows, whose 16-row form has one product: 108 us spread, 104 not).
+// 48 tokens over up to 9000 positions, window 4096, 16 heads of 128, 389 MB: 85 us (4.6 TB/s).  48 over 4000 each: 112 us, 125 in the 16-row form; bf16 rows, whose
+// 16-row form has one product, 108 spread and 104 not.
 #define KV_FEW_WAVES 4
 template <typename IT, typename CT, int HD, int SP>
 __global__ void __launch_bounds__(KV_FEW_WAVES * 64, KvType<CT>::code == MLH_CACHE_Q4 ? 3 : 2) k_kvattn_few(KvAttnArgs A) {
@@ -845,7 +847,7 @@ __global__ void __launch_bounds__(KV_FEW_WAVES * 64, KvType<CT>::code == MLH_CAC
 // (the 16-byte pieces of a row in an order that keeps both readings free of bank conflicts), those of 4 bits through registers, where codes become halves; fp16 rows too
 // meet K and V rounded to halves here (error against the result's norm 4.4e-4, 2.1e-4 the rounding of the result).
 // Bound by the matrix cores at the clock that their power leaves (1.8 GHz) and the vector ALU's exponentials between them: 16384 rows, 32 heads of 128 in fp16, window 4096
-// 1.10 ms, 0.89 PFLOP/s of what is seen (a library product of 8192 cubed: 1.05).  Eight prompts of 2048, window 1024: 0.17 ms, 0.61 PFLOP/s: of 19 tiles that a
+// 1.10 to 1.15 ms on two cards, 0.89 to 0.85 PFLOP/s of what is seen (a library product of 8192 cubed: 1.05).  Eight prompts of 2048, window 1024: 0.17 ms, 0.61 PFLOP/s: of 19 tiles that a
 // workgroup's rows touch 16 are seen whole, and every workgroup starts with a lookup and a tile that nothing hides.  1289 rows behind 3000 to 7000 positions in 4 bits, heads
 // of 64: 108 us, 0.48 PFLOP/s (an exponential and its conversion for every 256 operations of the products).
 // ----------------------------------------------------------------------------
@@ -1117,7 +1119,7 @@ __global__ void __launch_bounds__(NW * 64, HD == 64 ? 3 : 2) k_kvattn_many(KvAtt
 // ----------------------------------------------------------------------------
 // The shares of nsplit workgroups of a row and head: a lane a share for the factors, 256 / (HD / 4) groups of threads for the sums.
 // ----------------------------------------------------------------------------
-// (2048 rows of 16 shares: 4.8 us, latency)
+// (32 of 64 shares: 4 us, latency)
 #define KV_MAX_SPLIT 64
 template <typename IT, int HD>
 __global__ void __launch_bounds__(256) k_kvattn_join(KvAttnArgs A) {
@@ -1204,7 +1206,7 @@ static std::string attn_check(const mlh_kv_cache* c, const mlh_kv_batch* b, cons
 
 // Which kernel (32 query heads on 8, heads of 128, bf16, 4000 positions; "rows" are a sequence's, over the heads of one K/V head):
 //   16-bit pages: k_kvattn_many from 17 rows on.  16 sequences of 4, 16, 32, 64 rows: k_kvattn_few 49, 59, 111, 174 us, k_kvattn_many 50, 53, 57, 73; one sequence: 12, 12, 19, 19
-//     and 15, 15, 16, 18; 64 of 4 rows over 100 to 12000 positions: 316 and 377 (it splits less).
+//     and 15, 15, 16, 18; 64 of 4 rows over 100 to 12000 positions: 290 and 377 (it splits less).
 //   4-bit pages: from 65 on.  16 sequences of 32, 64, 96 rows: k_kvattn_few 44, 68, 95 us, k_kvattn_many 53, 69, 77 (its tiles pass through LDS as halves).
 //   fp16 rows over 4-bit pages that leave a column for each of their groups: spread (above).
 // How keys are split, a second kernel joining the shares:
