@@ -1117,33 +1117,40 @@ __global__ void __launch_bounds__(NW * 64, HD == 64 ? 3 : 2) k_kvattn_many(KvAtt
 }
 
 // ----------------------------------------------------------------------------
-// The shares of nsplit workgroups of a row and head: a lane a share for the factors, 256 / (HD / 4) groups of threads for the sums.
+// The shares of nsplit workgroups of a row and head, MOST at most: a lane a share (or several) for the factors, 256 / (HD / 4) groups of threads for the sums.
 // ----------------------------------------------------------------------------
 // (32 of 64 shares: 4 us, latency)
-#define KV_MAX_SPLIT 64
-template <typename IT, int HD>
+#define KV_MAX_SPLIT 256 // (one token over 200000 positions in 4 bits, one K/V head: 23 us; 128: 30, 64: 49)
+template <typename IT, int HD, int MOST>
 __global__ void __launch_bounds__(256) k_kvattn_join(KvAttnArgs A) {
-    constexpr int T = HD / 4, G = 256 / T;
+    constexpr int T = HD / 4, G = 256 / T, L = MOST / 64; // L: shares of a lane, lane + 64 i
     __shared__ f32x4 sum[G][T];
     const size_t rh = blockIdx.x, n = (size_t)A.rows * A.heads;
     const int row = (int)(rh / A.heads), h = (int)(rh % A.heads), lane = threadIdx.x & 63, t = threadIdx.x % T, g = threadIdx.x / T;
     const float2* stat = reinterpret_cast<const float2*>(A.part + (size_t)A.nsplit * n * HD);
-    const float2 ml = lane < A.nsplit ? stat[lane * n + rh] : make_float2(-INFINITY, 0.f);
-    f32x4 v[KV_MAX_SPLIT / G]; // (everything on its way before anything is waited for)
+    float2 ml[L];
 #pragma unroll
-    for (int i = 0; i < KV_MAX_SPLIT / G; i++) v[i] = *reinterpret_cast<const f32x4*>(A.part + (min(i * G + g, A.nsplit - 1) * n + rh) * HD + 4 * t);
+    for (int i = 0; i < L; i++) ml[i] = lane + 64 * i < A.nsplit ? stat[(lane + 64 * i) * n + rh] : make_float2(-INFINITY, 0.f);
+    f32x4 v[MOST / G]; // (everything on its way before anything is waited for)
+#pragma unroll
+    for (int i = 0; i < MOST / G; i++) v[i] = *reinterpret_cast<const f32x4*>(A.part + (min(i * G + g, A.nsplit - 1) * n + rh) * HD + 4 * t);
     if (row < A.start[0] || row >= A.start[A.nseq]) return;
-    float M = ml.x;
+    float M = -INFINITY, den = 0.f, f[L];
+#pragma unroll
+    for (int i = 0; i < L; i++) M = fmaxf(M, ml[i].x);
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
-    const float f = kv_exp2(ml.x - (M == -INFINITY ? 0.f : M));
-    float den = ml.y * f;
+#pragma unroll
+    for (int i = 0; i < L; i++) {
+        f[i] = kv_exp2(ml[i].x - (M == -INFINITY ? 0.f : M));
+        den = fmaf(ml[i].y, f[i], den);
+    }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) den += __shfl_xor(den, o, 64);
     f32x4 o = (f32x4)(0.f);
 #pragma unroll
-    for (int i = 0; i < KV_MAX_SPLIT / G; i++) {
-        const float w = __shfl(f, i * G + g, 64); // (of a share that is not there: 2^-inf)
+    for (int i = 0; i < MOST / G; i++) {
+        const float w = __shfl(f[i * G / 64], (i * G + g) % 64, 64); // (of a share that is not there: 2^-inf)
         if (i * G + g < A.nsplit) o += v[i] * w;
     }
     sum[g][t] = o;
@@ -1261,7 +1268,8 @@ template <typename IT, typename CT, int HD, int NW> static hipError_t launch_man
 template <typename IT, int HD> static void launch_join(hipStream_t st, const KvAttnArgs& A) {
     const unsigned n = (unsigned)(A.rows * A.heads), per = 256 / (HD / 4);
     if (A.nsplit <= KV_JOIN_FEW) hipLaunchKernelGGL((k_kvattn_join_few<IT, HD>), dim3((n + per - 1) / per), dim3(256), 0, st, A);
-    else hipLaunchKernelGGL((k_kvattn_join<IT, HD>), dim3(n), dim3(256), 0, st, A);
+    else if (A.nsplit <= 64) hipLaunchKernelGGL((k_kvattn_join<IT, HD, 64>), dim3(n), dim3(256), 0, st, A);
+    else hipLaunchKernelGGL((k_kvattn_join<IT, HD, KV_MAX_SPLIT>), dim3(n), dim3(256), 0, st, A);
 }
 static int launch_join(hipStream_t st, int type, int hd, const KvAttnArgs& A) {
     if (A.nsplit == 1) return 0;

@@ -277,6 +277,15 @@ def test_hints_decide_nothing_else(pkg, kind, cache):
             c.check()
 
 
+@pytest.mark.parametrize("kind,cache", KINDS)
+@pytest.mark.parametrize("hd,lens", [(64, [17000, 40]), (128, [33100])])
+def test_more_shares_than_lanes(pkg, kind, cache, hd, lens):
+    """One K/V head and a long sequence: its keys are split over more workgroups than a wave has lanes."""
+    c = Call(pkg, kind, cache, 3, 1, hd, [1] * len(lens), lens, seed=8)
+    assert c.args.workBytes > 64 * 3 * len(lens) * (hd + 2) * 4
+    c.check()
+
+
 @pytest.mark.parametrize("hd", [64, 128])
 @pytest.mark.parametrize("kind,spread,scale", [("bf16", 1e30, 1e-30), ("bf16", 1e-25, 1e24), ("bf16", 3e4, 1e-5), ("f16", 1.2e4, 1e-5), ("f16", 1e-5, 1e4)])
 def test_sizes_of_rows(pkg, kind, spread, scale, hd):
