@@ -323,6 +323,18 @@ def test_many_sequences(pkg):
     assert _same_bits(a.pools.dk.cpu(), a.pools.k) and _same_bits(a.pools.dv.cpu(), a.pools.v)
 
 
+@pytest.mark.parametrize("n", [2, 8, 9, 33, 64, 65])
+@pytest.mark.parametrize("kind,cache", [("bf16", "bf16"), ("f32", "q4"), ("f16", "q4")])
+def test_order_of_sequences(pkg, kind, cache, n):
+    """Sequences are taken longest first, up to 64 of them: single tokens, rows of every number, equal lengths, some without rows, the last rows of all untouched."""
+    one = [1] * n
+    some = [(5 * i + 2) % 4 for i in range(n)]
+    most = [70 if i % 7 == 3 else (3 * i) % 5 for i in range(n)]
+    for new in (one, some, most):
+        lens = [m + (53 * i) % 130 if i % 3 else 80 for i, m in enumerate(new)]
+        Call(pkg, kind, cache, 2, 1, 64, new, lens, 90, 2, seed=n, pad=3).check()
+
+
 def test_small_work_is_refused(pkg):
     c = Call(pkg, "bf16", "bf16", 2, 1, 64, [1], [9000], seed=1)
     assert c.args.workBytes > 0
