@@ -129,6 +129,9 @@ __device__ __forceinline__ bool kv_finite(float v) { return (__float_as_uint(v) 
 __device__ __forceinline__ float kv_exp2(float v) { return __builtin_amdgcn_exp2f(v); }
 // The larger of two (as a median: fmaxf would first quiet both, an instruction each; where one is no number, either, and the row's sum is none then)
 __device__ __forceinline__ float kv_max(float a, float b) { return __builtin_amdgcn_fmed3f(a, b, INFINITY); }
+// The running maximum follows when a score is 2^8 times beyond it and not before (weights up to 256 are as good as up to one, in halves too): with every new maximum, of 32 rows
+// some have one in most tiles, and sums and result are multiplied again.
+#define KV_SLACK 8.f
 __device__ __forceinline__ float kv_halves_max(float v) { // of a lane and the one 32 further
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     return kv_max(__uint_as_float(r[0]), __uint_as_float(r[1]));
@@ -719,9 +722,15 @@ __global__ void __launch_bounds__(KV_FEW_WAVES * 64, KvType<CT>::code == MLH_CAC
         for (int b = 0; b < 2; b++)
 #pragma unroll
             for (int e = 0; e < 4; e++) mx = kv_max(mx, s[b][e]);
-        const float mt = fmaxf(m, kv_quad_max(mx) * scale), ref = mt == -INFINITY ? 0.f : mt, corr = kv_exp2(m - ref);
-        m = mt;
-        l *= corr;
+        const float mt = kv_quad_max(mx) * scale;
+        if (__any(mt > m + KV_SLACK)) {
+            const float mn = mt > m + KV_SLACK ? mt : m, corr = m == -INFINITY ? 0.f : kv_exp2(m - mn); // (each row for itself)
+            m = mn;
+            l *= corr;
+#pragma unroll
+            for (int b = 0; b < VB; b++) acc[b] *= corr;
+        }
+        const float ref = m == -INFINITY ? 0.f : m;
 #pragma unroll
         for (int b = 0; b < 2; b++)
 #pragma unroll
@@ -729,10 +738,6 @@ __global__ void __launch_bounds__(KV_FEW_WAVES * 64, KvType<CT>::code == MLH_CAC
                 p[b][e] = kv_exp2(fmaf(s[b][e], scale, -ref));
                 l += p[b][e];
             }
-        if (__any(corr != 1.f)) { // (a maximum that moves gets rare)
-#pragma unroll
-            for (int b = 0; b < VB; b++) acc[b] *= corr;
-        }
         if (repair) {
 #pragma unroll
             for (int b = 0; b < 2; b++) {
@@ -1015,17 +1020,17 @@ __global__ void __launch_bounds__(NW * 64, HD == 64 ? 3 : 2) k_kvattn_many(KvAtt
         for (int b = 0; b < 2; b++)
 #pragma unroll
             for (int e = 0; e < 16; e++) mx = kv_max(mx, s[b][e]);
-        const float mn = fmaxf(m, kv_halves_max(mx) * scale);
-        if (__any(mn > m)) {
-            const float corr = m == -INFINITY ? 0.f : kv_exp2(m - mn);
+        const float mt = kv_halves_max(mx) * scale;
+        if (__any(mt > m + KV_SLACK)) {
+            const float mn = mt > m + KV_SLACK ? mt : m, corr = m == -INFINITY ? 0.f : kv_exp2(m - mn); // (each row for itself)
+            m = mn;
             l *= corr;
 #pragma unroll
             for (int b = 0; b < MB; b++)
 #pragma unroll
                 for (int e = 0; e < 16; e++) acc[b][e] *= corr;
         }
-        m = mn;
-        const float ref = mn == -INFINITY ? 0.f : -mn;
+        const float ref = m == -INFINITY ? 0.f : -m;
 #pragma unroll
         for (int b = 0; b < 2; b++)
 #pragma unroll
