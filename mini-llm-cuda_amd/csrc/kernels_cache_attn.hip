@@ -130,7 +130,7 @@ __device__ __forceinline__ float kv_exp2(float v) { return __builtin_amdgcn_exp2
 // The larger of two (as a median: fmaxf would first quiet both, an instruction each; where one is no number, either, and the row's sum is none then)
 __device__ __forceinline__ float kv_max(float a, float b) { return __builtin_amdgcn_fmed3f(a, b, INFINITY); }
 // The running maximum follows when a score is 2^8 times beyond it and not before (weights up to 256 are as good as up to one, in halves too): with every new maximum, of 32 rows
-// some have one in most tiles, and sums and result are multiplied again.
+// some have one in most tiles, and sums and result are multiplied again (the prompts below: 1071 and 171 us for 1017 and 158).
 #define KV_SLACK 8.f
 __device__ __forceinline__ float kv_halves_max(float v) { // of a lane and the one 32 further
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
@@ -607,7 +607,7 @@ template <typename IT, int HD> struct KvRaw16<IT, q4_t, HD> { // the same, eleme
 // SP > 1 (fp16 rows over 4-bit pages, at most 16 / SP of them a sequence): column n of the first product is row n / SP with the elements of group n % SP alone.  A sum's codes
 // then share minimum and scale: codes go in as they are (kv_tiny), the scale is one multiplication a key and group in fp32 behind them, exact where the 16-row form
 // needs two products, and the groups' sums meet in the neighbouring columns.  The minima meet the row's sums of elements in one product more.
-// 48 tokens over up to 9000 positions, window 4096, 16 heads of 128, 389 MB: 85 us (4.6 TB/s).  48 over 4000 each: 112 us, 125 in the 16-row form; bf16 rows, whose
+// 48 tokens over up to 9000 positions, window 4096, 16 heads of 128, 389 MB: 79 us (4.9 TB/s).  48 over 4000 each: 112 us, 125 in the 16-row form; bf16 rows, whose
 // 16-row form has one product, 108 spread and 104 not.
 #define KV_FEW_WAVES 4
 template <typename IT, typename CT, int HD, int SP>
@@ -852,9 +852,9 @@ __global__ void __launch_bounds__(KV_FEW_WAVES * 64, KvType<CT>::code == MLH_CAC
 // (the 16-byte pieces of a row in an order that keeps both readings free of bank conflicts), those of 4 bits through registers, where codes become halves; fp16 rows too
 // meet K and V rounded to halves here (error against the result's norm 4.4e-4, 2.1e-4 the rounding of the result).
 // Bound by the matrix cores at the clock that their power leaves (1.8 GHz) and the vector ALU's exponentials between them: 16384 rows, 32 heads of 128 in fp16, window 4096
-// 1.10 to 1.15 ms on two cards, 0.89 to 0.85 PFLOP/s of what is seen (a library product of 8192 cubed: 1.05).  Eight prompts of 2048, window 1024: 0.17 ms, 0.61 PFLOP/s: of 19 tiles that a
+// 1.02 ms, 0.95 PFLOP/s of what is seen (a library product of 8192 cubed: 1.05).  Eight prompts of 2048, window 1024: 0.16 ms, 0.64 PFLOP/s: of 19 tiles that a
 // workgroup's rows touch 16 are seen whole, and every workgroup starts with a lookup and a tile that nothing hides.  1289 rows behind 3000 to 7000 positions in 4 bits, heads
-// of 64: 108 us, 0.48 PFLOP/s (an exponential and its conversion for every 256 operations of the products).
+// of 64: 101 us, 0.51 PFLOP/s (an exponential and its conversion for every 256 operations of the products).
 // ----------------------------------------------------------------------------
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 template <bool BF> __device__ __forceinline__ float kv_add2(uint32_t w, float sum) { // two 16-bit numbers onto a sum
