@@ -1223,7 +1223,7 @@ static std::string attn_check(const mlh_kv_cache* c, const mlh_kv_batch* b, cons
 //   fp16 rows over 4-bit pages that leave a column for each of their groups: spread (above).
 // How keys are split, a second kernel joining the shares:
 #define KV_SPLIT_WGS 768 // k_kvattn_few, k_kvattn_f32: until a call has this many workgroups of at least four turns each, or two until each compute unit has one
-                         // (64 tokens over 100 to 12000, 64 over 3000 positions, 48 over up to 9000 in 4 bits: 291, 150, 87 us; 512: 339, 141, 87; 1536: 293, 152, 90; 3072: 303, 162, 98;
+                         // (64 tokens over 100 to 12000, 64 over 3000 positions, 48 over up to 9000 in 4 bits: 291, 150, 87 us; 512: 339, 141, 87; 1536: 293, 152, 90;
                          // four turns always: one token over 4000 15 us for 12; two always: 64 over 300 30 for 17)
 #define KV_SPLIT_MANY 1024 // k_kvattn_many: the same (512 to 3000: no difference within 3 of 118 us) ...
 #define KV_SPLIT_LEAST 8   // ... of at least eight tiles each, four until each compute unit has a workgroup (one sequence, 32 rows: 16 us, 21 with eight; two: 14, but 512 rows 44 for 32)
