@@ -567,7 +567,8 @@ template <typename IT, typename CT, int HD> struct KvRaw16 { // a lane's part of
 };
 // Rows in halves over 4-bit pages (16 rows a workgroup): rounding K's values to halves costs such rows more than all else together, so that they are multiplied as what they are, minimum +
 // (high + low part of the scale) * code: parts of six and five bits times a code of four are exact in halves, two products instead of one, and the minima meet the sum of
-// the row's elements (as two halves) in one product more.  The weights are two halves as well.  (Error of a result, normal values, 4000 keys, against its norm: 4.4e-4 with
+// the row's elements (as two halves) in one product more.  (15 times a scale may be beyond the halves' range where the values are not: of the high part, whose last place is 2^-19 at
+// least, a sixteenth is multiplied, exact as well, and the sum is 16 times as much; the low part is below a 32nd of the scale.)  The weights are two halves as well.  (Error of a result, normal values, 4000 keys, against its norm: 4.4e-4 with
 // K, V and weights each rounded to halves, 2.8e-4 so, 2.1e-4 the rounding of the result alone.)  Rows in bf16 round their results eight times as far.
 template <typename IT, typename CT> constexpr bool kv_in_parts() { return KvType<CT>::code == MLH_CACHE_Q4 && KvType<IT>::code == MLH_DTYPE_F16; }
 __device__ __forceinline__ u32x4 kv_times(const u32x4& codes, uint32_t scaleBits) {
@@ -679,15 +680,19 @@ __global__ void __launch_bounds__(KV_FEW_WAVES * 64, KvType<CT>::code == MLH_CAC
                     s[b][e] = fmaf(v, 1024.f, base[e]);
                 }
             } else if constexpr (PARTS) {
-                const uint32_t par = raw[set].kp[b], high = par >> 16 & 0xffe0u;
-                const _Float16 low = __builtin_bit_cast(_Float16, (uint16_t)(par >> 16)) - __builtin_bit_cast(_Float16, (uint16_t)high);
+                const uint32_t par = raw[set].kp[b];
+                const _Float16 top = __builtin_bit_cast(_Float16, (uint16_t)(par >> 16 & 0xffe0u));
+                const _Float16 low = __builtin_bit_cast(_Float16, (uint16_t)(par >> 16)) - top, high = top * (_Float16)0.0625f;
+                f32x4 most = (f32x4)(0.f); // a sixteenth of the high part's sum
                 s[b] = mfma16<false>(u32x4{(par & 0xffffu) | par << 16, 0u, 0u, 0u}, qsum, s[b]);
 #pragma unroll
                 for (int t = 0; t < KS; t++) {
                     const u32x4 codes = kv_codes(raw[set].k[b][t]);
-                    s[b] = mfma16<false>(kv_times(codes, high), q[t], s[b]);
+                    most = mfma16<false>(kv_times(codes, __builtin_bit_cast(uint16_t, high)), q[t], most);
                     s[b] = mfma16<false>(kv_times(codes, __builtin_bit_cast(uint16_t, low)), q[t], s[b]);
                 }
+#pragma unroll
+                for (int e = 0; e < 4; e++) s[b][e] = fmaf(most[e], 16.f, s[b][e]);
             } else {
 #pragma unroll
                 for (int t = 0; t < KS; t++) s[b] = mfma16<BF>(raw[set].key(b, t), q[t], s[b]);
