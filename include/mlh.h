@@ -430,7 +430,7 @@ int mlh_kv_read_device(const mlh_kv_cache* cache, const mlh_kv_batch* batch, con
 
 /* Attention of the batch's rows over what their sequences hold (their own k and v are in the cache by then).  Position p sees key position j when j <= p and,
  * with window > 0, p - j < window or j < sinks.  out = sum over those of softmax(scale * q . k) v (inference.cu:136-239); zeros for a row that sees
- * nothing.  Keys that a row does not see do not count for it, whatever they hold (infinities and NaN too); pages no row sees are not read, so their table entries may be
+ * nothing (one at a negative position).  NaN, as the softmax is, where a score is NaN or +infinity, or every one is -infinity.  Keys that a row does not see do not count for it, whatever they hold (infinities and NaN too); pages no row sees are not read, so their table entries may be
  * stale.  A row that sees a position beyond the page table or in a page outside the pool is NaN.
  * Scores, softmax statistics and sums are fp32, and with fp32 rows everything is.  With rows of 16 bits over pages of the same type the weights are rounded to it for the product
  * with v.  Over 4-bit pages both products are of halves: v's values and the weights are rounded to them, q times a power of two (exactly, but for what is 2^-24 of its row's

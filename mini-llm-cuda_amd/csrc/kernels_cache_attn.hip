@@ -208,18 +208,15 @@ __device__ __forceinline__ void kv_finish16(const KvAttnArgs& A, const KvBlock& 
         }
         const int qi = (B.r0 + r) / A.group, h = kh * A.group + (B.r0 + r) % A.group, row = B.row0 + qi;
         if (B.pos0 + qi >= B.cap) { den = KV_NAN; M = 0.f; } // (its own position is behind the page table)
+        if (B.pos0 + qi < 0) { den = 1.f; M = 0.f; } // sees nothing: o is zero.  (Every other row sees itself: no weight at all means that each score is -infinity, and 0 / 0 is what that is)
         if (A.nsplit > 1) {
             const size_t rh = (size_t)split * A.rows * A.heads + (size_t)row * A.heads + h;
             *reinterpret_cast<f32x4*>(A.part + rh * HD + d) = o;
             if (d == 0) *reinterpret_cast<float2*>(A.part + (size_t)A.nsplit * A.rows * A.heads * HD + rh * 2) = make_float2(M, den);
         } else {
-            const float inv = den == 0.f ? 0.f : 1.0f / den;
-            if constexpr (sizeof(IT) == 4) { // (a division's rounding, not a product's with a rounded inverse)
-                o = den == 0.f ? (f32x4)(0.f) : f32x4{o.x / den, o.y / den, o.z / den, o.w / den};
-                kv_put4((IT*)A.out + (size_t)row * A.outStride + (size_t)h * HD + d, o);
-            } else {
-                kv_put4((IT*)A.out + (size_t)row * A.outStride + (size_t)h * HD + d, den == 0.f ? (f32x4)(0.f) : o * inv);
-            }
+            if constexpr (sizeof(IT) == 4) o = f32x4{o.x / den, o.y / den, o.z / den, o.w / den}; // (a division's rounding, not a product's with a rounded inverse)
+            else o = o * (1.0f / den);
+            kv_put4((IT*)A.out + (size_t)row * A.outStride + (size_t)h * HD + d, o);
         }
     }
 }
@@ -1105,18 +1102,17 @@ __global__ void __launch_bounds__(NW * 64, HD == 64 ? 3 : 2) k_kvattn_many(KvAtt
     if (!active || wave * 32 + n >= B.nr) return;
     l += __shfl_xor(l, 32, 64);
     const int qi = r / A.group;
-    const bool beyond = B.pos0 + qi >= B.cap; // (its own position is behind the page table)
-    const float inv = A.nsplit > 1 ? 1.f : beyond ? KV_NAN : l == 0.f ? 0.f : 1.0f / l;
+    const bool beyond = B.pos0 + qi >= B.cap, none = B.pos0 + qi < 0; // its own position is behind the page table; it sees nothing (as in kv_finish16)
+    const float inv = A.nsplit > 1 || none ? 1.f : beyond ? KV_NAN : 1.0f / l;
     IT* out = (IT*)A.out + (size_t)(B.row0 + qi) * A.outStride + (size_t)h * HD;
     const size_t shares = (size_t)A.rows * A.heads, rh = split * shares + (size_t)(B.row0 + qi) * A.heads + h;
     float* part = A.part + rh * HD;
-    if (A.nsplit > 1 && half == 0) *reinterpret_cast<float2*>(A.part + A.nsplit * shares * HD + rh * 2) = beyond ? make_float2(0.f, KV_NAN) : make_float2(m, l);
+    if (A.nsplit > 1 && half == 0) *reinterpret_cast<float2*>(A.part + A.nsplit * shares * HD + rh * 2) = beyond ? make_float2(0.f, KV_NAN) : none ? make_float2(0.f, 1.f) : make_float2(m, l);
 #pragma unroll
     for (int c = 0; c < MB; c++)
 #pragma unroll
         for (int e = 0; e < 4; e++) {
             f32x4 o = f32x4{acc[c][4 * e], acc[c][4 * e + 1], acc[c][4 * e + 2], acc[c][4 * e + 3]} * inv;
-            if (inv == 0.f) o = (f32x4)(0.f);
             if (FOUR) { // columns (0, 4, 1, 5) here, (2, 6, 3, 7) in the other half: four neighbours each
                 const float a = __shfl_xor(half ? o.x : o.y, 32, 64), b = __shfl_xor(half ? o.z : o.w, 32, 64);
                 o = half ? f32x4{a, b, o.y, o.w} : f32x4{o.x, o.z, a, b};
@@ -1168,7 +1164,7 @@ __global__ void __launch_bounds__(256) k_kvattn_join(KvAttnArgs A) {
     if (g > 0) return;
 #pragma unroll
     for (int i = 1; i < G; i++) o += sum[i][t];
-    o = den == 0.f ? (f32x4)(0.f) : f32x4{o.x / den, o.y / den, o.z / den, o.w / den};
+    o = f32x4{o.x / den, o.y / den, o.z / den, o.w / den};
     kv_put4((IT*)A.out + (size_t)row * A.outStride + (size_t)h * HD + 4 * t, o);
 }
 
@@ -1200,7 +1196,7 @@ __global__ void __launch_bounds__(256) k_kvattn_join_few(KvAttnArgs A) {
         den = fmaf(ml[s].y, f, den);
         o += v[s] * f;
     }
-    o = den == 0.f ? (f32x4)(0.f) : f32x4{o.x / den, o.y / den, o.z / den, o.w / den};
+    o = f32x4{o.x / den, o.y / den, o.z / den, o.w / den};
     kv_put4((IT*)A.out + (size_t)row * A.outStride + (size_t)h * HD + d, o);
 }
 

@@ -1,9 +1,11 @@
 """Attention over a paged K/V cache where numbers are at their limits."""
+import math
+
 import pytest
 import torch
 
 from kv_oracle import GROUP, quantise
-from test_gpu_cache import Call
+from test_gpu_cache import KINDS, Call
 
 pytestmark = pytest.mark.gpu
 
@@ -43,3 +45,69 @@ def test_wide_groups(pkg, kind, hd, H, new, lens):
         _store(c, "k", s, _wide(gen, n, 1, hd, 40000.0))
         assert c.keys[s].abs().max() < 65504 < 15 * float(quantise(_wide(gen, 1, 1, hd, 40000.0))[1][..., 1].min())
     c.check()
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# scores of -infinity
+# ---------------------------------------------------------------------------------------------------------------------
+SIGHTS = [([3], [3], 0), ([1], [200], 0), ([5, 1], [90, 300], 60), ([70], [100], 0), ([150], [400], 70), ([1], [9000], 0)]
+
+
+@pytest.mark.parametrize("kind,cache", KINDS)
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("new,lens,window", SIGHTS)
+def test_nothing_but_minus_infinity(pkg, kind, cache, hd, new, lens, window):
+    """An infinite element of q that meets one sign in every key: each score is -infinity, the softmax is undefined and the row NaN, as 0 / 0 is; not zero as for a row that
+    sees nothing.  Its neighbours are as without it."""
+    c = Call(pkg, kind, cache, 2, 1, hd, new, lens, window, 2, seed=50)
+    for s, n in enumerate(lens):
+        k = c.keys[s].float().clone()
+        k[..., 7] = -1.5  # (over 4 bits not a group's minimum, whose code is zero: zero times infinity is no number anyway)
+        k[..., 8] = -4.0
+        _store(c, "k", s, k)
+    clean = c.run().clone()
+    c.dq[0, 7] = math.inf
+    c.dq[c.rows.used - 1, hd + 7] = math.inf
+    got = c.run()
+    for i in range(c.rows.used):
+        for h in range(2):
+            a, b = got[i, hd * h:hd * h + hd], clean[i, hd * h:hd * h + hd]
+            hit = (i, h) in ((0, 0), (c.rows.used - 1, 1))
+            assert torch.isnan(a).all() if hit else torch.equal(a, b), (i, h)
+
+
+@pytest.mark.parametrize("new,lens", [([3], [3]), ([1], [300]), ([40], [90]), ([1], [9000])])
+def test_scores_that_overflow(pkg, new, lens):
+    """fp32 products beyond the largest number: a row whose every score is one is NaN, keys with such a score beside others weigh nothing."""
+    c = Call(pkg, "f32", "f32", 2, 1, 64, new, lens, seed=51)
+    n = lens[0]
+    k = torch.zeros(n, 1, 64)
+    k[:, 0, 5] = -1e30
+    k[::3, 0, 6] = 1e30
+    _store(c, "k", 0, k)
+    q = torch.zeros(new[0], 2, 64)
+    q[:, 0, 5] = 1e30  # each score -infinity
+    q[:, 1, 6] = -1e30  # of every third key
+    _query(c, q.flatten(1))
+    got = c.run().double()
+    assert torch.isnan(got[:new[0], :64]).all()
+    for i in range(new[0]):
+        p = n - new[0] + i
+        some = [j for j in range(p + 1) if j % 3]
+        if not some:
+            assert torch.isnan(got[i, 64:]).all()
+            continue
+        v = c.vals[0][some, 0]
+        # equal weights: fp32 sums in any order, 64 terms of the size of the values at most between roundings
+        assert ((got[i, 64:] - v.mean(0)).abs() <= (len(some) + 8) * 2.0 ** -24 * v.abs().mean(0)).all()
+
+
+@pytest.mark.parametrize("kind,cache", KINDS)
+@pytest.mark.parametrize("new,lens", [([4, 2], [66, 70]), ([90, 2], [66, 9000]), ([4, 2], [66, 9000])])
+def test_nothing_seen_is_zero(pkg, kind, cache, new, lens):
+    """Rows at negative positions are zero whatever stands in them; with keys split over workgroups too."""
+    c = Call(pkg, kind, cache, 2, 1, 64, new, lens, seed=52)
+    c.rows.dlen.copy_(torch.tensor([new[0] - 3, lens[1]], dtype=torch.int32))
+    c.dq[0], c.dq[1] = math.nan, math.inf
+    got = c.run()
+    assert (got[:3] == 0).all() and not (got[3:] == 0).any(1).all()
