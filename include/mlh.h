@@ -434,7 +434,8 @@ int mlh_kv_read_device(const mlh_kv_cache* cache, const mlh_kv_batch* batch, con
  * stale.  A row that sees a position beyond the page table or in a page outside the pool is NaN.
  * Scores, softmax statistics and sums are fp32, and with fp32 rows everything is.  With rows of 16 bits over pages of the same type the weights are rounded to it for the product
  * with v.  Over 4-bit pages both products are of halves: v's values and the weights are rounded to them, q times a power of two (exactly, but for what is 2^-24 of its row's
- * largest), and k's values, except in calls of fp16 rows whose maxNew * heads / cache.heads is at most 64: these take k as it is and the weights to 22 bits.
+ * largest), and k's values, except in calls of fp16 rows whose maxNew * heads / cache.heads is at most 64: these take k as it is and the weights to 22 bits.  A weight that is held in
+ * halves, one or two, is off by 2^-32 of the row's largest at least.
  * Values of 4-bit pages beyond the halves' range count as infinite where they are rounded to halves; a group whose scale is an infinity or NaN counts as NaN or infinite.
  * maxLen, maxNew: what no len and no number of rows of a sequence exceeds (0: the page table's, rows).  They decide which kernel runs and how the work is split; a call that
  * exceeds them is right, and slower.

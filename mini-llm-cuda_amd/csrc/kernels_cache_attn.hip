@@ -132,6 +132,11 @@ __device__ __forceinline__ float kv_max(float a, float b) { return __builtin_amd
 // The running maximum follows when a score is 2^8 times beyond it and not before (weights up to 256 are as good as up to one, in halves too): with every new maximum, of 32 rows
 // some have one in most tiles, and sums and result are multiplied again (the prompts below: 1071 and 171 us for 1017 and 158).
 #define KV_SLACK 8.f
+// m is the maximum less KvRaise: a weight is 2^KvRaise at a new maximum, and up to 2^(KvRaise + KV_SLACK) before there is another.
+// Halves: 2^7, the largest then 2^15, so that half of their smallest step, which is what a weight is off by at least, is 2^-32 of the largest weight.  (With 1 for 2^7, of one key and 60000
+// others whose scores are 17 lower, 0.0025 of the result in all, each counted 1.4 times or not at all.)  bf16, which has room below: 2^-8, no weight above one, so that
+// sums stay as far from the end of fp32's range as they can.
+template <bool BF> struct KvRaise { static constexpr float value = BF ? -KV_SLACK : 7.f; };
 __device__ __forceinline__ float kv_halves_max(float v) { // of a lane and the one 32 further
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     return kv_max(__uint_as_float(r[0]), __uint_as_float(r[1]));
@@ -612,6 +617,7 @@ template <typename IT, typename CT, int HD, int SP>
 __global__ void __launch_bounds__(KV_FEW_WAVES * 64, KvType<CT>::code == MLH_CACHE_Q4 ? 3 : 2) k_kvattn_few(KvAttnArgs A) {
     constexpr bool FOUR = KvType<CT>::code == MLH_CACHE_Q4, BF = !FOUR && KvType<IT>::code == MLH_DTYPE_BF16; // products in bf16
     constexpr bool PARTS = kv_in_parts<IT, CT>();
+    constexpr float RAISE = KvRaise<BF>::value;
     constexpr int NW = KV_FEW_WAVES, KS = HD / 32, VB = HD / 16;
     static_assert(SP == 1 || (PARTS && SP == HD / KV_GROUP), "a column for each group of a row");
     constexpr int VP = HD * 2 + 16; // bytes of a row of V in LDS: four rows start in different banks
@@ -725,8 +731,8 @@ __global__ void __launch_bounds__(KV_FEW_WAVES * 64, KvType<CT>::code == MLH_CAC
 #pragma unroll
             for (int e = 0; e < 4; e++) mx = kv_max(mx, s[b][e]);
         const float mt = kv_quad_max(mx) * scale;
-        if (__any(mt > m + KV_SLACK)) {
-            const float mn = mt > m + KV_SLACK ? mt : m, corr = m == -INFINITY ? 0.f : kv_exp2(m - mn); // (each row for itself)
+        if (__any(mt > m + (RAISE + KV_SLACK))) {
+            const float mn = mt > m + (RAISE + KV_SLACK) ? mt - RAISE : m, corr = m == -INFINITY ? 0.f : kv_exp2(m - mn); // (each row for itself)
             m = mn;
             l *= corr;
 #pragma unroll
@@ -874,6 +880,7 @@ template <int HD> __device__ __forceinline__ int kv_place_v(int r, int c) { retu
 template <typename IT, typename CT, int HD, int NW>
 __global__ void __launch_bounds__(NW * 64, HD == 64 ? 3 : 2) k_kvattn_many(KvAttnArgs A) {
     constexpr bool FOUR = KvType<CT>::code == MLH_CACHE_Q4, BF = !FOUR && KvType<IT>::code == MLH_DTYPE_BF16;
+    constexpr float RAISE = KvRaise<BF>::value;
     constexpr int KS = HD / 16, MB = HD / 32, TB = 64 * HD * 2, QB = NW * 32; // TB: bytes of a tile of K or V
     extern __shared__ __attribute__((aligned(16))) unsigned char lds[]; // K, V of two tiles; keys to repair; a row of V for each wave
     uint32_t* const flags = reinterpret_cast<uint32_t*>(lds + 4 * TB);
@@ -1023,8 +1030,8 @@ __global__ void __launch_bounds__(NW * 64, HD == 64 ? 3 : 2) k_kvattn_many(KvAtt
 #pragma unroll
             for (int e = 0; e < 16; e++) mx = kv_max(mx, s[b][e]);
         const float mt = kv_halves_max(mx) * scale;
-        if (__any(mt > m + KV_SLACK)) {
-            const float mn = mt > m + KV_SLACK ? mt : m, corr = m == -INFINITY ? 0.f : kv_exp2(m - mn); // (each row for itself)
+        if (__any(mt > m + (RAISE + KV_SLACK))) {
+            const float mn = mt > m + (RAISE + KV_SLACK) ? mt - RAISE : m, corr = m == -INFINITY ? 0.f : kv_exp2(m - mn); // (each row for itself)
             m = mn;
             l *= corr;
 #pragma unroll

@@ -4,7 +4,7 @@ import math
 import pytest
 import torch
 
-from kv_oracle import GROUP, quantise
+from kv_oracle import GROUP, U, quantise
 from test_gpu_cache import KINDS, Call
 
 pytestmark = pytest.mark.gpu
@@ -111,3 +111,35 @@ def test_nothing_seen_is_zero(pkg, kind, cache, new, lens):
     c.dq[0], c.dq[1] = math.nan, math.inf
     got = c.run()
     assert (got[:3] == 0).all() and not (got[3:] == 0).any(1).all()
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# weights
+# ---------------------------------------------------------------------------------------------------------------------
+HALVES = [("f16", "f16"), ("f16", "q4"), ("bf16", "q4")]
+
+
+@pytest.mark.parametrize("kind,cache", HALVES)
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("new", [1, 6, 80])
+def test_small_weights_of_a_long_sequence(pkg, kind, cache, hd, new):
+    """One key whose score is 17 above those of 60000 others that make up the whole result, 60000 e^-17 = 0.0025: each weight is below half a step of the smallest halves.
+    Weights are held to 2^-32 of the largest at least; maxLen keeps the keys in one workgroup, as they are in a call of many sequences."""
+    n = 60000
+    c = Call(pkg, kind, cache, 1, 1, hd, [new], [n], seed=53)
+    k, v = torch.zeros(n, 1, hd), torch.ones(n, 1, hd)
+    k[0], v[0] = 1.0, 0.0
+    _store(c, "k", 0, k)
+    _store(c, "v", 0, v)
+    _query(c, torch.full((new, hd), 17.0 / math.sqrt(hd)))
+    c.args.maxLen = 1
+    c.work_for(c.args)
+    assert c.args.workBytes == 0
+    got = c.run().double()
+    q = c.q.double()[0, 0]
+    for i in range(new):
+        others = (n - new + i) * math.exp(-float(q) * hd * c.scale)
+        want = others / (1 + others)
+        # scores of equal products: hd + 4 roundings; weights: 2^-32 of the largest each, or 2^-11 of their own size, the coarser one
+        bound = U[kind] * want + want * (2 * 17 * (hd + 4) * 2.0 ** -24 + U["f16"] + 2.0 ** -18) + (n - new + i) * 2.0 ** -32 + (2.0 ** -25 if kind == "f16" else 0)
+        assert ((got[i] - want).abs() <= bound).all(), (i, got[i, 0].item(), want, bound)
