@@ -472,6 +472,10 @@ template <bool BF> __device__ __forceinline__ uint32_t kv_pack(float a, float b)
     if constexpr (BF) { typedef __bf16 bf16x2 __attribute__((ext_vector_type(2))); return __builtin_bit_cast(uint32_t, bf16x2{(__bf16)a, (__bf16)b}); }
     else return pack_f16(a, b);
 }
+template <bool BF> __device__ __forceinline__ float kv_add2(uint32_t w, float sum) { // two 16-bit numbers onto a sum
+    if constexpr (BF) { typedef __bf16 bf16x2 __attribute__((ext_vector_type(2))); return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, w), bf16x2{(__bf16)1.f, (__bf16)1.f}, sum, false); }
+    else return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, w), f16x2{(_Float16)1.f, (_Float16)1.f}, sum, false);
+}
 __device__ __forceinline__ u32x2 lds_transposed(const void* p) { // 4 rows x 16 columns of 16 bits from 16 lanes' addresses
     return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p));
 }
@@ -742,10 +746,7 @@ __global__ void __launch_bounds__(KV_FEW_WAVES * 64, KvType<CT>::code == MLH_CAC
 #pragma unroll
         for (int b = 0; b < 2; b++)
 #pragma unroll
-            for (int e = 0; e < 4; e++) { // (hidden: 2^-inf)
-                p[b][e] = kv_exp2(fmaf(s[b][e], scale, -ref));
-                l += p[b][e];
-            }
+            for (int e = 0; e < 4; e++) p[b][e] = kv_exp2(fmaf(s[b][e], scale, -ref)); // (hidden: 2^-inf)
         if (repair) {
 #pragma unroll
             for (int b = 0; b < 2; b++) {
@@ -778,6 +779,11 @@ __global__ void __launch_bounds__(KV_FEW_WAVES * 64, KvType<CT>::code == MLH_CAC
         if constexpr (PARTS) {
             auto left = [&](uint32_t w, float a, float b) { return pack_f16(a - kv_half(w & 0xffffu), b - kv_half(w >> 16)); };
             rest = u32x4{left(pw.x, p[0][0], p[0][1]), left(pw.y, p[0][2], p[0][3]), left(pw.z, p[1][0], p[1][1]), left(pw.w, p[1][2], p[1][3])};
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) { // (the weights as the products have them)
+            l = kv_add2<BF>(pw[i], l);
+            if constexpr (PARTS) l = kv_add2<BF>(rest[i], l);
         }
         // lane i of a group of 16 gives the address of row i / 4, columns 4 (i % 4) ..
         const unsigned char* va = vt + (4 * g + (n >> 2)) * VP + (n & 3) * 8;
@@ -865,10 +871,6 @@ __global__ void __launch_bounds__(KV_FEW_WAVES * 64, KvType<CT>::code == MLH_CAC
 // of 64: 101 us, 0.51 PFLOP/s (an exponential and its conversion for every 256 operations of the products).
 // ----------------------------------------------------------------------------
 typedef float f32x16 __attribute__((ext_vector_type(16)));
-template <bool BF> __device__ __forceinline__ float kv_add2(uint32_t w, float sum) { // two 16-bit numbers onto a sum
-    if constexpr (BF) { typedef __bf16 bf16x2 __attribute__((ext_vector_type(2))); return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, w), bf16x2{(__bf16)1.f, (__bf16)1.f}, sum, false); }
-    else return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, w), f16x2{(_Float16)1.f, (_Float16)1.f}, sum, false);
-}
 template <bool BF> __device__ __forceinline__ f32x16 mfma32(const u32x4& a, const u32x4& b, const f32x16& c) {
     if constexpr (BF) return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
     else return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);

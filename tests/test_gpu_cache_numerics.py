@@ -143,3 +143,24 @@ def test_small_weights_of_a_long_sequence(pkg, kind, cache, hd, new):
         # scores of equal products: hd + 4 roundings; weights: 2^-32 of the largest each, or 2^-11 of their own size, the coarser one
         bound = U[kind] * want + want * (2 * 17 * (hd + 4) * 2.0 ** -24 + U["f16"] + 2.0 ** -18) + (n - new + i) * 2.0 ** -32 + (2.0 ** -25 if kind == "f16" else 0)
         assert ((got[i] - want).abs() <= bound).all(), (i, got[i, 0].item(), want, bound)
+
+
+@pytest.mark.parametrize("kind,cache", KINDS)
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("new,lens", [([1], [700]), ([6, 1], [300, 5000]), ([90], [400])])
+def test_weights_sum_to_one(pkg, kind, cache, hd, new, lens):
+    """Values that are all one: the result is one, whatever the weights are rounded to, as what is summed is what is multiplied.  (fp32 sums of both in their orders: off by a few
+    2^-24 for each key, which a 16-bit result does not show; fp32 rows by twice that.)  One key in 16 weighs 1, the others 1/2 (1 + 0.45 steps): rounded, all err to one side."""
+    weight = 0.5 * (1 + 0.45 * 2 * U[kind if cache == kind else "f16"])
+    c = Call(pkg, kind, cache, 1, 1, hd, new, lens, seed=54, scale=-math.log(weight) / hd)
+    for s, n in enumerate(lens):
+        k = torch.full((n, 1, hd), -1.0)
+        k[3::16] = 0.0
+        _store(c, "k", s, k)
+        _store(c, "v", s, torch.ones(n, 1, hd))
+    _query(c, torch.ones(c.rows.used, hd))
+    got = c.run().double()[:c.rows.used]
+    if kind == "f32":
+        assert ((got - 1).abs() <= 2 * max(lens) * 2.0 ** -24).all()
+    else:
+        assert (got == 1).all(), (got - 1).abs().max().item()
