@@ -202,9 +202,9 @@ extern "C" uint64_t mlh_kv_page_bytes(int type, int heads, int headDim) {
     return kv_float_type(type) ? (uint64_t)MLH_KV_PAGE * heads * headDim * kv_elem_bytes(type) : 0;
 }
 
-int kv_launched() {
-    const hipError_t e = hipGetLastError();
+int kv_status(hipError_t e) {
     if (e == hipSuccess) return 0;
+    (void)hipGetLastError(); // (reported here)
     mlh_set_thread_error(std::string("launch failed: ") + hipGetErrorString(e));
     return -2;
 }
@@ -232,21 +232,17 @@ extern "C" int mlh_kv_append_device(const mlh_kv_cache* c, const mlh_kv_batch* b
     const dim3 grid(kv_grid(b->rows, pieces), pieces);
     const bool nt = (double)b->rows * (b->heads + 2 * c->heads) * hd * kv_elem_bytes(b->type) > 32e6; // eight L2s of 4 MB
 #define KV_GO(IT_, CT_) \
-    do { \
-        if (hd == 64 && nt) hipLaunchKernelGGL((k_kv_append<IT_, CT_, 64, true>), grid, dim3(KV_WG), 0, (hipStream_t)stream, A); \
-        else if (hd == 64) hipLaunchKernelGGL((k_kv_append<IT_, CT_, 64, false>), grid, dim3(KV_WG), 0, (hipStream_t)stream, A); \
-        else if (nt) hipLaunchKernelGGL((k_kv_append<IT_, CT_, 128, true>), grid, dim3(KV_WG), 0, (hipStream_t)stream, A); \
-        else hipLaunchKernelGGL((k_kv_append<IT_, CT_, 128, false>), grid, dim3(KV_WG), 0, (hipStream_t)stream, A); \
-    } while (0)
+    return kv_launch(hd == 64 ? (nt ? &k_kv_append<IT_, CT_, 64, true> : &k_kv_append<IT_, CT_, 64, false>) \
+                              : (nt ? &k_kv_append<IT_, CT_, 128, true> : &k_kv_append<IT_, CT_, 128, false>), grid, KV_WG, 0, stream, A)
     if (c->type == MLH_CACHE_Q4) {
         if (b->type == MLH_DTYPE_F32) KV_GO(float, q4_t);
-        else if (b->type == MLH_DTYPE_BF16) KV_GO(bf16_t, q4_t);
-        else KV_GO(f16_t, q4_t);
-    } else if (b->type == MLH_DTYPE_F32) KV_GO(float, float);
-    else if (b->type == MLH_DTYPE_BF16) KV_GO(bf16_t, bf16_t);
-    else KV_GO(f16_t, f16_t);
+        if (b->type == MLH_DTYPE_BF16) KV_GO(bf16_t, q4_t);
+        KV_GO(f16_t, q4_t);
+    }
+    if (b->type == MLH_DTYPE_F32) KV_GO(float, float);
+    if (b->type == MLH_DTYPE_BF16) KV_GO(bf16_t, bf16_t);
+    KV_GO(f16_t, f16_t);
 #undef KV_GO
-    return kv_launched();
 }
 
 extern "C" int mlh_kv_read_device(const mlh_kv_cache* c, const mlh_kv_batch* b, const mlh_kv_read* a, void* stream) {
@@ -261,22 +257,17 @@ extern "C" int mlh_kv_read_device(const mlh_kv_cache* c, const mlh_kv_batch* b, 
     KvReadArgs A = {kv_rows_of(c, b), c->k, c->v, a->k, a->v, a->stride};
     const int pieces = (2 * c->heads * (hd / 8) + KV_WG - 1) / KV_WG;
     const dim3 grid(kv_grid(b->rows, pieces), pieces);
-#define KV_GO2(OT_, CT_) \
-    do { \
-        if (hd == 64) hipLaunchKernelGGL((k_kv_read<OT_, CT_, 64>), grid, dim3(KV_WG), 0, (hipStream_t)stream, A); \
-        else hipLaunchKernelGGL((k_kv_read<OT_, CT_, 128>), grid, dim3(KV_WG), 0, (hipStream_t)stream, A); \
-    } while (0)
+#define KV_GO2(OT_, CT_) return kv_launch(hd == 64 ? &k_kv_read<OT_, CT_, 64> : &k_kv_read<OT_, CT_, 128>, grid, KV_WG, 0, stream, A)
 #define KV_GO(CT_) \
     do { \
         if (b->type == MLH_DTYPE_F32) KV_GO2(float, CT_); \
-        else if (b->type == MLH_DTYPE_BF16) KV_GO2(bf16_t, CT_); \
-        else KV_GO2(f16_t, CT_); \
+        if (b->type == MLH_DTYPE_BF16) KV_GO2(bf16_t, CT_); \
+        KV_GO2(f16_t, CT_); \
     } while (0)
     if (c->type == MLH_CACHE_Q4) KV_GO(q4_t);
-    else if (c->type == MLH_DTYPE_F32) KV_GO(float);
-    else if (c->type == MLH_DTYPE_BF16) KV_GO(bf16_t);
-    else KV_GO(f16_t);
+    if (c->type == MLH_DTYPE_F32) KV_GO(float);
+    if (c->type == MLH_DTYPE_BF16) KV_GO(bf16_t);
+    KV_GO(f16_t);
 #undef KV_GO
 #undef KV_GO2
-    return kv_launched();
 }

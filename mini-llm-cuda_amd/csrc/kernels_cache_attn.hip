@@ -1270,30 +1270,27 @@ static AttnPlan attn_plan(const mlh_kv_cache* c, const mlh_kv_batch* b, const ml
 // A workgroup has 16 rows at most, and nsplit times their number is below KV_SPLIT_WGS and once more their own, which is below that where keys are split.
 size_t mlh_attention_work_most(int headDim) { return (size_t)2 * KV_SPLIT_WGS * 16 * (headDim + 2) * 4; }
 
-template <typename IT, typename CT, int HD, int NW> static hipError_t launch_many(dim3 grid, hipStream_t st, const KvAttnArgs& A) {
+template <typename IT, typename CT, int HD, int NW> static int launch_many(dim3 grid, void* stream, const KvAttnArgs& A) {
     constexpr int bytes = 4 * 64 * HD * 2 + 32 + NW * HD * 4;
     if (bytes > 65536) { // (asked for on every call: the attribute belongs to the device that is current)
         const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&k_kvattn_many<IT, CT, HD, NW>), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
-        if (e != hipSuccess) return e;
+        if (e != hipSuccess) return kv_status(e);
     }
-    hipLaunchKernelGGL((k_kvattn_many<IT, CT, HD, NW>), grid, dim3(NW * 64), bytes, st, A);
-    return hipSuccess;
+    return kv_launch(&k_kvattn_many<IT, CT, HD, NW>, grid, NW * 64, bytes, stream, A);
 }
 
-template <typename IT, int HD> static void launch_join(hipStream_t st, const KvAttnArgs& A) {
+template <typename IT, int HD> static int launch_join(void* stream, const KvAttnArgs& A) {
     const unsigned n = (unsigned)(A.rows * A.heads), per = 256 / (HD / 4);
-    if (A.nsplit <= KV_JOIN_FEW) hipLaunchKernelGGL((k_kvattn_join_few<IT, HD>), dim3((n + per - 1) / per), dim3(256), 0, st, A);
-    else if (A.nsplit <= 64) hipLaunchKernelGGL((k_kvattn_join<IT, HD, 64>), dim3(n), dim3(256), 0, st, A);
-    else hipLaunchKernelGGL((k_kvattn_join<IT, HD, KV_MAX_SPLIT>), dim3(n), dim3(256), 0, st, A);
+    if (A.nsplit <= KV_JOIN_FEW) return kv_launch(&k_kvattn_join_few<IT, HD>, dim3((n + per - 1) / per), 256, 0, stream, A);
+    return kv_launch(A.nsplit <= 64 ? &k_kvattn_join<IT, HD, 64> : &k_kvattn_join<IT, HD, KV_MAX_SPLIT>, dim3(n), 256, 0, stream, A);
 }
-static int launch_join(hipStream_t st, int type, int hd, const KvAttnArgs& A) {
+static int launch_join(void* stream, int type, int hd, const KvAttnArgs& A) {
     if (A.nsplit == 1) return 0;
-#define JOIN(IT_) do { if (hd == 64) launch_join<IT_, 64>(st, A); else launch_join<IT_, 128>(st, A); } while (0)
+#define JOIN(IT_) return hd == 64 ? launch_join<IT_, 64>(stream, A) : launch_join<IT_, 128>(stream, A)
     if (type == MLH_DTYPE_F32) JOIN(float);
-    else if (type == MLH_DTYPE_BF16) JOIN(bf16_t);
-    else JOIN(f16_t);
+    if (type == MLH_DTYPE_BF16) JOIN(bf16_t);
+    JOIN(f16_t);
 #undef JOIN
-    return kv_launched();
 }
 
 extern "C" uint64_t mlh_attention_work_bytes(const mlh_kv_cache* c, const mlh_kv_batch* b, const mlh_attention* a) {
@@ -1312,35 +1309,22 @@ extern "C" int mlh_attention_device(const mlh_kv_cache* c, const mlh_kv_batch* b
     const KvAttnArgs A = {c->k, c->v, c->table, b->start, b->len, a->q, a->out, (float*)a->work, a->qStride, a->outStride, c->nseq, b->rows, b->heads, c->heads, b->heads / c->heads,
                           c->pagesPerSeq, c->numPages, a->window, a->sinks, P.nsplit, (a->scale > 0.f ? a->scale : 1.0f / sqrtf((float)hd)) * 1.44269504088896341f};
     const dim3 grid = P.many ? dim3(c->heads * P.blocks, P.nsplit) : dim3(c->heads * P.blocks * P.nsplit);
-    hipStream_t st = (hipStream_t)stream;
+    int rc;
     if (P.many) {
-        hipError_t e;
-#define MANY(IT_, CT_) (hd == 64 ? launch_many<IT_, CT_, 64, 4>(grid, st, A) : launch_many<IT_, CT_, 128, 4>(grid, st, A))
-        if (b->type == MLH_DTYPE_BF16) e = c->type == MLH_CACHE_Q4 ? MANY(bf16_t, q4_t) : MANY(bf16_t, bf16_t);
-        else e = c->type == MLH_CACHE_Q4 ? MANY(f16_t, q4_t) : MANY(f16_t, f16_t);
+#define MANY(IT_, CT_) (hd == 64 ? launch_many<IT_, CT_, 64, 4>(grid, stream, A) : launch_many<IT_, CT_, 128, 4>(grid, stream, A))
+        if (b->type == MLH_DTYPE_BF16) rc = c->type == MLH_CACHE_Q4 ? MANY(bf16_t, q4_t) : MANY(bf16_t, bf16_t);
+        else rc = c->type == MLH_CACHE_Q4 ? MANY(f16_t, q4_t) : MANY(f16_t, f16_t);
 #undef MANY
-        if (e != hipSuccess) { mlh_set_thread_error(std::string("launch failed: ") + hipGetErrorString(e)); return -2; }
     } else if (b->type == MLH_DTYPE_F32) {
-#define F32_ROWS(CT_, HD_) hipLaunchKernelGGL((k_kvattn_f32<CT_, HD_>), grid, dim3(KV_F32_WAVES * 64), 0, st, A)
-        if (c->type == MLH_CACHE_Q4) { if (hd == 64) F32_ROWS(q4_t, 64); else F32_ROWS(q4_t, 128); }
-        else { if (hd == 64) F32_ROWS(float, 64); else F32_ROWS(float, 128); }
+#define F32_ROWS(CT_) kv_launch(hd == 64 ? &k_kvattn_f32<CT_, 64> : &k_kvattn_f32<CT_, 128>, grid, KV_F32_WAVES * 64, 0, stream, A)
+        rc = c->type == MLH_CACHE_Q4 ? F32_ROWS(q4_t) : F32_ROWS(float);
 #undef F32_ROWS
     } else {
-#define FEW(IT_, CT_) \
-    do { \
-        if (hd == 64) hipLaunchKernelGGL((k_kvattn_few<IT_, CT_, 64, SP64>), grid, dim3(KV_FEW_WAVES * 64), 0, st, A); \
-        else hipLaunchKernelGGL((k_kvattn_few<IT_, CT_, 128, SP64 * SP64>), grid, dim3(KV_FEW_WAVES * 64), 0, st, A); \
-    } while (0)
-        if (P.rowsPer < 16) {
-            constexpr int SP64 = 2; // (4 for heads of 128)
-            FEW(f16_t, q4_t);
-        } else {
-            constexpr int SP64 = 1;
-            if (b->type == MLH_DTYPE_BF16) { if (c->type == MLH_CACHE_Q4) FEW(bf16_t, q4_t); else FEW(bf16_t, bf16_t); }
-            else { if (c->type == MLH_CACHE_Q4) FEW(f16_t, q4_t); else FEW(f16_t, f16_t); }
-        }
+#define FEW(IT_, CT_, SP64_) kv_launch(hd == 64 ? &k_kvattn_few<IT_, CT_, 64, SP64_> : &k_kvattn_few<IT_, CT_, 128, SP64_ * SP64_>, grid, KV_FEW_WAVES * 64, 0, stream, A)
+        if (P.rowsPer < 16) rc = FEW(f16_t, q4_t, 2); // (spread: a column for each of 2 groups, 4 for heads of 128)
+        else if (b->type == MLH_DTYPE_BF16) rc = c->type == MLH_CACHE_Q4 ? FEW(bf16_t, q4_t, 1) : FEW(bf16_t, bf16_t, 1);
+        else rc = c->type == MLH_CACHE_Q4 ? FEW(f16_t, q4_t, 1) : FEW(f16_t, f16_t, 1);
 #undef FEW
     }
-    if (const int rc = kv_launched()) return rc;
-    return launch_join(st, b->type, hd, A);
+    return rc ? rc : launch_join(stream, b->type, hd, A);
 }

@@ -98,5 +98,10 @@ __device__ __forceinline__ void kv_values8(uint32_t codes, uint32_t params, floa
 std::string kv_check(const mlh_kv_cache* cache, const mlh_kv_batch* batch, bool anyType);
 std::string kv_check_rows(const char* what, const void* p, long long stride, long long width, int type);
 int kv_fail(const std::string& msg); // -1, with the text for mlh_last_error(NULL)
-int kv_launched();                    // 0, or -2 and the text of what the last launch left
+int kv_status(hipError_t e);         // of a launch: 0, or -2, with the text
+// What this launch returned, and not hipGetLastError, which also gives what an earlier call of the program left.
+template <typename Args> int kv_launch(void (*kernel)(Args), dim3 grid, int threads, size_t lds, void* stream, const Args& a) {
+    void* args[] = {const_cast<Args*>(&a)};
+    return kv_status(hipLaunchKernel(reinterpret_cast<const void*>(kernel), grid, dim3(threads), args, lds, (hipStream_t)stream));
+}
 inline size_t kv_elem_bytes(int type) { return type == MLH_DTYPE_F32 ? 4 : 2; }
