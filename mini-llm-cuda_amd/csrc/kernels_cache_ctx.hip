@@ -28,15 +28,18 @@ static int* cache_start(const mlh_ctx* c) { return c->cacheMeta; }
 static int* cache_len(const mlh_ctx* c) { return c->cacheMeta + c->hp.maxSeqs + 1; }
 static int* cache_table(const mlh_ctx* c) { return c->cacheMeta + 2 * c->hp.maxSeqs + 1; }
 
-static int prepare(mlh_ctx* c) {
-    if (c->cacheMeta) return 0;
+// Tables of the calls, and room for the shares of split keys: each is kept from its first need on (a second try after a failure finds what the first one got).
+static int prepare(mlh_ctx* c, bool attention) {
     const size_t S = c->hp.maxSeqs;
-    void *meta = nullptr, *work = nullptr;
-    int rc = mlh_dev_alloc_bytes(c, &meta, (2 * S + 1 + S * c->pagesPerSeq) * 4);
-    if (rc == 0) rc = mlh_dev_alloc_bytes(c, &work, mlh_attention_work_most(c->hp.headDim));
-    if (rc) return rc;
-    c->cacheMeta = (int*)meta;
-    c->cacheWork = work;
+    void* p = nullptr;
+    if (!c->cacheMeta) {
+        if (const int rc = mlh_dev_alloc_bytes(c, &p, (2 * S + 1 + S * c->pagesPerSeq) * 4)) return rc;
+        c->cacheMeta = (int*)p;
+    }
+    if (attention && !c->cacheWork) {
+        if (const int rc = mlh_dev_alloc_bytes(c, &p, mlh_attention_work_most(c->hp.headDim))) return rc;
+        c->cacheWork = p;
+    }
     return 0;
 }
 
@@ -114,7 +117,7 @@ extern "C" int mlh_set_attention_window(mlh_ctx* c, int window, int sinks) {
     if (!c) return -1;
     if (window < 0 || sinks < 0) { c->err = "window and sinks must not be negative"; return -1; }
     (void)hipSetDevice(c->device);
-    if (const int rc = prepare(c)) return rc;
+    if (const int rc = window ? prepare(c, true) : 0) return rc;
     mlh_drop_graphs(c); // recorded launches hold the old values
     c->window = window;
     c->sinks = window ? sinks : 0;
@@ -128,7 +131,7 @@ extern "C" int mlh_set_kv_type(mlh_ctx* c, int type) {
     for (int n : c->h_len)
         if (n > 0) { c->err = "the type of the pages can be changed while all sequences are empty (mlh_reset)"; return -1; }
     (void)hipSetDevice(c->device);
-    if (const int rc = prepare(c)) return rc;
+    if (const int rc = type == MLH_CACHE_Q4 ? prepare(c, true) : 0) return rc;
     const size_t bytes = (size_t)c->hp.maxSeqs * c->pagesPerSeq * mlh_kv_page_bytes(type, c->hp.attnHeads, c->hp.headDim);
     std::vector<void*> fresh; // the new pools first: the context stays as it is when they do not fit
     auto drop = [&]() { for (void* p : fresh) (void)hipFree(p); };
@@ -164,7 +167,7 @@ extern "C" int mlh_read_kv(mlh_ctx* c, int layer, int seq, int pos, int n, float
     if (seq < 0 || seq >= c->hp.maxSeqs) { c->err = "sequence index out of range"; return -1; }
     if (!k || !v || pos < 0 || n <= 0 || n > c->h_len[seq] || pos > c->h_len[seq] - n) { c->err = "positions beyond what the sequence holds, or a null output"; return -1; }
     (void)hipSetDevice(c->device);
-    if (const int rc = prepare(c)) return rc;
+    if (const int rc = prepare(c, false)) return rc;
     const size_t d = c->hp.dim, bytes = (size_t)n * d * 4;
     float* tmp = nullptr;
     MLH_CHECK(c, hipStreamSynchronize(c->stream));

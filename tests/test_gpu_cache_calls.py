@@ -1,10 +1,12 @@
 """Calls around the operators on a paged K/V cache."""
 import ctypes
 
+import numpy as np
 import pytest
 import torch
 
 from test_gpu_cache import Append, Call, _same_bits, _stream
+from test_gpu_cache_context import _hp, _model
 from kv_oracle import TORCH
 
 pytestmark = pytest.mark.gpu
@@ -38,3 +40,25 @@ def test_errors_of_earlier_calls(pkg):
     torch.cuda.synchronize()
     a.expect()
     assert _same_bits(a.pools.dk.cpu(), a.pools.k) and torch.equal(c.out.cpu(), want)
+
+
+def test_reading_rows_keeps_no_workspace(pkg):
+    """A context that reads its rows back, or sets the window that it has, keeps a few words of tables for it and not the memory that split keys need."""
+    hp = _hp(pkg, 1, 128, 4, maxL=200)
+    work = 2 * 768 * 16 * (128 + 2) * 4  # what shares of split keys need
+    tokens = np.arange(30, dtype=np.int32)
+    kept = []
+    for _ in range(2):  # (the first context loads code)
+        dev = pkg.Device(hp, 0)
+        dev.upload(_model(pkg, hp))
+        dev.prefill(0, tokens)
+        torch.cuda.synchronize()
+        before = torch.cuda.mem_get_info()[0]
+        dev.set_attention_window(0, 0)
+        dev.read_kv(0, 0, 0, 30)
+        kept.append(before - torch.cuda.mem_get_info()[0])
+        dev.set_attention_window(20, 2)
+        dev.prefill(0, tokens)
+        assert np.isfinite(dev.logits(0)).all()
+        dev.close()
+    assert kept[1] < work // 2, kept
