@@ -164,3 +164,90 @@ def test_weights_sum_to_one(pkg, kind, cache, hd, new, lens):
         assert ((got - 1).abs() <= 2 * max(lens) * 2.0 ** -24).all()
     else:
         assert (got == 1).all(), (got - 1).abs().max().item()
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# few fp16 rows over 4-bit pages: K as it is, weights to 22 bits
+# ---------------------------------------------------------------------------------------------------------------------
+FORMS = [(1, 1, 64), (1, 1, 128), (1, 20, 64), (1, 20, 128), (20, 1, 64), (20, 1, 128)]  # query heads, rows of a sequence, head size: a column for each group (the first two); 16 rows a workgroup
+
+
+def _few(c, seq, keys, weights):
+    """Results [n, H, hd] of a sequence in 64 bits, and their bound: K as the codes have it, weights to 2^-22 of their size or 2^-32 of the largest, values that are halves.
+    Scores: fp32 sums of minimum * (sum of the row's elements) and of code * scale * element in two parts, a rounding of that size for each element that is not zero and 16 more;
+    the row's sum as two halves, and elements of the row below 2^-24 of its largest.  keys: what the scores are of; weights: what is done to them (a mistake to be found)."""
+    r0, n = int(c.rows.start[seq]), c.rows.new[seq]
+    q = c.q[r0:r0 + n, :c.H * c.hd].double().unflatten(1, (c.H, c.hd))
+    k, v = keys[:, 0], c.vals[seq][:, 0]
+    low = k.unflatten(-1, (-1, GROUP)).amin(-1, keepdim=True).expand(-1, -1, GROUP).flatten(1)
+    want, bound = torch.zeros(n, c.H, c.hd, dtype=torch.float64), torch.zeros(n, c.H, c.hd, dtype=torch.float64)
+    for i in range(n):
+        at = c.rows.lens[seq] - n + i + 1
+        for h in range(c.H):
+            s = k[:at] @ q[i, h] * c.scale
+            size = (low[:at].abs() + (k - low)[:at].abs()) @ q[i, h].abs() * c.scale
+            ds = size * (2 * int((q[i, h] != 0).sum()) + 16) * 2.0 ** -24 + 2.0 ** -22 * (low[:at].abs() @ q[i, h].abs()) * c.scale
+            ds = ds + 2.0 ** -24 * q[i, h].abs().max() * (low.abs() + (k - low))[:at].sum(1) * c.scale + s.abs().max() * 2.0 ** -22
+            p = weights(torch.exp(s - s.max()))
+            l = p.sum()
+            p = p / l
+            want[i, h] = p @ v[:at]
+            e = 2.0 ** -22 + 2 * (ds + (p * ds).sum()) + (at ** 0.5 + 16) * 2.0 ** -22
+            bound[i, h] = (p * e) @ v[:at].abs() + 2.0 ** -32 / l * v[:at].abs().sum(0) + U["f16"] * want[i, h].abs() + 2.0 ** -25
+    return want, bound
+
+
+def _found(c, got, keys=lambda k: k, weights=lambda p: p):
+    """The largest difference from that, in bounds."""
+    worst = 0.0
+    for s, n in enumerate(c.rows.new):
+        want, bound = _few(c, s, keys(c.keys[s]), weights)
+        g = got[int(c.rows.start[s]):int(c.rows.start[s]) + n, :c.H * c.hd].double().unflatten(1, (c.H, c.hd))
+        worst = max(worst, ((g - want).abs() / bound).nan_to_num(1e9).max().item())
+    return worst
+
+
+def _two_of_a_row(gen, c):
+    """Rows of two elements that are not zero: the roundings of longer sums would hide what is looked for."""
+    q = torch.randn(c.rows.used, c.H, c.hd, generator=gen)
+    some = torch.rand(c.rows.used, c.H, c.hd, generator=gen).argsort(-1) < 2
+    return torch.where(some, q, torch.zeros_like(q)).flatten(1)
+
+
+@pytest.mark.parametrize("H,rows,hd", FORMS)
+def test_weights_of_few_rows(pkg, H, rows, hd):
+    """Keys in pairs with almost the same score and opposite values, so that the result is a small difference of large sums: weights of 11 bits would miss the bound."""
+    lens = [rows + i % 10 for i in range(1, 41)] if rows == 1 else [rows + 2 * i for i in range(1, 13)]
+    c = Call(pkg, "f16", "q4", H, 1, hd, [rows] * len(lens), lens, seed=55, scale=0.1)
+    gen = torch.Generator().manual_seed(56)
+    for s, n in enumerate(lens):
+        k = torch.randn((n + 1) // 2, 1, hd, generator=gen).repeat_interleave(2, 0)
+        k[1::2] *= 1.01
+        v = torch.where(torch.rand((n + 1) // 2, 1, hd // GROUP, generator=gen) < 0.5, 1.0, -1.0).repeat_interleave(2, 0)
+        v[1::2] *= -1
+        _store(c, "k", s, k[:n])
+        _store(c, "v", s, v.repeat_interleave(GROUP, -1)[:n])  # (one value a group: exact)
+        assert (c.vals[s].abs() == 1).all()
+    _query(c, _two_of_a_row(gen, c))
+    got = c.run()
+    assert _found(c, got) <= 1
+    assert _found(c, got, weights=lambda p: p.half().double()) > 2
+
+
+@pytest.mark.parametrize("H,rows,hd", FORMS)
+@pytest.mark.parametrize("low,span,scale,spread", [(1000.0, 2.0, 0.1, 1.0), (-40000.0, 80000.0, 1e-3, 0.02), (0.0, 1e-5, 2.0 ** 16, 1.0), (0.25, 3e-4, 2.0 ** 9, 1.0)])
+def test_keys_of_few_rows(pkg, H, rows, hd, low, span, scale, spread):
+    """Keys whose differences halves would lose (from 1000 to 1002), whose groups span more than they hold, and with scales below the normal halves: taken as they are."""
+    lens = [rows + i % 10 for i in range(1, 41)] if rows == 1 else [rows + 3 * i for i in range(1, 13)]
+    c = Call(pkg, "f16", "q4", H, 1, hd, [rows] * len(lens), lens, seed=57, scale=scale / 8)
+    gen = torch.Generator().manual_seed(58)
+    for s, n in enumerate(lens):
+        x = torch.rand(n, 1, hd // GROUP, GROUP, generator=gen)
+        x[..., 3], x[..., 9] = 0.0, 1.0
+        _store(c, "k", s, (low + span * x).flatten(2))
+        _store(c, "v", s, torch.where(torch.rand(n, 1, hd // GROUP, generator=gen) < 0.5, 1.0, -1.0).repeat_interleave(GROUP, -1))
+    _query(c, _two_of_a_row(gen, c) * spread)
+    got = c.run()
+    assert _found(c, got) <= 1
+    if low > 0:
+        assert _found(c, got, keys=lambda k: k.half().double()) > 2
