@@ -250,10 +250,12 @@ int mlh_debug_inject_abort_at_step(mlh_ctx* ctx, int step);
 int mlh_debug_set_xcd_tag(mlh_ctx* ctx, unsigned tagsUsed);
 
 /* Attention layers that forget: with window > 0 a position sees the `window` positions up to its own and the first `sinks`
- * positions of its sequence (mlh_attention_device); 0 (the default): everything before it.  From the next call on; what the pages hold stays, so a window can be widened
- * again.  mlh_set_kv_type: what the pages of the attention layers are, MLH_DTYPE_F32 (the default) or MLH_CACHE_Q4 (mlh_kv_append_device: 5 bits an
- * element instead of 32); all sequences must be empty, and the pools are allocated anew.  With either, decode runs as the kernel sequence (the single-launch modes know neither), and attention is that of
- * mlh_kv_append_device and mlh_attention_device in fp32, in prefills too.  (No counterpart in the reference, whose attention recomputes every column, inference.cu:511-573.) */
+ * positions of its sequence (mlh_attention_device); 0 (the default): everything before it.  From the next call on; what the pages
+ * hold stays, so a window can be widened again.  mlh_set_kv_type: what the pages of the attention layers are, MLH_DTYPE_F32 (the
+ * default) or MLH_CACHE_Q4 (mlh_kv_append_device: 5 bits an element instead of 32); all sequences must be empty, and the pools are
+ * allocated anew.  With either, decode runs as the kernel sequence (the single-launch modes know neither; one sequence then takes
+ * two to three times as long a token), and attention is that of mlh_kv_append_device and mlh_attention_device in fp32, in prefills
+ * too.  (No counterpart in the reference, whose attention recomputes every column, inference.cu:511-573.) */
 int mlh_set_attention_window(mlh_ctx* ctx, int window, int sinks);
 int mlh_set_kv_type(mlh_ctx* ctx, int type);
 /* K and V rows [n, dim] of positions pos .. pos + n - 1 of a sequence as an attention layer's pages hold them (layer: FILE block index; after per-head
@@ -437,8 +439,9 @@ int mlh_kv_read_device(const mlh_kv_cache* cache, const mlh_kv_batch* batch, con
  * largest), and k's values, except in calls of fp16 rows whose maxNew * heads / cache.heads is at most 64: these take k as it is and the weights to 22 bits.  A weight that is held in
  * halves, one or two, is off by 2^-32 of the row's largest at least.
  * Values of 4-bit pages beyond the halves' range count as infinite where they are rounded to halves; a group whose scale is an infinity or NaN counts as NaN or infinite.
- * maxLen, maxNew: what no len and no number of rows of a sequence exceeds (0: the page table's, rows).  They decide which kernel runs and how the work is split; a call that
- * exceeds them is right, and slower.
+ * maxLen, maxNew: what no len and no number of rows of a sequence exceeds (0: the page table's, rows).  They decide which kernel runs and how the work is split, and with that the
+ * order of sums and, of fp16 rows over 4-bit pages, what K and the weights are rounded to (above): a token inside a prompt and the same token alone differ by that.  A call
+ * that exceeds them is right, and slower.  Calls of more than 64 sequences take them in their order: the longest are best brought first.
  * work: mlh_attention_work_bytes() bytes (of the same structures; 0: none), 16-byte aligned, undefined before and after, not shared by calls that may overlap. */
 typedef struct {
     const void* q;

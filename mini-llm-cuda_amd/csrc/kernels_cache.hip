@@ -34,8 +34,8 @@ struct KvAppendArgs {
     int ropeRows;
 };
 
-// The code of x: the nearest whole number to (x - base) / scale.  The fp32 quotient is off by less than 2^-20 (three roundings of values up to 15, and inv's): only
-// next to a half is it done again in 64 bits.
+// The code of x: the nearest whole number to (x - base) / scale.  The fp32 quotient, up to 16 where it is not clamped, is off by less than 2^-18 (three roundings: difference, inverse
+// and product): only within 1e-4 of a half, 26 times that, is it done again in 64 bits.
 __device__ __forceinline__ uint32_t kv_code(float x, float base, float scale, float inv) {
     const float u = (x - base) * inv;
     float c = rintf(u);
@@ -45,8 +45,9 @@ __device__ __forceinline__ uint32_t kv_code(float x, float base, float scale, fl
 
 // One thread: eight elements of a head's row of q, k or v.  HD / 8 neighbouring threads hold the row (norm), four a group of 32 (4-bit codes).  Grid: rows x pieces of the
 // heads.  Norm and rotation are in 64 bits and rounded once, as the plain form's products of fp32 numbers are exact there.
-// Bound by memory: 17435 rows of 32 + 8 + 8 heads of 128 in bf16, 429 MB read and written, 80 us (5.3 TB/s; a copy of 1 GiB: 5.2).  11071 rows of the same heads in fp16
-// into 4-bit pages 59 us (4.2 TB/s: the codes' arithmetic).  A single token: 2.2 us, the latency of start, table and row in turn.  Streaming stores (NT) for
+// Bound by memory: 17435 rows of 32 + 8 + 8 heads of 128 in bf16, 429 MB read and written, 80 us (5.4 TB/s; a copy of 1 GiB: 5.2).  11071 rows of the same heads in fp16
+// into 4-bit pages 57 to 59 us (240 MB, 4.2 TB/s): the vector ALU, busy in 0.84 of the cycles.  With gains 127 and 85 us, by the norm's arithmetic in 64 bits (a division an element).
+// A single token: 2.2 us, the latency of start, table and row in turn.  Streaming stores (NT) for
 // calls that write more than the L2s hold: 112 us without.  Two, four and eight rows a workgroup, their loads together: 95, 107 and 149 us against 91 for one (all before the row
 // was loaded ahead of the lookup).
 template <typename IT, typename CT, int HD, bool NT>

@@ -57,8 +57,8 @@ template <int QB> __device__ __forceinline__ bool kv_block(const KvAttnArgs& A, 
 }
 
 // The same for calls of at most 64 sequences, the longest ones' blocks first: what starts last is short then, and the numbers without rows come behind all others
-// (64 tokens over 100 to 12000 positions 316 -> 292 us, 60 chunks of up to 120 rows behind up to 2000 139 -> 108).  LAST: of a sequence the last rows first, which see
-// most.  A lane a sequence: the blocks of longer ones are before its own.  From nine on, each of the four waves looks at a quarter of them (64 tokens over 300
+// (64 tokens over 100 to 12000 positions 316 -> 292 us, 60 chunks of up to 120 rows behind up to 2000 139 -> 108).  Beyond 64 it is the caller's order: 65 of those tokens take 342 us
+// in the order of the 64, 332 when the shortest come first and 297 when the longest do.  LAST: of a sequence the last rows first, which see most.  A lane a sequence: the blocks of longer ones are before its own.  From nine on, each of the four waves looks at a quarter of them (64 tokens over 300
 // each: 20 us where every wave looks at all, 17).  For workgroups of four waves, all together.
 template <int QB, bool LAST = false> __device__ __forceinline__ bool kv_block_longest_first(const KvAttnArgs& A, int blk, KvBlock& B) {
     __shared__ int parts[4][64];
@@ -129,8 +129,8 @@ __device__ __forceinline__ bool kv_finite(float v) { return (__float_as_uint(v) 
 __device__ __forceinline__ float kv_exp2(float v) { return __builtin_amdgcn_exp2f(v); }
 // The larger of two (as a median: fmaxf would first quiet both, an instruction each; where one is no number, either, and the row's sum is none then)
 __device__ __forceinline__ float kv_max(float a, float b) { return __builtin_amdgcn_fmed3f(a, b, INFINITY); }
-// The running maximum follows when a score is 2^8 times beyond it and not before (weights up to 256 are as good as up to one, in halves too): with every new maximum, of 32 rows
-// some have one in most tiles, and sums and result are multiplied again (the prompts below: 1071 and 171 us for 1017 and 158).
+// The running maximum follows when a weight is 2^8 times beyond that of the last one and not before: with every new maximum, of 32 rows some have one in most tiles, and sums and
+// result are multiplied again (the prompts below: 1071 and 171 us for 1017 and 158).
 #define KV_SLACK 8.f
 // m is the maximum less KvRaise: a weight is 2^KvRaise at a new maximum, and up to 2^(KvRaise + KV_SLACK) before there is another.
 // Halves: 2^7, the largest then 2^15, so that half of their smallest step, which is what a weight is off by at least, is 2^-32 of the largest weight.  (With 1 for 2^7, of one key and 60000
@@ -454,8 +454,10 @@ __global__ void __launch_bounds__(KV_F32_WAVES * 64, 2) k_kvattn_f32(KvAttnArgs 
 // are minimum + code * scale in halves, one rounding), all products are in halves, and rows are scaled by a power of two first.
 // 16-bit pages are bound by memory: 64 tokens over 100 to 12000 positions, 32 heads on 8 of 128 in bf16, 1.59 GB, 288 us (5.5 TB/s; reads alone reach 6.1); 64 over 3000
 // each 150 us.  Eight waves a workgroup, one of them a compute unit then, before the longest came first: 307 and 170 us for 316 and 156, one token over 4000 17 for 12.  4-bit
-// pages by the instructions that unpack them: one token over 65000 positions, bf16, 21 us (83 MB, 3.9 TB/s); eight waves a workgroup 146 us for 116 (48 tokens, before the
-// spread below).
+// pages by the instructions that unpack them: one token over 65000 positions, bf16, 21 us (83 MB, 3.9 TB/s; the vector ALU busy in 0.58 of the cycles, the rest is the start of 768
+// workgroups of five turns); eight waves a workgroup 146 us for 116 (48 tokens, before the spread below).
+// Weights are rounded to 16 bits for the second product, and summed as rounded: errors against the results' norm 2.1e-3 (bf16) and 2.8e-4 (fp16) where rounding the results alone gives
+// 1.7e-3 and 2.1e-4.  In two parts they would take a second product of each; only the few rows in halves over 4-bit pages, which keep K as it is, do.
 // ----------------------------------------------------------------------------
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
@@ -614,8 +616,8 @@ template <typename IT, int HD> struct KvRaw16<IT, q4_t, HD> { // the same, eleme
 // SP > 1 (fp16 rows over 4-bit pages, at most 16 / SP of them a sequence): column n of the first product is row n / SP with the elements of group n % SP alone.  A sum's codes
 // then share minimum and scale: codes go in as they are (kv_tiny), the scale is one multiplication a key and group in fp32 behind them, exact where the 16-row form
 // needs two products, and the groups' sums meet in the neighbouring columns.  The minima meet the row's sums of elements in one product more.
-// 48 tokens over up to 9000 positions, window 4096, 16 heads of 128, 389 MB: 79 us (4.9 TB/s).  48 over 4000 each: 112 us, 125 in the 16-row form; bf16 rows, whose
-// 16-row form has one product, 108 spread and 104 not.
+// 48 tokens over up to 9000 positions, window 4096, 16 heads of 128, 389 MB: 79 us (4.9 TB/s).  48 over 4000 each: 103 us, 120 in the 16-row form; bf16 rows, whose
+// 16-row form has one product, 98, and spread 4 % more.
 #define KV_FEW_WAVES 4
 template <typename IT, typename CT, int HD, int SP>
 __global__ void __launch_bounds__(KV_FEW_WAVES * 64, KvType<CT>::code == MLH_CACHE_Q4 ? 3 : 2) k_kvattn_few(KvAttnArgs A) {
@@ -864,11 +866,13 @@ __global__ void __launch_bounds__(KV_FEW_WAVES * 64, KvType<CT>::code == MLH_CAC
 // products: every lane owns one row (element i of lane l: key 8 (i / 4) + 4 (l / 32) + i % 4, row l % 32), so maximum and sum run down registers, with one
 // exchange between the lane halves; O^T += V^T . P^T takes the weights as they lie and V through the transposing LDS read.  Pages of 16 bits go straight to LDS
 // (the 16-byte pieces of a row in an order that keeps both readings free of bank conflicts), those of 4 bits through registers, where codes become halves; fp16 rows too
-// meet K and V rounded to halves here (error against the result's norm 4.4e-4, 2.1e-4 the rounding of the result).
+// meet K and V rounded to halves here (error against the result's norm 4.4e-4, 2.1e-4 the rounding of the result).  Weights are rounded to 16 bits as above: in two parts the
+// products would be half as many again.
 // Bound by the matrix cores at the clock that their power leaves (1.8 GHz) and the vector ALU's exponentials between them: 16384 rows, 32 heads of 128 in fp16, window 4096
-// 1.02 ms, 0.95 PFLOP/s of what is seen (a library product of 8192 cubed: 1.05).  Eight prompts of 2048, window 1024: 0.16 ms, 0.64 PFLOP/s: of 19 tiles that a
-// workgroup's rows touch 16 are seen whole, and every workgroup starts with a lookup and a tile that nothing hides.  1289 rows behind 3000 to 7000 positions in 4 bits, heads
-// of 64: 101 us, 0.51 PFLOP/s (an exponential and its conversion for every 256 operations of the products).
+// 1.02 to 1.10 ms on different cards, 0.95 to 0.89 PFLOP/s of what is seen (a library product of 8192 cubed: 1.07).  Eight prompts of 2048, window 1024: 0.16 to 0.18 ms, 0.64 to
+// 0.57 PFLOP/s: of 19 tiles that a workgroup's rows touch 16 are seen whole, and every workgroup starts with a lookup and a tile that nothing hides; matrix cores and vector ALU
+// are busy in 0.35 and 0.41 of the cycles.  1289 rows behind 3000 to 7000 positions in 4 bits, heads of 64: 101 us, 0.51 PFLOP/s: the vector ALU, busy in 0.64 of the cycles to the
+// matrix cores' 0.28, unpacks every tile for 128 rows.
 // ----------------------------------------------------------------------------
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 template <bool BF> __device__ __forceinline__ f32x16 mfma32(const u32x4& a, const u32x4& b, const f32x16& c) {
@@ -1229,7 +1233,8 @@ static std::string attn_check(const mlh_kv_cache* c, const mlh_kv_batch* b, cons
 // Which kernel (32 query heads on 8, heads of 128, bf16, 4000 positions; "rows" are a sequence's, over the heads of one K/V head):
 //   16-bit pages: k_kvattn_many from 17 rows on.  16 sequences of 4, 16, 32, 64 rows: k_kvattn_few 49, 59, 111, 174 us, k_kvattn_many 50, 53, 57, 73; one sequence: 12, 12, 19, 19
 //     and 15, 15, 16, 18; 64 of 4 rows over 100 to 12000 positions: 290 and 377 (it splits less).
-//   4-bit pages: from 65 on.  16 sequences of 32, 64, 96 rows: k_kvattn_few 44, 68, 95 us, k_kvattn_many 53, 69, 77 (its tiles pass through LDS as halves).
+//   4-bit pages: from 65 on.  16 sequences of 32, 64, 96 rows: k_kvattn_few 44, 68, 95 us, k_kvattn_many 53, 69, 77 (its tiles pass through LDS as halves).  fp16 rows, whose
+//     products are two there: 44 and 76 for 50 and 58 us at 32 and 64, for the keys that it keeps.
 //   fp16 rows over 4-bit pages that leave a column for each of their groups: spread (above).
 // How keys are split, a second kernel joining the shares:
 #define KV_SPLIT_WGS 768 // k_kvattn_few, k_kvattn_f32: until a call has this many workgroups of at least four turns each, or two until each compute unit has one
