@@ -432,12 +432,12 @@ int mlh_kv_read_device(const mlh_kv_cache* cache, const mlh_kv_batch* batch, con
 
 /* Attention of the batch's rows over what their sequences hold (their own k and v are in the cache by then).  Position p sees key position j when j <= p and,
  * with window > 0, p - j < window or j < sinks.  out = sum over those of softmax(scale * q . k) v (inference.cu:136-239); zeros for a row that sees
- * nothing (one at a negative position).  NaN, as the softmax is, where a score is NaN or +infinity, or every one is -infinity.  Keys that a row does not see do not count for it, whatever they hold (infinities and NaN too); pages no row sees are not read, so their table entries may be
- * stale.  A row that sees a position beyond the page table or in a page outside the pool is NaN.
+ * nothing (one at a negative position); NaN, as the softmax is, where a score is NaN or +infinity, or every one is -infinity.  Keys that a row does not see do not count for it,
+ * whatever they hold (infinities and NaN too); pages no row sees are not read, so their table entries may be stale.  A row that sees a position beyond the page table or in a page outside the pool is NaN.
  * Scores, softmax statistics and sums are fp32, and with fp32 rows everything is.  With rows of 16 bits over pages of the same type the weights are rounded to it for the product
  * with v.  Over 4-bit pages both products are of halves: v's values and the weights are rounded to them, q times a power of two (exactly, but for what is 2^-24 of its row's
- * largest), and k's values, except in calls of fp16 rows whose maxNew * heads / cache.heads is at most 64: these take k as it is and the weights to 22 bits.  A weight that is held in
- * halves, one or two, is off by 2^-32 of the row's largest at least.
+ * largest), and k's values, except in calls of fp16 rows whose maxNew * heads / cache.heads is at most 64: these take k as it is and the weights to 22 bits.  Weights held in halves,
+ * one or two, are off by that or by 2^-32 of the row's largest, whichever is more.
  * Values of 4-bit pages beyond the halves' range count as infinite where they are rounded to halves; a group whose scale is an infinity or NaN counts as NaN or infinite.
  * maxLen, maxNew: what no len and no number of rows of a sequence exceeds (0: the page table's, rows).  They decide which kernel runs and how the work is split, and with that the
  * order of sums and, of fp16 rows over 4-bit pages, what K and the weights are rounded to (above): a token inside a prompt and the same token alone differ by that.  A call
