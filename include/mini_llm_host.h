@@ -40,6 +40,17 @@ void mll_set_layer_pattern(mlh_hparams* hp, int gdnPerAttn);
 /* getPreComputedRopeTheta (inference.cu:364-374), with headDim/base as arguments. */
 void mll_rope_table(float* tab, int maxL, int headDim, float base);
 
+/* Frequencies for mlh_rotate_device (radians a position, to be copied to the device): out[t] = f(t) = base^(-2t / rotated), t = 0 .. rotated / 2 - 1, as in that table, and
+ * their forms for texts longer than the `original` positions a model was trained on:
+ *   MLL_ROPE_PLAIN   f(t) (factor, original, low and high are not looked at);
+ *   MLL_ROPE_LINEAR  f(t) / factor: positions squeezed together;
+ *   MLL_ROPE_BASE    f(t) with base * factor^(rotated / (rotated - 2)) for base (rotated >= 4): the slowest pair is slowed by factor, the fastest not at all;
+ *   MLL_ROPE_BLEND   by the turns n = original * f(t) / (2 pi) that a pair makes in the original length: f(t) where n >= high, f(t) / factor where n <= low, and
+ *                    in between f(t) * (w + (1 - w) / factor) with w = (n - low) / (high - low).
+ * 1, or 0 for arguments out of range (rotated even and 2 to 512, base > 1, factor >= 1, original > 0, 0 <= low < high).  No counterpart in the reference. */
+enum { MLL_ROPE_PLAIN = 0, MLL_ROPE_LINEAR = 1, MLL_ROPE_BASE = 2, MLL_ROPE_BLEND = 3 };
+int mll_rope_frequencies(double* out, int rotated, double base, int kind, double factor, double original, double low, double high);
+
 /* ---- model.bin ---------------------------------------------------------- */
 
 typedef struct mll_model mll_model;

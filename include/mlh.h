@@ -457,6 +457,97 @@ typedef struct {
 uint64_t mlh_attention_work_bytes(const mlh_kv_cache* cache, const mlh_kv_batch* batch, const mlh_attention* args);
 int mlh_attention_device(const mlh_kv_cache* cache, const mlh_kv_batch* batch, const mlh_attention* args, void* stream);
 
+/* Rows of q and k turned to their positions: rotary embedding with frequencies of the caller's, for the layouts and lengths that the table of
+ * mlh_kv_append_device does not cover (inference.cu:113-134 has adjacent pairs of whole heads).  The first `rotated` elements of every head are pairs,
+ * (2t, 2t + 1) with MLH_ROTATE_PAIRS and (t, t + rotated / 2) with MLH_ROTATE_HALVES; pair t of a row at position p becomes
+ * amplitude * (c a - s b, s a + c b), c and s the cosine and sine of p * freq[t].  Elements behind them stay as they are.  Positions may be negative, which turns back:
+ * rows read from a cache (mlh_kv_read_device) move to another place by the difference.  The angle is in 64 bits (off by 2^-52 of itself) and reduced there; with fp32 rows the
+ * products are in 64 bits too, with rows of 16 bits cosine, sine and products are fp32.  Infinities and NaN stay in their pair.  freq: see mll_rope_frequencies.
+ * Pointers 16-byte aligned (pos 4, freq 8), rows `stride` elements apart, strides multiples of 16 bytes.  qOut may be q with the same stride, kOut k likewise; rows must not overlap in any
+ * other way.  k may be null (with kOut; kvHeads is not looked at then).  As the operators above: one launch on `stream`, no allocation, recordable, 0 / -1 / -2. */
+enum { MLH_ROTATE_PAIRS = 0, MLH_ROTATE_HALVES = 1 };
+typedef struct {
+    const void *q, *k;
+    void *qOut, *kOut;
+    int64_t qStride, qOutStride, kStride, kOutStride;
+    const int32_t* pos; /* [rows] */
+    const double* freq; /* [rotated / 2], radians a position */
+    int32_t rows;       /* 0 to 2^24 */
+    int32_t type;       /* MLH_DTYPE_F32, _BF16 or _F16 */
+    int32_t heads, kvHeads;
+    int32_t headDim;    /* a multiple of 8 up to 512 */
+    int32_t rotated;    /* even, 2 to headDim */
+    int32_t layout;     /* MLH_ROTATE_PAIRS or MLH_ROTATE_HALVES */
+    float amplitude;    /* 1e-30 to 1e30; 0: 1 */
+} mlh_rotate;
+int mlh_rotate_device(const mlh_rotate* args, void* stream);
+
+/* Matrices of 4-bit codes: row n of W [N, K] in groups of 32, 64 or 128 neighbouring elements (the last one may be shorter), each with a pair of IEEE
+ * halves (minimum, scale); an element stands for minimum + code * scale: 5, 4.5 or 4.25 bits an element.  `data` holds them in the order that mlh_gemm4_device reads (which no caller
+ * needs to know): mlh_weights4_bytes() bytes, 16-byte aligned, written once by one of the first two calls below, which quantise a matrix (rows
+ * `stride` elements apart) or take codes of the caller's.  K is a multiple of 32 up to 2^17, N is 1 to 2^20.
+ * Quantising is that of mlh_kv_append_device: minimum = half(min x), scale = half((max x - min x) * (1 / 15)), code = the nearest whole number to (x - minimum) / scale in 0 .. 15 (ties to
+ * even; scale 0: code 0); minima beyond the halves' range count as their largest, and a group with an infinity or NaN, or whose scale is beyond that range, becomes NaN.
+ * Codes of the caller's: codes [N, K / 2] with the even element of a pair in the low half of a byte, params [N, ceil(K / group), 2] minima and scales.
+ * mlh_weights4_read_device gives the values back, rounded to fp32 and then to `type`. */
+typedef struct {
+    void* data;
+    int32_t N, K;
+    int32_t group; /* 32, 64 or 128 */
+} mlh_weights4;
+uint64_t mlh_weights4_bytes(int N, int K, int group); /* 0: no such matrix */
+int mlh_weights4_pack_device(const mlh_weights4* w, int type, const void* src, int64_t stride, void* stream);
+int mlh_weights4_set_device(const mlh_weights4* w, const uint8_t* codes, const uint16_t* params, void* stream);
+int mlh_weights4_read_device(const mlh_weights4* w, int type, void* dst, int64_t stride, void* stream);
+
+/* C[M,N] = A[M,K] . W^T (+ R[M,N]) for few rows, as mlh_gemm_device with W in 4 bits; or, with swiglu, rows 2j and 2j + 1 of W are gate and up of unit j (N even,
+ * no R) and C is [M, N/2], silu(gate) * up (inference.cu:262-281).  A, R and C are of one type, C is rounded to it once.  The codes are multiplied as whole numbers and
+ * minimum and scale applied to the sums of a group, in fp32: products are exact (fp32 activations as three bf16 planes) and sums fp32, so no weight is rounded.  Rows of A with an infinity or NaN give
+ * infinities or NaN, not always the ones that products with the values would give; fp32 elements of 3.3962e38 or more count as such.  What a row gives does not depend on what the other rows hold.
+ * rStride may be 0: one row for all (a bias).  c may be r with the same stride.  Pointers 16-byte aligned, rows a multiple of 16 bytes apart, except those of R and C: aligned to their elements.
+ * work: mlh_gemm4_work_bytes() bytes (of the same structures; 0: none), 16-byte aligned, undefined before and after, not shared by calls that may overlap.  As the
+ * operators above: launches on `stream`, no allocation, recordable, 0 / -1 / -2. */
+typedef struct {
+    const void *a, *r; /* r may be null */
+    void* c;
+    int64_t aStride, rStride, cStride;
+    int32_t M;    /* 0 to 64 */
+    int32_t type; /* MLH_DTYPE_F32, _BF16 or _F16 */
+    int32_t swiglu;
+    void* work;
+    uint64_t workBytes;
+} mlh_gemm4;
+uint64_t mlh_gemm4_work_bytes(const mlh_weights4* w, const mlh_gemm4* args);
+int mlh_gemm4_device(const mlh_weights4* w, const mlh_gemm4* args, void* stream);
+
+/* What rows of logits say: with p = softmax(logits / temperature) of a row, logProb = log p of `given` tokens of the caller's, entropy = -sum p log p (an element of p = 0 adds 0),
+ * and the `top` most likely tokens, most likely first and of equal logits the lower id first, with their log p (inference_orchestrator.cu:68-84 sorts the probabilities of a row on the host).
+ * Sums of exponentials are in 64 bits, the largest logit is their 1, so that log p of a token that is nearly certain keeps its digits down to 2^-40; results are rounded to fp32.  A masked token is a logit of -infinity: its
+ * log p is -infinity.  A row with NaN or +infinity in it, or with nothing but -infinity, has no distribution: all its log probabilities and its entropy are NaN (its top tokens are those of
+ * the largest logits, NaN as -infinity).  A given token below 0 asks for nothing: its log p is 0; one of vocab or more is NaN.
+ * Rows `stride` elements apart, aligned to their elements (odd vocabularies; 16-byte aligned rows are read faster).  tokens and logProb [rows, given], entropy [rows] (may be null), topIds and topLogProb [rows, top].
+ * work: mlh_logprobs_work_bytes() bytes (of the same structure; 0: none), 16-byte aligned, undefined before and after, not shared by calls that may overlap.  As the
+ * operators above: launches on `stream`, no allocation, recordable, 0 / -1 / -2. */
+typedef struct {
+    const void* logits;
+    int64_t stride;
+    const int32_t* tokens; /* null with given 0 */
+    float* logProb;
+    float* entropy;
+    int32_t* topIds;       /* null with top 0 */
+    float* topLogProb;
+    int32_t rows;          /* 0 to 2^24 */
+    int32_t vocab;         /* 1 to 2^22 */
+    int32_t type;          /* MLH_DTYPE_F32, _BF16 or _F16 */
+    int32_t given;         /* 0 to 64 */
+    int32_t top;           /* 0 to 64, at most vocab */
+    float temperature;     /* 1e-4 to 1e4; 0: 1 */
+    void* work;
+    uint64_t workBytes;
+} mlh_logprobs;
+uint64_t mlh_logprobs_work_bytes(const mlh_logprobs* args);
+int mlh_logprobs_device(const mlh_logprobs* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

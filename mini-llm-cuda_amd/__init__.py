@@ -25,6 +25,8 @@ DTYPE_F32, DTYPE_BF16, DTYPE_F16 = 0, 1, 2
 CACHE_Q4 = 5  # pages of 4-bit codes (KvCache.type)
 PREFILL_BY_TOKEN, PREFILL_ROWS, PREFILL_HALVES, PREFILL_PAIRS, PREFILL_PLANES = range(5)  # Device.prefill_route
 
+ROTATE_PAIRS, ROTATE_HALVES = range(2)  # Rotate.layout
+ROPE_PLAIN, ROPE_LINEAR, ROPE_BASE, ROPE_BLEND = range(4)  # rope_frequencies
 DECODE_GEMV, DECODE_ROWS, DECODE_BARRIER, DECODE_XCD, DECODE_RANKS, DECODE_WIDE = range(6)  # Device.decode_route
 
 # tensor ids (include/mlh.h)
@@ -95,6 +97,30 @@ class Attention(ctypes.Structure):
                 ("maxLen", c_int32), ("maxNew", c_int32), ("scale", c_float), ("work", c_void_p), ("workBytes", c_uint64)]
 
 
+class Rotate(ctypes.Structure):
+    """mlh_rotate: rows of q and k, their positions and frequencies."""
+    _fields_ = [("q", c_void_p), ("k", c_void_p), ("qOut", c_void_p), ("kOut", c_void_p), ("qStride", c_int64), ("qOutStride", c_int64), ("kStride", c_int64),
+                ("kOutStride", c_int64), ("pos", c_void_p), ("freq", c_void_p), ("rows", c_int32), ("type", c_int32), ("heads", c_int32), ("kvHeads", c_int32),
+                ("headDim", c_int32), ("rotated", c_int32), ("layout", c_int32), ("amplitude", c_float)]
+
+
+class Weights4(ctypes.Structure):
+    """mlh_weights4: a matrix of 4-bit codes with a minimum and a scale for every group of a row's elements."""
+    _fields_ = [("data", c_void_p), ("N", c_int32), ("K", c_int32), ("group", c_int32)]
+
+
+class Gemm4(ctypes.Structure):
+    """mlh_gemm4: rows, residual and result of a product with such a matrix."""
+    _fields_ = [("a", c_void_p), ("r", c_void_p), ("c", c_void_p), ("aStride", c_int64), ("rStride", c_int64), ("cStride", c_int64), ("M", c_int32), ("type", c_int32),
+                ("swiglu", c_int32), ("work", c_void_p), ("workBytes", c_uint64)]
+
+
+class LogProbs(ctypes.Structure):
+    """mlh_logprobs: rows of logits, given tokens, and where the results go."""
+    _fields_ = [("logits", c_void_p), ("stride", c_int64), ("tokens", c_void_p), ("logProb", c_void_p), ("entropy", c_void_p), ("topIds", c_void_p), ("topLogProb", c_void_p),
+                ("rows", c_int32), ("vocab", c_int32), ("type", c_int32), ("given", c_int32), ("top", c_int32), ("temperature", c_float), ("work", c_void_p), ("workBytes", c_uint64)]
+
+
 _P = POINTER
 _sigs_dev = {
     "mlh_last_error": (c_char_p, [c_void_p]),
@@ -149,6 +175,15 @@ _sigs_dev = {
     "mlh_kv_read_device": (c_int, [_P(KvCache), _P(KvBatch), _P(KvRead), c_void_p]),
     "mlh_attention_work_bytes": (c_uint64, [_P(KvCache), _P(KvBatch), _P(Attention)]),
     "mlh_attention_device": (c_int, [_P(KvCache), _P(KvBatch), _P(Attention), c_void_p]),
+    "mlh_rotate_device": (c_int, [_P(Rotate), c_void_p]),
+    "mlh_weights4_bytes": (c_uint64, [c_int, c_int, c_int]),
+    "mlh_weights4_pack_device": (c_int, [_P(Weights4), c_int, c_void_p, c_int64, c_void_p]),
+    "mlh_weights4_set_device": (c_int, [_P(Weights4), c_void_p, c_void_p, c_void_p]),
+    "mlh_weights4_read_device": (c_int, [_P(Weights4), c_int, c_void_p, c_int64, c_void_p]),
+    "mlh_gemm4_work_bytes": (c_uint64, [_P(Weights4), _P(Gemm4)]),
+    "mlh_gemm4_device": (c_int, [_P(Weights4), _P(Gemm4), c_void_p]),
+    "mlh_logprobs_work_bytes": (c_uint64, [_P(LogProbs)]),
+    "mlh_logprobs_device": (c_int, [_P(LogProbs), c_void_p]),
     "mlh_probe_hops": (c_int, [c_void_p, c_int, _P(c_double)]),
     "mlh_probe_mfma": (c_int, [c_void_p, c_int, c_int, c_int, _P(c_double)]),
     "mlh_probe_lds_loads": (c_int, [c_void_p, c_int, _P(c_double)]),
@@ -159,6 +194,7 @@ _sigs_host = {
     "mll_hparams_config": (c_int, [c_int, _P(HParams)]),
     "mll_set_layer_pattern": (None, [_P(HParams), c_int]),
     "mll_rope_table": (None, [c_void_p, c_int, c_int, c_float]),
+    "mll_rope_frequencies": (c_int, [c_void_p, c_int, c_double, c_int, c_double, c_double, c_double, c_double]),
     "mll_model_new": (c_void_p, [_P(HParams)]),
     "mll_model_free": (None, [c_void_p]),
     "mll_model_hparams": (_P(HParams), [c_void_p]),
@@ -331,6 +367,59 @@ def attention_work_bytes(cache, batch, args):
 def attention(cache, batch, args, stream=None):
     """Attention of a batch's rows over a KvCache, with an optional window and first positions that stay visible (mlh_attention_device)."""
     _checked(dev.mlh_attention_device(byref(cache), byref(batch), byref(args), stream))
+
+
+def rope_frequencies(rotated, base=10000.0, kind=ROPE_PLAIN, factor=1.0, original=0, low=1.0, high=4.0):
+    """Radians a position of the rotated / 2 pairs of a head, float64 (mll_rope_frequencies): what Rotate.freq points at, on the device."""
+    out = np.empty(max(int(rotated) // 2, 0), dtype=np.float64)
+    if not host.mll_rope_frequencies(out.ctypes.data, rotated, base, kind, factor, original, low, high):
+        raise MlhError("rope_frequencies: bad arguments")
+    return out
+
+
+def rotate(args, stream=None):
+    """Rows of q and k turned to their positions (mlh_rotate_device).  stream: a raw stream handle."""
+    _checked(dev.mlh_rotate_device(byref(args), stream))
+
+
+def weights4_bytes(n, k, group):
+    """Bytes of Weights4.data; 0 where there is no such matrix."""
+    return dev.mlh_weights4_bytes(n, k, group)
+
+
+def weights4_pack(w, type, src, stride, stream=None):
+    """Quantises a matrix of device memory into w (mlh_weights4_pack_device)."""
+    _checked(dev.mlh_weights4_pack_device(byref(w), type, src, stride, stream))
+
+
+def weights4_set(w, codes, params, stream=None):
+    """Lays codes [N, K / 2] and (minimum, scale) pairs of the caller's out in w (mlh_weights4_set_device)."""
+    _checked(dev.mlh_weights4_set_device(byref(w), codes, params, stream))
+
+
+def weights4_read(w, type, dst, stride, stream=None):
+    """The values that w stands for (mlh_weights4_read_device)."""
+    _checked(dev.mlh_weights4_read_device(byref(w), type, dst, stride, stream))
+
+
+def gemm4_work_bytes(w, args):
+    """Bytes of Gemm4.work that such a call needs."""
+    return dev.mlh_gemm4_work_bytes(byref(w), byref(args))
+
+
+def gemm4(w, args, stream=None):
+    """Product of few rows with a matrix in 4 bits (mlh_gemm4_device)."""
+    _checked(dev.mlh_gemm4_device(byref(w), byref(args), stream))
+
+
+def logprobs_work_bytes(args):
+    """Bytes of LogProbs.work that such a call needs."""
+    return dev.mlh_logprobs_work_bytes(byref(args))
+
+
+def logprobs(args, stream=None):
+    """Log probabilities of given tokens, entropy and most likely tokens of rows of logits (mlh_logprobs_device)."""
+    _checked(dev.mlh_logprobs_device(byref(args), stream))
 
 
 class Device:

@@ -34,15 +34,6 @@ struct KvAppendArgs {
     int ropeRows;
 };
 
-// The code of x: the nearest whole number to (x - base) / scale.  The fp32 quotient, up to 16 where it is not clamped, is off by less than 2^-18 (three roundings: difference, inverse
-// and product): only within 1e-4 of a half, 26 times that, is it done again in 64 bits.
-__device__ __forceinline__ uint32_t kv_code(float x, float base, float scale, float inv) {
-    const float u = (x - base) * inv;
-    float c = rintf(u);
-    if (fabsf(u - c) > 0.4999f) c = (float)rint(((double)x - (double)base) / (double)scale);
-    return (uint32_t)fminf(fmaxf(c, 0.f), 15.f);
-}
-
 // One thread: eight elements of a head's row of q, k or v.  HD / 8 neighbouring threads hold the row (norm), four a group of 32 (4-bit codes).  Grid: rows x pieces of the
 // heads.  Norm and rotation are in 64 bits and rounded once, as the plain form's products of fp32 numbers are exact there.
 // Bound by memory: 17435 rows of 32 + 8 + 8 heads of 128 in bf16, 429 MB read and written, 80 us (5.4 TB/s; a copy of 1 GiB: 5.2).  11071 rows of the same heads in fp16

@@ -94,6 +94,15 @@ __device__ __forceinline__ void kv_values8(uint32_t codes, uint32_t params, floa
     for (int i = 0; i < 8; i++) x[i] = fmaf((float)((codes >> (4 * i)) & 15u), scale, base);
 }
 
+// The code of x: the nearest whole number to (x - base) / scale.  The fp32 quotient, up to 16 where it is not clamped, is off by less than 2^-18 (three roundings: difference, inverse
+// and product): only within 1e-4 of a half, 26 times that, is it done again in 64 bits.
+__device__ __forceinline__ uint32_t kv_code(float x, float base, float scale, float inv) {
+    const float u = (x - base) * inv;
+    float c = rintf(u);
+    if (fabsf(u - c) > 0.4999f) c = (float)rint(((double)x - (double)base) / (double)scale);
+    return (uint32_t)fminf(fmaxf(c, 0.f), 15.f);
+}
+
 // mlh_kv_append_device's and its fellows' checks, also made by the context's calls: empty, or what is wrong
 std::string kv_check(const mlh_kv_cache* cache, const mlh_kv_batch* batch, bool anyType);
 std::string kv_check_rows(const char* what, const void* p, long long stride, long long width, int type);

@@ -5,6 +5,8 @@
 #include <stdlib.h>
 #include <string.h>
 
+#include <algorithm>
+#include <cmath>
 #include <string>
 #include <vector>
 
@@ -84,6 +86,27 @@ extern "C" void mll_rope_table(float* tab, int maxL_, int headDim_, float base) 
             tab[colOffset + pairIndex * 2 + 1] = sinf(theta);
         }
     }
+}
+
+extern "C" int mll_rope_frequencies(double* out, int rotated, double base, int kind, double factor, double original, double low, double high) {
+    if (!out || rotated < 2 || rotated > 512 || rotated % 2 || !(base > 1.0) || !std::isfinite(base) || kind < MLL_ROPE_PLAIN || kind > MLL_ROPE_BLEND) return 0;
+    if (kind != MLL_ROPE_PLAIN && (!(factor >= 1.0) || !std::isfinite(factor))) return 0;
+    if (kind == MLL_ROPE_BASE) {
+        if (rotated < 4) return 0;
+        base *= std::pow(factor, rotated / (rotated - 2.0));
+        if (!std::isfinite(base)) return 0;
+    }
+    if (kind == MLL_ROPE_BLEND && (!(original > 0.0) || !std::isfinite(original) || !(low >= 0.0) || !(high > low) || !std::isfinite(high))) return 0;
+    for (int t = 0; t < rotated / 2; t++) {
+        double f = std::pow(base, -2.0 * t / rotated);
+        if (kind == MLL_ROPE_LINEAR) f /= factor;
+        if (kind == MLL_ROPE_BLEND) {
+            const double turns = original * f / 6.283185307179586477, w = std::min(std::max((turns - low) / (high - low), 0.0), 1.0);
+            f *= w + (1.0 - w) / factor;
+        }
+        out[t] = f;
+    }
+    return 1;
 }
 
 // ---------------------------------------------------------------------------

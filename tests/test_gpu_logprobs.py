@@ -1,0 +1,188 @@
+"""mlh_logprobs_device against its formula in 64 bits."""
+import ctypes
+import math
+
+import pytest
+import torch
+
+import step_oracle as so
+
+pytestmark = pytest.mark.gpu
+INF, NAN = math.inf, math.nan
+
+
+class Call:
+    def __init__(self, pkg, x, tokens=None, top=0, t=0.0, pad=0, shift=0, entropy=True):
+        """x [rows, vocab] in its type; pad: elements between rows (NaN); shift: elements that the first row starts behind an aligned address."""
+        self.x, self.top, self.t = x, top, ctypes.c_float(t).value  # (the temperature of a call is a float)
+        rows, vocab = x.shape
+        self.tokens = torch.zeros(rows, 0, dtype=torch.int32) if tokens is None else tokens.to(torch.int32)
+        given = self.tokens.shape[1]
+        flat = torch.full((rows * (vocab + pad) + shift + 8,), NAN, dtype=x.dtype)
+        flat[shift:shift + rows * (vocab + pad)].unflatten(0, (rows, vocab + pad))[:, :vocab] = x
+        self.buf = flat.cuda()
+        self.dtok = self.tokens.cuda()
+        self.lp, self.ent = torch.full((rows + 1, given), 55.0, device="cuda"), torch.full((rows + 1,), 55.0, device="cuda")
+        self.ids, self.tlp = torch.full((rows + 1, top), -55, dtype=torch.int32, device="cuda"), torch.full((rows + 1, top), 55.0, device="cuda")
+        kind = {v: k for k, v in so.TORCH.items()}[x.dtype]
+        self.args = pkg.LogProbs(logits=self.buf.data_ptr() + shift * x.element_size(), stride=vocab + pad, tokens=self.dtok.data_ptr() if given else None,
+                                 logProb=self.lp.data_ptr() if given else None, entropy=self.ent.data_ptr() if entropy else None, topIds=self.ids.data_ptr() if top else None,
+                                 topLogProb=self.tlp.data_ptr() if top else None, rows=rows, vocab=vocab, type=so.code_of(pkg, kind), given=given, top=top, temperature=t)
+        size = pkg.logprobs_work_bytes(self.args)
+        self.work = torch.full((max(size, 16) + 64,), 255, dtype=torch.uint8, device="cuda")
+        self.args.work, self.args.workBytes = self.work.data_ptr(), size
+        self.size, self.entropy = size, entropy
+
+    def check(self, what=""):
+        torch.cuda.synchronize()
+        (lp, ent, ids, tlp), (blp, bent, btlp) = so.logprobs(self.x, self.tokens, self.top, self.t or 1.0)
+        rows = self.x.shape[0]
+        assert torch.equal(self.ids[:rows].cpu(), ids), f"{what}: ids {(self.ids[:rows].cpu() != ids).nonzero()[:4].tolist()}"
+        so.close(self.lp[:rows].cpu(), lp, blp, what + " given")
+        so.close(self.tlp[:rows].cpu(), tlp, btlp, what + " top")
+        if self.entropy:
+            so.close(self.ent[:rows].cpu(), ent, bent, what + " entropy")
+            assert float(self.ent[rows]) == 55.0
+        else:
+            assert bool((self.ent == 55.0).all())
+        assert bool((self.lp[rows] == 55.0).all()) and bool((self.tlp[rows] == 55.0).all()) and bool((self.ids[rows] == -55).all())
+        assert bool((self.work[max(self.size, 0):] == 255).all())
+
+
+def logits(kind, rows, vocab, seed, spread=2.0):
+    gen = torch.Generator().manual_seed(seed)
+    return (torch.randn(rows, vocab, generator=gen) * spread).to(so.TORCH[kind]), gen
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("rows,vocab,given,top,pad,shift", [(1, 1, 1, 1, 0, 0), (1, 8192, 1, 5, 0, 0), (3, 7, 2, 7, 0, 1), (5, 100, 1, 64, 4, 0), (2, 2049, 3, 20, 0, 3), (17, 4099, 1, 1, 1, 5),
+                                                            (4, 20160, 0, 10, 0, 0), (64, 777, 1, 0, 0, 0), (7, 50257, 4, 64, 0, 7), (2, 131075, 1, 20, 0, 0), (1, 262144, 1, 50, 0, 0), (600, 513, 1, 3, 0, 0),
+                                                            (1, 300001, 1, 64, 0, 1), (130, 9001, 2, 33, 7, 2)])
+def test_against_the_formula(pkg, kind, rows, vocab, given, top, pad, shift):
+    x, gen = logits(kind, rows, vocab, rows * 7 + vocab)
+    c = Call(pkg, x, torch.randint(0, vocab, (rows, given), generator=gen), top, pad=pad, shift=shift)
+    pkg.logprobs(c.args)
+    c.check()
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("t", [1e-4, 0.25, 1.0, 7.0, 1e4])
+def test_temperatures(pkg, kind, t):
+    x, gen = logits(kind, 6, 3001, 11)
+    c = Call(pkg, x, torch.randint(0, 3001, (6, 2), generator=gen), 9, t)
+    pkg.logprobs(c.args)
+    c.check()
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("vocab", [97, 5003, 140001])
+def test_masks(pkg, kind, vocab):
+    """Rows with few tokens left, with one, with none; masks of -infinity and of the type's lowest value; +infinity and NaN."""
+    x, gen = logits(kind, 14, vocab, vocab)
+    low = torch.finfo(x.dtype).min
+    keep = torch.rand(14, vocab, generator=gen) < 3.0 / vocab
+    for r, fill in ((0, -INF), (1, low), (2, -INF), (3, low)):
+        x[r][~keep[r]] = fill
+    x[4] = -INF
+    x[5] = low
+    x[6] = -INF
+    x[6, vocab // 2] = -3.0
+    x[7] = low
+    x[7, vocab - 1] = low / 2
+    x[8, vocab // 3] = INF
+    x[9, vocab // 5] = NAN
+    x[10] = NAN
+    x[11] = -INF
+    x[11, 1::2] = NAN
+    x[12] = torch.finfo(x.dtype).max
+    x[13, :vocab // 2] = low
+    x[13, vocab // 2:] = torch.finfo(x.dtype).max
+    c = Call(pkg, x, torch.randint(0, vocab, (14, 3), generator=gen), 40)
+    pkg.logprobs(c.args)
+    c.check()
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("order", ["up", "down", "equal", "steps", "stripes", "zeros", "last"])
+@pytest.mark.parametrize("vocab", [2000, 33333, 131072])
+def test_orders_and_ties(pkg, kind, order, vocab):
+    """Rows in which the largest come last, in which many are equal, or in which they stand where one thread finds them all."""
+    i = torch.arange(vocab, dtype=torch.float64)
+    x = {"up": i / vocab * 8, "down": -i / vocab * 8, "equal": i * 0 + 1.5, "steps": (i // 700) % 11, "stripes": ((i // 8) % 256 == 17) * 3.0 + (i % 97) / 97, "zeros": torch.where(i % 2 == 0, -0.0, 0.0),
+         "last": torch.where(i >= vocab - 70, 4.0, 0.0)}[order]
+    x = x[None].repeat(3, 1).to(so.TORCH[kind])
+    x[1] = x[1].flip(0)
+    c = Call(pkg, x, torch.tensor([[0, vocab - 1], [5, 6], [vocab // 2, 1]]), 64)
+    pkg.logprobs(c.args)
+    c.check()
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_a_nearly_certain_token_keeps_its_digits(pkg, kind):
+    x, gen = logits(kind, 8, 30000, 5, 1.0)
+    for r in range(8):
+        x[r, 1000 + r] = 14.0 + 4 * r
+    tok = torch.arange(1000, 1008)[:, None]
+    c = Call(pkg, x, tok, 2)
+    pkg.logprobs(c.args)
+    c.check()
+    assert float(c.lp[7, 0]) < 0  # (exp(-42 + ...) beside 1)
+
+
+def test_tokens_that_are_none(pkg):
+    x, _ = logits("bf16", 5, 1000, 1)
+    x[4] = -INF
+    c = Call(pkg, x, torch.tensor([[-1, 0], [999, 1000], [-2 ** 31, 2 ** 31 - 1], [3, -7], [-1, 5]]), 1, entropy=False)
+    pkg.logprobs(c.args)
+    c.check()
+
+
+def test_entropy_alone_and_no_rows(pkg):
+    x, _ = logits("f16", 33, 6007, 2)
+    c = Call(pkg, x)
+    c.args.rows = 0
+    pkg.logprobs(c.args)
+    torch.cuda.synchronize()
+    assert bool((c.ent == 55.0).all())
+    c.args.rows = 33
+    pkg.logprobs(c.args)
+    c.check()
+
+
+def test_the_same_call_gives_the_same_bits(pkg):
+    x, gen = logits("bf16", 70, 60001, 3)
+    tok = torch.randint(0, 60001, (70, 2), generator=gen)
+    c = Call(pkg, x, tok, 20)
+    seen = []
+    for _ in range(4):
+        pkg.logprobs(c.args)
+        torch.cuda.synchronize()
+        seen.append([v.clone() for v in (c.lp, c.ent, c.ids, c.tlp)])
+    for other in seen[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(seen[0], other))
+
+
+@pytest.mark.parametrize("rows,vocab", [(2, 90001), (40, 5000)])
+def test_on_a_stream_and_in_a_graph(pkg, rows, vocab):
+    x, gen = logits("f32", rows, vocab, 4)
+    c = Call(pkg, x, torch.randint(0, vocab, (rows, 1), generator=gen), 12)
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    pkg.logprobs(c.args, st.cuda_stream)
+    st.synchronize()
+    c.check("stream")
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=st):
+        pkg.logprobs(c.args, st.cuda_stream)
+    for i in range(4):
+        c.x, gen = logits("f32", rows, vocab, 50 + i)
+        c.buf[:rows * vocab] = c.x.flatten().cuda()
+        c.tokens = torch.randint(0, vocab, (rows, 1), generator=gen, dtype=torch.int32)
+        c.dtok.copy_(c.tokens)
+        torch.cuda.synchronize()
+        g.replay()
+        c.check(f"replay {i}")
+        y, _ = logits("bf16", 3, 4001, 90 + i)
+        other = Call(pkg, y, top=3)
+        pkg.logprobs(other.args)
+        other.check("between")
