@@ -1,4 +1,9 @@
 // Log probabilities of given tokens, entropy and most likely tokens of rows of logits (mlh_logprobs_device).
+//
+// One pass over a row.  A thread keeps its running maximum m, the sum s of exp((x - m) / T) and the sum t of that times its exponent; a larger maximum scales both.  Threads, waves and
+// parts of a row are joined by the same rule.  For the top tokens a thread also notes the largest of every 32 elements it has seen (a group).  The k-th largest of the threads' maxima is
+// a bound that k tokens reach, so only groups that reach it can hold one of the k most likely: about as many groups as tokens are asked for.  Those are read again, their elements
+// that reach the bound are ranked by counting how many are larger, and the row is done.
 #include <math.h>
 
 #include <algorithm>
@@ -6,6 +11,14 @@
 #include "kv_cache.h"
 
 #define LP_WG 256
+#define LP_WAVES (LP_WG / 64)
+#define LP_CHUNK 16                            // elements a thread takes at once
+#define LP_GROUP 32                            // ... and whose largest it notes
+#define LP_GROUPS 16                           // groups of a thread, at most
+#define LP_PART (LP_WG * LP_GROUP * LP_GROUPS) // elements of a part, at most
+#define LP_TOP 64
+#define LP_CANDS (LP_TOP * LP_GROUP)           // elements that are ranked, at most
+#define LP_PARTS 64                            // of a row, at most
 
 struct LpArgs {
     const void* logits;
@@ -15,69 +28,406 @@ struct LpArgs {
     int32_t* topIds;
     float* topLogProb;
     int rows, vocab, given, top;
-    double inv; // 1 / temperature
+    double inv;  // 1 / temperature
+    float scale; // ... times log2(e)
+    int parts, partGranules;
+    unsigned char* work; // with several parts: what they leave
 };
+struct LpSums { double s; float m, t; }; // of a part; behind those of all parts their best keys, `top` each
+
+template <typename T> struct LpType;
+template <> struct LpType<float> { static constexpr int V = 4; };
+template <> struct LpType<bf16_t> { static constexpr int V = 8; };
+template <> struct LpType<f16_t> { static constexpr int V = 8; };
 
 __device__ __forceinline__ float lp_get(const float* p) { return *p; }
 __device__ __forceinline__ float lp_get(const bf16_t* p) { return kv_bf16(*p); }
 __device__ __forceinline__ float lp_get(const f16_t* p) { return kv_half(p->bits); }
+// element i of 16 bytes
+__device__ __forceinline__ float lp_elem(const kv_u32x4& v, int i, float) { return __uint_as_float(v[i]); }
+__device__ __forceinline__ float lp_elem(const kv_u32x4& v, int i, bf16_t) { return i & 1 ? __uint_as_float(v[i >> 1] & 0xffff0000u) : kv_bf16(v[i >> 1] & 0xffffu); }
+__device__ __forceinline__ float lp_elem(const kv_u32x4& v, int i, f16_t) { return kv_half(i & 1 ? v[i >> 1] >> 16 : v[i >> 1] & 0xffffu); }
 
-// What a token is ranked by: the larger the likelier, of equal logits the lower id.  NaN counts as -infinity, and the zeros are equal.
-__device__ __forceinline__ uint64_t lp_key(float x, int id) {
+// What a token is ranked by: the larger the likelier, of equal logits the lower id.  NaN counts as -infinity, and the zeros are equal.  0 is no token.
+__device__ __forceinline__ uint32_t lp_rank(float x) {
     if (!(x > -INFINITY)) x = -INFINITY;
     const uint32_t u = __float_as_uint(x + 0.f);
-    return (uint64_t)((u & 0x80000000u) ? ~u : u | 0x80000000u) << 32 | (uint32_t)~id;
+    return (u & 0x80000000u) ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ uint64_t lp_key(uint32_t rank, int id) { return (uint64_t)rank << 32 | (uint32_t)~id; }
+__device__ __forceinline__ int lp_id(uint64_t key) { return (int)~(uint32_t)key; }
+__device__ __forceinline__ float lp_value(uint64_t key) {
+    const uint32_t r = (uint32_t)(key >> 32);
+    return __uint_as_float((r & 0x80000000u) ? r & 0x7fffffffu : ~r);
 }
 
-// One workgroup a row, the row again for each of its top tokens.
-template <typename T>
-__global__ void __launch_bounds__(LP_WG) k_logprobs(LpArgs A) {
-    __shared__ float best[LP_WG];
-    __shared__ double sums[2 * LP_WG];
-    __shared__ uint64_t keys[LP_WG];
+// (m, s, t) as seen from a maximum `to` that is not smaller.  Nothing seen: m is -infinity and s and t are 0.
+__device__ __forceinline__ void lp_scale(float& m, double& s, float& t, float to, float scale) {
+    if (m < to) {
+        const float d = fmaxf((m - to) * scale, -1e4f), f = __builtin_amdgcn_exp2f(d); // (2^-1e4 is 0; an infinity would make NaN of 0)
+        t = f * fmaf((float)s, d, t);
+        s *= f;
+        m = to;
+    }
+}
+
+// A row's granules of 16 bytes; the first and the last may hold elements of other rows.
+struct LpRow {
+    const kv_u32x4* at;
+    int lead, granules, vocab;
+};
+template <typename T> __device__ __forceinline__ LpRow lp_row(const LpArgs& A, int row) {
+    constexpr int V = LpType<T>::V;
+    const T* x = (const T*)A.logits + (size_t)row * A.stride;
+    const int lead = (int)(((uintptr_t)x & 15) / sizeof(T));
+    return {(const kv_u32x4*)(x - lead), lead, (A.vocab + lead + V - 1) / V, A.vocab};
+}
+
+// Sums and maxima over a wave, in its last lane: row_shr 1, 2, 4, 8, then row_bcast 15 and 31.  `none`: what a lane without a partner takes.
+template <typename T, int CTRL, typename F> __device__ __forceinline__ T lp_step(T v, T none, F f) {
+    T o;
+    if constexpr (sizeof(T) == 8) {
+        const uint64_t x = __builtin_bit_cast(uint64_t, v), n = __builtin_bit_cast(uint64_t, none);
+        const uint32_t lo = __builtin_amdgcn_update_dpp((int)(uint32_t)n, (int)(uint32_t)x, CTRL, 0xf, 0xf, false);
+        const uint32_t hi = __builtin_amdgcn_update_dpp((int)(n >> 32), (int)(x >> 32), CTRL, 0xf, 0xf, false);
+        o = __builtin_bit_cast(T, (uint64_t)hi << 32 | lo);
+    } else
+        o = __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(__builtin_bit_cast(int, none), __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, false));
+    return f(v, o);
+}
+template <typename T, typename F> __device__ __forceinline__ T lp_wave(T v, T none, F f) {
+    v = lp_step<T, 0x111>(v, none, f);
+    v = lp_step<T, 0x112>(v, none, f);
+    v = lp_step<T, 0x114>(v, none, f);
+    v = lp_step<T, 0x118>(v, none, f);
+    v = lp_step<T, 0x142>(v, none, f);
+    return lp_step<T, 0x143>(v, none, f);
+}
+__device__ __forceinline__ uint32_t lp_last(uint32_t v) { return (uint32_t)__builtin_amdgcn_readlane((int)v, 63); }
+__device__ __forceinline__ float lp_last(float v) { return __uint_as_float(lp_last(__float_as_uint(v))); }
+__device__ __forceinline__ float lp_wave_max(float v) { return lp_last(lp_wave(v, -INFINITY, [](float a, float b) { return fmaxf(a, b); })); }
+template <typename T> __device__ __forceinline__ T lp_wave_sum(T v) { return lp_wave(v, T(0), [](T a, T b) { return a + b; }); } // (in lane 63)
+
+// The sum of the threads' counts.  Two calls in a row take different slots.
+__device__ __forceinline__ int lp_count(int mine, int* slot) {
+    const int sum = lp_wave_sum(mine);
+    if ((threadIdx.x & 63) == 63) slot[threadIdx.x >> 6] = sum;
+    __syncthreads();
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < LP_WAVES; i++) n += slot[i];
+    return n;
+}
+
+// Ranks the n keys in cand (all different; written before a barrier) and puts the first `top` of them into best, in order.  More than LP_WG are first cut down to few more than top, by
+// bisection.  All threads; best is whole after a barrier.
+__device__ void lp_best(const uint64_t* cand, int n, int top, int (*slot)[LP_WAVES], uint64_t* best) {
+    uint64_t least = 0;
+    if (n > LP_WG) {
+        uint64_t lo = 0, hi = ~0ull; // as many as top reach lo, not hi
+        for (int step = 0, seen = n; seen > top + 32 && hi - lo > 1; step++) {
+            const uint64_t mid = lo + (hi - lo) / 2;
+            int mine = 0;
+            for (int i = threadIdx.x; i < n; i += LP_WG) mine += cand[i] >= mid;
+            const int c = lp_count(mine, slot[step & 1]);
+            if (c >= top) { lo = mid; seen = c; } else hi = mid;
+        }
+        least = lo;
+    }
+    for (int i = threadIdx.x; i < n; i += LP_WG) {
+        const uint64_t key = cand[i];
+        if (key < least) continue;
+        int r = 0;
+        for (int j = 0; j < n; j++) r += cand[j] > key;
+        if (r < top) best[r] = key;
+    }
+    for (int r = n + threadIdx.x; r < top; r += LP_WG) best[r] = 0; // (a short part)
+}
+
+struct LpShared {
+    union {
+        uint32_t group[LP_GROUPS][LP_WG]; // rank of the largest of every group; 0: none
+        uint64_t cand[LP_CANDS];          // (once the groups that matter are known)
+    };
+    uint32_t most[LP_WG];
+    uint64_t best[LP_TOP];
+    int list[LP_TOP];
+    int count, found;
+    uint32_t bound;
+    int slot[2][LP_WAVES];
+    float m[LP_WAVES], t[LP_WAVES];
+    double s[LP_WAVES];
+};
+
+// The elements of granule g of a row that belong to it
+template <typename T, typename F> __device__ __forceinline__ void lp_granule(const LpRow& R, int g, F f) {
+    constexpr int V = LpType<T>::V;
+    const kv_u32x4 v = R.at[g];
+#pragma unroll
+    for (int i = 0; i < V; i++) {
+        const int id = g * V - R.lead + i;
+        if (id >= 0 && id < R.vocab) f(lp_elem(v, i, T{}), id);
+    }
+}
+
+// sh.best: the most likely tokens of granules first .. end - 1, of which this thread's largest has the rank `mine` and whose groups' largest ranks are in sh.group (lost).  All threads.
+template <typename T> __device__ void lp_tops(LpShared& sh, const LpRow& R, int first, int end, int groups, uint32_t mine, int top) {
+    constexpr int V = LpType<T>::V, U = LP_GROUP / V; // granules of a group
     const int t = threadIdx.x;
+    sh.most[t] = mine;
+    if (t == 0) sh.count = sh.found = 0;
+    __syncthreads();
+    if (t < 64) { // a bound that at least top threads reach, and not many more
+        uint32_t b[LP_WAVES], lo = ~0u, hi = 0u;
+#pragma unroll
+        for (int i = 0; i < LP_WAVES; i++) { b[i] = sh.most[i * 64 + t]; lo = min(lo, b[i]); hi = max(hi, b[i]); }
+        hi = lp_last(lp_wave(hi, 0u, [](uint32_t a, uint32_t c) { return max(a, c); })) + 1;
+        lo = top == 1 ? hi - 1 : lp_last(lp_wave(lo, ~0u, [](uint32_t a, uint32_t c) { return min(a, c); }));
+        for (int seen = LP_WG; seen > top + top / 4 && hi - lo > 1;) {
+            const uint32_t mid = lo + (hi - lo) / 2;
+            int c = 0;
+#pragma unroll
+            for (int i = 0; i < LP_WAVES; i++) c += __builtin_popcountll(__ballot(b[i] >= mid));
+            if (c >= top) { lo = mid; seen = c; } else hi = mid;
+        }
+        if (t == 0) sh.bound = max(lo, 1u);
+    }
+    __syncthreads();
+    uint32_t bound = sh.bound;
+    const auto list = [&](uint32_t least) { // this thread's groups that reach it
+        for (int j = 0; j < groups; j++)
+            if (sh.group[j][t] >= least) {
+                const int i = atomicAdd(&sh.count, 1);
+                if (i < LP_TOP) sh.list[i] = j << 8 | t;
+            }
+    };
+    if (mine >= bound) list(bound);
+    __syncthreads();
+    const bool many = sh.count > LP_TOP;
+    if (many) { // the top-th largest group itself: fewer than top groups are larger
+        uint32_t lo = bound, hi = ~0u;
+        for (int step = 0; hi - lo > 1; step++) {
+            const uint32_t mid = step == 0 ? lo + 1 : lo + (hi - lo) / 2; // (most often it is the bound: masked tokens fill the groups up)
+            int c = 0;
+            if (mine >= mid)
+                for (int j = 0; j < groups; j++) c += sh.group[j][t] >= mid;
+            if (lp_count(c, sh.slot[step & 1]) >= top) lo = mid; else hi = mid;
+        }
+        bound = lo;
+        if (t == 0) sh.count = 0;
+        __syncthreads();
+        if (mine > bound) list(bound + 1);
+        __syncthreads();
+    }
+    const int listed = sh.count;
+    for (int i = t; i < listed * U; i += LP_WG) {
+        const int where = sh.list[i / U], g = first + ((where >> 8) * U + i % U) * LP_WG + (where & 255);
+        if (g < end)
+            lp_granule<T>(R, g, [&](float x, int id) {
+                const uint32_t r = lp_rank(x);
+                if (many ? r > bound : r >= bound) sh.cand[atomicAdd(&sh.found, 1)] = lp_key(r, id);
+            });
+    }
+    __syncthreads();
+    int n = sh.found;
+    if (many && n < top) { // of those that equal the bound the first ones: granule by granule in the order of ids
+        int need = top - n;
+        for (int g0 = first, step = 0; g0 < end && need > 0; g0 += LP_WG, step++) {
+            const int g = g0 + t;
+            uint32_t equal = 0;
+            if (g < end) lp_granule<T>(R, g, [&](float x, int id) { equal |= (uint32_t)(lp_rank(x) == bound) << (id - g * V + R.lead); });
+            int before = __builtin_popcount(equal);
+            const int own = before;
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) {
+                const int v = __shfl_up(before, o, 64);
+                if ((t & 63) >= o) before += v;
+            }
+            if ((t & 63) == 63) sh.slot[step & 1][t >> 6] = before;
+            before -= own;
+            __syncthreads();
+            int all = 0;
+#pragma unroll
+            for (int i = 0; i < LP_WAVES; i++) {
+                if (i < t >> 6) before += sh.slot[step & 1][i];
+                all += sh.slot[step & 1][i];
+            }
+            while (equal && before < need) {
+                const int i = __builtin_ctz(equal);
+                equal &= equal - 1;
+                sh.cand[n + before++] = lp_key(bound, g * V - R.lead + i);
+            }
+            const int took = min(all, need);
+            n += took;
+            need -= took;
+        }
+        __syncthreads();
+    }
+    lp_best(sh.cand, n, top, sh.slot, sh.best);
+    __syncthreads();
+}
+
+// What a row's maximum, sums, given tokens' logits and most likely tokens come to: the first wave, one thread a token.
+__device__ __forceinline__ void lp_finish(const LpArgs& A, int row, float m, double s, float ent, int token, float given, const uint64_t* best) {
+    const int t = threadIdx.x;
+    const double logz = m > -INFINITY ? log(s) : NAN;
+    if (t == 0 && A.entropy) A.entropy[row] = (float)(logz - (double)ent * 0.69314718055994530942 / s);
+    if (t < A.given) A.logProb[(size_t)row * A.given + t] = token < 0 ? 0.f : token >= A.vocab ? NAN : (float)(((double)given - (double)m) * A.inv - logz);
+    if (t < A.top) {
+        const uint64_t key = best[t];
+        A.topIds[(size_t)row * A.top + t] = lp_id(key);
+        A.topLogProb[(size_t)row * A.top + t] = (float)(((double)lp_value(key) - (double)m) * A.inv - logz);
+    }
+}
+
+template <typename T, bool TOP>
+__global__ void __launch_bounds__(LP_WG, sizeof(T) == 4 ? 5 : 6) k_logprobs(LpArgs A) {
+    constexpr int V = LpType<T>::V, U = LP_CHUNK / V;
+    __shared__ LpShared sh;
+    const int t = threadIdx.x, wave = t >> 6;
+    const unsigned items = (unsigned)A.rows * A.parts; // (2^30 at most)
+    for (unsigned item = blockIdx.x; item < items; item += gridDim.x) {
+        const int row = (int)(item / A.parts), part = (int)(item % A.parts);
+        const LpRow R = lp_row<T>(A, row);
+        const int first = min(part * A.partGranules, R.granules), end = min(first + A.partGranules, R.granules);
+        const int chunks = (end - first + LP_WG * U - 1) / (LP_WG * U);
+        kv_u32x4 next[U];
+        const auto load = [&](int j) {
+            const int g0 = first + j * LP_WG * U + t;
+#pragma unroll
+            for (int u = 0; u < U; u++) next[u] = R.at[min(g0 + u * LP_WG, end - 1)]; // (behind the end the last one again)
+        };
+        load(0);
+        float given = 0.f;
+        int token = -1;
+        if (A.parts == 1 && t < A.given) {
+            token = A.tokens[(size_t)row * A.given + t];
+            if (token >= 0 && token < A.vocab) given = lp_get((const T*)A.logits + (size_t)row * A.stride + token);
+        }
+        float m = -INFINITY, ent = 0.f; // m: the wave's
+        double s = 0.0;
+        uint32_t mine = 0, grp = 0;
+        for (int j = 0; j < chunks; j++) {
+            const int g0 = first + j * LP_WG * U;
+            kv_u32x4 v[U];
+#pragma unroll
+            for (int u = 0; u < U; u++) v[u] = next[u];
+            load(j + 1);
+            float x[LP_CHUNK];
+#pragma unroll
+            for (int u = 0; u < U; u++)
+#pragma unroll
+                for (int i = 0; i < V; i++) x[u * V + i] = lp_elem(v[u], i, T{});
+            bool any = true;
+            if ((g0 == 0 && R.lead) || g0 + LP_WG * U >= R.granules || g0 + LP_WG * U > end) { // an end of the row or of the part
+                any = g0 + t < end;
+#pragma unroll
+                for (int u = 0; u < U; u++) {
+                    const int g = g0 + u * LP_WG + t, id = g * V - R.lead, room = g < end ? R.vocab - id : 0;
+#pragma unroll
+                    for (int i = 0; i < V; i++) x[u * V + i] = i >= -id && i < room ? x[u * V + i] : -INFINITY;
+                }
+            }
+            float c = x[0];
+#pragma unroll
+            for (int i = 1; i < LP_CHUNK; i++) c = fmaxf(c, x[i]);
+            if (!(c > -INFINITY)) c = -INFINITY; // (NaN alone)
+            if (TOP) {
+                grp = max(j & 1 ? grp : 0u, any ? lp_rank(c) : 0u);
+                mine = max(mine, grp);
+                if (j & 1 || j + 1 == chunks) sh.group[j / 2][t] = grp;
+            }
+            const float cw = lp_wave_max(c);
+            if (cw > m) lp_scale(m, s, ent, cw, A.scale); // (seldom)
+            const float from = m > -INFINITY ? m : 0.f;
+            if (cw < m) {
+                float e4[2] = {}, t4[2] = {};
+#pragma unroll
+                for (int i = 0; i < LP_CHUNK; i++) {
+                    const float d = (x[i] - from) * A.scale, e = __builtin_amdgcn_exp2f(d);
+                    e4[i & 1] += e;
+                    t4[i & 1] = fmaf(e, fmaxf(d, -1e4f), t4[i & 1]);
+                }
+                s += (double)(e4[0] + e4[1]);
+                ent += t4[0] + t4[1];
+            } else { // the maximum's 1 is among them, beside which fp32 would lose the others
+#pragma unroll
+                for (int i = 0; i < LP_CHUNK; i++) {
+                    const float d = (x[i] - from) * A.scale, e = __builtin_amdgcn_exp2f(d);
+                    s += (double)e;
+                    ent = fmaf(e, fmaxf(d, -1e4f), ent);
+                }
+            }
+        }
+        s = lp_wave_sum(s);
+        ent = lp_wave_sum(ent);
+        if ((t & 63) == 63) { sh.m[wave] = m; sh.s[wave] = s; sh.t[wave] = ent; }
+        if (TOP) lp_tops<T>(sh, R, first, end, (chunks + 1) / 2, mine, A.top); // (with the barriers that the sums need)
+        else __syncthreads();
+        if (wave == 0) {
+            m = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < LP_WAVES; i++) m = fmaxf(m, sh.m[i]);
+            s = 0.0;
+            ent = 0.f;
+#pragma unroll
+            for (int i = 0; i < LP_WAVES; i++) {
+                float from = sh.m[i], e = sh.t[i];
+                double z = sh.s[i];
+                lp_scale(from, z, e, m, A.scale);
+                s += z;
+                ent += e;
+            }
+            if (A.parts > 1) {
+                if (t == 0) reinterpret_cast<LpSums*>(A.work)[item] = LpSums{s, m, ent};
+                if (t < A.top) reinterpret_cast<uint64_t*>(A.work + (size_t)items * sizeof(LpSums))[(size_t)item * A.top + t] = sh.best[t];
+            } else
+                lp_finish(A, row, m, s, ent, token, given, sh.best);
+        }
+        if (item + gridDim.x < items) __syncthreads();
+    }
+}
+
+// One workgroup a row: the parts' sums and best tokens.  A part's own top-th key is a bound that the row's reach.
+template <typename T>
+__global__ void __launch_bounds__(LP_WG) k_logprobs_join(LpArgs A) {
+    __shared__ uint64_t cand[LP_PARTS * LP_TOP], best[LP_TOP];
+    __shared__ int slot[2][LP_WAVES], found;
+    const int t = threadIdx.x, lane = t & 63;
+    const size_t items = (size_t)A.rows * A.parts;
     for (int row = blockIdx.x; row < A.rows; row += gridDim.x) {
-        const T* x = (const T*)A.logits + (size_t)row * A.stride;
-        float m = -INFINITY;
-        for (int i = t; i < A.vocab; i += LP_WG) m = fmaxf(m, lp_get(x + i));
-        __syncthreads();
-        best[t] = m;
-        __syncthreads();
-        for (int i = 0; i < LP_WG; i++) m = fmaxf(m, best[i]);
-        double z = 0, e = 0;
-        for (int i = t; i < A.vocab; i += LP_WG) {
-            const double d = ((double)lp_get(x + i) - (double)m) * A.inv, p = exp(d);
-            z += p;
-            e += p > 0 ? p * d : 0;
-        }
-        sums[t] = z;
-        sums[LP_WG + t] = e;
-        __syncthreads();
-        z = e = 0;
-        for (int i = 0; i < LP_WG; i++) { z += sums[i]; e += sums[LP_WG + i]; }
-        const double logz = log1p(z - 1.0);
-        if (t == 0 && A.entropy) A.entropy[row] = (float)(logz - e / z);
+        const LpSums* sums = reinterpret_cast<const LpSums*>(A.work) + (size_t)row * A.parts;
+        const uint64_t* keys = reinterpret_cast<const uint64_t*>(A.work + items * sizeof(LpSums)) + (size_t)row * A.parts * A.top;
+        float given = 0.f;
+        int token = -1;
         if (t < A.given) {
-            const int id = A.tokens[(size_t)row * A.given + t];
-            A.logProb[(size_t)row * A.given + t] = id < 0 ? 0.f : id >= A.vocab ? NAN : (float)(((double)lp_get(x + id) - (double)m) * A.inv - logz);
+            token = A.tokens[(size_t)row * A.given + t];
+            if (token >= 0 && token < A.vocab) given = lp_get((const T*)A.logits + (size_t)row * A.stride + token);
         }
-        uint64_t last = ~0ull;
-        for (int j = 0; j < A.top; j++) {
-            uint64_t k = 0;
-            for (int i = t; i < A.vocab; i += LP_WG) {
-                const uint64_t y = lp_key(lp_get(x + i), i);
-                if (y < last && y > k) k = y;
+        if (A.top) {
+            if (t == 0) found = 0;
+            __syncthreads();
+            uint64_t bound = lane < A.parts ? keys[(lane + 1) * A.top - 1] : 0;
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) {
+                const uint64_t other = (uint64_t)__shfl_xor((unsigned long long)bound, o, 64);
+                bound = other > bound ? other : bound;
+            }
+            for (int i = t; i < A.parts * A.top; i += LP_WG) {
+                const uint64_t key = keys[i];
+                if (key && key >= bound) cand[atomicAdd(&found, 1)] = key;
             }
             __syncthreads();
-            keys[t] = k;
+            lp_best(cand, found, A.top, slot, best);
             __syncthreads();
-            for (int i = 0; i < LP_WG; i++) k = keys[i] > k ? keys[i] : k;
-            last = k;
-            const int id = (int)~(uint32_t)k;
-            if (t == 0) {
-                A.topIds[(size_t)row * A.top + j] = id;
-                A.topLogProb[(size_t)row * A.top + j] = (float)(((double)lp_get(x + id) - (double)m) * A.inv - logz);
-            }
+        }
+        if (t < 64) {
+            LpSums mine = {0.0, -INFINITY, 0.f};
+            if (lane < A.parts) mine = sums[lane];
+            const float m = lp_wave_max(mine.m);
+            lp_scale(mine.m, mine.s, mine.t, m, A.scale);
+            const double s = __shfl(lp_wave_sum(mine.s), 63, 64);
+            lp_finish(A, row, m, s, lp_last(lp_wave_sum(mine.t)), token, given, best);
         }
     }
 }
@@ -99,15 +449,44 @@ static std::string lp_check(const mlh_logprobs* a) {
     return "";
 }
 
-extern "C" uint64_t mlh_logprobs_work_bytes(const mlh_logprobs* a) { return 0; }
+// Elements of a part, a multiple of LP_WG granules: rows that fill the chip by themselves are not cut (up to LP_PART elements), fewer are.
+static int lp_part_granules(const mlh_logprobs* a) {
+    const int V = 16 / (int)kv_elem_bytes(a->type), granules = (a->vocab + 2 * V - 2) / V, most = LP_PART / V;
+    const int want = getenv("LP_WANT") ? atoi(getenv("LP_WANT")) : 1024, least = getenv("LP_LEAST") ? atoi(getenv("LP_LEAST")) : 4;
+    const int parts = std::min(LP_PARTS, std::max((granules + most - 1) / most, want / std::max(a->rows, 1)));
+    int per = ((granules + parts - 1) / parts + LP_WG - 1) / LP_WG * LP_WG;
+    per = std::min(std::max(per, least * LP_WG), most);
+    return per;
+}
+static int lp_parts(const mlh_logprobs* a, int per) {
+    const int V = 16 / (int)kv_elem_bytes(a->type), granules = (a->vocab + 2 * V - 2) / V;
+    return (granules + per - 1) / per;
+}
+
+extern "C" uint64_t mlh_logprobs_work_bytes(const mlh_logprobs* a) {
+    if (!lp_check(a).empty()) return 0;
+    const int parts = lp_parts(a, lp_part_granules(a));
+    return parts > 1 ? (uint64_t)a->rows * parts * (sizeof(LpSums) + 8 * a->top) : 0;
+}
+
+template <typename T> static int lp_go(const LpArgs& A, void* stream) {
+    const dim3 grid((unsigned)std::min<long long>((long long)A.rows * A.parts, 1 << 22));
+    const int rc = kv_launch(A.top ? &k_logprobs<T, true> : &k_logprobs<T, false>, grid, LP_WG, 0, stream, A);
+    if (rc || A.parts == 1) return rc;
+    return kv_launch(&k_logprobs_join<T>, dim3((unsigned)std::min(A.rows, 1 << 22)), LP_WG, 0, stream, A);
+}
 
 extern "C" int mlh_logprobs_device(const mlh_logprobs* a, void* stream) {
     const std::string bad = lp_check(a);
     if (!bad.empty()) return kv_fail(bad);
     if (a->rows == 0) return 0;
-    LpArgs A = {a->logits, a->stride, a->tokens, a->logProb, a->entropy, a->topIds, a->topLogProb, a->rows, a->vocab, a->given, a->top, a->temperature == 0.f ? 1.0 : 1.0 / (double)a->temperature};
-    const dim3 grid((unsigned)std::min(a->rows, 1 << 20));
-    if (a->type == MLH_DTYPE_F32) return kv_launch(&k_logprobs<float>, grid, LP_WG, 0, stream, A);
-    if (a->type == MLH_DTYPE_BF16) return kv_launch(&k_logprobs<bf16_t>, grid, LP_WG, 0, stream, A);
-    return kv_launch(&k_logprobs<f16_t>, grid, LP_WG, 0, stream, A);
+    const uint64_t need = mlh_logprobs_work_bytes(a);
+    if (need && (!a->work || (uintptr_t)a->work % 16 || a->workBytes < need)) return kv_fail("work must be 16-byte aligned and have mlh_logprobs_work_bytes");
+    const double inv = a->temperature == 0.f ? 1.0 : 1.0 / (double)a->temperature;
+    const int per = lp_part_granules(a);
+    LpArgs A = {a->logits, a->stride, a->tokens, a->logProb, a->entropy, a->topIds, a->topLogProb, a->rows, a->vocab, a->given, a->top, inv, (float)(inv * 1.4426950408889634074),
+                lp_parts(a, per), per, (unsigned char*)a->work};
+    if (a->type == MLH_DTYPE_F32) return lp_go<float>(A, stream);
+    if (a->type == MLH_DTYPE_BF16) return lp_go<bf16_t>(A, stream);
+    return lp_go<f16_t>(A, stream);
 }
