@@ -18,6 +18,7 @@
 #define LP_PART (LP_WG * LP_GROUP * LP_GROUPS) // elements of a part, at most
 #define LP_TOP 64
 #define LP_CANDS (LP_TOP * LP_GROUP)           // elements that are ranked, at most
+#define LP_PAD 8
 #define LP_PARTS 64                            // of a row, at most
 
 struct LpArgs {
@@ -119,10 +120,12 @@ __device__ __forceinline__ int lp_count(int mine, int* slot) {
     return n;
 }
 
-// Ranks the n keys in cand (all different; written before a barrier) and puts the first `top` of them into best, in order.  More than LP_WG are first cut down to few more than top, by
+// Ranks the n keys in cand (all different; written before a barrier; with room for LP_PAD more) and puts the first `top` of them into best, in order.  More than LP_WG are first cut down to few more than top, by
 // bisection.  All threads; best is whole after a barrier.
-__device__ void lp_best(const uint64_t* cand, int n, int top, int (*slot)[LP_WAVES], uint64_t* best) {
+__device__ void lp_best(uint64_t* cand, int n, int top, int (*slot)[LP_WAVES], uint64_t* best) {
     uint64_t least = 0;
+    if (threadIdx.x < LP_PAD) cand[n + threadIdx.x] = 0;
+    __syncthreads();
     if (n > LP_WG) {
         uint64_t lo = 0, hi = ~0ull; // as many as top reach lo, not hi
         for (int step = 0, seen = n; seen > top + 32 && hi - lo > 1; step++) {
@@ -138,7 +141,13 @@ __device__ void lp_best(const uint64_t* cand, int n, int top, int (*slot)[LP_WAV
         const uint64_t key = cand[i];
         if (key < least) continue;
         int r = 0;
-        for (int j = 0; j < n; j++) r += cand[j] > key;
+        for (int j = 0; j < n; j += LP_PAD) { // (one after the other, each would wait for the LDS by itself)
+            uint64_t other[LP_PAD];
+#pragma unroll
+            for (int q = 0; q < LP_PAD; q++) other[q] = cand[j + q];
+#pragma unroll
+            for (int q = 0; q < LP_PAD; q++) r += other[q] > key;
+        }
         if (r < top) best[r] = key;
     }
     for (int r = n + threadIdx.x; r < top; r += LP_WG) best[r] = 0; // (a short part)
@@ -147,12 +156,12 @@ __device__ void lp_best(const uint64_t* cand, int n, int top, int (*slot)[LP_WAV
 struct LpShared {
     union {
         uint32_t group[LP_GROUPS][LP_WG]; // rank of the largest of every group; 0: none
-        uint64_t cand[LP_CANDS];          // (once the groups that matter are known)
+        uint64_t cand[LP_CANDS + LP_PAD]; // (once the groups that matter are known)
     };
     uint32_t most[LP_WG];
     uint64_t best[LP_TOP];
     int list[LP_TOP];
-    int count, found;
+    int count, found, seen;
     uint32_t bound;
     int slot[2][LP_WAVES];
     float m[LP_WAVES], t[LP_WAVES];
@@ -182,41 +191,59 @@ template <typename T> __device__ void lp_tops(LpShared& sh, const LpRow& R, int 
 #pragma unroll
         for (int i = 0; i < LP_WAVES; i++) { b[i] = sh.most[i * 64 + t]; lo = min(lo, b[i]); hi = max(hi, b[i]); }
         hi = lp_last(lp_wave(hi, 0u, [](uint32_t a, uint32_t c) { return max(a, c); })) + 1;
-        lo = top == 1 ? hi - 1 : lp_last(lp_wave(lo, ~0u, [](uint32_t a, uint32_t c) { return min(a, c); }));
-        for (int seen = LP_WG; seen > top + top / 4 && hi - lo > 1;) {
-            const uint32_t mid = lo + (hi - lo) / 2;
+        lo = lp_last(lp_wave(lo, ~0u, [](uint32_t a, uint32_t c) { return min(a, c); }));
+        const auto reach = [&](uint32_t least) {
             int c = 0;
 #pragma unroll
-            for (int i = 0; i < LP_WAVES; i++) c += __builtin_popcountll(__ballot(b[i] >= mid));
+            for (int i = 0; i < LP_WAVES; i++) c += __builtin_popcountll(__ballot(b[i] >= least));
+            return c;
+        };
+        if (top == 1) lo = hi - 1;
+        if (reach(lo + 1) < top) hi = lo + 1; // (masked tokens fill most threads, or top is 1)
+        int seen = reach(lo);
+        while (seen > top + top / 4 && hi - lo > 1) {
+            const uint32_t mid = lo + (hi - lo) / 2;
+            const int c = reach(mid);
             if (c >= top) { lo = mid; seen = c; } else hi = mid;
         }
-        if (t == 0) sh.bound = max(lo, 1u);
+        if (t == 0) {
+            sh.bound = max(lo, 1u);
+            sh.seen = lo ? seen : 0;
+        }
     }
     __syncthreads();
     uint32_t bound = sh.bound;
     const auto list = [&](uint32_t least) { // this thread's groups that reach it
-        for (int j = 0; j < groups; j++)
-            if (sh.group[j][t] >= least) {
-                const int i = atomicAdd(&sh.count, 1);
-                if (i < LP_TOP) sh.list[i] = j << 8 | t;
-            }
+        uint32_t those = 0;
+#pragma unroll
+        for (int j = 0; j < LP_GROUPS; j++) those |= (uint32_t)(j < groups && sh.group[j][t] >= least) << j;
+        while (those) {
+            const int i = atomicAdd(&sh.count, 1);
+            if (i < LP_TOP) sh.list[i] = __builtin_ctz(those) << 8 | t;
+            those &= those - 1;
+        }
     };
-    if (mine >= bound) list(bound);
-    __syncthreads();
-    const bool many = sh.count > LP_TOP;
-    if (many) { // the top-th largest group itself: fewer than top groups are larger
+    bool many = sh.seen > LP_TOP; // (threads that are equal at the bound)
+    if (!many) {
+        if (mine >= bound) list(bound);
+        __syncthreads();
+        many = sh.count > LP_TOP;
+    }
+    if (many) { // a bound that at least top groups reach and at most LP_TOP; if there is none, the top-th largest group itself: fewer than top are larger
         uint32_t lo = bound, hi = ~0u;
-        for (int step = 0; hi - lo > 1; step++) {
-            const uint32_t mid = step == 0 ? lo + 1 : lo + (hi - lo) / 2; // (most often it is the bound: masked tokens fill the groups up)
+        for (int step = 0; many && hi - lo > 1; step++) {
+            const uint32_t mid = step == 0 ? lo + 1 : lo + (hi - lo) / 2; // (most often masked tokens are what is at the bound)
             int c = 0;
             if (mine >= mid)
                 for (int j = 0; j < groups; j++) c += sh.group[j][t] >= mid;
-            if (lp_count(c, sh.slot[step & 1]) >= top) lo = mid; else hi = mid;
+            c = lp_count(c, sh.slot[step & 1]);
+            if (c >= top) lo = mid; else hi = mid;
+            many = c < top || c > LP_TOP;
         }
         bound = lo;
         if (t == 0) sh.count = 0;
         __syncthreads();
-        if (mine > bound) list(bound + 1);
+        if (mine >= bound) list(many ? bound + 1 : bound);
         __syncthreads();
     }
     const int listed = sh.count;
@@ -391,7 +418,7 @@ __global__ void __launch_bounds__(LP_WG, sizeof(T) == 4 ? 5 : 6) k_logprobs(LpAr
 // One workgroup a row: the parts' sums and best tokens.  A part's own top-th key is a bound that the row's reach.
 template <typename T>
 __global__ void __launch_bounds__(LP_WG) k_logprobs_join(LpArgs A) {
-    __shared__ uint64_t cand[LP_PARTS * LP_TOP], best[LP_TOP];
+    __shared__ uint64_t cand[LP_PARTS * LP_TOP + LP_PAD], best[LP_TOP];
     __shared__ int slot[2][LP_WAVES], found;
     const int t = threadIdx.x, lane = t & 63;
     const size_t items = (size_t)A.rows * A.parts;
@@ -449,14 +476,15 @@ static std::string lp_check(const mlh_logprobs* a) {
     return "";
 }
 
-// Elements of a part, a multiple of LP_WG granules: rows that fill the chip by themselves are not cut (up to LP_PART elements), fewer are.
+// Granules of a part.  A row is one workgroup's where it can be (LP_PART): a second launch costs about 4 us, and many rows fill the chip.  Few and long rows are cut, since one
+// compute unit takes 0.1 us for 1000 elements: in bf16 with the 20 most likely, rows whole / cut, 1 row of 32768 10.6 / 12.8 us, 50000 13.1 / 12.7, 100000 19.5 / 13.5; 64 rows 11.6 / 13.7,
+// 14.4 / 14.2, 20.8 / 16.2; 128 rows of 50000 14.8 / 16.0, of 131072 21.4 / 21.3.  Parts of eight granules a thread or more (four: 14.5 for one row of 100000 in bf16, 22.4 for 13.4 in fp32).
 static int lp_part_granules(const mlh_logprobs* a) {
     const int V = 16 / (int)kv_elem_bytes(a->type), granules = (a->vocab + 2 * V - 2) / V, most = LP_PART / V;
-    const int want = getenv("LP_WANT") ? atoi(getenv("LP_WANT")) : 1024, least = getenv("LP_LEAST") ? atoi(getenv("LP_LEAST")) : 4;
-    const int parts = std::min(LP_PARTS, std::max((granules + most - 1) / most, want / std::max(a->rows, 1)));
-    int per = ((granules + parts - 1) / parts + LP_WG - 1) / LP_WG * LP_WG;
-    per = std::min(std::max(per, least * LP_WG), most);
-    return per;
+    int parts = (granules + most - 1) / most;
+    if (a->rows <= 64 && a->vocab >= 49152) parts = std::max(parts, std::min(LP_PARTS, 256 / std::max(a->rows, 1)));
+    const int per = ((granules + parts - 1) / parts + LP_WG - 1) / LP_WG * LP_WG;
+    return std::min(std::max(per, 8 * LP_WG), most);
 }
 static int lp_parts(const mlh_logprobs* a, int per) {
     const int V = 16 / (int)kv_elem_bytes(a->type), granules = (a->vocab + 2 * V - 2) / V;
