@@ -13,7 +13,8 @@ typedef __bf16 w4_bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 w4_f16x8 __attribute__((ext_vector_type(8)));
 
 #define W4_WG 256   // threads of the kernels that lay out and read
-#define W4_WAVES 8  // waves of a product's workgroup
+#define W4_WAVES 8   // waves of a product's workgroup that multiply
+#define W4_LOADERS 4 // ... and that bring A, where it goes through LDS
 
 // ----------------------------------------------------------------------------
 // laying out
@@ -96,35 +97,35 @@ struct Gemm4Args {
     int M, N, K, swiglu;
 };
 
-// How codes and activations meet on the matrix cores, exactly.  PLANES: of an activation.  codes(x, i): eight codes of a word as an operand that stands for UNIT * (code + SHIFT).
+// Columns 2j and 2j + 1 of a word of codes, each in bits 3 to 6 of a half
+template <int J> __device__ __forceinline__ uint32_t w4_turn(uint32_t x) { return J == 0 ? x : J == 3 ? __builtin_amdgcn_alignbit(x, x, 12) : x >> (4 * J); }
+
+// How codes and activations meet on the matrix cores, exactly.  PLANES: of an activation.  codes(x): a word of eight codes as an operand that stands for UNIT * (code + SHIFT); unit(): one of UNIT.
 template <typename T> struct W4Mul;
-template <> struct W4Mul<f16_t> { // codes as the smallest halves, code * 2^-24
+template <> struct W4Mul<f16_t> { // codes as halves below 2^-14, code * 2^-21
     static constexpr int PLANES = 1;
-    static constexpr float UNIT = 0x1p-24f, SHIFT = 0.f;
+    static constexpr float UNIT = 0x1p-21f, SHIFT = 0.f;
     typedef w4_f16x8 V;
     static __device__ __forceinline__ V codes(uint32_t x) {
-        return __builtin_bit_cast(V, w4_u32x4{x & 0x000f000fu, x >> 4 & 0x000f000fu, x >> 8 & 0x000f000fu, x >> 12 & 0x000f000fu});
+        return __builtin_bit_cast(V, w4_u32x4{w4_turn<0>(x) & 0x00780078u, w4_turn<1>(x) & 0x00780078u, w4_turn<2>(x) & 0x00780078u, w4_turn<3>(x) & 0x00780078u});
     }
-    static __device__ __forceinline__ V ones() { return V{1, 1, 1, 1, 1, 1, 1, 1}; }
+    static __device__ __forceinline__ V unit() { return __builtin_bit_cast(V, w4_u32x4{0x00080008u, 0x00080008u, 0x00080008u, 0x00080008u}); }
     static __device__ __forceinline__ w4_f32x4 mul(V a, V b, w4_f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 };
-template <> struct W4Mul<bf16_t> { // codes behind 16: 16 + code is a bf16 with the code in bits 3 to 6
+template <> struct W4Mul<bf16_t> { // codes behind 16: a bf16 of 16 + code has the code in bits 3 to 6
     static constexpr int PLANES = 1;
     static constexpr float UNIT = 1.f, SHIFT = 16.f;
     typedef w4_bf16x8 V;
     static __device__ __forceinline__ V codes(uint32_t x) {
-        return __builtin_bit_cast(V, w4_u32x4{(x << 3 & 0x00780078u) | 0x41804180u, (x >> 1 & 0x00780078u) | 0x41804180u, (x >> 5 & 0x00780078u) | 0x41804180u, (x >> 9 & 0x00780078u) | 0x41804180u});
+        uint32_t base = 0x41804180u;
+        asm("" : "+v"(base)); // (a register: with two literals the mask and the base would take an instruction each)
+        return __builtin_bit_cast(V, w4_u32x4{(w4_turn<0>(x) & 0x00780078u) | base, (w4_turn<1>(x) & 0x00780078u) | base, (w4_turn<2>(x) & 0x00780078u) | base, (w4_turn<3>(x) & 0x00780078u) | base});
     }
-    static __device__ __forceinline__ V ones() { return __builtin_bit_cast(V, w4_u32x4{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u}); }
+    static __device__ __forceinline__ V unit() { return __builtin_bit_cast(V, w4_u32x4{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u}); }
     static __device__ __forceinline__ w4_f32x4 mul(V a, V b, w4_f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 };
-template <> struct W4Mul<float> { // the same with activations as three planes (p3.h): every product exact
+template <> struct W4Mul<float> : W4Mul<bf16_t> { // the same with activations as three planes (p3.h): every product exact
     static constexpr int PLANES = 3;
-    static constexpr float UNIT = 1.f, SHIFT = 16.f;
-    typedef w4_bf16x8 V;
-    static __device__ __forceinline__ V codes(uint32_t x) { return W4Mul<bf16_t>::codes(x); }
-    static __device__ __forceinline__ V ones() { return W4Mul<bf16_t>::ones(); }
-    static __device__ __forceinline__ w4_f32x4 mul(V a, V b, w4_f32x4 c) { return W4Mul<bf16_t>::mul(a, b, c); }
 };
 
 __device__ __forceinline__ float w4_get(const float* p) { return *p; }
@@ -134,145 +135,29 @@ __device__ __forceinline__ void w4_put(float* p, float v) { *p = v; }
 __device__ __forceinline__ void w4_put(bf16_t* p, float v) { *p = (bf16_t)kv_to_bf16(v); }
 __device__ __forceinline__ void w4_put(f16_t* p, float v) { p->bits = (uint16_t)kv_to_half(v); }
 
-// Eight neighbouring elements of a row of A on their way into LDS: raw, then as the planes that are multiplied
+// Eight neighbouring elements of a row of A: as loaded, and as the operands that are multiplied
 template <typename T> struct W4Raw {
     w4_u32x4 x;
     __device__ __forceinline__ void load(const T* p) { x = *reinterpret_cast<const w4_u32x4*>(p); }
     __device__ __forceinline__ void zero() { x = w4_u32x4{}; }
-    __device__ __forceinline__ void put(w4_u32x4* at, int) const { *at = x; }
+    __device__ __forceinline__ void split(w4_u32x4 (&v)[1]) const { v[0] = x; }
 };
 template <> struct W4Raw<float> {
     w4_u32x4 x[2];
     __device__ __forceinline__ void load(const float* p) { x[0] = *reinterpret_cast<const w4_u32x4*>(p); x[1] = *reinterpret_cast<const w4_u32x4*>(p + 4); }
     __device__ __forceinline__ void zero() { x[0] = x[1] = w4_u32x4{}; }
-    __device__ __forceinline__ void put(w4_u32x4* at, int plane) const {
+    __device__ __forceinline__ void split(w4_u32x4 (&v)[3]) const {
         uint32_t s[4][3];
 #pragma unroll
         for (int i = 0; i < 4; i++) p3_split2(__uint_as_float(x[i / 2][i % 2 * 2]), __uint_as_float(x[i / 2][i % 2 * 2 + 1]), s[i]);
 #pragma unroll
-        for (int pl = 0; pl < 3; pl++) at[pl * plane] = w4_u32x4{s[0][pl], s[1][pl], s[2][pl], s[3][pl]};
+        for (int pl = 0; pl < 3; pl++) v[pl] = w4_u32x4{s[0][pl], s[1][pl], s[2][pl], s[3][pl]};
     }
 };
 
-// A workgroup of WN x WK waves: WN * NT * 16 rows of W against all rows of A, K in blocks of WK * TPW tiles.  A block of A goes through LDS, once for all waves (asked for a block ahead,
-// into registers); wave (wn, wk) multiplies TPW tiles of it with its NT times 16 rows, whose codes it asks for a block ahead, too.  Sums over K stay in registers; those of the WK waves are
-// added up in LDS at the end, in order.
-// With sum over a group of a (min + scale code) = (scale / UNIT) D + (min - scale SHIFT) S, D the sum of a (UNIT (code + SHIFT)) and S the sum of a: both come from the matrix cores, S as a product with ones.
-// Lane l of a result holds column l % 16 (a row of W) and the instruction's rows 4 (l / 16) + i, i = 0 .. 3.  RG of the four are used: row m of A is row m / RG * 4 + m % RG of the
-// instruction, so that few rows cost few multiplications by scales.
-template <typename T, int G, int MT, int RG, int WN, int WK, int NT, int TPW>
-__global__ void __launch_bounds__(W4_WAVES * 64) k_gemm4(Gemm4Args A) {
-    typedef W4Mul<T> X;
-    static_assert(WN * WK == W4_WAVES && (MT == 1 || RG == 4), "waves, rows");
-    constexpr int S = G / 32, TG = w4_groups(G), KB = WK * TPW * W4_COLS, THREADS = W4_WAVES * 64, ROWS = MT * 4 * RG, UPT = (ROWS * KB / 8 + THREADS - 1) / THREADS;
-    typedef uint32_t Pairs __attribute__((ext_vector_type(TG)));
-    extern __shared__ w4_u32x4 lds[];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wn = wave / WK, wk = wave % WK, row = lane & 15, quad = lane >> 4;
-    const int tiles = w4_tiles(A.K), blocks = (tiles + WK * TPW - 1) / (WK * TPW), bands = (A.N + W4_ROWS - 1) / W4_ROWS;
-    const int held = MT == 1 ? A.M : ROWS; // rows of A in LDS
-    const int plane = KB / 32 * held * 4;  // pieces of 16 bytes of a plane: [KB / 32][held][4], the four of a row's 32 columns swapped so that the lanes' reads meet no bank twice
-    const uint8_t* w[NT];
-#pragma unroll
-    for (int nt = 0; nt < NT; nt++) w[nt] = A.w + (size_t)min((int)(blockIdx.x * WN + wn) * NT + nt, bands - 1) * tiles * w4_tile(G);
-
-    w4_u32x4 codes[TPW][NT];
-    Pairs pairs[TPW][NT];
-    const auto ask = [&](int b, int j) {
-        const int t = min((b * WK + wk) * TPW + j, tiles - 1);
-#pragma unroll
-        for (int nt = 0; nt < NT; nt++) {
-            codes[j][nt] = *reinterpret_cast<const w4_u32x4*>(w[nt] + (size_t)t * w4_tile(G) + lane * 16);
-            pairs[j][nt] = *reinterpret_cast<const Pairs*>(w[nt] + (size_t)t * w4_tile(G) + W4_CODES + row * (TG * 4));
-        }
-    };
-    W4Raw<T> raw[UPT];
-    const auto ask_a = [&](int b) { // unit u: piece u % 4 of row u / 4 % held of 32 columns u / (4 held)
-#pragma unroll
-        for (int i = 0; i < UPT; i++) {
-            const int u = i * THREADS + threadIdx.x, m = u / 4 % held, k = b * KB + u / (4 * held) * 32 + u % 4 * 8;
-            if (u < plane) {
-                if (k < A.K) raw[i].load((const T*)A.a + (size_t)min(m, A.M - 1) * A.aStride + k);
-                else raw[i].zero();
-            }
-        }
-    };
-    const auto put_a = [&]() {
-#pragma unroll
-        for (int i = 0; i < UPT; i++) {
-            const int u = i * THREADS + threadIdx.x, m = u / 4 % held;
-            if (u < plane) raw[i].put(lds + (u ^ (m >> 2 & 3)), plane);
-        }
-    };
-    ask_a(0);
-#pragma unroll
-    for (int j = 0; j < TPW; j++) ask(0, j);
-
-    const typename X::V one = X::ones();
-    w4_f32x4 acc[NT][MT] = {};
-    const w4_u32x4* mine[MT]; // this lane's piece of the first 32 columns
-#pragma unroll
-    for (int mt = 0; mt < MT; mt++) {
-        const int m = MT == 1 ? min(row / 4 * RG + min(row % 4, RG - 1), held - 1) : mt * 16 + row;
-        mine[mt] = lds + m * 4 + (quad ^ (m >> 2 & 3));
-    }
-    for (int b = 0; b < blocks; b++) {
-        if (b) __syncthreads();
-        put_a();
-        __syncthreads();
-        if (b + 1 < blocks) ask_a(b + 1);
-#pragma unroll
-        for (int j = 0; j < TPW; j++) {
-            if ((b * WK + wk) * TPW + j < tiles) {
-#pragma unroll
-                for (int g = 0; g < TG; g++) {
-                    w4_f32x4 d[NT][MT] = {}, s[MT] = {};
-#pragma unroll
-                    for (int q = 0; q < S; q++) {
-                        const int step = g * S + q;
-                        typename X::V c[NT];
-#pragma unroll
-                        for (int nt = 0; nt < NT; nt++) c[nt] = X::codes(codes[j][nt][step]);
-#pragma unroll
-                        for (int mt = 0; mt < MT; mt++) {
-#pragma unroll
-                            for (int p = X::PLANES - 1; p >= 0; p--) {
-                                const typename X::V a = __builtin_bit_cast(typename X::V, mine[mt][p * plane + ((wk * TPW + j) * 4 + step) * held * 4]);
-                                s[mt] = X::mul(a, one, s[mt]);
-#pragma unroll
-                                for (int nt = 0; nt < NT; nt++) d[nt][mt] = X::mul(a, c[nt], d[nt][mt]);
-                            }
-                        }
-                    }
-#pragma unroll
-                    for (int nt = 0; nt < NT; nt++) {
-                        const float sc = kv_half(pairs[j][nt][g] >> 16), scale = sc * (1.f / X::UNIT), low = kv_half(pairs[j][nt][g] & 0xffffu) - sc * X::SHIFT;
-#pragma unroll
-                        for (int mt = 0; mt < MT; mt++)
-#pragma unroll
-                            for (int i = 0; i < RG; i++) acc[nt][mt][i] = fmaf(scale, d[nt][mt][i], fmaf(low, s[mt][i], acc[nt][mt][i]));
-                    }
-                }
-            }
-            if (b + 1 < blocks) ask(b + 1, j);
-        }
-    }
-    // [WK][WN * NT][ROWS][16]
-    __syncthreads();
-    float* part = reinterpret_cast<float*>(lds);
-#pragma unroll
-    for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-        for (int mt = 0; mt < MT; mt++)
-#pragma unroll
-            for (int i = 0; i < RG; i++) part[((wk * WN * NT + wn * NT + nt) * ROWS + mt * 16 + quad * RG + i) * 16 + row] = acc[nt][mt][i];
-    __syncthreads();
-    const auto sum = [&](int m, int n) { // element (m, n) of this workgroup's columns
-        float v = 0.f;
-#pragma unroll
-        for (int q = 0; q < WK; q++) v += part[((q * WN * NT + n / 16) * ROWS + m) * 16 + n % 16];
-        return v;
-    };
-    constexpr int COLS = WN * NT * 16;
+// The epilogue of BANDS times 16 columns: sum(m, n) is their element (m, n)
+template <typename T, int BANDS, int THREADS, typename F> __device__ __forceinline__ void w4_finish(const Gemm4Args& A, F sum) {
+    constexpr int COLS = BANDS * 16;
     if (A.swiglu) {
         for (int u = threadIdx.x; u < A.M * (COLS / 2); u += THREADS) {
             const int m = u / (COLS / 2), j = u % (COLS / 2), n = (int)blockIdx.x * (COLS / 2) + j;
@@ -289,6 +174,260 @@ __global__ void __launch_bounds__(W4_WAVES * 64) k_gemm4(Gemm4Args A) {
             w4_put((T*)A.c + (size_t)m * A.cStride + n, v);
         }
     }
+}
+
+// Products with minimum and scale behind the sums: the sum over a group of a (min + scale code) is (scale D + (min - scale SHIFT) S) / UNIT, D the sum of a UNIT (code + SHIFT) and S that of
+// a UNIT; both come from the matrix cores, S as a product with UNIT.  Lane l of a result holds column l % 16 (a row of W) and the instruction's rows 4 (l / 16) + i, i = 0 .. 3.
+//
+// Few rows, four in an operand: the instruction's row 4 m + s is row m of A in the s-th 32 columns of a tile, so that one load brings a tile's share of A to the lanes that multiply it and the product with
+// the s-th step's codes has that step's sums, of row m, in element s of lanes 16 m to 16 m + 15.  (The other elements are of rows and codes that do not belong together.)  One product with UNIT gives the S of
+// all four steps.  No LDS and no barrier but for the sums of WK waves at the end.
+// A workgroup is WN x WK waves, WN * NT * 16 rows of W; a wave has TPW tiles of its share of K on their way.
+template <typename T, int G, int MR, int WN, int WK, int NT, int TPW>
+__global__ void __launch_bounds__(W4_WAVES * 64) k_gemm4_few(Gemm4Args A) {
+    typedef W4Mul<T> X;
+    constexpr int S = G / 32, TG = w4_groups(G);
+    static_assert(WN * WK == W4_WAVES, "waves");
+    typedef uint32_t Pairs __attribute__((ext_vector_type(TG)));
+    __shared__ float part[WK][WN * NT][MR][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wn = wave / WK, wk = wave % WK, row = lane & 15, quad = lane >> 4;
+    const int tiles = w4_tiles(A.K), bands = (A.N + W4_ROWS - 1) / W4_ROWS, k0 = (row & 3) * 32 + quad * 8;
+    const uint8_t* w[NT];
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) w[nt] = A.w + (size_t)min((int)(blockIdx.x * WN + wn) * NT + nt, bands - 1) * tiles * w4_tile(G);
+    const T* from[MR];
+#pragma unroll
+    for (int r = 0; r < MR; r++) from[r] = (const T*)A.a + (size_t)min(r * 4 + (row >> 2), A.M - 1) * A.aStride;
+
+    w4_u32x4 codes[TPW][NT];
+    Pairs pairs[TPW][NT];
+    W4Raw<T> raw[TPW][MR];
+    const auto ask = [&](int t, int j) { // (behind the end the last tile again, so that there is always as much on its way)
+        t = min(t, tiles - 1);
+        const int k = min(t * W4_COLS + k0, A.K - 8);
+#pragma unroll
+        for (int r = 0; r < MR; r++) raw[j][r].load(from[r] + k);
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+            const uint8_t* at = w[nt] + (size_t)t * w4_tile(G);
+            codes[j][nt] = *reinterpret_cast<const w4_u32x4*>(at + lane * 16);
+            pairs[j][nt] = *reinterpret_cast<const Pairs*>(at + W4_CODES + row * (TG * 4));
+        }
+    };
+#pragma unroll
+    for (int j = 0; j < TPW; j++) ask(j * WK + wk, j);
+    const typename X::V unit = X::unit();
+    float acc[NT][MR] = {};
+    for (int t0 = wk; t0 < tiles; t0 += WK * TPW) {
+#pragma unroll
+        for (int j = 0; j < TPW; j++) {
+            const int t = t0 + j * WK;
+            if (t < tiles) {
+                if (t * W4_COLS + W4_COLS > A.K && t * W4_COLS + k0 >= A.K) {
+#pragma unroll
+                    for (int r = 0; r < MR; r++) raw[j][r].zero();
+                }
+                w4_u32x4 a[MR][X::PLANES];
+                w4_f32x4 s[MR] = {};
+#pragma unroll
+                for (int r = 0; r < MR; r++) {
+                    raw[j][r].split(a[r]);
+#pragma unroll
+                    for (int p = X::PLANES - 1; p >= 0; p--) s[r] = X::mul(__builtin_bit_cast(typename X::V, a[r][p]), unit, s[r]);
+                }
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) {
+#pragma unroll
+                    for (int step = 0; step < 4; step++) {
+                        const int g = step / S;
+                        const typename X::V c = X::codes(codes[j][nt][step]);
+                        const float scale = kv_half(pairs[j][nt][g] >> 16), low = kv_half(pairs[j][nt][g] & 0xffffu) - scale * X::SHIFT;
+#pragma unroll
+                        for (int r = 0; r < MR; r++) {
+                            w4_f32x4 d = {};
+#pragma unroll
+                            for (int p = X::PLANES - 1; p >= 0; p--) d = X::mul(__builtin_bit_cast(typename X::V, a[r][p]), c, d);
+                            acc[nt][r] = fmaf(scale, d[step], acc[nt][r]);
+                            if (step % S == S - 1) {
+                                float sum = s[r][g * S];
+#pragma unroll
+                                for (int q = 1; q < S; q++) sum += s[r][g * S + q];
+                                acc[nt][r] = fmaf(low, sum, acc[nt][r]);
+                            }
+                        }
+                    }
+                }
+            }
+            ask(t + WK * TPW, j);
+        }
+    }
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+        for (int r = 0; r < MR; r++) part[wk][wn * NT + nt][r][lane] = acc[nt][r] * (1.f / X::UNIT);
+    __syncthreads();
+    w4_finish<T, WN * NT, W4_WAVES * 64>(A, [&](int m, int n) {
+        float v = 0.f;
+#pragma unroll
+        for (int q = 0; q < WK; q++) v += part[q][n / 16][m / 4][m % 4 * 16 + n % 16];
+        return v;
+    });
+}
+
+// More rows, MT times 16: the instruction's rows are rows of A.  A goes through LDS, once for all waves of a workgroup, a block of WK * TPW tiles of K at a time and two blocks in turn; W4_LOADERS
+// further waves bring it there, since loads come back in the order they were asked for: a wave that waits for A, which is near, would wait for codes that are far and not needed yet.  Wave (wn, wk) of the
+// others multiplies TPW tiles of every block with its NT times 16 rows of W, whose codes it asks for AHEAD blocks ahead.
+// In LDS piece q (eight columns) of step s (32 columns) of row m stands at [m][s ^ (m / 4 % 4)][q ^ (m % 4)], so that neither the lanes of a store, which share a row, nor those of a load, which share
+// step and piece, meet in a bank.
+template <typename T, int G, int MT, int WN, int WK, int NT, int TPW, int AHEAD>
+__global__ void __launch_bounds__((W4_WAVES + W4_LOADERS) * 64) k_gemm4_many(Gemm4Args A) {
+    typedef W4Mul<T> X;
+    constexpr int S = G / 32, TG = w4_groups(G), ROWS = MT * 16, STEPS = WK * TPW * 4, PIECES = STEPS * 4, PLANE = ROWS * PIECES, BUF = PLANE * X::PLANES;
+    typedef uint32_t Pairs __attribute__((ext_vector_type(TG)));
+    extern __shared__ w4_u32x4 lds[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int tiles = w4_tiles(A.K), blocks = (tiles + WK * TPW - 1) / (WK * TPW);
+    const int wn = wave / WK, wk = wave % WK, row = lane & 15, quad = lane >> 4;
+    float* part = reinterpret_cast<float*>(lds); // [WK][WN * NT][ROWS][16], at the end
+    if (wave >= W4_WAVES) {
+        constexpr int THREADS = W4_LOADERS * 64, UNITS = PLANE / THREADS, EVERY = THREADS / PIECES; // EVERY: rows from one of a thread's pieces to the next
+        static_assert(WN * WK == W4_WAVES && PIECES <= THREADS && PLANE % THREADS == 0, "waves, pieces of A");
+        const int thread = threadIdx.x - W4_WAVES * 64, row0 = PIECES < 64 ? thread / PIECES : (wave - W4_WAVES) * 64 / PIECES, piece = thread % PIECES;
+        W4Raw<T> raw[UNITS];
+        const T* from[UNITS]; // rows, the last one again behind the end
+#pragma unroll
+        for (int i = 0; i < UNITS; i++) from[i] = (const T*)A.a + (size_t)min(row0 + i * EVERY, A.M - 1) * A.aStride;
+        const auto ask = [&](int b) { // (behind the end of a row its last piece again)
+            const unsigned k = min(b * (STEPS * 32) + piece * 8, A.K - 8);
+#pragma unroll
+            for (int i = 0; i < UNITS; i++) raw[i].load(from[i] + k);
+        };
+        // the place of row m's piece: EVERY divides or is a multiple of 4, so that the bits of m that are swapped in are those of row0 and of i * EVERY put together
+        const int place = row0 * PIECES + (((piece >> 2) ^ (row0 >> 2 & 3)) * 4 | ((piece & 3) ^ (row0 & 3)));
+        const auto put = [&](int b) {
+            w4_u32x4* const buf = lds + (b & 1) * BUF;
+            if ((b + 1) * (STEPS * 32) > A.K && b * (STEPS * 32) + piece * 8 >= A.K) {
+#pragma unroll
+                for (int i = 0; i < UNITS; i++) raw[i].zero();
+            }
+#pragma unroll
+            for (int i = 0; i < UNITS; i++) {
+                w4_u32x4 v[X::PLANES];
+                raw[i].split(v);
+#pragma unroll
+                for (int p = 0; p < X::PLANES; p++) buf[(place ^ ((i * EVERY >> 2 & 3) * 4 | (i * EVERY & 3))) + (p * PLANE + i * EVERY * PIECES)] = v[p];
+            }
+        };
+        ask(0);
+        put(0);
+        ask(1);
+        __syncthreads();
+        for (int b = 0; b < blocks; b++) { // (while the others multiply block b)
+            if (b + 1 < blocks) put(b + 1);
+            ask(b + 2);
+            __syncthreads();
+        }
+    } else {
+        const int bands = (A.N + W4_ROWS - 1) / W4_ROWS;
+        const uint8_t* w[NT];
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) w[nt] = A.w + (size_t)min((int)(blockIdx.x * WN + wn) * NT + nt, bands - 1) * tiles * w4_tile(G);
+        w4_u32x4 codes[AHEAD][TPW][NT];
+        Pairs pairs[AHEAD][TPW][NT];
+        const auto ask = [&](int b, int a, int j) { // (behind the end the last tile again, so that there is always as much on its way)
+            const int t = min((b * WK + wk) * TPW + j, tiles - 1);
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) {
+                const uint8_t* at = w[nt] + (size_t)t * w4_tile(G);
+                codes[a][j][nt] = *reinterpret_cast<const w4_u32x4*>(at + lane * 16);
+                pairs[a][j][nt] = *reinterpret_cast<const Pairs*>(at + W4_CODES + row * (TG * 4));
+            }
+        };
+#pragma unroll
+        for (int a = 0; a < AHEAD; a++)
+#pragma unroll
+            for (int j = 0; j < TPW; j++) ask(a, a, j);
+        int at[4]; // this lane's piece of step s of the block's first tile, in its first 16 rows
+#pragma unroll
+        for (int s = 0; s < 4; s++) at[s] = (row * STEPS + (s ^ (row >> 2 & 3))) * 4 + (quad ^ (row & 3));
+        const typename X::V unit = X::unit();
+        w4_f32x4 acc[NT][MT] = {};
+        __syncthreads();
+        for (int b0 = 0; b0 < blocks; b0 += AHEAD) {
+#pragma unroll
+            for (int u = 0; u < AHEAD; u++) {
+                const int b = b0 + u;
+                if (b < blocks) {
+                    const w4_u32x4* const buf = lds + (b & 1) * BUF;
+
+                    // Sixteen rows of A by a group of columns at a time; A's pieces for the next ones are asked for in front of the products, between which the scales of the last ones are applied.
+                    // (Behind the last tile A is zero.)
+                    constexpr int PARTS = TPW * TG * MT;
+                    typename X::V a[2][S][X::PLANES];
+                    const auto fetch = [&](int i) {
+#pragma unroll
+                        for (int q = 0; q < S; q++)
+#pragma unroll
+                            for (int p = 0; p < X::PLANES; p++)
+                                a[i & 1][q][p] = __builtin_bit_cast(typename X::V, buf[p * PLANE + at[i / MT % TG * S + q] + i % MT * 16 * PIECES + (wk * TPW + i / MT / TG) * 16]);
+                    };
+                    fetch(0);
+                    typename X::V c[S][NT];
+                    float scale[2][NT], low[2][NT];
+                    w4_f32x4 d[2][NT], s[2];
+                    const auto apply = [&](int i) {
+                        const int mt = i % MT, h = i / MT & 1;
+#pragma unroll
+                        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                            for (int e = 0; e < 4; e++) acc[nt][mt][e] = fmaf(scale[h][nt], d[i & 1][nt][e], fmaf(low[h][nt], s[i & 1][e], acc[nt][mt][e]));
+                    };
+#pragma unroll
+                    for (int i = 0; i < PARTS; i++) {
+                        const int mt = i % MT, g = i / MT % TG, j = i / MT / TG, h = i / MT & 1;
+                        if (i + 1 < PARTS) fetch(i + 1);
+                        if (mt == 0) {
+#pragma unroll
+                            for (int nt = 0; nt < NT; nt++) {
+#pragma unroll
+                                for (int q = 0; q < S; q++) c[q][nt] = X::codes(codes[u][j][nt][g * S + q]);
+                                scale[h][nt] = kv_half(pairs[u][j][nt][g] >> 16);
+                                low[h][nt] = kv_half(pairs[u][j][nt][g] & 0xffffu) - scale[h][nt] * X::SHIFT;
+                            }
+                        }
+                        s[i & 1] = w4_f32x4{};
+#pragma unroll
+                        for (int nt = 0; nt < NT; nt++) d[i & 1][nt] = w4_f32x4{};
+#pragma unroll
+                        for (int q = 0; q < S; q++)
+#pragma unroll
+                            for (int p = X::PLANES - 1; p >= 0; p--) {
+                                s[i & 1] = X::mul(a[i & 1][q][p], unit, s[i & 1]);
+#pragma unroll
+                                for (int nt = 0; nt < NT; nt++) d[i & 1][nt] = X::mul(a[i & 1][q][p], c[q][nt], d[i & 1][nt]);
+                            }
+                        if (i > 0) apply(i - 1);
+                        if (mt == MT - 1 && g == TG - 1) ask(b + AHEAD, u, j);
+                    }
+                    apply(PARTS - 1);
+                    __syncthreads();
+                }
+            }
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+            for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) part[((wk * WN * NT + wn * NT + nt) * ROWS + mt * 16 + quad * 4 + i) * 16 + row] = acc[nt][mt][i] * (1.f / X::UNIT);
+    }
+    __syncthreads();
+    w4_finish<T, WN * NT, (W4_WAVES + W4_LOADERS) * 64>(A, [&](int m, int n) {
+        float v = 0.f;
+#pragma unroll
+        for (int q = 0; q < WK; q++) v += part[((q * WN * NT + n / 16) * ROWS + m) * 16 + n % 16];
+        return v;
+    });
 }
 
 // ----------------------------------------------------------------------------
@@ -374,31 +513,42 @@ static std::string gemm4_check(const mlh_weights4* w, const mlh_gemm4* a) {
 
 extern "C" uint64_t mlh_gemm4_work_bytes(const mlh_weights4* w, const mlh_gemm4* a) { return 0; }
 
-template <typename T, int G, int MT, int RG, int WN, int WK, int NT, int TPW> static int gemm4_run(const Gemm4Args& A, void* stream) {
-    constexpr int planes = W4Mul<T>::PLANES, rows = MT * 4 * RG;
-    const int held = MT == 1 ? A.M : rows;
-    const size_t lds = std::max<size_t>((size_t)WK * TPW * W4_COLS * held * 2 * planes, (size_t)WK * WN * NT * rows * 16 * 4);
+template <typename T, int G, int MR, int WN, int WK, int NT, int TPW> static int gemm4_few(const Gemm4Args& A, void* stream) {
+    const unsigned grid = ((A.N + W4_ROWS - 1) / W4_ROWS + WN * NT - 1) / (WN * NT);
+    return kv_launch(&k_gemm4_few<T, G, MR, WN, WK, NT, TPW>, dim3(grid), W4_WAVES * 64, 0, stream, A);
+}
+template <typename T, int G, int MT, int WN, int WK, int NT, int TPW, int AHEAD> static int gemm4_many(const Gemm4Args& A, void* stream) {
+    constexpr int rows = MT * 16, lds = std::max(2 * WK * TPW * 4 * rows * 64 * W4Mul<T>::PLANES, WK * WN * NT * rows * 16 * 4);
+    static_assert(lds <= 163840, "LDS of a compute unit");
     const unsigned grid = ((A.N + W4_ROWS - 1) / W4_ROWS + WN * NT - 1) / (WN * NT);
     if (lds > 65536) { // (asked for on every call: the attribute belongs to the device that is current)
-        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&k_gemm4<T, G, MT, RG, WN, WK, NT, TPW>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&k_gemm4_many<T, G, MT, WN, WK, NT, TPW, AHEAD>), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
         if (e != hipSuccess) return kv_status(e);
     }
-    return kv_launch(&k_gemm4<T, G, MT, RG, WN, WK, NT, TPW>, dim3(grid), W4_WAVES * 64, lds, stream, A);
+    return kv_launch(&k_gemm4_many<T, G, MT, WN, WK, NT, TPW, AHEAD>, dim3(grid), (W4_WAVES + W4_LOADERS) * 64, lds, stream, A);
 }
 
+// Which kernel, and how its waves are dealt, goes by the rows of A, their type, and the number of 16-row bands of W: many bands fill the chip by themselves, so that a workgroup takes several, for
+// fewer reads of A and fewer starts; few are cut along K.  Microseconds by events around graph replays, one way / the other:
+//   M 1:  fp16, 256 bands, K 4096 4.5 / 7.6 (eight waves of a band / four of two and two); 1792 bands, K 8192 27.6 / 30.1; 2000 bands, K 2048 11.9 / 10.3; fp32 the same three 6.0 / 11.3, 43.6 / 38.4, 18.7 / 11.8
+//   M 8:  fp16, 256 bands, K 4096 5.2 / 6.2 (a band a wave / two); M 5, 512 bands, K 28672 37 / 32; 1792 bands, K 8192 37.7 / 31.2, four of two and two 31.8
+//   M 16: fp16, 256 bands, K 4096 few 5.8, many 8.2; M 10, 512 bands, K 28672 33.5, 35; 1792 bands, K 8192 50, 35
+//   M 32: fp16, 256 bands, K 4096 8.3 / 15.8 (two times four waves of a band / four times two of two); 1792 bands, K 8192 60 / 39
+//   M 64: fp16, 256 bands, K 4096 13.3 / 24.4; 1792 bands, K 8192 101 / 57
 template <typename T, int G> static int gemm4_go(const Gemm4Args& A, void* stream) {
-    static const int cfg = getenv("G4") ? atoi(getenv("G4")) : 0;
-    if constexpr (sizeof(T) == 2) {
-        if (A.M <= 4) return cfg == 1 ? gemm4_run<T, G, 1, 1, 1, 8, 1, 2>(A, stream) : cfg == 2 ? gemm4_run<T, G, 1, 1, 1, 8, 2, 2>(A, stream) : cfg == 3 ? gemm4_run<T, G, 1, 1, 2, 4, 1, 4>(A, stream) : gemm4_run<T, G, 1, 1, 1, 8, 1, 4>(A, stream);
-        if (A.M <= 8) return cfg == 1 ? gemm4_run<T, G, 1, 2, 1, 8, 1, 2>(A, stream) : cfg == 2 ? gemm4_run<T, G, 1, 2, 1, 8, 2, 2>(A, stream) : cfg == 3 ? gemm4_run<T, G, 1, 2, 2, 4, 1, 4>(A, stream) : gemm4_run<T, G, 1, 2, 1, 8, 1, 4>(A, stream);
-        if (A.M <= 16) return cfg == 1 ? gemm4_run<T, G, 1, 4, 1, 8, 1, 2>(A, stream) : cfg == 2 ? gemm4_run<T, G, 1, 4, 1, 8, 2, 2>(A, stream) : cfg == 3 ? gemm4_run<T, G, 1, 4, 2, 4, 2, 2>(A, stream) : gemm4_run<T, G, 1, 4, 1, 8, 2, 1>(A, stream);
-        if (A.M <= 32) return cfg == 1 ? gemm4_run<T, G, 2, 4, 1, 8, 1, 1>(A, stream) : cfg == 2 ? gemm4_run<T, G, 2, 4, 2, 4, 1, 2>(A, stream) : cfg == 3 ? gemm4_run<T, G, 2, 4, 4, 2, 2, 2>(A, stream) : gemm4_run<T, G, 2, 4, 2, 4, 2, 2>(A, stream);
-        return cfg == 1 ? gemm4_run<T, G, 4, 4, 2, 4, 1, 1>(A, stream) : cfg == 2 ? gemm4_run<T, G, 4, 4, 4, 2, 2, 2>(A, stream) : cfg == 3 ? gemm4_run<T, G, 4, 4, 4, 2, 1, 2>(A, stream) : gemm4_run<T, G, 4, 4, 2, 4, 2, 1>(A, stream);
+    constexpr bool f32 = sizeof(T) == 4;
+    const int bands = (A.N + W4_ROWS - 1) / W4_ROWS;
+    const bool wide = bands >= 1024;
+    if (A.M <= 4) return wide && (f32 || A.K <= 4096) ? gemm4_few<T, G, 1, 2, 4, 2, 2>(A, stream) : gemm4_few<T, G, 1, 1, 8, 1, 2>(A, stream);
+    if (A.M <= 8) return wide ? gemm4_few<T, G, 2, 2, 4, 2, 2>(A, stream) : bands >= 512 ? gemm4_few<T, G, 2, 1, 8, 2, 2>(A, stream) : gemm4_few<T, G, 2, 1, 8, 1, 2>(A, stream);
+    if constexpr (f32) {
+        if (A.M <= 16) return wide ? gemm4_many<T, G, 1, 4, 2, 2, 2, 1>(A, stream) : gemm4_many<T, G, 1, 2, 4, 1, 1, 2>(A, stream);
+        if (A.M <= 32) return wide ? gemm4_many<T, G, 2, 4, 2, 2, 1, 2>(A, stream) : gemm4_many<T, G, 2, 4, 2, 1, 1, 2>(A, stream);
+        return gemm4_many<T, G, 4, 8, 1, 1, 1, 2>(A, stream);
     } else {
-        if (A.M <= 4) return gemm4_run<T, G, 1, 1, 1, 8, 1, 2>(A, stream);
-        if (A.M <= 16) return gemm4_run<T, G, 1, 4, 1, 8, 1, 1>(A, stream);
-        if (A.M <= 32) return gemm4_run<T, G, 2, 4, 4, 2, 1, 1>(A, stream);
-        return gemm4_run<T, G, 4, 4, 4, 2, 1, 1>(A, stream);
+        if (A.M <= 16) return wide ? gemm4_many<T, G, 1, 4, 2, 2, 2, 2>(A, stream) : bands >= 512 ? gemm4_few<T, G, 4, 1, 8, 2, 2>(A, stream) : gemm4_few<T, G, 4, 1, 8, 1, 2>(A, stream);
+        if (A.M <= 32) return wide ? gemm4_many<T, G, 2, 4, 2, 2, 2, 1>(A, stream) : gemm4_many<T, G, 2, 2, 4, 1, 1, 3>(A, stream);
+        return wide ? gemm4_many<T, G, 4, 4, 2, 2, 2, 1>(A, stream) : gemm4_many<T, G, 4, 2, 4, 1, 1, 3>(A, stream);
     }
 }
 
