@@ -2,10 +2,12 @@
 #include <math.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "kv_cache.h"
 
 #define ROT_WG 256
+#define ROT_LDS 8192 // bytes of cosines and sines: two rows of 512 turned elements in 64 bits
 
 struct RotateArgs {
     const void *q, *k;
@@ -13,46 +15,94 @@ struct RotateArgs {
     long long qStride, qOutStride, kStride, kOutStride;
     const int32_t* pos;
     const double* freq;
-    int rows, heads, kvHeads, hd, rotated;
+    int rows, heads, kvHeads, hd, rotated, rowsAtOnce;
+    bool copy; // elements behind the turned ones
     double amplitude;
 };
 
-__device__ __forceinline__ double rot_get(const float* p) { return *p; }
-__device__ __forceinline__ double rot_get(const bf16_t* p) { return kv_bf16(*p); }
-__device__ __forceinline__ double rot_get(const f16_t* p) { return kv_half(p->bits); }
-__device__ __forceinline__ void rot_put(float* p, double v) { *p = (float)v; }
-__device__ __forceinline__ void rot_put(bf16_t* p, double v) { *p = (bf16_t)kv_to_bf16((float)v); }
-__device__ __forceinline__ void rot_put(f16_t* p, double v) { p->bits = (uint16_t)kv_to_half((float)v); }
+// V neighbouring elements, which stand on a multiple of their size, <-> floats
+__device__ __forceinline__ float rot_get(float v) { return v; }
+__device__ __forceinline__ float rot_get(bf16_t v) { return kv_bf16(v); }
+__device__ __forceinline__ float rot_get(f16_t v) { return kv_half(v.bits); }
+__device__ __forceinline__ void rot_put(float& p, float v) { p = v; }
+__device__ __forceinline__ void rot_put(bf16_t& p, float v) { p = (bf16_t)kv_to_bf16(v); }
+__device__ __forceinline__ void rot_put(f16_t& p, float v) { p.bits = (uint16_t)kv_to_half(v); }
+template <typename T, int V> struct __align__(sizeof(T) * V) RotVec { T v[V]; };
+template <int V, typename T> __device__ __forceinline__ void rot_load(const T* p, float (&x)[V]) {
+    if constexpr (V == 8) kv_load8(p, x);
+    else {
+        const RotVec<T, V> r = *reinterpret_cast<const RotVec<T, V>*>(p);
+#pragma unroll
+        for (int i = 0; i < V; i++) x[i] = rot_get(r.v[i]);
+    }
+}
+template <bool NT, int V, typename T> __device__ __forceinline__ void rot_store(T* p, const float (&x)[V]) {
+    if constexpr (V == 8) kv_store8<NT>(p, x);
+    else {
+        RotVec<T, V> r;
+#pragma unroll
+        for (int i = 0; i < V; i++) rot_put(r.v[i], x[i]);
+        *reinterpret_cast<RotVec<T, V>*>(p) = r;
+    }
+}
 
-// One workgroup a row: cosines and sines of its pairs once, into LDS, then its heads.  The angle is counted in half turns, whose whole ones are taken off in 64 bits.
-template <typename T, bool HALVES>
+// A workgroup takes a few rows at a time: their cosines and sines once, into LDS, for all heads, then the heads.  The angle is counted in half turns, whose whole ones are taken off in 64 bits.
+// A piece is V elements of a head: with halves the two times V that are V pairs, with pairs V neighbours, or V elements behind the turned ones.
+// Bound by memory: 16384 rows of 32 + 8 heads of 128 in bf16, 336 MB read and written, 58 us (5.8 TB/s; a copy of 1 GiB 5.2), fp32 rows 63 us for as many bytes (5.3).  A single token 2.6 us, the latency
+// of position, angle and LDS in turn.  Rows at once: about as many as give every thread a piece; of 40 heads one, two and four 58, 62 and 65 us, of 3 heads one, four and eight 18, 11 and 9.5.
+template <typename T, bool HALVES, int V, bool NT>
 __global__ void __launch_bounds__(ROT_WG) k_rotate(RotateArgs A) {
-    __shared__ double cs[2 * 256];
-    const int half = A.rotated / 2, rest = A.hd - A.rotated;
-    for (int row = blockIdx.x; row < A.rows; row += gridDim.x) {
-        __syncthreads();
-        for (int t = threadIdx.x; t < half; t += ROT_WG) {
-            const double turns = (double)A.pos[row] * (A.freq[t] * 0.31830988618379067154);
+    typedef std::conditional_t<sizeof(T) == 4, double, float> C; // (64-bit products of fp32 rows)
+    __shared__ __align__(16) C cs[ROT_LDS / sizeof(C)]; // [rows][half] pairs
+    const int half = A.rotated / 2, rest = A.hd - A.rotated, heads = A.heads + A.kvHeads;
+    const int turned = (HALVES ? half : A.rotated) / V, pieces = turned + (A.copy ? rest / V : 0); // of a head
+    for (int row0 = blockIdx.x * A.rowsAtOnce; row0 < A.rows; row0 += gridDim.x * A.rowsAtOnce) {
+        const int rows = min(A.rowsAtOnce, A.rows - row0);
+        if (row0 != (int)blockIdx.x * A.rowsAtOnce) __syncthreads();
+        for (int u = threadIdx.x; u < rows * half; u += ROT_WG) {
+            const int t = u % half;
+            const double turns = (double)A.pos[row0 + u / half] * (A.freq[t] * 0.31830988618379067154);
             double s, c;
             sincospi(turns - 2.0 * rint(turns * 0.5), &s, &c);
-            cs[2 * t] = c * A.amplitude;
-            cs[2 * t + 1] = s * A.amplitude;
+            cs[2 * u] = (C)(c * A.amplitude);
+            cs[2 * u + 1] = (C)(s * A.amplitude);
         }
         __syncthreads();
-        for (int u = threadIdx.x; u < (A.heads + A.kvHeads) * (half + rest); u += ROT_WG) {
-            const int g = u / (half + rest), t = u % (half + rest);
-            const bool isK = g >= A.heads;
-            const int h = isK ? g - A.heads : g;
-            const T* x = (const T*)(isK ? A.k : A.q) + (size_t)row * (isK ? A.kStride : A.qStride) + (size_t)h * A.hd;
-            T* y = (T*)(isK ? A.kOut : A.qOut) + (size_t)row * (isK ? A.kOutStride : A.qOutStride) + (size_t)h * A.hd;
-            if (t >= half) {
-                y[A.rotated + t - half] = x[A.rotated + t - half];
-                continue;
+        for (int u = threadIdx.x; u < rows * heads * pieces; u += ROT_WG) {
+            const int p = u % pieces, g = u / pieces, h = g % heads, r = g / heads;
+            const bool isK = h >= A.heads;
+            const size_t row = row0 + r;
+            const T* x = (const T*)(isK ? A.k : A.q) + row * (isK ? A.kStride : A.qStride) + (size_t)(isK ? h - A.heads : h) * A.hd;
+            T* y = (T*)(isK ? A.kOut : A.qOut) + row * (isK ? A.kOutStride : A.qOutStride) + (size_t)(isK ? h - A.heads : h) * A.hd;
+            float a[V], b[V];
+            if (p >= turned) {
+                const int i = A.rotated + (p - turned) * V;
+                rot_load<V>(x + i, a);
+                rot_store<NT, V>(y + i, a);
+            } else if constexpr (HALVES) {
+                const int i = p * V, j = half + p * V;
+                const C* w = cs + 2 * ((size_t)r * half + p * V);
+                rot_load<V>(x + i, a);
+                rot_load<V>(x + j, b);
+#pragma unroll
+                for (int e = 0; e < V; e++) {
+                    const C c = w[2 * e], s = w[2 * e + 1], f = a[e], g2 = b[e];
+                    a[e] = (float)(c * f - s * g2);
+                    b[e] = (float)(s * f + c * g2);
+                }
+                rot_store<NT, V>(y + i, a);
+                rot_store<NT, V>(y + j, b);
+            } else {
+                const C* w = cs + (size_t)r * half * 2 + p * V;
+                rot_load<V>(x + p * V, a);
+#pragma unroll
+                for (int e = 0; e < V; e += 2) {
+                    const C c = w[e], s = w[e + 1], f = a[e], g2 = a[e + 1];
+                    a[e] = (float)(c * f - s * g2);
+                    a[e + 1] = (float)(s * f + c * g2);
+                }
+                rot_store<NT, V>(y + p * V, a);
             }
-            const int i = HALVES ? t : 2 * t, j = HALVES ? t + half : 2 * t + 1;
-            const double a = rot_get(x + i), b = rot_get(x + j), c = cs[2 * t], s = cs[2 * t + 1];
-            rot_put(y + i, c * a - s * b);
-            rot_put(y + j, s * a + c * b);
         }
     }
 }
@@ -84,11 +134,25 @@ extern "C" int mlh_rotate_device(const mlh_rotate* a, void* stream) {
     const std::string bad = rot_check(a);
     if (!bad.empty()) return kv_fail(bad);
     if (a->rows == 0) return 0;
-    RotateArgs A = {a->q, a->k, a->qOut, a->kOut, a->qStride, a->qOutStride, a->kStride, a->kOutStride, a->pos, a->freq, a->rows, a->heads, a->k ? a->kvHeads : 0, a->headDim, a->rotated,
-                    a->amplitude == 0.f ? 1.0 : (double)a->amplitude};
-    const dim3 grid((unsigned)std::min(a->rows, 1 << 20));
+    const int kvHeads = a->k ? a->kvHeads : 0;
     const bool halves = a->layout == MLH_ROTATE_HALVES;
-#define ROT_GO(T_) return kv_launch(halves ? &k_rotate<T_, true> : &k_rotate<T_, false>, grid, ROT_WG, 0, stream, A)
+    const bool copy = a->rotated < a->headDim && (a->q != a->qOut || (a->k && a->k != a->kOut));
+    const size_t bytes = (size_t)a->rows * (a->heads + kvHeads) * a->headDim * kv_elem_bytes(a->type);
+    int v = 8; // elements of a piece
+    while (v > 1 && (halves ? a->rotated / 2 : a->rotated) % v) v /= 2;
+    const int pieces = (a->heads + kvHeads) * ((halves ? a->rotated / 2 : a->rotated) + (copy ? a->headDim - a->rotated : 0)) / v; // of a row
+    const int most = ROT_LDS / (a->rotated * (a->type == MLH_DTYPE_F32 ? 8 : 4)), atOnce = std::max(1, std::min(most, ROT_WG / pieces));
+    RotateArgs A = {a->q, a->k, a->qOut, a->kOut, a->qStride, a->qOutStride, a->kStride, a->kOutStride, a->pos, a->freq, a->rows, a->heads, kvHeads, a->headDim, a->rotated, atOnce, copy,
+                    a->amplitude == 0.f ? 1.0 : (double)a->amplitude};
+    const dim3 grid((unsigned)std::min((a->rows + atOnce - 1) / atOnce, 1 << 20));
+    const bool nt = bytes > 32e6; // streaming stores for calls that write more than the L2s hold
+#define ROT_GO(T_) \
+    do { \
+        if (v == 8) return kv_launch(halves ? (nt ? &k_rotate<T_, true, 8, true> : &k_rotate<T_, true, 8, false>) : (nt ? &k_rotate<T_, false, 8, true> : &k_rotate<T_, false, 8, false>), grid, ROT_WG, 0, stream, A); \
+        if (v == 4) return kv_launch(halves ? &k_rotate<T_, true, 4, false> : &k_rotate<T_, false, 4, false>, grid, ROT_WG, 0, stream, A); \
+        if (v == 2) return kv_launch(halves ? &k_rotate<T_, true, 2, false> : &k_rotate<T_, false, 2, false>, grid, ROT_WG, 0, stream, A); \
+        return kv_launch(&k_rotate<T_, true, 1, false>, grid, ROT_WG, 0, stream, A); \
+    } while (0)
     if (a->type == MLH_DTYPE_F32) ROT_GO(float);
     if (a->type == MLH_DTYPE_BF16) ROT_GO(bf16_t);
     ROT_GO(f16_t);
