@@ -162,6 +162,12 @@ int mlh_prefill_batch(mlh_ctx* ctx, int nseg, const int32_t* seqs, const int32_t
  * 512 MB stay with the context for the next call; from 4 MB of results on, four host threads live for the call. */
 int mlh_forward_full(mlh_ctx* ctx, int seq, const int32_t* ids, int n, float* logits_out, float* probs_out, float* mean_nll);
 
+/* The same forward for callers that want to know how likely a text is: per position i of the n tokens, logProb[i] = log p(ids[i + 1] | everything up to ids[i]) (0 for the last one, which has
+ * no next token here), the entropy of that distribution, and its `top` (0 to 64) most likely tokens with their log p, [n, top], as mlh_logprobs_device defines them; temperature 0: 1.  logProb
+ * and entropy may be null.  The logits stay on the device: of a text of 517 tokens and 20160 words 42 MB that mlh_forward_full would bring to the host.  Its work buffers
+ * are that call's.  (The reference copies the probabilities of all columns to the host and sorts the last one there, inference_orchestrator.cu:68-84.) */
+int mlh_score(mlh_ctx* ctx, int seq, const int32_t* ids, int n, int top, float temperature, float* logProb, float* entropy, int32_t* topIds, float* topLogProb);
+
 /* 0 (default): MFMA products when the call has two or more tokens and dim, ffnDim,
  * pleDim and the mixing widths are multiples of 32 (fp32) / 64 (bf16), and in decode steps of up to 64 sequences;
  * 1: always token by token, and decode steps through the GEMV kernels. */

@@ -143,6 +143,7 @@ _sigs_dev = {
     "mlh_prefill_batch": (c_int, [c_void_p, c_int, c_void_p, c_void_p, c_void_p]),
     "mlh_set_prefill_mode": (c_int, [c_void_p, c_int]),
     "mlh_forward_full": (c_int, [c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p, _P(c_float)]),
+    "mlh_score": (c_int, [c_void_p, c_int, c_void_p, c_int, c_int, c_float, c_void_p, c_void_p, c_void_p, c_void_p]),
     "mlh_decode_step": (c_int, [c_void_p, c_void_p, c_int, c_void_p]),
     "mlh_decode_loop": (c_int, [c_void_p, c_void_p, c_int, c_int, c_void_p]),
     "mlh_greedy_token": (c_int, [c_void_p, c_int, _P(c_int32)]),
@@ -493,6 +494,15 @@ class Device:
         self._check(dev.mlh_forward_full(self._h, seq, a.ctypes.data, a.size, lg.ctypes.data,
                                          pr.ctypes.data if pr is not None else None, byref(nll)))
         return lg, pr, float(nll.value)
+
+    def score(self, seq, ids, top=0, temperature=0.0):
+        """Teacher-forced forward over ids appended to seq (mlh_score): (log p of each next token [n], the last one 0; entropy [n]; the `top`
+        most likely tokens [n, top]; their log p [n, top])."""
+        a = np.ascontiguousarray(ids, dtype=np.int32)
+        lp, ent = (np.empty(a.size, dtype=np.float32) for _ in range(2))
+        tid, tlp = np.empty((a.size, max(top, 0)), dtype=np.int32), np.empty((a.size, max(top, 0)), dtype=np.float32)
+        self._check(dev.mlh_score(self._h, seq, a.ctypes.data, a.size, top, temperature, lp.ctypes.data, ent.ctypes.data, tid.ctypes.data, tlp.ctypes.data))
+        return lp, ent, tid, tlp
 
     def set_prefill_mode(self, mode):
         self._check(dev.mlh_set_prefill_mode(self._h, int(mode)))

@@ -582,27 +582,59 @@ extern "C" int mlh_prefill(mlh_ctx* c, int seq, const int32_t* ids, int n) {
 
 // Teacher-forced forward over n tokens appended to `seq`: what runInference(L) leaves in vocabScores_DEVICE and
 // vocabScores_postSoftmax_DEVICE for all L columns (inference.cu:723-749), plus the mean next-token cross-entropy.
-extern "C" int mlh_forward_full(mlh_ctx* c, int seq, const int32_t* ids, int n, float* logitsOut, float* probsOut, float* meanNll) {
+// What mlh_forward_full and mlh_score ask of their input
+static int check_full(mlh_ctx* c, int seq, const int32_t* ids, int n) {
     int rc = check_ready(c);
     if (rc) return rc;
     const mlh_hparams& hp = c->hp;
-    const size_t V = hp.vocabSize;
     if (seq < 0 || seq >= hp.maxSeqs) { c->err = "sequence index out of range"; return -1; }
     if (!ids || n <= 0) { c->err = "empty input"; return -1; }
     if (c->h_len[seq] + n > hp.maxL) { c->err = "input does not fit in maxL"; return -1; }
     for (int i = 0; i < n; i++)
         if (ids[i] < 0 || ids[i] >= hp.vocabSize) { c->err = "token id out of range"; return -1; }
     touch(c, seq, seq + 1);
-    if ((rc = mlh_ranks_settle(c, &seq, 1))) return rc;
+    return mlh_ranks_settle(c, &seq, 1);
+}
+
+// ... their device results, at least so many bytes: kept by the context for the next call, unless they are large
+static int full_buffer(mlh_ctx* c, size_t need) {
+    if (need <= c->fullBytes) return 0;
+    MLH_CHECK(c, hipStreamSynchronize(c->stream));
+    if (c->fullBuf) (void)hipFree(c->fullBuf);
+    c->fullBuf = nullptr; c->fullBytes = 0;
+    MLH_CHECK(c, hipMalloc((void**)&c->fullBuf, need));
+    c->fullBytes = need;
+    return 0;
+}
+static void drop_large_full_buffer(mlh_ctx* c, size_t need) {
+    if (need <= ((size_t)512 << 20)) return; // (2 048 tokens of a 32 K vocabulary with probabilities are kept)
+    (void)hipFree(c->fullBuf);
+    c->fullBuf = nullptr; c->fullBytes = 0;
+}
+
+// ... and the forward itself: appends the tokens and leaves the logits of all of them [n, vocabSize]
+static int full_logits(mlh_ctx* c, int seq, const int32_t* ids, int n, float* dLogits, const char* what) {
+    const size_t V = c->hp.vocabSize;
+    if (c->prefillMode == 0 && n > 1 && mlh_prefill_gemm_supported(c)) return mlh_run_prefill_gemm(c, 1, &seq, ids, &n, dLogits);
+    // token by token through the decode kernels, LM head at every position
+    int rc = set_slots(c, &seq, 1);
+    if (rc == 0 && hipMemcpyAsync(c->d_prompt, ids, (size_t)n * 4, hipMemcpyHostToDevice, c->stream) != hipSuccess) rc = -2;
+    for (int i = 0; i < n && rc == 0; i++) {
+        rc = mlh_launch_step(c, 1, c->d_prompt + i, true);
+        if (rc == 0 && hipMemcpyAsync(dLogits + (size_t)i * V, c->logits + (size_t)seq * V, V * 4, hipMemcpyDeviceToDevice, c->stream) != hipSuccess) rc = -2;
+    }
+    if (rc == 0) { if (hipStreamSynchronize(c->stream) != hipSuccess) rc = -2; else c->h_len[seq] += n; }
+    if (rc == -2 && c->err.empty()) c->err = std::string(what) + ": HIP call failed";
+    return rc;
+}
+
+extern "C" int mlh_forward_full(mlh_ctx* c, int seq, const int32_t* ids, int n, float* logitsOut, float* probsOut, float* meanNll) {
+    int rc = check_full(c, seq, ids, n);
+    if (rc) return rc;
+    const size_t V = c->hp.vocabSize;
     // device results: logits, probabilities, targets, losses
     const size_t mat = (size_t)n * V * 4, need = mat * (probsOut ? 2 : 1) + (size_t)n * 8;
-    if (need > c->fullBytes) {
-        MLH_CHECK(c, hipStreamSynchronize(c->stream));
-        if (c->fullBuf) (void)hipFree(c->fullBuf);
-        c->fullBuf = nullptr; c->fullBytes = 0;
-        MLH_CHECK(c, hipMalloc((void**)&c->fullBuf, need));
-        c->fullBytes = need;
-    }
+    if ((rc = full_buffer(c, need))) return rc;
     if ((rc = mlh_pin(c, c->pinStage, RB_RING * RB_CHUNK)) || (rc = mlh_pin(c, c->pinIo, (size_t)n * 8))) return rc;
     float *dLogits = c->fullBuf, *dProbs = probsOut ? dLogits + (size_t)n * V : nullptr, *dNll = dLogits + (size_t)n * V * (probsOut ? 2 : 1) + n;
     int* dTarget = (int*)dNll - n;
@@ -616,18 +648,7 @@ extern "C" int mlh_forward_full(mlh_ctx* c, int seq, const int32_t* ids, int n, 
     Readback out(parts, np); // its threads map the callers' pages from here on
     hipError_t e = hipMemcpyAsync(dTarget, target, (size_t)n * 4, hipMemcpyHostToDevice, c->stream);
     if (e != hipSuccess) { c->err = std::string("forward_full: ") + hipGetErrorString(e); return -2; }
-    if (c->prefillMode == 0 && n > 1 && mlh_prefill_gemm_supported(c)) {
-        rc = mlh_run_prefill_gemm(c, 1, &seq, ids, &n, dLogits);
-    } else { // token by token through the decode kernels, LM head at every position
-        rc = set_slots(c, &seq, 1);
-        if (rc == 0 && hipMemcpyAsync(c->d_prompt, ids, (size_t)n * 4, hipMemcpyHostToDevice, c->stream) != hipSuccess) rc = -2;
-        for (int i = 0; i < n && rc == 0; i++) {
-            rc = mlh_launch_step(c, 1, c->d_prompt + i, true);
-            if (rc == 0 && hipMemcpyAsync(dLogits + (size_t)i * V, c->logits + (size_t)seq * V, V * 4, hipMemcpyDeviceToDevice, c->stream) != hipSuccess) rc = -2;
-        }
-        if (rc == 0) { if (hipStreamSynchronize(c->stream) != hipSuccess) rc = -2; else c->h_len[seq] += n; }
-        if (rc == -2 && c->err.empty()) c->err = "forward_full: HIP call failed";
-    }
+    rc = full_logits(c, seq, ids, n, dLogits, "forward_full");
     if (rc == 0) rc = mlh_launch_softmax_rows(c, dLogits, dProbs, dTarget, dNll, n);
     if (rc == 0) {
         e = hipMemcpyAsync(nll, dNll, (size_t)n * 4, hipMemcpyDeviceToHost, c->stream);
@@ -636,16 +657,59 @@ extern "C" int mlh_forward_full(mlh_ctx* c, int seq, const int32_t* ids, int n, 
         if (e != hipSuccess) { c->err = std::string("forward_full read-back: ") + hipGetErrorString(e); rc = -2; }
     }
     if (rc) (void)hipStreamSynchronize(c->stream);
-    if (need > ((size_t)512 << 20)) { // (2 048 tokens of a 32 K vocabulary with probabilities are kept)
-        (void)hipFree(c->fullBuf);
-        c->fullBuf = nullptr; c->fullBytes = 0;
-    }
+    drop_large_full_buffer(c, need);
     if (rc == 0 && meanNll) {
         double s = 0;
         for (int i = 0; i + 1 < n; i++) s += nll[i];
         *meanNll = n > 1 ? (float)(s / (n - 1)) : 0.f;
     }
     return rc;
+}
+
+extern "C" int mlh_score(mlh_ctx* c, int seq, const int32_t* ids, int n, int top, float temperature, float* logProb, float* entropy, int32_t* topIds, float* topLogProb) {
+    if (c && (top < 0 || top > 64 || (c->hp.vocabSize < top) || (top && (!topIds || !topLogProb)))) { c->err = "top must be 0 to 64, at most the vocabulary, with room for its results"; return -1; }
+    if (c && temperature != 0.f && !(temperature >= 1e-4f && temperature <= 1e4f)) { c->err = "temperature must be 0 or 1e-4 to 1e4"; return -1; }
+    int rc = check_full(c, seq, ids, n);
+    if (rc) return rc;
+    // device results: logits, then per row its next token, log probability, entropy, best tokens and theirs; the operator's workspace
+    const size_t V = c->hp.vocabSize, rows = n, words = rows * (3 + 2 * (size_t)top), at = (rows * V + 3) / 4 * 4;
+    mlh_logprobs a = {nullptr, (int64_t)V, nullptr, nullptr, nullptr, nullptr, nullptr, n, (int32_t)V, MLH_DTYPE_F32, 1, top, temperature, nullptr, 0};
+    a.logits = a.tokens = (const int32_t*)16; // (what the workspace takes does not go by them)
+    a.logProb = a.entropy = a.topLogProb = (float*)16;
+    a.topIds = (int32_t*)16;
+    a.workBytes = mlh_logprobs_work_bytes(&a);
+    const size_t workAt = (at + words + 3) / 4 * 4, need = workAt * 4 + a.workBytes;
+    if ((rc = full_buffer(c, need)) || (rc = mlh_pin(c, c->pinIo, words * 4))) return rc;
+    float* const d = c->fullBuf + at;
+    int* const next = c->pinIo.p;
+    for (int i = 0; i < n; i++) next[i] = i + 1 < n ? ids[i + 1] : -1;
+    a.logits = c->fullBuf;
+    a.tokens = (const int32_t*)d;
+    a.logProb = d + rows;
+    a.entropy = d + 2 * rows;
+    a.topIds = (int32_t*)(d + 3 * rows);
+    a.topLogProb = d + (3 + (size_t)top) * rows;
+    a.work = c->fullBuf + workAt;
+    hipError_t e = hipMemcpyAsync(d, next, rows * 4, hipMemcpyHostToDevice, c->stream);
+    if (e != hipSuccess) { c->err = std::string("score: ") + hipGetErrorString(e); return -2; }
+    rc = full_logits(c, seq, ids, n, c->fullBuf, "score");
+    if (rc == 0 && (rc = mlh_logprobs_device(&a, c->stream))) c->err = mlh_last_error(nullptr);
+    if (rc == 0) {
+        e = hipMemcpyAsync(c->pinIo.p, d, words * 4, hipMemcpyDeviceToHost, c->stream);
+        if (e == hipSuccess) e = hipStreamSynchronize(c->stream);
+        if (e != hipSuccess) { c->err = std::string("score read-back: ") + hipGetErrorString(e); rc = -2; }
+    }
+    if (rc) (void)hipStreamSynchronize(c->stream);
+    drop_large_full_buffer(c, need);
+    if (rc) return rc;
+    const float* const r = (const float*)c->pinIo.p;
+    if (logProb) memcpy(logProb, r + rows, rows * 4);
+    if (entropy) memcpy(entropy, r + 2 * rows, rows * 4);
+    if (top) {
+        memcpy(topIds, r + 3 * rows, rows * top * 4);
+        memcpy(topLogProb, r + (3 + (size_t)top) * rows, rows * top * 4);
+    }
+    return 0;
 }
 
 extern "C" int mlh_set_prefill_mode(mlh_ctx* c, int mode) {
