@@ -28,61 +28,98 @@ struct W4Args {
     long long stride;
 };
 
-// A thread: eight columns of a row.  group / 8 neighbouring threads share a pair (whole tiles of 128 columns are gone through, so they are of one wave); those behind K bring no value.
+// A wave: a tile, as the lanes of a product hold it: lane l row l % 16, eight columns of each of the four steps.  The columns of a group are those of 1, 2 or 4 steps in the four lanes of a row.
+// Bound by memory.  28672 columns of 8192 rows, groups of 32: codes laid out in 99 us (a thread for eight columns wrote four bytes at places 64 apart: 142), packed from bf16 in 153, read back in 171.
+struct W4Place { int n, k, lane; }; // row and first column of step 0
+__device__ __forceinline__ W4Place w4_place(const W4Args& A, size_t tile) {
+    const int perBand = w4_tiles(A.K), lane = threadIdx.x & 63;
+    return {(int)(tile / perBand) * W4_ROWS + (lane & 15), (int)(tile % perBand) * W4_COLS + (lane >> 4) * 8, lane};
+}
+#define W4_EACH_TILE(PLACE_) \
+    for (size_t tile = (size_t)blockIdx.x * (W4_WG / 64) + (threadIdx.x >> 6), tiles = (size_t)(A.rows / W4_ROWS) * w4_tiles(A.K); tile < tiles; tile += (size_t)gridDim.x * (W4_WG / 64)) \
+        if (const W4Place PLACE_ = w4_place(A, tile); true)
+
 template <typename T, int G>
 __global__ void __launch_bounds__(W4_WG) k_w4_pack(W4Args A) {
-    constexpr int L = G / 8;
-    const int perRow = w4_tiles(A.K) * (W4_COLS / 8);
-    const size_t units = (size_t)A.rows * perRow;
-    for (size_t u = (size_t)blockIdx.x * W4_WG + threadIdx.x; u < units; u += (size_t)gridDim.x * W4_WG) {
-        const int n = (int)(u / perRow), k = (int)(u % perRow) * 8;
-        const bool live = n < A.N && k < A.K;
-        float x[8], lo = INFINITY, hi = -INFINITY, bad = 0.f;
-        if (live) {
-            kv_load8((const T*)A.src + (size_t)n * A.stride + k, x);
+    constexpr int S = G / 32, TG = w4_groups(G);
+    W4_EACH_TILE(P) {
+        float x[4][8];
+        bool live[4];
 #pragma unroll
-            for (int i = 0; i < 8; i++) { lo = fminf(lo, x[i]); hi = fmaxf(hi, x[i]); bad += x[i] * 0.f; }
+        for (int s = 0; s < 4; s++) {
+            live[s] = P.n < A.N && P.k + s * 32 < A.K;
+            if (live[s]) kv_load8((const T*)A.src + (size_t)P.n * A.stride + P.k + s * 32, x[s]);
         }
+        uint32_t pairs[TG], words[4];
 #pragma unroll
-        for (int o = 1; o < L; o <<= 1) { lo = fminf(lo, __shfl_xor(lo, o, 64)); hi = fmaxf(hi, __shfl_xor(hi, o, 64)); bad += __shfl_xor(bad, o, 64); }
-        float step = (hi - lo) * (1.0f / 15.0f);
-        asm volatile("" : "+v"(step)); // (rounded to fp32 first; in one instruction with the conversion the product is not)
-        uint32_t minBits = kv_to_half(__builtin_amdgcn_fmed3f(lo, -65504.f, 65504.f)), scaleBits = kv_to_half(step);
-        const float base = kv_half(minBits), scale = kv_half(scaleBits);
-        uint32_t codes = 0;
-        if (lo > hi && bad == 0.f) minBits = scaleBits = 0; // (nobody brought a value)
-        else if (!(bad == 0.f) || scaleBits == 0x7c00u) { minBits = 0x7e00u; scaleBits = 0; }
-        else if (live && scale > 0.f) {
+        for (int g = 0; g < TG; g++) {
+            float lo = INFINITY, hi = -INFINITY, bad = 0.f;
+#pragma unroll
+            for (int s = g * S; s < g * S + S; s++)
+                if (live[s]) {
+#pragma unroll
+                    for (int i = 0; i < 8; i++) { lo = fminf(lo, x[s][i]); hi = fmaxf(hi, x[s][i]); bad += x[s][i] * 0.f; }
+                }
+#pragma unroll
+            for (int o = 16; o < 64; o <<= 1) { lo = fminf(lo, __shfl_xor(lo, o, 64)); hi = fmaxf(hi, __shfl_xor(hi, o, 64)); bad += __shfl_xor(bad, o, 64); }
+            float step = (hi - lo) * (1.0f / 15.0f);
+            asm volatile("" : "+v"(step)); // (rounded to fp32 first; in one instruction with the conversion the product is not)
+            uint32_t minBits = kv_to_half(__builtin_amdgcn_fmed3f(lo, -65504.f, 65504.f)), scaleBits = kv_to_half(step);
+            const float base = kv_half(minBits), scale = kv_half(scaleBits);
+            const bool none = lo > hi && bad == 0.f, odd = !none && (!(bad == 0.f) || scaleBits == 0x7c00u); // (nobody brought a value; a value is no number)
+            if (none) minBits = scaleBits = 0;
+            if (odd) { minBits = 0x7e00u; scaleBits = 0; }
             const float inv = 1.0f / scale;
 #pragma unroll
-            for (int i = 0; i < 8; i++) codes |= kv_code(x[i], base, scale, inv) << (4 * i);
+            for (int s = g * S; s < g * S + S; s++) {
+                uint32_t codes = 0;
+                if (live[s] && !odd && scale > 0.f) {
+#pragma unroll
+                    for (int i = 0; i < 8; i++) codes |= kv_code(x[s][i], base, scale, inv) << (4 * i);
+                }
+                words[s] = w4_spread(codes);
+            }
+            pairs[g] = minBits | scaleBits << 16;
         }
-        *reinterpret_cast<uint32_t*>(A.data + w4_code_at(n, k, A.K, G)) = w4_spread(codes);
-        if (k % G == 0) *reinterpret_cast<uint32_t*>(A.data + w4_param_at(n, k, A.K, G)) = minBits | scaleBits << 16;
+        uint8_t* at = A.data + tile * w4_tile(G);
+        *reinterpret_cast<w4_u32x4*>(at + P.lane * 16) = w4_u32x4{words[0], words[1], words[2], words[3]};
+        if (P.lane < W4_ROWS) {
+#pragma unroll
+            for (int g = 0; g < TG; g++) *reinterpret_cast<uint32_t*>(at + W4_CODES + (P.lane * TG + g) * 4) = pairs[g];
+        }
     }
 }
 
 template <int G>
 __global__ void __launch_bounds__(W4_WG) k_w4_set(W4Args A) {
-    const int perRow = w4_tiles(A.K) * (W4_COLS / 8);
-    const size_t units = (size_t)A.rows * perRow;
-    for (size_t u = (size_t)blockIdx.x * W4_WG + threadIdx.x; u < units; u += (size_t)gridDim.x * W4_WG) {
-        const int n = (int)(u / perRow), k = (int)(u % perRow) * 8;
-        const bool live = n < A.N && k < A.K;
-        *reinterpret_cast<uint32_t*>(A.data + w4_code_at(n, k, A.K, G)) = live ? w4_spread(((const uint32_t*)A.src)[((size_t)n * A.K + k) / 8]) : 0u;
-        if (k % G == 0) *reinterpret_cast<uint32_t*>(A.data + w4_param_at(n, k, A.K, G)) = live ? A.params[(size_t)n * ((A.K + G - 1) / G) + k / G] : 0u;
+    constexpr int TG = w4_groups(G);
+    W4_EACH_TILE(P) {
+        w4_u32x4 words = {};
+#pragma unroll
+        for (int s = 0; s < 4; s++)
+            if (P.n < A.N && P.k + s * 32 < A.K) words[s] = w4_spread(((const uint32_t*)A.src)[((size_t)P.n * A.K + P.k + s * 32) / 8]);
+        uint8_t* at = A.data + tile * w4_tile(G);
+        *reinterpret_cast<w4_u32x4*>(at + P.lane * 16) = words;
+        if (P.lane < W4_ROWS) {
+#pragma unroll
+            for (int g = 0; g < TG; g++)
+                *reinterpret_cast<uint32_t*>(at + W4_CODES + (P.lane * TG + g) * 4) = P.n < A.N && P.k + g * G < A.K ? A.params[(size_t)P.n * ((A.K + G - 1) / G) + (P.k + g * G) / G] : 0u;
+        }
     }
 }
 
 template <typename T, int G>
 __global__ void __launch_bounds__(W4_WG) k_w4_read(W4Args A) {
-    const int perRow = A.K / 8;
-    const size_t units = (size_t)A.N * perRow;
-    for (size_t u = (size_t)blockIdx.x * W4_WG + threadIdx.x; u < units; u += (size_t)gridDim.x * W4_WG) {
-        const int n = (int)(u / perRow), k = (int)(u % perRow) * 8;
-        float x[8];
-        kv_values8(w4_gather(*reinterpret_cast<const uint32_t*>(A.data + w4_code_at(n, k, A.K, G))), *reinterpret_cast<const uint32_t*>(A.data + w4_param_at(n, k, A.K, G)), x);
-        kv_store8<false>((T*)A.dst + (size_t)n * A.stride + k, x);
+    constexpr int S = G / 32, TG = w4_groups(G);
+    W4_EACH_TILE(P) {
+        const uint8_t* at = A.data + tile * w4_tile(G);
+        const w4_u32x4 words = *reinterpret_cast<const w4_u32x4*>(at + P.lane * 16);
+#pragma unroll
+        for (int s = 0; s < 4; s++) {
+            float x[8];
+            kv_values8(w4_gather(words[s]), *reinterpret_cast<const uint32_t*>(at + W4_CODES + ((P.lane & 15) * TG + s / S) * 4), x);
+            if (P.n < A.N && P.k + s * 32 < A.K) kv_store8<false>((T*)A.dst + (size_t)P.n * A.stride + P.k + s * 32, x);
+        }
     }
 }
 
@@ -447,7 +484,7 @@ static std::string w4_check(const mlh_weights4* w) {
     return "";
 }
 
-static unsigned w4_grid(size_t units) { return (unsigned)std::min<size_t>((units + W4_WG - 1) / W4_WG, 1 << 20); }
+static unsigned w4_grid(const W4Args& A) { return (unsigned)std::min<size_t>(((size_t)(A.rows / W4_ROWS) * w4_tiles(A.K) + W4_WG / 64 - 1) / (W4_WG / 64), 1 << 20); }
 static W4Args w4_args(const mlh_weights4* w) { return {(uint8_t*)w->data, w->N, w->K, (w->N + W4_ROWS - 1) / W4_ROWS * W4_ROWS, nullptr, nullptr, nullptr, 0}; }
 
 #define W4_BY_GROUP(KERNEL_, ...) (w->group == 32 ? &KERNEL_<__VA_ARGS__ 32> : w->group == 64 ? &KERNEL_<__VA_ARGS__ 64> : &KERNEL_<__VA_ARGS__ 128>)
@@ -461,7 +498,7 @@ extern "C" int mlh_weights4_pack_device(const mlh_weights4* w, int type, const v
     W4Args A = w4_args(w);
     A.src = src;
     A.stride = stride;
-    const unsigned grid = w4_grid((size_t)A.rows * w4_tiles(A.K) * (W4_COLS / 8));
+    const unsigned grid = w4_grid(A);
     if (type == MLH_DTYPE_F32) return kv_launch(W4_BY_GROUP(k_w4_pack, float W4_COMMA), dim3(grid), W4_WG, 0, stream, A);
     if (type == MLH_DTYPE_BF16) return kv_launch(W4_BY_GROUP(k_w4_pack, bf16_t W4_COMMA), dim3(grid), W4_WG, 0, stream, A);
     return kv_launch(W4_BY_GROUP(k_w4_pack, f16_t W4_COMMA), dim3(grid), W4_WG, 0, stream, A);
@@ -475,7 +512,7 @@ extern "C" int mlh_weights4_set_device(const mlh_weights4* w, const uint8_t* cod
     W4Args A = w4_args(w);
     A.src = codes;
     A.params = (const uint32_t*)params;
-    return kv_launch(W4_BY_GROUP(k_w4_set, ), dim3(w4_grid((size_t)A.rows * w4_tiles(A.K) * (W4_COLS / 8))), W4_WG, 0, stream, A);
+    return kv_launch(W4_BY_GROUP(k_w4_set, ), dim3(w4_grid(A)), W4_WG, 0, stream, A);
 }
 
 extern "C" int mlh_weights4_read_device(const mlh_weights4* w, int type, void* dst, int64_t stride, void* stream) {
@@ -486,7 +523,7 @@ extern "C" int mlh_weights4_read_device(const mlh_weights4* w, int type, void* d
     W4Args A = w4_args(w);
     A.dst = dst;
     A.stride = stride;
-    const unsigned grid = w4_grid((size_t)A.N * (A.K / 8));
+    const unsigned grid = w4_grid(A);
     if (type == MLH_DTYPE_F32) return kv_launch(W4_BY_GROUP(k_w4_read, float W4_COMMA), dim3(grid), W4_WG, 0, stream, A);
     if (type == MLH_DTYPE_BF16) return kv_launch(W4_BY_GROUP(k_w4_read, bf16_t W4_COMMA), dim3(grid), W4_WG, 0, stream, A);
     return kv_launch(W4_BY_GROUP(k_w4_read, f16_t W4_COMMA), dim3(grid), W4_WG, 0, stream, A);
@@ -529,26 +566,26 @@ template <typename T, int G, int MT, int WN, int WK, int NT, int TPW, int AHEAD>
 }
 
 // Which kernel, and how its waves are dealt, goes by the rows of A, their type, and the number of 16-row bands of W: many bands fill the chip by themselves, so that a workgroup takes several, for
-// fewer reads of A and fewer starts; few are cut along K.  Microseconds by events around graph replays, one way / the other:
-//   M 1:  fp16, 256 bands, K 4096 4.5 / 7.6 (eight waves of a band / four of two and two); 1792 bands, K 8192 27.6 / 30.1; 2000 bands, K 2048 11.9 / 10.3; fp32 the same three 6.0 / 11.3, 43.6 / 38.4, 18.7 / 11.8
-//   M 8:  fp16, 256 bands, K 4096 5.2 / 6.2 (a band a wave / two); M 5, 512 bands, K 28672 37 / 32; 1792 bands, K 8192 37.7 / 31.2, four of two and two 31.8
-//   M 16: fp16, 256 bands, K 4096 few 5.8, many 8.2; M 10, 512 bands, K 28672 33.5, 35; 1792 bands, K 8192 50, 35
-//   M 32: fp16, 256 bands, K 4096 8.3 / 15.8 (two times four waves of a band / four times two of two); 1792 bands, K 8192 60 / 39
-//   M 64: fp16, 256 bands, K 4096 13.3 / 24.4; 1792 bands, K 8192 101 / 57
+// fewer reads of A and fewer starts; few are cut along K.  Microseconds by events around graph replays, fp16, groups of 64 unless said:
+//   M 1:  256 bands, K 4096 4.5 with eight waves a band, 7.6 with four of two and two; 1792, K 8192, groups of 32 27.6 / 30.1; 2000, K 2048 11.9 / 10.3; fp32 the same three 6.0 / 11.3, 43.6 / 38.4, 18.7 / 11.8
+//   M 8:  256 bands, K 4096 5.2 with eight waves of a band, 6.2 of two; M 5, 512, K 28672 37 / 32; 1792, K 8192 37.7 / 31.2, four of two and two 31.8
+//   M 16: 256 bands, K 4096 5.8 as few rows, 8.2 as many; 512, K 8192 14.0 / 16.6; 704, K 2048 8.0 / 6.5; 1792, K 8192 46.6 / 33
+//   M 32: 512 bands, K 8192 with 2, 4 and 8 bands a workgroup 16.4, 21.1, 32.9; 1024, K 4096 18.6, 15.3, 19.5; 1280, K 4096 25.9, 24.9, 20.3
+//   M 64: 512 bands, K 8192 29, 32, 47; 1024, K 4096 31, 20.4, 27; 1280, K 4096 42.7, 35.0, 28.3
 template <typename T, int G> static int gemm4_go(const Gemm4Args& A, void* stream) {
     constexpr bool f32 = sizeof(T) == 4;
     const int bands = (A.N + W4_ROWS - 1) / W4_ROWS;
-    const bool wide = bands >= 1024;
-    if (A.M <= 4) return wide && (f32 || A.K <= 4096) ? gemm4_few<T, G, 1, 2, 4, 2, 2>(A, stream) : gemm4_few<T, G, 1, 1, 8, 1, 2>(A, stream);
-    if (A.M <= 8) return wide ? gemm4_few<T, G, 2, 2, 4, 2, 2>(A, stream) : bands >= 512 ? gemm4_few<T, G, 2, 1, 8, 2, 2>(A, stream) : gemm4_few<T, G, 2, 1, 8, 1, 2>(A, stream);
+    if (A.M <= 4) return bands >= 1024 && (f32 || A.K <= 4096) ? gemm4_few<T, G, 1, 2, 4, 2, 2>(A, stream) : gemm4_few<T, G, 1, 1, 8, 1, 2>(A, stream);
+    if (A.M <= 8) return bands >= 1024 ? gemm4_few<T, G, 2, 2, 4, 2, 2>(A, stream) : bands >= 512 ? gemm4_few<T, G, 2, 1, 8, 2, 2>(A, stream) : gemm4_few<T, G, 2, 1, 8, 1, 2>(A, stream);
     if constexpr (f32) {
-        if (A.M <= 16) return wide ? gemm4_many<T, G, 1, 4, 2, 2, 2, 1>(A, stream) : gemm4_many<T, G, 1, 2, 4, 1, 1, 2>(A, stream);
-        if (A.M <= 32) return wide ? gemm4_many<T, G, 2, 4, 2, 2, 1, 2>(A, stream) : gemm4_many<T, G, 2, 4, 2, 1, 1, 2>(A, stream);
+        if (A.M <= 16) return bands >= 1024 ? gemm4_many<T, G, 1, 4, 2, 2, 2, 1>(A, stream) : gemm4_many<T, G, 1, 2, 4, 1, 1, 2>(A, stream);
+        if (A.M <= 32) return bands >= 1024 ? gemm4_many<T, G, 2, 4, 2, 2, 1, 2>(A, stream) : gemm4_many<T, G, 2, 4, 2, 1, 1, 2>(A, stream);
         return gemm4_many<T, G, 4, 8, 1, 1, 1, 2>(A, stream);
     } else {
-        if (A.M <= 16) return wide ? gemm4_many<T, G, 1, 4, 2, 2, 2, 2>(A, stream) : bands >= 512 ? gemm4_few<T, G, 4, 1, 8, 2, 2>(A, stream) : gemm4_few<T, G, 4, 1, 8, 1, 2>(A, stream);
-        if (A.M <= 32) return wide ? gemm4_many<T, G, 2, 4, 2, 2, 2, 1>(A, stream) : gemm4_many<T, G, 2, 2, 4, 1, 1, 3>(A, stream);
-        return wide ? gemm4_many<T, G, 4, 4, 2, 2, 2, 1>(A, stream) : gemm4_many<T, G, 4, 2, 4, 1, 1, 3>(A, stream);
+        if (A.M <= 16 && bands <= 512) return bands > 384 ? gemm4_few<T, G, 4, 1, 8, 2, 2>(A, stream) : gemm4_few<T, G, 4, 1, 8, 1, 2>(A, stream);
+        if (A.M <= 16) return bands > 1024 ? gemm4_many<T, G, 1, 4, 2, 2, 2, 2>(A, stream) : gemm4_many<T, G, 1, 2, 4, 2, 2, 1>(A, stream);
+        if (A.M <= 32) return bands > 1024 ? gemm4_many<T, G, 2, 4, 2, 2, 2, 1>(A, stream) : bands > 512 ? gemm4_many<T, G, 2, 2, 4, 2, 2, 1>(A, stream) : gemm4_many<T, G, 2, 2, 4, 1, 1, 3>(A, stream);
+        return bands > 1024 ? gemm4_many<T, G, 4, 4, 2, 2, 2, 1>(A, stream) : bands > 512 ? gemm4_many<T, G, 4, 2, 4, 2, 1, 1>(A, stream) : gemm4_many<T, G, 4, 2, 4, 1, 1, 3>(A, stream);
     }
 }
 

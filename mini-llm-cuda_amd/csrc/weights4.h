@@ -12,15 +12,8 @@
 #define W4_COLS 128
 #define W4_CODES (W4_ROWS * W4_COLS / 2)
 __host__ __device__ constexpr int w4_groups(int group) { return W4_COLS / group; } // of a tile
-__host__ __device__ constexpr int w4_tile(int group) { return W4_CODES + W4_ROWS * w4_groups(group) * 4; }
+__host__ __device__ constexpr int w4_tile(int group) { return W4_CODES + W4_ROWS * w4_groups(group) * 4; } // bytes of it
 __host__ __device__ constexpr int w4_tiles(int K) { return (K + W4_COLS - 1) / W4_COLS; } // of a row
-// the word that holds row n's columns k .. k + 7 (k a multiple of 8), and the pair of a column's group
-__host__ __device__ inline size_t w4_code_at(int n, int k, int K, int group) {
-    return ((size_t)(n / W4_ROWS) * w4_tiles(K) + k / W4_COLS) * w4_tile(group) + ((k / 8 % 4) * W4_ROWS + n % W4_ROWS) * 16 + k / 32 % 4 * 4;
-}
-__host__ __device__ inline size_t w4_param_at(int n, int k, int K, int group) {
-    return ((size_t)(n / W4_ROWS) * w4_tiles(K) + k / W4_COLS) * w4_tile(group) + W4_CODES + (n % W4_ROWS * w4_groups(group) + k % W4_COLS / group) * 4;
-}
 // eight codes in the order of their columns, a nibble each, <-> that word
 __host__ __device__ inline uint32_t w4_spread(uint32_t x) {
     uint32_t y = 0;
