@@ -166,6 +166,10 @@ struct LpShared {
     int slot[2][LP_WAVES];
     float m[LP_WAVES], t[LP_WAVES];
     double s[LP_WAVES];
+    float rowMax;
+    double logz;
+    int token[64];
+    float given[64];
 };
 
 // The elements of granule g of a row that belong to it
@@ -179,7 +183,7 @@ template <typename T, typename F> __device__ __forceinline__ void lp_granule(con
     }
 }
 
-// sh.best: the most likely tokens of granules first .. end - 1, of which this thread's largest has the rank `mine` and whose groups' largest ranks are in sh.group (lost).  All threads.
+// sh.best: the most likely tokens of granules first .. end - 1, of which this thread's largest has the rank `mine` and whose groups' largest ranks are in sh.group (lost).  All threads; whole after a barrier.
 template <typename T> __device__ void lp_tops(LpShared& sh, const LpRow& R, int first, int end, int groups, uint32_t mine, int top) {
     constexpr int V = LpType<T>::V, U = LP_GROUP / V; // granules of a group
     const int t = threadIdx.x;
@@ -291,15 +295,19 @@ template <typename T> __device__ void lp_tops(LpShared& sh, const LpRow& R, int 
         __syncthreads();
     }
     lp_best(sh.cand, n, top, sh.slot, sh.best);
-    __syncthreads();
 }
 
-// What a row's maximum, sums, given tokens' logits and most likely tokens come to: the first wave, one thread a token.
-__device__ __forceinline__ void lp_finish(const LpArgs& A, int row, float m, double s, float ent, int token, float given, const uint64_t* best) {
-    const int t = threadIdx.x;
+// What a row's maximum and sums come to: its entropy, its given tokens, and the logarithm of its sum, which its most likely tokens need.  One wave.
+__device__ __forceinline__ double lp_finish(const LpArgs& A, int row, float m, double s, float ent, int token, float given) {
+    const int lane = threadIdx.x & 63;
     const double logz = m > -INFINITY ? log(s) : NAN;
-    if (t == 0 && A.entropy) A.entropy[row] = (float)(logz - (double)ent * 0.69314718055994530942 / s);
-    if (t < A.given) A.logProb[(size_t)row * A.given + t] = token < 0 ? 0.f : token >= A.vocab ? NAN : (float)(((double)given - (double)m) * A.inv - logz);
+    if (lane == 0 && A.entropy) A.entropy[row] = (float)(logz - (double)ent * 0.69314718055994530942 / s);
+    if (lane < A.given) A.logProb[(size_t)row * A.given + lane] = token < 0 ? 0.f : token >= A.vocab ? NAN : (float)(((double)given - (double)m) * A.inv - logz);
+    return logz;
+}
+// Its most likely tokens: the first wave, one thread a token.
+__device__ __forceinline__ void lp_finish_top(const LpArgs& A, int row, float m, double logz, const uint64_t* best) {
+    const int t = threadIdx.x;
     if (t < A.top) {
         const uint64_t key = best[t];
         A.topIds[(size_t)row * A.top + t] = lp_id(key);
@@ -307,11 +315,14 @@ __device__ __forceinline__ void lp_finish(const LpArgs& A, int row, float m, dou
     }
 }
 
+// What bounds it: many rows memory (8192 of 50257 in bf16, 823 MB: 160 us, 5.1 TB/s), with the instructions for 16 exponentials a chunk close behind; few rows the latencies of one workgroup (a row
+// of 8192 in fp32, five tokens: 6 us, of which the launch is 2).  Workgroups of 512 and 1024 threads were no faster: a compute unit takes 0.1 us for 1000 elements however they are dealt.
+// Parts joined by the last of them to end, counted by atomics, took 25 to 52 us for 64 rows of 131075, which the second launch brings to 17.
 template <typename T, bool TOP>
 __global__ void __launch_bounds__(LP_WG, sizeof(T) == 4 ? 5 : 6) k_logprobs(LpArgs A) {
     constexpr int V = LpType<T>::V, U = LP_CHUNK / V;
     __shared__ LpShared sh;
-    const int t = threadIdx.x, wave = t >> 6;
+    const int t = threadIdx.x, wave = t >> 6, lane = t & 63;
     const unsigned items = (unsigned)A.rows * A.parts; // (2^30 at most)
     for (unsigned item = blockIdx.x; item < items; item += gridDim.x) {
         const int row = (int)(item / A.parts), part = (int)(item % A.parts);
@@ -325,11 +336,10 @@ __global__ void __launch_bounds__(LP_WG, sizeof(T) == 4 ? 5 : 6) k_logprobs(LpAr
             for (int u = 0; u < U; u++) next[u] = R.at[min(g0 + u * LP_WG, end - 1)]; // (behind the end the last one again)
         };
         load(0);
-        float given = 0.f;
-        int token = -1;
-        if (A.parts == 1 && t < A.given) {
-            token = A.tokens[(size_t)row * A.given + t];
-            if (token >= 0 && token < A.vocab) given = lp_get((const T*)A.logits + (size_t)row * A.stride + token);
+        if (A.parts == 1 && wave == LP_WAVES - 1 && lane < A.given) { // (kept in LDS: the loop has no registers left)
+            const int token = A.tokens[(size_t)row * A.given + lane];
+            sh.token[lane] = token;
+            sh.given[lane] = token >= 0 && token < A.vocab ? lp_get((const T*)A.logits + (size_t)row * A.stride + token) : 0.f;
         }
         float m = -INFINITY, ent = 0.f; // m: the wave's
         double s = 0.0;
@@ -388,15 +398,12 @@ __global__ void __launch_bounds__(LP_WG, sizeof(T) == 4 ? 5 : 6) k_logprobs(LpAr
         }
         s = lp_wave_sum(s);
         ent = lp_wave_sum(ent);
-        if ((t & 63) == 63) { sh.m[wave] = m; sh.s[wave] = s; sh.t[wave] = ent; }
-        if (TOP) lp_tops<T>(sh, R, first, end, (chunks + 1) / 2, mine, A.top); // (with the barriers that the sums need)
-        else __syncthreads();
-        if (wave == 0) {
-            m = -INFINITY;
+        if (lane == 63) { sh.m[wave] = m; sh.s[wave] = s; sh.t[wave] = ent; }
+        const auto join = [&] { // the last wave
+            float m = -INFINITY, ent = 0.f;
+            double s = 0.0;
 #pragma unroll
             for (int i = 0; i < LP_WAVES; i++) m = fmaxf(m, sh.m[i]);
-            s = 0.0;
-            ent = 0.f;
 #pragma unroll
             for (int i = 0; i < LP_WAVES; i++) {
                 float from = sh.m[i], e = sh.t[i];
@@ -406,10 +413,19 @@ __global__ void __launch_bounds__(LP_WG, sizeof(T) == 4 ? 5 : 6) k_logprobs(LpAr
                 ent += e;
             }
             if (A.parts > 1) {
-                if (t == 0) reinterpret_cast<LpSums*>(A.work)[item] = LpSums{s, m, ent};
-                if (t < A.top) reinterpret_cast<uint64_t*>(A.work + (size_t)items * sizeof(LpSums))[(size_t)item * A.top + t] = sh.best[t];
-            } else
-                lp_finish(A, row, m, s, ent, token, given, sh.best);
+                if (lane == 0) reinterpret_cast<LpSums*>(A.work)[item] = LpSums{s, m, ent};
+            } else {
+                const double logz = lp_finish(A, row, m, s, ent, sh.token[lane], sh.given[lane]);
+                if (TOP && lane == 0) { sh.rowMax = m; sh.logz = logz; }
+            }
+        };
+        if (TOP) lp_tops<T>(sh, R, first, end, (chunks + 1) / 2, mine, A.top);
+        else __syncthreads();
+        if (wave == LP_WAVES - 1) join(); // (it has less to rank than the first, or nothing)
+        if (TOP) {
+            __syncthreads();
+            if (A.parts == 1) lp_finish_top(A, row, sh.rowMax, sh.logz, sh.best);
+            else if (t < A.top) reinterpret_cast<uint64_t*>(A.work + (size_t)items * sizeof(LpSums))[(size_t)item * A.top + t] = sh.best[t];
         }
         if (item + gridDim.x < items) __syncthreads();
     }
@@ -420,17 +436,22 @@ template <typename T>
 __global__ void __launch_bounds__(LP_WG) k_logprobs_join(LpArgs A) {
     __shared__ uint64_t cand[LP_PARTS * LP_TOP + LP_PAD], best[LP_TOP];
     __shared__ int slot[2][LP_WAVES], found;
+    __shared__ float rowMax;
+    __shared__ double logz;
     const int t = threadIdx.x, lane = t & 63;
     const size_t items = (size_t)A.rows * A.parts;
     for (int row = blockIdx.x; row < A.rows; row += gridDim.x) {
         const LpSums* sums = reinterpret_cast<const LpSums*>(A.work) + (size_t)row * A.parts;
         const uint64_t* keys = reinterpret_cast<const uint64_t*>(A.work + items * sizeof(LpSums)) + (size_t)row * A.parts * A.top;
+        const bool last = t >= LP_WG - 64; // the wave that takes the sums, while the first ranks
         float given = 0.f;
         int token = -1;
-        if (t < A.given) {
-            token = A.tokens[(size_t)row * A.given + t];
+        LpSums mine = {0.0, -INFINITY, 0.f};
+        if (last && lane < A.given) {
+            token = A.tokens[(size_t)row * A.given + lane];
             if (token >= 0 && token < A.vocab) given = lp_get((const T*)A.logits + (size_t)row * A.stride + token);
         }
+        if (last && lane < A.parts) mine = sums[lane];
         if (A.top) {
             if (t == 0) found = 0;
             __syncthreads();
@@ -446,15 +467,17 @@ __global__ void __launch_bounds__(LP_WG) k_logprobs_join(LpArgs A) {
             }
             __syncthreads();
             lp_best(cand, found, A.top, slot, best);
-            __syncthreads();
         }
-        if (t < 64) {
-            LpSums mine = {0.0, -INFINITY, 0.f};
-            if (lane < A.parts) mine = sums[lane];
+        if (last) {
             const float m = lp_wave_max(mine.m);
             lp_scale(mine.m, mine.s, mine.t, m, A.scale);
             const double s = __shfl(lp_wave_sum(mine.s), 63, 64);
-            lp_finish(A, row, m, s, lp_last(lp_wave_sum(mine.t)), token, given, best);
+            const double z = lp_finish(A, row, m, s, lp_last(lp_wave_sum(mine.t)), token, given);
+            if (lane == 0) { rowMax = m; logz = z; }
+        }
+        if (A.top) {
+            __syncthreads();
+            lp_finish_top(A, row, rowMax, logz, best);
         }
     }
 }
@@ -477,12 +500,12 @@ static std::string lp_check(const mlh_logprobs* a) {
 }
 
 // Granules of a part.  A row is one workgroup's where it can be (LP_PART): a second launch costs about 4 us, and many rows fill the chip.  Few and long rows are cut, since one
-// compute unit takes 0.1 us for 1000 elements: in bf16 with the 20 most likely, rows whole / cut, 1 row of 32768 10.6 / 12.8 us, 50000 13.1 / 12.7, 100000 19.5 / 13.5; 64 rows 11.6 / 13.7,
-// 14.4 / 14.2, 20.8 / 16.2; 128 rows of 50000 14.8 / 16.0, of 131072 21.4 / 21.3.  Parts of eight granules a thread or more (four: 14.5 for one row of 100000 in bf16, 22.4 for 13.4 in fp32).
+// compute unit takes 0.1 us for 1000 elements: in bf16 with the 20 most likely, rows whole / cut, 1 row of 32768 10.4 / 11.9 us, 50000 13.0 / 13.7, 100000 19.7 / 14.0; 64 rows 11.1 / 12.8,
+// 13.9 / 14.2, 20.6 / 15.7; 128 rows of 50000 14.0 / 15.1, of 131072 20.7 / 20.4.  Parts of eight granules a thread or more (four: 14.5 for 13.5 for one row of 100000 in bf16, 22.4 for 13.4 in fp32).
 static int lp_part_granules(const mlh_logprobs* a) {
     const int V = 16 / (int)kv_elem_bytes(a->type), granules = (a->vocab + 2 * V - 2) / V, most = LP_PART / V;
     int parts = (granules + most - 1) / most;
-    if (a->rows <= 64 && a->vocab >= 49152) parts = std::max(parts, std::min(LP_PARTS, 256 / std::max(a->rows, 1)));
+    if (a->rows <= 64 && a->vocab >= 65536) parts = std::max(parts, std::min(LP_PARTS, 256 / std::max(a->rows, 1)));
     const int per = ((granules + parts - 1) / parts + LP_WG - 1) / LP_WG * LP_WG;
     return std::min(std::max(per, 8 * LP_WG), most);
 }
