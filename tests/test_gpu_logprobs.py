@@ -186,3 +186,46 @@ def test_on_a_stream_and_in_a_graph(pkg, rows, vocab):
         other = Call(pkg, y, top=3)
         pkg.logprobs(other.args)
         other.check("between")
+
+
+@pytest.mark.parametrize("kind,rows,vocab,given,top,pad,shift", [("bf16", 1, 1 << 22, 2, 64, 0, 0), ("f32", 2, (1 << 22) - 1, 1, 3, 1, 3), ("f16", 70, 131080, 1, 2, 1, 1), ("bf16", 64, 65536, 1, 64, 1, 7),
+                                                                 ("f32", 65, 65537, 0, 5, 0, 2), ("bf16", 63, 65535, 64, 0, 0, 0), ("f32", 70000, 3, 1, 2, 0, 1), ("f16", 4, 70001, 64, 64, 0, 5)])
+def test_largest_rows_and_many(pkg, kind, rows, vocab, given, top, pad, shift):
+    x, gen = logits(kind, rows, vocab, vocab)
+    c = Call(pkg, x, torch.randint(0, vocab, (rows, given), generator=gen), top, pad=pad, shift=shift)
+    pkg.logprobs(c.args)
+    c.check()
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+def test_parts_of_which_some_hold_nothing(pkg, kind):
+    """Rows cut into parts (few of a long vocabulary): masked but for one part, or one token, or with a NaN or an infinity in one part only."""
+    x, gen = logits(kind, 7, 200003, 3)
+    x[0, :150000] = -INF
+    x[1, 5:] = -INF
+    x[2] = -INF
+    x[2, 123456] = 2.0
+    x[3] = -INF
+    x[4, 7] = NAN
+    x[5, 200002] = INF
+    x[6, 8192:] = torch.finfo(x.dtype).min
+    c = Call(pkg, x, torch.randint(0, 200003, (7, 5), generator=gen), 64, 0.5)
+    assert c.size > 0
+    pkg.logprobs(c.args)
+    c.check()
+
+
+@pytest.mark.parametrize("rows,vocab", [(3, 100001), (300, 7001)])
+def test_two_calls_at_once(pkg, rows, vocab):
+    """On two streams, of the same logits, each with work of its own."""
+    x, gen = logits("bf16", rows, vocab, 8)
+    tok = torch.randint(0, vocab, (rows, 2), generator=gen)
+    calls = [Call(pkg, x, tok, 20), Call(pkg, x, tok, 20, 0.7)]
+    calls[1].args.logits = calls[0].args.logits
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in calls]
+    for _ in range(3):
+        for c, s in zip(calls, streams):
+            pkg.logprobs(c.args, s.cuda_stream)
+    for c in calls:
+        c.check()

@@ -213,3 +213,43 @@ def test_on_a_stream_and_in_a_graph(pkg, m, kind):
         g.replay()
         p.check(f"replay {i}")
         Product(pkg, "bf16", 2, 50, 96, 32, seed=i).run().check("between")
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("n,k,group", [(4500, 416, 64), (6201, 1056, 32), (8190, 160, 128), (8193, 736, 64), (16383, 1184, 128), (16400, 288, 32), (20481, 416, 64)])
+def test_every_way_that_waves_are_dealt(pkg, kind, n, k, group):
+    """Rows of A and bands of W on both sides of every bound that chooses a kernel or its shape."""
+    weights = set_from(pkg, n, k, group, n)
+    for m in (1, 4, 5, 8, 9, 16, 17, 32, 33, 64):
+        Product(pkg, kind, m, n, k, group, weights=weights, pad=8).run().check(f"M {m}")
+    if n % 2 == 0:
+        Product(pkg, kind, 64, n, k, group, "swiglu", weights=weights).run().check("swiglu")
+
+
+def test_two_products_at_once(pkg):
+    """On two streams, of the same matrix and of the same A."""
+    weights = set_from(pkg, 5000, 2048, 64, 3)
+    p = [Product(pkg, "bf16", m, 5000, 2048, 64, weights=weights, seed=7) for m in (33, 33, 2)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in p]
+    for _ in range(3):
+        for x, s in zip(p, streams):
+            x.run(s.cuda_stream)
+    for x in p:
+        x.check()
+    assert torch.equal(p[0].c, p[1].c)
+
+
+@pytest.mark.parametrize("n,k,group", [(4097, 1184, 32), (1 << 16, 96, 64), (50, 1 << 17, 128)])
+def test_laid_out_and_read_at_large_sizes(pkg, n, k, group):
+    w, data, codes, params = set_from(pkg, n, k, group, 5)
+    out = torch.full((n + 1, k), 9.0, device="cuda")
+    pkg.weights4_read(w, pkg.DTYPE_F32, out.data_ptr(), k)
+    want = so.values4(codes, params, group).float()
+    assert torch.equal(out[:n].cpu(), want) and bool((out[n] == 9.0).all())
+    again, other = matrix(pkg, n, k, group)
+    pkg.weights4_pack(again, pkg.DTYPE_F32, out.data_ptr(), k)
+    c2, p2 = so.quantise4(want, group)
+    pkg.weights4_read(again, pkg.DTYPE_F32, out.data_ptr(), k)
+    torch.cuda.synchronize()
+    assert torch.equal(out[:n].cpu(), so.values4(c2, p2, group).float()) and bool((other[-64:] == 255).all())

@@ -104,6 +104,17 @@ def test_logprobs(pkg, kw, what):
     assert pkg.logprobs_work_bytes(_logprobs(pkg, **kw)) == 0
 
 
+@pytest.mark.parametrize("kw", [dict(work=None), dict(work=(1 << 26) + 8), dict(workBytes=0), dict(workBytes=-1)])
+def test_logprobs_of_rows_in_parts_want_their_work(pkg, kw):
+    long = dict(rows=2, vocab=200000, stride=200000)
+    need = pkg.logprobs_work_bytes(_logprobs(pkg, **long))
+    assert need > 0 and pkg.logprobs_work_bytes(_logprobs(pkg)) == 0
+    if kw.get("workBytes") == -1:
+        kw = dict(workBytes=need - 1)
+    with pytest.raises(pkg.MlhError, match="work"):
+        pkg.logprobs(_logprobs(pkg, **long, **kw))
+
+
 def test_null_structures(pkg):
     assert pkg.dev.mlh_rotate_device(None, None) == -1 and b"null" in pkg.dev.mlh_last_error(None)
     assert pkg.dev.mlh_logprobs_device(None, None) == -1 and b"null" in pkg.dev.mlh_last_error(None)
