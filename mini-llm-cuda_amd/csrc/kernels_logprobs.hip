@@ -4,6 +4,7 @@
 // parts of a row are joined by the same rule.  For the top tokens a thread also notes the largest of every 32 elements it has seen (a group).  The k-th largest of the threads' maxima is
 // a bound that k tokens reach, so only groups that reach it can hold one of the k most likely: about as many groups as tokens are asked for.  Those are read again, their elements
 // that reach the bound are ranked by counting how many are larger, and the row is done.
+// A row is a workgroup's, or, few and long ones, cut into parts, whose sums and groups a second launch takes up with a workgroup a row.
 #include <math.h>
 
 #include <algorithm>
@@ -14,8 +15,8 @@
 #define LP_WAVES (LP_WG / 64)
 #define LP_CHUNK 16                            // elements a thread takes at once
 #define LP_GROUP 32                            // ... and whose largest it notes
-#define LP_GROUPS 16                           // groups of a thread, at most
-#define LP_PART (LP_WG * LP_GROUP * LP_GROUPS) // elements of a part, at most
+#define LP_UNIT (LP_WG * LP_GROUP)             // elements of which every thread has a group; parts are whole units
+#define LP_GROUPS 16                           // groups of a thread, at most, where one workgroup has a row
 #define LP_TOP 64
 #define LP_CANDS (LP_TOP * LP_GROUP)           // elements that are ranked, at most
 #define LP_PAD 8
@@ -31,10 +32,11 @@ struct LpArgs {
     int rows, vocab, given, top;
     double inv;  // 1 / temperature
     float scale; // ... times log2(e)
-    int parts, partGranules;
-    unsigned char* work; // with several parts: what they leave
+    int parts, partGranules, units; // units: of a row, at most
+    unsigned char* work;            // with parts: what they leave
 };
-struct LpSums { double s; float m, t; }; // of a part; behind those of all parts their best keys, `top` each
+struct LpSums { double s; float m, t; }; // of a part; behind those of all parts the ranks of the groups, [rows][units][LP_WG]
+__device__ __forceinline__ uint32_t* lp_ranks(const LpArgs& A, int row) { return reinterpret_cast<uint32_t*>(A.work + (size_t)A.rows * A.parts * sizeof(LpSums)) + (size_t)row * A.units * LP_WG; }
 
 template <typename T> struct LpType;
 template <> struct LpType<float> { static constexpr int V = 4; };
@@ -150,12 +152,11 @@ __device__ void lp_best(uint64_t* cand, int n, int top, int (*slot)[LP_WAVES], u
         }
         if (r < top) best[r] = key;
     }
-    for (int r = n + threadIdx.x; r < top; r += LP_WG) best[r] = 0; // (a short part)
 }
 
-struct LpShared {
+template <int GROUPS> struct LpTops {
     union {
-        uint32_t group[LP_GROUPS][LP_WG]; // rank of the largest of every group; 0: none
+        uint32_t group[GROUPS][LP_WG];    // rank of the largest of every group; 0: none
         uint64_t cand[LP_CANDS + LP_PAD]; // (once the groups that matter are known)
     };
     uint32_t most[LP_WG];
@@ -164,12 +165,6 @@ struct LpShared {
     int count, found, seen;
     uint32_t bound;
     int slot[2][LP_WAVES];
-    float m[LP_WAVES], t[LP_WAVES];
-    double s[LP_WAVES];
-    float rowMax;
-    double logz;
-    int token[64];
-    float given[64];
 };
 
 // The elements of granule g of a row that belong to it
@@ -179,12 +174,14 @@ template <typename T, typename F> __device__ __forceinline__ void lp_granule(con
 #pragma unroll
     for (int i = 0; i < V; i++) {
         const int id = g * V - R.lead + i;
-        if (id >= 0 && id < R.vocab) f(lp_elem(v, i, T{}), id);
+        if (id >= 0 && id < R.vocab) f(lp_elem(v, i, T{}), id, i);
     }
 }
 
-// sh.best: the most likely tokens of granules first .. end - 1, of which this thread's largest has the rank `mine` and whose groups' largest ranks are in sh.group (lost).  All threads; whole after a barrier.
-template <typename T> __device__ void lp_tops(LpShared& sh, const LpRow& R, int first, int end, int groups, uint32_t mine, int top) {
+// sh.best: the row's most likely tokens.  group: the ranks of its groups, [groups][LP_WG] (in LDS they are sh.group, and lost), of which a thread has every LP_WG-th, or (WIDE) four
+// in every 4 * LP_WG; `mine`: the largest of this thread's.  All threads; whole after a barrier.  (Few workgroups run this, once each, so that fetching the code counts: loops are not unrolled
+// but where loads have to be on their way together.)
+template <typename T, bool WIDE, int GROUPS> __device__ void lp_tops(LpTops<GROUPS>& sh, const LpRow& R, int groups, const uint32_t* group, uint32_t mine, int top) {
     constexpr int V = LpType<T>::V, U = LP_GROUP / V; // granules of a group
     const int t = threadIdx.x;
     sh.most[t] = mine;
@@ -217,15 +214,29 @@ template <typename T> __device__ void lp_tops(LpShared& sh, const LpRow& R, int 
     }
     __syncthreads();
     uint32_t bound = sh.bound;
-    const auto list = [&](uint32_t least) { // this thread's groups that reach it
-        uint32_t those = 0;
+    const auto each = [&](auto f) { // four of this thread's groups at a time: f(ranks, index of the first, from one to the next)
+        if constexpr (WIDE) {
+#pragma unroll 1
+            for (int at = t * 4; at < groups * LP_WG; at += LP_WG * 4) f(*reinterpret_cast<const kv_u32x4*>(group + at), at, 1);
+        } else {
+#pragma unroll 1
+            for (int at = t; at < groups * LP_WG; at += LP_WG * 4) {
+                kv_u32x4 r;
 #pragma unroll
-        for (int j = 0; j < LP_GROUPS; j++) those |= (uint32_t)(j < groups && sh.group[j][t] >= least) << j;
-        while (those) {
-            const int i = atomicAdd(&sh.count, 1);
-            if (i < LP_TOP) sh.list[i] = __builtin_ctz(those) << 8 | t;
-            those &= those - 1;
+                for (int e = 0; e < 4; e++) r[e] = at + e * LP_WG < groups * LP_WG ? group[at + e * LP_WG] : 0u;
+                f(r, at, LP_WG);
+            }
         }
+    };
+    const auto list = [&](uint32_t least) { // this thread's groups that reach it
+        each([&](kv_u32x4 r, int at, int by) {
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                if (r[e] >= least) {
+                    const int i = atomicAdd(&sh.count, 1);
+                    if (i < LP_TOP) sh.list[i] = at + e * by;
+                }
+        });
     };
     bool many = sh.seen > LP_TOP; // (threads that are equal at the bound)
     if (!many) {
@@ -239,7 +250,10 @@ template <typename T> __device__ void lp_tops(LpShared& sh, const LpRow& R, int 
             const uint32_t mid = step == 0 ? lo + 1 : lo + (hi - lo) / 2; // (most often masked tokens are what is at the bound)
             int c = 0;
             if (mine >= mid)
-                for (int j = 0; j < groups; j++) c += sh.group[j][t] >= mid;
+                each([&](kv_u32x4 r, int, int) {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) c += r[e] >= mid;
+                });
             c = lp_count(c, sh.slot[step & 1]);
             if (c >= top) lo = mid; else hi = mid;
             many = c < top || c > LP_TOP;
@@ -252,21 +266,31 @@ template <typename T> __device__ void lp_tops(LpShared& sh, const LpRow& R, int 
     }
     const int listed = sh.count;
     for (int i = t; i < listed * U; i += LP_WG) {
-        const int where = sh.list[i / U], g = first + ((where >> 8) * U + i % U) * LP_WG + (where & 255);
-        if (g < end)
-            lp_granule<T>(R, g, [&](float x, int id) {
+        const int where = sh.list[i / U], g = ((where >> 8) * U + i % U) * LP_WG + (where & 255);
+        if (g < R.granules) {
+            uint64_t keys[V];
+            uint32_t those = 0;
+            lp_granule<T>(R, g, [&](float x, int id, int e) {
                 const uint32_t r = lp_rank(x);
-                if (many ? r > bound : r >= bound) sh.cand[atomicAdd(&sh.found, 1)] = lp_key(r, id);
+                keys[e] = lp_key(r, id);
+                those |= (uint32_t)(r >= bound + many) << e; // (no rank is 2^32 - 1)
             });
+            if (those) {
+                int at = atomicAdd(&sh.found, __builtin_popcount(those));
+#pragma unroll
+                for (int e = 0; e < V; e++)
+                    if (those >> e & 1) sh.cand[at++] = keys[e];
+            }
+        }
     }
     __syncthreads();
     int n = sh.found;
     if (many && n < top) { // of those that equal the bound the first ones: granule by granule in the order of ids
         int need = top - n;
-        for (int g0 = first, step = 0; g0 < end && need > 0; g0 += LP_WG, step++) {
+        for (int g0 = 0, step = 0; g0 < R.granules && need > 0; g0 += LP_WG, step++) {
             const int g = g0 + t;
             uint32_t equal = 0;
-            if (g < end) lp_granule<T>(R, g, [&](float x, int id) { equal |= (uint32_t)(lp_rank(x) == bound) << (id - g * V + R.lead); });
+            if (g < R.granules) lp_granule<T>(R, g, [&](float x, int, int e) { equal |= (uint32_t)(lp_rank(x) == bound) << e; });
             int before = __builtin_popcount(equal);
             const int own = before;
 #pragma unroll
@@ -317,11 +341,17 @@ __device__ __forceinline__ void lp_finish_top(const LpArgs& A, int row, float m,
 
 // What bounds it: many rows memory (8192 of 50257 in bf16, 823 MB: 160 us, 5.1 TB/s), with the instructions for 16 exponentials a chunk close behind; few rows the latencies of one workgroup (a row
 // of 8192 in fp32, five tokens: 6 us, of which the launch is 2).  Workgroups of 512 and 1024 threads were no faster: a compute unit takes 0.1 us for 1000 elements however they are dealt.
-// Parts joined by the last of them to end, counted by atomics, took 25 to 52 us for 64 rows of 131075, which the second launch brings to 17.
-template <typename T, bool TOP>
+// Rows in parts: 64 of 131075 in bf16 16 us, of which the parts take 7.5 and the join 8.4, a row alone 3.8 and 6.9: the join waits for memory three times (ranks, groups, given tokens' logits) and for
+// its own code.  Parts that picked their own top tokens took 14 + 5 us; joined by the last part to end, counted by atomics, 25 to 52.
+enum { LP_SUMS, LP_WHOLE, LP_PARTLY }; // no top tokens; with them, of rows that are one workgroup's; the groups left in work
+template <typename T, int KIND>
 __global__ void __launch_bounds__(LP_WG, sizeof(T) == 4 ? 5 : 6) k_logprobs(LpArgs A) {
     constexpr int V = LpType<T>::V, U = LP_CHUNK / V;
-    __shared__ LpShared sh;
+    __shared__ LpTops<KIND == LP_WHOLE ? LP_GROUPS : 1> sh;
+    __shared__ LpSums of[LP_WAVES];
+    __shared__ double logz;
+    __shared__ float rowMax, given[64];
+    __shared__ int token[64];
     const int t = threadIdx.x, wave = t >> 6, lane = t & 63;
     const unsigned items = (unsigned)A.rows * A.parts; // (2^30 at most)
     for (unsigned item = blockIdx.x; item < items; item += gridDim.x) {
@@ -336,11 +366,13 @@ __global__ void __launch_bounds__(LP_WG, sizeof(T) == 4 ? 5 : 6) k_logprobs(LpAr
             for (int u = 0; u < U; u++) next[u] = R.at[min(g0 + u * LP_WG, end - 1)]; // (behind the end the last one again)
         };
         load(0);
-        if (A.parts == 1 && wave == LP_WAVES - 1 && lane < A.given) { // (kept in LDS: the loop has no registers left)
-            const int token = A.tokens[(size_t)row * A.given + lane];
-            sh.token[lane] = token;
-            sh.given[lane] = token >= 0 && token < A.vocab ? lp_get((const T*)A.logits + (size_t)row * A.stride + token) : 0.f;
+        const bool whole = KIND == LP_WHOLE || (KIND == LP_SUMS && A.parts == 1);
+        if (whole && wave == LP_WAVES - 1 && lane < A.given) { // (kept in LDS: the loop has no registers left)
+            const int id = A.tokens[(size_t)row * A.given + lane];
+            token[lane] = id;
+            given[lane] = id >= 0 && id < A.vocab ? lp_get((const T*)A.logits + (size_t)row * A.stride + id) : 0.f;
         }
+        uint32_t* const ranks = KIND == LP_PARTLY ? lp_ranks(A, row) + first / (LP_UNIT / V) * LP_WG + t : nullptr;
         float m = -INFINITY, ent = 0.f; // m: the wave's
         double s = 0.0;
         uint32_t mine = 0, grp = 0;
@@ -369,10 +401,13 @@ __global__ void __launch_bounds__(LP_WG, sizeof(T) == 4 ? 5 : 6) k_logprobs(LpAr
 #pragma unroll
             for (int i = 1; i < LP_CHUNK; i++) c = fmaxf(c, x[i]);
             if (!(c > -INFINITY)) c = -INFINITY; // (NaN alone)
-            if (TOP) {
+            if (KIND != LP_SUMS) {
                 grp = max(j & 1 ? grp : 0u, any ? lp_rank(c) : 0u);
-                mine = max(mine, grp);
-                if (j & 1 || j + 1 == chunks) sh.group[j / 2][t] = grp;
+                if (KIND == LP_WHOLE) mine = max(mine, grp);
+                if (j & 1 || j + 1 == chunks) {
+                    if (KIND == LP_WHOLE) sh.group[j / 2][t] = grp;
+                    else ranks[j / 2 * LP_WG] = grp;
+                }
             }
             const float cw = lp_wave_max(c);
             if (cw > m) lp_scale(m, s, ent, cw, A.scale); // (seldom)
@@ -398,52 +433,43 @@ __global__ void __launch_bounds__(LP_WG, sizeof(T) == 4 ? 5 : 6) k_logprobs(LpAr
         }
         s = lp_wave_sum(s);
         ent = lp_wave_sum(ent);
-        if (lane == 63) { sh.m[wave] = m; sh.s[wave] = s; sh.t[wave] = ent; }
-        const auto join = [&] { // the last wave
-            float m = -INFINITY, ent = 0.f;
-            double s = 0.0;
+        if (lane == 63) of[wave] = LpSums{s, m, ent};
+        if (KIND == LP_WHOLE) lp_tops<T, false>(sh, R, (chunks + 1) / 2, &sh.group[0][0], mine, A.top); // (with the barrier that the sums need)
+        else __syncthreads();
+        if (wave == LP_WAVES - 1) { // (it has less to rank than the first, or nothing)
+            LpSums all = {0.0, -INFINITY, 0.f};
 #pragma unroll
-            for (int i = 0; i < LP_WAVES; i++) m = fmaxf(m, sh.m[i]);
+            for (int i = 0; i < LP_WAVES; i++) all.m = fmaxf(all.m, of[i].m);
 #pragma unroll
             for (int i = 0; i < LP_WAVES; i++) {
-                float from = sh.m[i], e = sh.t[i];
-                double z = sh.s[i];
-                lp_scale(from, z, e, m, A.scale);
-                s += z;
-                ent += e;
+                LpSums one = of[i];
+                lp_scale(one.m, one.s, one.t, all.m, A.scale);
+                all.s += one.s;
+                all.t += one.t;
             }
-            if (A.parts > 1) {
-                if (lane == 0) reinterpret_cast<LpSums*>(A.work)[item] = LpSums{s, m, ent};
-            } else {
-                const double logz = lp_finish(A, row, m, s, ent, sh.token[lane], sh.given[lane]);
-                if (TOP && lane == 0) { sh.rowMax = m; sh.logz = logz; }
-            }
-        };
-        if (TOP) lp_tops<T>(sh, R, first, end, (chunks + 1) / 2, mine, A.top);
-        else __syncthreads();
-        if (wave == LP_WAVES - 1) join(); // (it has less to rank than the first, or nothing)
-        if (TOP) {
+            if (whole) {
+                const double z = lp_finish(A, row, all.m, all.s, all.t, token[lane], given[lane]);
+                if (KIND == LP_WHOLE && lane == 0) { rowMax = all.m; logz = z; }
+            } else if (lane == 0)
+                reinterpret_cast<LpSums*>(A.work)[item] = all;
+        }
+        if (KIND == LP_WHOLE) {
             __syncthreads();
-            if (A.parts == 1) lp_finish_top(A, row, sh.rowMax, sh.logz, sh.best);
-            else if (t < A.top) reinterpret_cast<uint64_t*>(A.work + (size_t)items * sizeof(LpSums))[(size_t)item * A.top + t] = sh.best[t];
+            lp_finish_top(A, row, rowMax, logz, sh.best);
         }
         if (item + gridDim.x < items) __syncthreads();
     }
 }
 
-// One workgroup a row: the parts' sums and best tokens.  A part's own top-th key is a bound that the row's reach.
-template <typename T>
+// One workgroup a row: the parts' sums, and the tokens out of the groups' ranks.
+template <typename T, bool TOP>
 __global__ void __launch_bounds__(LP_WG) k_logprobs_join(LpArgs A) {
-    __shared__ uint64_t cand[LP_PARTS * LP_TOP + LP_PAD], best[LP_TOP];
-    __shared__ int slot[2][LP_WAVES], found;
-    __shared__ float rowMax;
+    __shared__ LpTops<1> sh;
     __shared__ double logz;
+    __shared__ float rowMax;
     const int t = threadIdx.x, lane = t & 63;
-    const size_t items = (size_t)A.rows * A.parts;
+    const bool last = t >= LP_WG - 64; // the wave that takes the sums, while the first ranks
     for (int row = blockIdx.x; row < A.rows; row += gridDim.x) {
-        const LpSums* sums = reinterpret_cast<const LpSums*>(A.work) + (size_t)row * A.parts;
-        const uint64_t* keys = reinterpret_cast<const uint64_t*>(A.work + items * sizeof(LpSums)) + (size_t)row * A.parts * A.top;
-        const bool last = t >= LP_WG - 64; // the wave that takes the sums, while the first ranks
         float given = 0.f;
         int token = -1;
         LpSums mine = {0.0, -INFINITY, 0.f};
@@ -451,22 +477,23 @@ __global__ void __launch_bounds__(LP_WG) k_logprobs_join(LpArgs A) {
             token = A.tokens[(size_t)row * A.given + lane];
             if (token >= 0 && token < A.vocab) given = lp_get((const T*)A.logits + (size_t)row * A.stride + token);
         }
-        if (last && lane < A.parts) mine = sums[lane];
-        if (A.top) {
-            if (t == 0) found = 0;
-            __syncthreads();
-            uint64_t bound = lane < A.parts ? keys[(lane + 1) * A.top - 1] : 0;
+        if (last && lane < A.parts) mine = reinterpret_cast<const LpSums*>(A.work)[(size_t)row * A.parts + lane];
+        if (TOP) {
+            constexpr int V = LpType<T>::V;
+            const LpRow R = lp_row<T>(A, row);
+            const int groups = (R.granules + LP_UNIT / V - 1) / (LP_UNIT / V);
+            const uint32_t* ranks = lp_ranks(A, row);
+            uint32_t most = 0;
+            for (int at = t * 4; at < groups * LP_WG; at += LP_WG * 32) {
+                kv_u32x4 r[8];
 #pragma unroll
-            for (int o = 1; o < 64; o <<= 1) {
-                const uint64_t other = (uint64_t)__shfl_xor((unsigned long long)bound, o, 64);
-                bound = other > bound ? other : bound;
+                for (int j = 0; j < 8; j++) r[j] = *reinterpret_cast<const kv_u32x4*>(ranks + min(at + j * LP_WG * 4, groups * LP_WG - 4));
+#pragma unroll
+                for (int j = 0; j < 8; j++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) most = max(most, at + j * LP_WG * 4 < groups * LP_WG ? r[j][e] : 0u);
             }
-            for (int i = t; i < A.parts * A.top; i += LP_WG) {
-                const uint64_t key = keys[i];
-                if (key && key >= bound) cand[atomicAdd(&found, 1)] = key;
-            }
-            __syncthreads();
-            lp_best(cand, found, A.top, slot, best);
+            lp_tops<T, true>(sh, R, groups, ranks, most, A.top);
         }
         if (last) {
             const float m = lp_wave_max(mine.m);
@@ -475,9 +502,10 @@ __global__ void __launch_bounds__(LP_WG) k_logprobs_join(LpArgs A) {
             const double z = lp_finish(A, row, m, s, lp_last(lp_wave_sum(mine.t)), token, given);
             if (lane == 0) { rowMax = m; logz = z; }
         }
-        if (A.top) {
+        if (TOP) {
             __syncthreads();
-            lp_finish_top(A, row, rowMax, logz, best);
+            lp_finish_top(A, row, rowMax, logz, sh.best);
+            if (row + (int)gridDim.x < A.rows) __syncthreads();
         }
     }
 }
@@ -499,32 +527,33 @@ static std::string lp_check(const mlh_logprobs* a) {
     return "";
 }
 
-// Granules of a part.  A row is one workgroup's where it can be (LP_PART): a second launch costs about 4 us, and many rows fill the chip.  Few and long rows are cut, since one
-// compute unit takes 0.1 us for 1000 elements: in bf16 with the 20 most likely, rows whole / cut, 1 row of 32768 10.4 / 11.9 us, 50000 13.0 / 13.7, 100000 19.7 / 14.0; 64 rows 11.1 / 12.8,
-// 13.9 / 14.2, 20.6 / 15.7; 128 rows of 50000 14.0 / 15.1, of 131072 20.7 / 20.4.  Parts of eight granules a thread or more (four: 14.5 for 13.5 for one row of 100000 in bf16, 22.4 for 13.4 in fp32).
-static int lp_part_granules(const mlh_logprobs* a) {
-    const int V = 16 / (int)kv_elem_bytes(a->type), granules = (a->vocab + 2 * V - 2) / V, most = LP_PART / V;
-    int parts = (granules + most - 1) / most;
-    if (a->rows <= 64 && a->vocab >= 65536) parts = std::max(parts, std::min(LP_PARTS, 256 / std::max(a->rows, 1)));
-    const int per = ((granules + parts - 1) / parts + LP_WG - 1) / LP_WG * LP_WG;
-    return std::min(std::max(per, 8 * LP_WG), most);
-}
-static int lp_parts(const mlh_logprobs* a, int per) {
-    const int V = 16 / (int)kv_elem_bytes(a->type), granules = (a->vocab + 2 * V - 2) / V;
-    return (granules + per - 1) / per;
+// How rows are cut.  A row is one workgroup's where it can be (LP_GROUPS): a second launch costs about 4 us, and many rows fill the chip.  Few and long rows are cut into as many parts as make 1024
+// workgroups of whole units (512: up to 1 us more), since one compute unit takes 0.1 us for 1000 elements.  bf16 with the 20 most likely, us whole / cut: 1 row of 32768 10.5 / 10.7, 40000 11.9 / 10.6,
+// 100000 20.6 / 11.2; 64 rows 11.2 / 11.9, 12.3 / 12.2, 21.3 / 14.3; 128 rows of 32768 11.3 / 13.1, 50000 14.4 / 13.8, 100000 21.8 / 17.1; 256 rows of 50000 14.5 / 16.9, 100000 22.8 / 23.3.
+struct LpCut { int units, parts, per; bool join; }; // units: of a row; per: of a part
+static LpCut lp_cut(const mlh_logprobs* a) {
+    const int V = 16 / (int)kv_elem_bytes(a->type), units = (a->vocab + V - 1 + LP_UNIT - 1) / LP_UNIT;
+    const bool few = a->rows <= 128 && a->vocab >= 40960;
+    LpCut c = {units, 1, units, (a->top && units > LP_GROUPS) || few};
+    if (c.join) {
+        const int parts = std::min(std::max(1024 / std::max(a->rows, 1), 1), LP_PARTS);
+        c.per = (units + parts - 1) / parts;
+        c.parts = (units + c.per - 1) / c.per;
+    }
+    return c;
 }
 
 extern "C" uint64_t mlh_logprobs_work_bytes(const mlh_logprobs* a) {
     if (!lp_check(a).empty()) return 0;
-    const int parts = lp_parts(a, lp_part_granules(a));
-    return parts > 1 ? (uint64_t)a->rows * parts * (sizeof(LpSums) + 8 * a->top) : 0;
+    const LpCut c = lp_cut(a);
+    return c.join ? (uint64_t)a->rows * (c.parts * sizeof(LpSums) + (a->top ? (uint64_t)c.units * LP_WG * 4 : 0)) : 0;
 }
 
-template <typename T> static int lp_go(const LpArgs& A, void* stream) {
-    const dim3 grid((unsigned)std::min<long long>((long long)A.rows * A.parts, 1 << 22));
-    const int rc = kv_launch(A.top ? &k_logprobs<T, true> : &k_logprobs<T, false>, grid, LP_WG, 0, stream, A);
-    if (rc || A.parts == 1) return rc;
-    return kv_launch(&k_logprobs_join<T>, dim3((unsigned)std::min(A.rows, 1 << 22)), LP_WG, 0, stream, A);
+template <typename T> static int lp_go(const LpArgs& A, bool join, void* stream) {
+    const dim3 grid((unsigned)std::min<long long>((long long)A.rows * A.parts, 1 << 22)), rows((unsigned)std::min(A.rows, 1 << 22));
+    const int rc = kv_launch(!A.top ? &k_logprobs<T, LP_SUMS> : join ? &k_logprobs<T, LP_PARTLY> : &k_logprobs<T, LP_WHOLE>, grid, LP_WG, 0, stream, A);
+    if (rc || !join) return rc;
+    return kv_launch(A.top ? &k_logprobs_join<T, true> : &k_logprobs_join<T, false>, rows, LP_WG, 0, stream, A);
 }
 
 extern "C" int mlh_logprobs_device(const mlh_logprobs* a, void* stream) {
@@ -534,10 +563,10 @@ extern "C" int mlh_logprobs_device(const mlh_logprobs* a, void* stream) {
     const uint64_t need = mlh_logprobs_work_bytes(a);
     if (need && (!a->work || (uintptr_t)a->work % 16 || a->workBytes < need)) return kv_fail("work must be 16-byte aligned and have mlh_logprobs_work_bytes");
     const double inv = a->temperature == 0.f ? 1.0 : 1.0 / (double)a->temperature;
-    const int per = lp_part_granules(a);
+    const LpCut c = lp_cut(a);
     LpArgs A = {a->logits, a->stride, a->tokens, a->logProb, a->entropy, a->topIds, a->topLogProb, a->rows, a->vocab, a->given, a->top, inv, (float)(inv * 1.4426950408889634074),
-                lp_parts(a, per), per, (unsigned char*)a->work};
-    if (a->type == MLH_DTYPE_F32) return lp_go<float>(A, stream);
-    if (a->type == MLH_DTYPE_BF16) return lp_go<bf16_t>(A, stream);
-    return lp_go<f16_t>(A, stream);
+                c.parts, c.per * (LP_UNIT / (16 / (int)kv_elem_bytes(a->type))), c.units, (unsigned char*)a->work};
+    if (a->type == MLH_DTYPE_F32) return lp_go<float>(A, c.join, stream);
+    if (a->type == MLH_DTYPE_BF16) return lp_go<bf16_t>(A, c.join, stream);
+    return lp_go<f16_t>(A, c.join, stream);
 }

@@ -189,7 +189,8 @@ def test_on_a_stream_and_in_a_graph(pkg, rows, vocab):
 
 
 @pytest.mark.parametrize("kind,rows,vocab,given,top,pad,shift", [("bf16", 1, 1 << 22, 2, 64, 0, 0), ("f32", 2, (1 << 22) - 1, 1, 3, 1, 3), ("f16", 70, 131080, 1, 2, 1, 1), ("bf16", 64, 65536, 1, 64, 1, 7),
-                                                                 ("f32", 65, 65537, 0, 5, 0, 2), ("bf16", 63, 65535, 64, 0, 0, 0), ("f32", 70000, 3, 1, 2, 0, 1), ("f16", 4, 70001, 64, 64, 0, 5)])
+                                                                 ("f32", 65, 65537, 0, 5, 0, 2), ("bf16", 128, 40960, 1, 20, 0, 1), ("f16", 129, 40960, 1, 20, 0, 1), ("f32", 128, 40959, 1, 20, 2, 1),
+                                                                 ("bf16", 140, 140000, 1, 0, 0, 3), ("f32", 9, 1048573, 1, 64, 1, 3), ("bf16", 63, 65535, 64, 0, 0, 0), ("f32", 70000, 3, 1, 2, 0, 1), ("f16", 4, 70001, 64, 64, 0, 5)])
 def test_largest_rows_and_many(pkg, kind, rows, vocab, given, top, pad, shift):
     x, gen = logits(kind, rows, vocab, vocab)
     c = Call(pkg, x, torch.randint(0, vocab, (rows, given), generator=gen), top, pad=pad, shift=shift)
