@@ -220,6 +220,15 @@ template <typename T, int BANDS, int THREADS, typename F> __device__ __forceinli
     }
 }
 
+// This workgroup's rows of A, ROWS at most.
+template <typename T, int ROWS> __device__ __forceinline__ void w4_rows(Gemm4Args& A) {
+    const int first = (int)blockIdx.y * ROWS;
+    A.M = min(A.M - first, ROWS);
+    A.a = (const T*)A.a + first * A.aStride;
+    if (A.r) A.r = (const T*)A.r + first * A.rStride;
+    A.c = (T*)A.c + first * A.cStride;
+}
+
 // Products with minimum and scale behind the sums: the sum over a group of a (min + scale code) is (scale D + (min - scale SHIFT) S) / UNIT, D the sum of a UNIT (code + SHIFT) and S that of
 // a UNIT; both come from the matrix cores, S as a product with UNIT.  Lane l of a result holds column l % 16 (a row of W) and the instruction's rows 4 (l / 16) + i, i = 0 .. 3.
 //
@@ -227,6 +236,8 @@ template <typename T, int BANDS, int THREADS, typename F> __device__ __forceinli
 // the s-th step's codes has that step's sums, of row m, in element s of lanes 16 m to 16 m + 15.  (The other elements are of rows and codes that do not belong together.)  One product with UNIT gives the S of
 // all four steps.  No LDS and no barrier but for the sums of WK waves at the end.
 // A workgroup is WN x WK waves, WN * NT * 16 rows of W; a wave has TPW tiles of its share of K on their way.
+// Bound by memory where W is large (5 rows, N 8192, K 28672, groups of 32, fp16: 147 MB in 28 us, 5.2 TB/s), else by the latency of a start, of a wave's first tiles and of its last sums (1 row, N 11264,
+// K 2048, groups of 64, bf16: 13 MB in 4.9 us).
 template <typename T, int G, int MR, int WN, int WK, int NT, int TPW>
 __global__ void __launch_bounds__(W4_WAVES * 64) k_gemm4_few(Gemm4Args A) {
     typedef W4Mul<T> X;
@@ -235,6 +246,7 @@ __global__ void __launch_bounds__(W4_WAVES * 64) k_gemm4_few(Gemm4Args A) {
     typedef uint32_t Pairs __attribute__((ext_vector_type(TG)));
     __shared__ float part[WK][WN * NT][MR][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wn = wave / WK, wk = wave % WK, row = lane & 15, quad = lane >> 4;
+    w4_rows<T, MR * 4>(A);
     const int tiles = w4_tiles(A.K), bands = (A.N + W4_ROWS - 1) / W4_ROWS, k0 = (row & 3) * 32 + quad * 8;
     const uint8_t* w[NT];
 #pragma unroll
@@ -318,9 +330,11 @@ __global__ void __launch_bounds__(W4_WAVES * 64) k_gemm4_few(Gemm4Args A) {
     });
 }
 
-// More rows, MT times 16: the instruction's rows are rows of A.  A goes through LDS, once for all waves of a workgroup, a block of WK * TPW tiles of K at a time and two blocks in turn; W4_LOADERS
+// More rows, MT times 16 of them a workgroup: the instruction's rows are rows of A.  A goes through LDS, once for all waves of a workgroup, a block of WK * TPW tiles of K at a time and two blocks in turn; W4_LOADERS
 // further waves bring it there, since loads come back in the order they were asked for: a wave that waits for A, which is near, would wait for codes that are far and not needed yet.  Wave (wn, wk) of the
 // others multiplies TPW tiles of every block with its NT times 16 rows of W, whose codes it asks for AHEAD blocks ahead.
+// 64 rows, N 28672, K 8192, groups of 64, fp16 take 55 us, 550 TFLOP/s, twice what the matrix cores alone need.  Left out in turn, the loads of W save 13 us, A's out of LDS 6, the loaders 2, and all three
+// half the time: the three wait for each other, with 37 KB of W on their way a compute unit, as many as the registers hold; of the cycles VALU take 70 % (codes, scales), MFMA 49, LDS 26.
 // In LDS piece q (eight columns) of step s (32 columns) of row m stands at [m][s ^ (m / 4 % 4)][q ^ (m % 4)], so that neither the lanes of a store, which share a row, nor those of a load, which share
 // step and piece, meet in a bank.
 template <typename T, int G, int MT, int WN, int WK, int NT, int TPW, int AHEAD>
@@ -329,6 +343,7 @@ __global__ void __launch_bounds__((W4_WAVES + W4_LOADERS) * 64) k_gemm4_many(Gem
     constexpr int S = G / 32, TG = w4_groups(G), ROWS = MT * 16, STEPS = WK * TPW * 4, PIECES = STEPS * 4, PLANE = ROWS * PIECES, BUF = PLANE * X::PLANES;
     typedef uint32_t Pairs __attribute__((ext_vector_type(TG)));
     extern __shared__ w4_u32x4 lds[];
+    w4_rows<T, ROWS>(A);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int tiles = w4_tiles(A.K), blocks = (tiles + WK * TPW - 1) / (WK * TPW);
     const int wn = wave / WK, wk = wave % WK, row = lane & 15, quad = lane >> 4;
@@ -559,7 +574,7 @@ extern "C" uint64_t mlh_gemm4_work_bytes(const mlh_weights4* w, const mlh_gemm4*
 
 template <typename T, int G, int MR, int WN, int WK, int NT, int TPW> static int gemm4_few(const Gemm4Args& A, void* stream) {
     const unsigned grid = ((A.N + W4_ROWS - 1) / W4_ROWS + WN * NT - 1) / (WN * NT);
-    return kv_launch(&k_gemm4_few<T, G, MR, WN, WK, NT, TPW>, dim3(grid), W4_WAVES * 64, 0, stream, A);
+    return kv_launch(&k_gemm4_few<T, G, MR, WN, WK, NT, TPW>, dim3(grid, (A.M + MR * 4 - 1) / (MR * 4)), W4_WAVES * 64, 0, stream, A);
 }
 template <typename T, int G, int MT, int WN, int WK, int NT, int TPW, int AHEAD> static int gemm4_many(const Gemm4Args& A, void* stream) {
     constexpr int rows = MT * 16, lds = std::max(2 * WK * TPW * 4 * rows * 64 * W4Mul<T>::PLANES, WK * WN * NT * rows * 16 * 4);
@@ -569,30 +584,53 @@ template <typename T, int G, int MT, int WN, int WK, int NT, int TPW, int AHEAD>
         const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&k_gemm4_many<T, G, MT, WN, WK, NT, TPW, AHEAD>), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
         if (e != hipSuccess) return kv_status(e);
     }
-    return kv_launch(&k_gemm4_many<T, G, MT, WN, WK, NT, TPW, AHEAD>, dim3(grid), (W4_WAVES + W4_LOADERS) * 64, lds, stream, A);
+    return kv_launch(&k_gemm4_many<T, G, MT, WN, WK, NT, TPW, AHEAD>, dim3(grid, (A.M + rows - 1) / rows), (W4_WAVES + W4_LOADERS) * 64, lds, stream, A);
 }
 
-// Which kernel, and how its waves are dealt, goes by the rows of A, their type, and the number of 16-row bands of W: many bands fill the chip by themselves, so that a workgroup takes several, for
-// fewer reads of A and fewer starts; few are cut along K.  Microseconds by events around graph replays, fp16, groups of 64 unless said:
+// A workgroup's share of a product of more than eight rows: rows of A times 16-row bands of W, and what a round of such workgroups, one a compute unit, takes (tenths of a us at K 8192, fp32 or fp16, groups of 64).
+// Large shares read A and W less often, small ones fill the chip when there are few: taken is the share whose rounds take least.  That was the fastest or within 5 % of it for 9 to 64 rows of
+// 48 to 1792 bands; for instance, us with the share taken / the next ones, fp16, K 4096: 64 rows, 256 bands 16 x 4 8.7 / 32 x 4 11.1, 16 x 2 13.2; 1024 bands 64 x 4 20.3 / 32 x 4 26.1, 64 x 8 27;
+// 32 rows, 1024 bands 32 x 4 15.0 / 16 x 8 16.2, 16 x 4 17.0; 16 rows, 256 bands 16 x 1 5.7 / 16 x 2 7.0, 16 x 4 8.2; fp32: 64 rows, 256 bands 16 x 4 15.0 / 16 x 8 19.9, 16 x 2 23.4, 32 x 8 28.9.
+struct W4Share { int rows, bands, us; };
+static int w4_share(const W4Share* s, int n, int M, int bands) {
+    int best = 0;
+    long long least = -1;
+    for (int i = 0; i < n; i++) {
+        const long long groups = (long long)((M + s[i].rows - 1) / s[i].rows) * ((bands + s[i].bands - 1) / s[i].bands), us = (groups + 255) / 256 * s[i].us;
+        if (least < 0 || us < least) { least = us; best = i; }
+    }
+    return best;
+}
+
+// Up to eight rows all of A is a wave's; with many bands of W a workgroup takes several, for fewer starts.  Microseconds by events around graph replays, fp16, groups of 64 unless said:
 //   M 1:  256 bands, K 4096 4.5 with eight waves a band, 7.6 with four of two and two; 1792, K 8192, groups of 32 27.6 / 30.1; 2000, K 2048 11.9 / 10.3; fp32 the same three 6.0 / 11.3, 43.6 / 38.4, 18.7 / 11.8
 //   M 8:  256 bands, K 4096 5.2 with eight waves of a band, 6.2 of two; M 5, 512, K 28672 37 / 32; 1792, K 8192 37.7 / 31.2, four of two and two 31.8
-//   M 16: 256 bands, K 4096 5.8 as few rows, 8.2 as many; 512, K 8192 14.0 / 16.6; 704, K 2048 8.0 / 6.5; 1792, K 8192 46.6 / 33
-//   M 32: 512 bands, K 8192 with 2, 4 and 8 bands a workgroup 16.4, 21.1, 32.9; 1024, K 4096 18.6, 15.3, 19.5; 1280, K 4096 25.9, 24.9, 20.3
-//   M 64: 512 bands, K 8192 29, 32, 47; 1024, K 4096 31, 20.4, 27; 1280, K 4096 42.7, 35.0, 28.3
 template <typename T, int G> static int gemm4_go(const Gemm4Args& A, void* stream) {
     constexpr bool f32 = sizeof(T) == 4;
     const int bands = (A.N + W4_ROWS - 1) / W4_ROWS;
     if (A.M <= 4) return bands >= 1024 && (f32 || A.K <= 4096) ? gemm4_few<T, G, 1, 2, 4, 2, 2>(A, stream) : gemm4_few<T, G, 1, 1, 8, 1, 2>(A, stream);
     if (A.M <= 8) return bands >= 1024 ? gemm4_few<T, G, 2, 2, 4, 2, 2>(A, stream) : bands >= 512 ? gemm4_few<T, G, 2, 1, 8, 2, 2>(A, stream) : gemm4_few<T, G, 2, 1, 8, 1, 2>(A, stream);
     if constexpr (f32) {
-        if (A.M <= 16) return bands >= 1024 ? gemm4_many<T, G, 1, 4, 2, 2, 2, 1>(A, stream) : gemm4_many<T, G, 1, 2, 4, 1, 1, 2>(A, stream);
-        if (A.M <= 32) return bands >= 1024 ? gemm4_many<T, G, 2, 4, 2, 2, 1, 2>(A, stream) : gemm4_many<T, G, 2, 4, 2, 1, 1, 2>(A, stream);
-        return gemm4_many<T, G, 4, 8, 1, 1, 1, 2>(A, stream);
+        static const W4Share shares[] = {{8, 1, 125}, {16, 2, 205}, {16, 4, 238}, {16, 8, 333}, {32, 8, 525}};
+        switch (w4_share(shares, 5, A.M, bands)) {
+        case 0: return gemm4_few<T, G, 2, 1, 8, 1, 2>(A, stream);
+        case 1: return gemm4_many<T, G, 1, 2, 4, 1, 1, 2>(A, stream);
+        case 2: return gemm4_many<T, G, 1, 2, 4, 2, 1, 2>(A, stream);
+        case 3: return gemm4_many<T, G, 1, 4, 2, 2, 2, 1>(A, stream);
+        default: return gemm4_many<T, G, 2, 4, 2, 2, 1, 1>(A, stream);
+        }
     } else {
-        if (A.M <= 16 && bands <= 512) return bands > 384 ? gemm4_few<T, G, 4, 1, 8, 2, 2>(A, stream) : gemm4_few<T, G, 4, 1, 8, 1, 2>(A, stream);
-        if (A.M <= 16) return bands > 1024 ? gemm4_many<T, G, 1, 4, 2, 2, 2, 2>(A, stream) : gemm4_many<T, G, 1, 2, 4, 2, 2, 1>(A, stream);
-        if (A.M <= 32) return bands > 1024 ? gemm4_many<T, G, 2, 4, 2, 2, 2, 1>(A, stream) : bands > 512 ? gemm4_many<T, G, 2, 2, 4, 2, 2, 1>(A, stream) : gemm4_many<T, G, 2, 2, 4, 1, 1, 3>(A, stream);
-        return bands > 1024 ? gemm4_many<T, G, 4, 4, 2, 2, 2, 1>(A, stream) : bands > 512 ? gemm4_many<T, G, 4, 2, 4, 2, 1, 1>(A, stream) : gemm4_many<T, G, 4, 2, 4, 1, 1, 3>(A, stream);
+        static const W4Share shares[] = {{16, 1, 80}, {16, 2, 103}, {16, 4, 126}, {16, 8, 206}, {32, 4, 170}, {32, 8, 330}, {64, 4, 260}, {64, 8, 470}};
+        switch (w4_share(shares, 8, A.M, bands)) {
+        case 0: return gemm4_few<T, G, 4, 1, 8, 1, 2>(A, stream);
+        case 1: return gemm4_few<T, G, 4, 1, 8, 2, 2>(A, stream);
+        case 2: return gemm4_many<T, G, 1, 2, 4, 2, 2, 1>(A, stream);
+        case 3: return gemm4_many<T, G, 1, 4, 2, 2, 2, 2>(A, stream);
+        case 4: return gemm4_many<T, G, 2, 2, 4, 2, 2, 1>(A, stream);
+        case 5: return gemm4_many<T, G, 2, 4, 2, 2, 2, 1>(A, stream);
+        case 6: return gemm4_many<T, G, 4, 2, 4, 2, 1, 1>(A, stream);
+        default: return gemm4_many<T, G, 4, 4, 2, 2, 2, 1>(A, stream);
+        }
     }
 }
 
