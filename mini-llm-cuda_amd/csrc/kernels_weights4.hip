@@ -14,7 +14,6 @@ typedef _Float16 w4_f16x8 __attribute__((ext_vector_type(8)));
 
 #define W4_WG 256   // threads of the kernels that lay out and read
 #define W4_WAVES 8   // waves of a product's workgroup that multiply
-#define W4_LOADERS 4 // ... and that bring A, where it goes through LDS
 
 // ----------------------------------------------------------------------------
 // laying out
@@ -153,7 +152,7 @@ template <> struct W4Mul<f16_t> { // codes as halves below 2^-14, code * 2^-21
     static __device__ __forceinline__ V codes(uint32_t x) {
         return __builtin_bit_cast(V, w4_u32x4{w4_turn<0>(x) & 0x00780078u, w4_turn<1>(x) & 0x00780078u, w4_turn<2>(x) & 0x00780078u, w4_turn<3>(x) & 0x00780078u});
     }
-    static __device__ __forceinline__ V unit() { return __builtin_bit_cast(V, w4_u32x4{0x00080008u, 0x00080008u, 0x00080008u, 0x00080008u}); }
+    static __device__ __forceinline__ V unit(bool on = true) { const uint32_t u = on ? 0x00080008u : 0u; return __builtin_bit_cast(V, w4_u32x4{u, u, u, u}); }
     static __device__ __forceinline__ w4_f32x4 mul(V a, V b, w4_f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 };
 template <> struct W4Mul<bf16_t> { // codes behind 16: a bf16 of 16 + code has the code in bits 3 to 6
@@ -165,7 +164,7 @@ template <> struct W4Mul<bf16_t> { // codes behind 16: a bf16 of 16 + code has t
         asm("" : "+v"(base)); // (a register: with two literals the mask and the base would take an instruction each)
         return __builtin_bit_cast(V, w4_u32x4{(w4_turn<0>(x) & 0x00780078u) | base, (w4_turn<1>(x) & 0x00780078u) | base, (w4_turn<2>(x) & 0x00780078u) | base, (w4_turn<3>(x) & 0x00780078u) | base});
     }
-    static __device__ __forceinline__ V unit() { return __builtin_bit_cast(V, w4_u32x4{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u}); }
+    static __device__ __forceinline__ V unit(bool on = true) { const uint32_t u = on ? 0x3f803f80u : 0u; return __builtin_bit_cast(V, w4_u32x4{u, u, u, u}); }
     static __device__ __forceinline__ w4_f32x4 mul(V a, V b, w4_f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 };
 template <> struct W4Mul<float> : W4Mul<bf16_t> { // the same with activations as three planes (p3.h): every product exact
@@ -330,26 +329,35 @@ __global__ void __launch_bounds__(W4_WAVES * 64) k_gemm4_few(Gemm4Args A) {
     });
 }
 
-// More rows, MT times 16 of them a workgroup: the instruction's rows are rows of A.  A goes through LDS, once for all waves of a workgroup, a block of WK * TPW tiles of K at a time and two blocks in turn; W4_LOADERS
+// More rows, MT times 16 of them a workgroup: the instruction's rows are rows of A.  A goes through LDS, once for all waves of a workgroup, a block of WK * TPW tiles of K at a time and two blocks in turn; LOADERS
 // further waves bring it there, since loads come back in the order they were asked for: a wave that waits for A, which is near, would wait for codes that are far and not needed yet.  Wave (wn, wk) of the
 // others multiplies TPW tiles of every block with its NT times 16 rows of W, whose codes it asks for AHEAD blocks ahead.
-// 64 rows, N 28672, K 8192, groups of 64, fp16 take 55 us, 550 TFLOP/s, twice what the matrix cores alone need.  Left out in turn, the loads of W save 13 us, A's out of LDS 6, the loaders 2, and all three
-// half the time: the three wait for each other, with 37 KB of W on their way a compute unit, as many as the registers hold; of the cycles VALU take 70 % (codes, scales), MFMA 49, LDS 26.
+// S does not depend on W: the loaders take it, with UNIT in the four rows of the instruction that belong to a group and zeros in the others, so that four groups add up in one result and stand where
+// v_mfma_f32_16x16x4_f32 wants them, which multiplies four groups' S with their minima at once, in fp32.  (With S and its products in every multiplying wave fp32 took 5 to 12 % longer, groups of 32 up to 15 %.)
+// Groups of 128 are two of 64 here, for fewer registers.  Eight loaders where the registers of 16 waves hold the shape (S and A in time: fp32, 16 rows, 7.8 us for 8.8 at 128 bands), four elsewhere.
+// 64 rows, N 28672, K 8192, groups of 64, fp16 take 55 us, 550 TFLOP/s, twice what the matrix cores alone need.  Left out in turn (before the loaders took S), the loads of W saved 13 us, A's out of LDS 6,
+// the loaders 2, and all three half the time: the three wait for each other; two and three blocks of codes ahead, other waves and shares were no faster.
 // In LDS piece q (eight columns) of step s (32 columns) of row m stands at [m][s ^ (m / 4 % 4)][q ^ (m % 4)], so that neither the lanes of a store, which share a row, nor those of a load, which share
 // step and piece, meet in a bank.
-template <typename T, int G, int MT, int WN, int WK, int NT, int TPW, int AHEAD>
-__global__ void __launch_bounds__((W4_WAVES + W4_LOADERS) * 64) k_gemm4_many(Gemm4Args A) {
+__host__ __device__ constexpr int w4_sums_at(int buf, int part) { return 2 * buf > part ? 2 * buf : part; } // bytes in front of the sums: two blocks of A, later the waves' results
+template <typename T, int G, int MT, int WN, int WK, int NT, int TPW, int AHEAD, int LOADERS>
+__global__ void __launch_bounds__((W4_WAVES + LOADERS) * 64) k_gemm4_many(Gemm4Args A) {
     typedef W4Mul<T> X;
-    constexpr int S = G / 32, TG = w4_groups(G), ROWS = MT * 16, STEPS = WK * TPW * 4, PIECES = STEPS * 4, PLANE = ROWS * PIECES, BUF = PLANE * X::PLANES;
-    typedef uint32_t Pairs __attribute__((ext_vector_type(TG)));
+    constexpr int S = G < 64 ? 1 : 2, TG = 4 / S, LOADED = w4_groups(G), ROWS = MT * 16, STEPS = WK * TPW * 4, PIECES = STEPS * 4, PLANE = ROWS * PIECES, BUF = PLANE * X::PLANES;
+    constexpr int FOURS = (TPW * TG + 3) / 4; // groups of a wave's share of a block, by four
+    typedef uint32_t Pairs __attribute__((ext_vector_type(LOADED)));
     extern __shared__ w4_u32x4 lds[];
     w4_rows<T, ROWS>(A);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int tiles = w4_tiles(A.K), blocks = (tiles + WK * TPW - 1) / (WK * TPW);
     const int wn = wave / WK, wk = wave % WK, row = lane & 15, quad = lane >> 4;
     float* part = reinterpret_cast<float*>(lds); // [WK][WN * NT][ROWS][16], at the end
+    float* sums = reinterpret_cast<float*>(lds) + w4_sums_at(BUF * 16, WK * WN * NT * ROWS * 64) / 4; // of blocks in turn, [2][WK][MT][FOURS][64]
+    int at[4]; // this lane's piece of step s of a block's first tile, in its first 16 rows
+#pragma unroll
+    for (int s = 0; s < 4; s++) at[s] = (row * STEPS + (s ^ (row >> 2 & 3))) * 4 + (quad ^ (row & 3));
     if (wave >= W4_WAVES) {
-        constexpr int THREADS = W4_LOADERS * 64, UNITS = PLANE / THREADS, EVERY = THREADS / PIECES; // EVERY: rows from one of a thread's pieces to the next
+        constexpr int THREADS = LOADERS * 64, UNITS = PLANE / THREADS, EVERY = THREADS / PIECES; // EVERY: rows from one of a thread's pieces to the next
         static_assert(WN * WK == W4_WAVES && PIECES <= THREADS && PLANE % THREADS == 0, "waves, pieces of A");
         const int thread = threadIdx.x - W4_WAVES * 64, row0 = PIECES < 64 ? thread / PIECES : (wave - W4_WAVES) * 64 / PIECES, piece = thread % PIECES;
         W4Raw<T> raw[UNITS];
@@ -377,11 +385,29 @@ __global__ void __launch_bounds__((W4_WAVES + W4_LOADERS) * 64) k_gemm4_many(Gem
                 for (int p = 0; p < X::PLANES; p++) buf[(place ^ ((i * EVERY >> 2 & 3) * 4 | (i * EVERY & 3))) + (p * PLANE + i * EVERY * PIECES)] = v[p];
             }
         };
+        // S of block b, four groups in a result: the instruction's rows of UNIT are where the group's lanes are, the others zero
+        const auto take = [&](int b) {
+            const w4_u32x4* const buf = lds + (b & 1) * BUF;
+            for (int u = wave - W4_WAVES; u < WK * MT * FOURS; u += LOADERS) { // [WK][MT][FOURS]
+                const w4_u32x4* const from = buf + u / FOURS % MT * 16 * PIECES + (u / FOURS / MT * TPW + u % FOURS * 4 / TG) * 16;
+                w4_f32x4 s[4] = {};
+#pragma unroll
+                for (int g = 0; g < 4 && g < TPW * TG; g++) {
+                    const typename X::V unit = X::unit(row >> 2 == g);
+#pragma unroll
+                    for (int q = 0; q < S; q++)
+#pragma unroll
+                        for (int p = X::PLANES - 1; p >= 0; p--) s[g] = X::mul(unit, __builtin_bit_cast(typename X::V, from[p * PLANE + at[g % TG * S + q] + g / TG * 16]), s[g]);
+                }
+                sums[((b & 1) * WK * MT * FOURS + u) * 64 + lane] = (s[0][0] + s[1][0]) + (s[2][0] + s[3][0]);
+            }
+        };
         ask(0);
         put(0);
         ask(1);
         __syncthreads();
         for (int b = 0; b < blocks; b++) { // (while the others multiply block b)
+            take(b);
             if (b + 1 < blocks) put(b + 1);
             ask(b + 2);
             __syncthreads();
@@ -399,18 +425,35 @@ __global__ void __launch_bounds__((W4_WAVES + W4_LOADERS) * 64) k_gemm4_many(Gem
             for (int nt = 0; nt < NT; nt++) {
                 const uint8_t* at = w[nt] + (size_t)t * w4_tile(G);
                 codes[a][j][nt] = *reinterpret_cast<const w4_u32x4*>(at + lane * 16);
-                pairs[a][j][nt] = *reinterpret_cast<const Pairs*>(at + W4_CODES + row * (TG * 4));
+                pairs[a][j][nt] = *reinterpret_cast<const Pairs*>(at + W4_CODES + row * (LOADED * 4));
             }
         };
 #pragma unroll
         for (int a = 0; a < AHEAD; a++)
 #pragma unroll
             for (int j = 0; j < TPW; j++) ask(a, a, j);
-        int at[4]; // this lane's piece of step s of the block's first tile, in its first 16 rows
-#pragma unroll
-        for (int s = 0; s < 4; s++) at[s] = (row * STEPS + (s ^ (row >> 2 & 3))) * 4 + (quad ^ (row & 3));
-        const typename X::V unit = X::unit();
         w4_f32x4 acc[NT][MT] = {};
+        uint32_t lows[NT][FOURS] = {}; // the pair of this lane's row and group of each four
+        // S times (min - scale SHIFT) for the block behind the last barrier: four groups in an instruction of fp32.  What it reads, and its products: with few rows at
+        // the end of the next block, where nothing waits for the LDS (16 rows, 1792 bands 28 us for 31), with more at once, for want of registers
+        float low[NT][FOURS], s[MT][FOURS];
+        const auto minima = [&](int b) {
+#pragma unroll
+            for (int f = 0; f < FOURS; f++) {
+#pragma unroll
+                for (int mt = 0; mt < MT; mt++) s[mt][f] = sums[((((b & 1) * WK + wk) * MT + mt) * FOURS + f) * 64 + lane];
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) low[nt][f] = kv_half(lows[nt][f] & 0xffffu) - kv_half(lows[nt][f] >> 16) * X::SHIFT;
+            }
+        };
+        const auto multiply = [&] {
+#pragma unroll
+            for (int f = 0; f < FOURS; f++)
+#pragma unroll
+                for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++) acc[nt][mt] = __builtin_amdgcn_mfma_f32_16x16x4f32(s[mt][f], low[nt][f], acc[nt][mt], 0, 0, 0);
+        };
         __syncthreads();
         for (int b0 = 0; b0 < blocks; b0 += AHEAD) {
 #pragma unroll
@@ -432,14 +475,18 @@ __global__ void __launch_bounds__((W4_WAVES + W4_LOADERS) * 64) k_gemm4_many(Gem
                     };
                     fetch(0);
                     typename X::V c[S][NT];
-                    float scale[2][NT], low[2][NT];
-                    w4_f32x4 d[2][NT], s[2];
+                    float scale[2][NT];
+                    w4_f32x4 d[2][NT];
+                    if (b > 0) {
+                        minima(b - 1);
+                        if (MT > 1) multiply();
+                    }
                     const auto apply = [&](int i) {
                         const int mt = i % MT, h = i / MT & 1;
 #pragma unroll
                         for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-                            for (int e = 0; e < 4; e++) acc[nt][mt][e] = fmaf(scale[h][nt], d[i & 1][nt][e], fmaf(low[h][nt], s[i & 1][e], acc[nt][mt][e]));
+                            for (int e = 0; e < 4; e++) acc[nt][mt][e] = fmaf(scale[h][nt], d[i & 1][nt][e], acc[nt][mt][e]);
                     };
 #pragma unroll
                     for (int i = 0; i < PARTS; i++) {
@@ -450,29 +497,30 @@ __global__ void __launch_bounds__((W4_WAVES + W4_LOADERS) * 64) k_gemm4_many(Gem
                             for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
                                 for (int q = 0; q < S; q++) c[q][nt] = X::codes(codes[u][j][nt][g * S + q]);
-                                scale[h][nt] = kv_half(pairs[u][j][nt][g] >> 16);
-                                low[h][nt] = kv_half(pairs[u][j][nt][g] & 0xffffu) - scale[h][nt] * X::SHIFT;
+                                scale[h][nt] = kv_half(pairs[u][j][nt][g * LOADED / TG] >> 16);
+                                lows[nt][(j * TG + g) / 4] = quad == (j * TG + g) % 4 ? pairs[u][j][nt][g * LOADED / TG] : (j * TG + g) % 4 ? lows[nt][(j * TG + g) / 4] : 0u;
                             }
                         }
-                        s[i & 1] = w4_f32x4{};
 #pragma unroll
                         for (int nt = 0; nt < NT; nt++) d[i & 1][nt] = w4_f32x4{};
 #pragma unroll
                         for (int q = 0; q < S; q++)
 #pragma unroll
                             for (int p = X::PLANES - 1; p >= 0; p--) {
-                                s[i & 1] = X::mul(a[i & 1][q][p], unit, s[i & 1]);
 #pragma unroll
                                 for (int nt = 0; nt < NT; nt++) d[i & 1][nt] = X::mul(a[i & 1][q][p], c[q][nt], d[i & 1][nt]);
                             }
                         if (i > 0) apply(i - 1);
                         if (mt == MT - 1 && g == TG - 1) ask(b + AHEAD, u, j);
                     }
+                    if (MT == 1 && b > 0) multiply();
                     apply(PARTS - 1);
                     __syncthreads();
                 }
             }
         }
+        minima(blocks - 1);
+        multiply();
 #pragma unroll
         for (int nt = 0; nt < NT; nt++)
 #pragma unroll
@@ -481,7 +529,7 @@ __global__ void __launch_bounds__((W4_WAVES + W4_LOADERS) * 64) k_gemm4_many(Gem
                 for (int i = 0; i < 4; i++) part[((wk * WN * NT + wn * NT + nt) * ROWS + mt * 16 + quad * 4 + i) * 16 + row] = acc[nt][mt][i] * (1.f / X::UNIT);
     }
     __syncthreads();
-    w4_finish<T, WN * NT, (W4_WAVES + W4_LOADERS) * 64>(A, [&](int m, int n) {
+    w4_finish<T, WN * NT, (W4_WAVES + LOADERS) * 64>(A, [&](int m, int n) {
         float v = 0.f;
 #pragma unroll
         for (int q = 0; q < WK; q++) v += part[((q * WN * NT + n / 16) * ROWS + m) * 16 + n % 16];
@@ -576,21 +624,22 @@ template <typename T, int G, int MR, int WN, int WK, int NT, int TPW> static int
     const unsigned grid = ((A.N + W4_ROWS - 1) / W4_ROWS + WN * NT - 1) / (WN * NT);
     return kv_launch(&k_gemm4_few<T, G, MR, WN, WK, NT, TPW>, dim3(grid, (A.M + MR * 4 - 1) / (MR * 4)), W4_WAVES * 64, 0, stream, A);
 }
-template <typename T, int G, int MT, int WN, int WK, int NT, int TPW, int AHEAD> static int gemm4_many(const Gemm4Args& A, void* stream) {
-    constexpr int rows = MT * 16, lds = std::max(2 * WK * TPW * 4 * rows * 64 * W4Mul<T>::PLANES, WK * WN * NT * rows * 16 * 4);
+template <typename T, int G, int MT, int WN, int WK, int NT, int TPW, int AHEAD, int LOADERS> static int gemm4_many(const Gemm4Args& A, void* stream) {
+    constexpr int rows = MT * 16, lds = w4_sums_at(WK * TPW * 4 * rows * 64 * W4Mul<T>::PLANES, WK * WN * NT * rows * 16 * 4) + 2 * WK * MT * ((TPW * (G < 64 ? 4 : 2) + 3) / 4) * 256;
     static_assert(lds <= 163840, "LDS of a compute unit");
     const unsigned grid = ((A.N + W4_ROWS - 1) / W4_ROWS + WN * NT - 1) / (WN * NT);
     if (lds > 65536) { // (asked for on every call: the attribute belongs to the device that is current)
-        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&k_gemm4_many<T, G, MT, WN, WK, NT, TPW, AHEAD>), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&k_gemm4_many<T, G, MT, WN, WK, NT, TPW, AHEAD, LOADERS>), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
         if (e != hipSuccess) return kv_status(e);
     }
-    return kv_launch(&k_gemm4_many<T, G, MT, WN, WK, NT, TPW, AHEAD>, dim3(grid, (A.M + rows - 1) / rows), (W4_WAVES + W4_LOADERS) * 64, lds, stream, A);
+    return kv_launch(&k_gemm4_many<T, G, MT, WN, WK, NT, TPW, AHEAD, LOADERS>, dim3(grid, (A.M + rows - 1) / rows), (W4_WAVES + LOADERS) * 64, lds, stream, A);
 }
 
-// A workgroup's share of a product of more than eight rows: rows of A times 16-row bands of W, and what a round of such workgroups, one a compute unit, takes (tenths of a us at K 8192, fp32 or fp16, groups of 64).
-// Large shares read A and W less often, small ones fill the chip when there are few: taken is the share whose rounds take least.  That was the fastest or within 5 % of it for 9 to 64 rows of
-// 48 to 1792 bands; for instance, us with the share taken / the next ones, fp16, K 4096: 64 rows, 256 bands 16 x 4 8.7 / 32 x 4 11.1, 16 x 2 13.2; 1024 bands 64 x 4 20.3 / 32 x 4 26.1, 64 x 8 27;
-// 32 rows, 1024 bands 32 x 4 15.0 / 16 x 8 16.2, 16 x 4 17.0; 16 rows, 256 bands 16 x 1 5.7 / 16 x 2 7.0, 16 x 4 8.2; fp32: 64 rows, 256 bands 16 x 4 15.0 / 16 x 8 19.9, 16 x 2 23.4, 32 x 8 28.9.
+// A workgroup's share of a product of more than eight rows: rows of A times 16-row bands of W, and what a round of such workgroups, one a compute unit, takes (tenths of a us at N 2048, K 8192, fp32 or
+// fp16, groups of 64).  Large shares read A and W less often, small ones fill the chip when there are few: taken is the share whose rounds take least, the fastest or within 6 % of it for 9 to 64
+// rows of 48 to 2000 bands.  For instance, us with the share taken / the next ones, fp16, K 4096: 64 rows, 256 bands 16 x 4 8.8 / 32 x 4 10.9, 16 x 8 11.8; 1024 bands 32 x 8 18.6 / 32 x 4 25.4, 64 x 8 26.8;
+// 1280 bands 64 x 8 27.4 / 32 x 8 31.9; 32 rows, 1024 bands 32 x 4 14.9 / 16 x 8 15.2, 32 x 8 18.0; 16 rows, 256 bands 16 x 1 5.6 / 16 x 2 7.0, 16 x 4 8.1; fp32: 64 rows, 256 bands 16 x 4 13.4 / 16 x 8 17.5,
+// 16 x 2 20.0, 32 x 8 26.3.  (64 x 4 takes longer than 32 x 8 everywhere: 21.1 for 18.6.)
 struct W4Share { int rows, bands, us; };
 static int w4_share(const W4Share* s, int n, int M, int bands) {
     int best = 0;
@@ -611,25 +660,24 @@ template <typename T, int G> static int gemm4_go(const Gemm4Args& A, void* strea
     if (A.M <= 4) return bands >= 1024 && (f32 || A.K <= 4096) ? gemm4_few<T, G, 1, 2, 4, 2, 2>(A, stream) : gemm4_few<T, G, 1, 1, 8, 1, 2>(A, stream);
     if (A.M <= 8) return bands >= 1024 ? gemm4_few<T, G, 2, 2, 4, 2, 2>(A, stream) : bands >= 512 ? gemm4_few<T, G, 2, 1, 8, 2, 2>(A, stream) : gemm4_few<T, G, 2, 1, 8, 1, 2>(A, stream);
     if constexpr (f32) {
-        static const W4Share shares[] = {{8, 1, 125}, {16, 2, 205}, {16, 4, 238}, {16, 8, 333}, {32, 8, 525}};
+        static const W4Share shares[] = {{8, 1, 127}, {16, 2, 174}, {16, 4, 209}, {16, 8, 304}, {32, 8, 488}};
         switch (w4_share(shares, 5, A.M, bands)) {
         case 0: return gemm4_few<T, G, 2, 1, 8, 1, 2>(A, stream);
-        case 1: return gemm4_many<T, G, 1, 2, 4, 1, 1, 2>(A, stream);
-        case 2: return gemm4_many<T, G, 1, 2, 4, 2, 1, 2>(A, stream);
-        case 3: return gemm4_many<T, G, 1, 4, 2, 2, 2, 1>(A, stream);
-        default: return gemm4_many<T, G, 2, 4, 2, 2, 1, 1>(A, stream);
+        case 1: return gemm4_many<T, G, 1, 2, 4, 1, 1, 2, 8>(A, stream);
+        case 2: return gemm4_many<T, G, 1, 2, 4, 2, 1, 2, 8>(A, stream);
+        case 3: return gemm4_many<T, G, 1, 4, 2, 2, 2, 1, 4>(A, stream);
+        default: return gemm4_many<T, G, 2, 4, 2, 2, 1, 1, 8>(A, stream);
         }
     } else {
-        static const W4Share shares[] = {{16, 1, 80}, {16, 2, 103}, {16, 4, 126}, {16, 8, 206}, {32, 4, 170}, {32, 8, 330}, {64, 4, 260}, {64, 8, 470}};
-        switch (w4_share(shares, 8, A.M, bands)) {
+        static const W4Share shares[] = {{16, 1, 80}, {16, 2, 103}, {16, 4, 124}, {16, 8, 192}, {32, 4, 171}, {32, 8, 264}, {64, 8, 406}};
+        switch (w4_share(shares, 7, A.M, bands)) {
         case 0: return gemm4_few<T, G, 4, 1, 8, 1, 2>(A, stream);
         case 1: return gemm4_few<T, G, 4, 1, 8, 2, 2>(A, stream);
-        case 2: return gemm4_many<T, G, 1, 2, 4, 2, 2, 1>(A, stream);
-        case 3: return gemm4_many<T, G, 1, 4, 2, 2, 2, 2>(A, stream);
-        case 4: return gemm4_many<T, G, 2, 2, 4, 2, 2, 1>(A, stream);
-        case 5: return gemm4_many<T, G, 2, 4, 2, 2, 2, 1>(A, stream);
-        case 6: return gemm4_many<T, G, 4, 2, 4, 2, 1, 1>(A, stream);
-        default: return gemm4_many<T, G, 4, 4, 2, 2, 2, 1>(A, stream);
+        case 2: return gemm4_many<T, G, 1, 2, 4, 2, 2, 1, 8>(A, stream);
+        case 3: return gemm4_many<T, G, 1, 4, 2, 2, 2, 2, G == 64 ? 8 : 4>(A, stream);
+        case 4: return gemm4_many<T, G, 2, 2, 4, 2, 2, 1, 8>(A, stream);
+        case 5: return gemm4_many<T, G, 2, 4, 2, 2, 2, 1, 4>(A, stream);
+        default: return gemm4_many<T, G, 4, 4, 2, 2, 2, 1, 4>(A, stream);
         }
     }
 }
