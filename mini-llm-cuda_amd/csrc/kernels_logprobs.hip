@@ -339,7 +339,7 @@ __device__ __forceinline__ void lp_finish_top(const LpArgs& A, int row, float m,
     }
 }
 
-// What bounds it: many rows memory (8192 of 50257 in bf16, 823 MB: 160 us, 5.1 TB/s), with the instructions for 16 exponentials a chunk close behind; few rows the latencies of one workgroup (a row
+// What bounds it: many rows memory (8192 of 50257 in bf16, 823 MB: 155 us, 5.3 TB/s), with the instructions for 16 exponentials a chunk close behind (162 with a maximum over the wave for every chunk); few rows the latencies of one workgroup (a row
 // of 8192 in fp32, five tokens: 6 us, of which the launch is 2).  Workgroups of 512 and 1024 threads were no faster: a compute unit takes 0.1 us for 1000 elements however they are dealt.
 // Rows in parts: 64 of 131075 in bf16 16 us, of which the parts take 7.5 and the join 8.4, a row alone 3.8 and 6.9: the join waits for memory three times (ranks, groups, given tokens' logits) and for
 // its own code.  Parts that picked their own top tokens took 14 + 5 us; joined by the last part to end, counted by atomics, 25 to 52.
@@ -375,7 +375,9 @@ __global__ void __launch_bounds__(LP_WG, sizeof(T) == 4 ? 5 : 6) k_logprobs(LpAr
         uint32_t* const ranks = KIND == LP_PARTLY ? lp_ranks(A, row) + first / (LP_UNIT / V) * LP_WG + t : nullptr;
         float m = -INFINITY, ent = 0.f; // m: the wave's
         double s = 0.0;
-        uint32_t mine = 0, grp = 0;
+        uint32_t mine = 0;
+        float grp = -INFINITY; // a group's largest, and whether it has any
+        bool some = false;
         for (int j = 0; j < chunks; j++) {
             const int g0 = first + j * LP_WG * U;
             kv_u32x4 v[U];
@@ -402,17 +404,24 @@ __global__ void __launch_bounds__(LP_WG, sizeof(T) == 4 ? 5 : 6) k_logprobs(LpAr
             for (int i = 1; i < LP_CHUNK; i++) c = fmaxf(c, x[i]);
             if (!(c > -INFINITY)) c = -INFINITY; // (NaN alone)
             if (KIND != LP_SUMS) {
-                grp = max(j & 1 ? grp : 0u, any ? lp_rank(c) : 0u);
-                if (KIND == LP_WHOLE) mine = max(mine, grp);
+                grp = j & 1 ? fmaxf(grp, c) : c;
+                some = any || (j & 1 && some);
                 if (j & 1 || j + 1 == chunks) {
-                    if (KIND == LP_WHOLE) sh.group[j / 2][t] = grp;
-                    else ranks[j / 2 * LP_WG] = grp;
+                    const uint32_t rank = some ? lp_rank(grp) : 0u;
+                    if (KIND == LP_WHOLE) {
+                        sh.group[j / 2][t] = rank;
+                        mine = max(mine, rank);
+                    } else
+                        ranks[j / 2 * LP_WG] = rank;
                 }
             }
-            const float cw = lp_wave_max(c);
-            if (cw > m) lp_scale(m, s, ent, cw, A.scale); // (seldom)
+            const bool less = __ballot(c >= m) == 0; // (most often)
+            if (!less) {
+                const float cw = lp_wave_max(c);
+                if (cw > m) lp_scale(m, s, ent, cw, A.scale);
+            }
             const float from = m > -INFINITY ? m : 0.f;
-            if (cw < m) {
+            if (less) {
                 float e4[2] = {}, t4[2] = {};
 #pragma unroll
                 for (int i = 0; i < LP_CHUNK; i++) {
