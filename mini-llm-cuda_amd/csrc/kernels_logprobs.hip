@@ -476,46 +476,43 @@ __global__ void __launch_bounds__(LP_WG) k_logprobs_join(LpArgs A) {
     __shared__ LpTops<1> sh;
     __shared__ double logz;
     __shared__ float rowMax;
-    const int t = threadIdx.x, lane = t & 63;
+    const int t = threadIdx.x, lane = t & 63, row = blockIdx.x;
     const bool last = t >= LP_WG - 64; // the wave that takes the sums, while the first ranks
-    for (int row = blockIdx.x; row < A.rows; row += gridDim.x) {
-        float given = 0.f;
-        int token = -1;
-        LpSums mine = {0.0, -INFINITY, 0.f};
-        if (last && lane < A.given) {
-            token = A.tokens[(size_t)row * A.given + lane];
-            if (token >= 0 && token < A.vocab) given = lp_get((const T*)A.logits + (size_t)row * A.stride + token);
-        }
-        if (last && lane < A.parts) mine = reinterpret_cast<const LpSums*>(A.work)[(size_t)row * A.parts + lane];
-        if (TOP) {
-            constexpr int V = LpType<T>::V;
-            const LpRow R = lp_row<T>(A, row);
-            const int groups = (R.granules + LP_UNIT / V - 1) / (LP_UNIT / V);
-            const uint32_t* ranks = lp_ranks(A, row);
-            uint32_t most = 0;
-            for (int at = t * 4; at < groups * LP_WG; at += LP_WG * 32) {
-                kv_u32x4 r[8];
+    float given = 0.f;
+    int token = -1;
+    LpSums mine = {0.0, -INFINITY, 0.f};
+    if (last && lane < A.given) {
+        token = A.tokens[(size_t)row * A.given + lane];
+        if (token >= 0 && token < A.vocab) given = lp_get((const T*)A.logits + (size_t)row * A.stride + token);
+    }
+    if (last && lane < A.parts) mine = reinterpret_cast<const LpSums*>(A.work)[(size_t)row * A.parts + lane];
+    if (TOP) {
+        constexpr int V = LpType<T>::V;
+        const LpRow R = lp_row<T>(A, row);
+        const int groups = (R.granules + LP_UNIT / V - 1) / (LP_UNIT / V);
+        const uint32_t* ranks = lp_ranks(A, row);
+        uint32_t most = 0;
+        for (int at = t * 4; at < groups * LP_WG; at += LP_WG * 32) {
+            kv_u32x4 r[8];
 #pragma unroll
-                for (int j = 0; j < 8; j++) r[j] = *reinterpret_cast<const kv_u32x4*>(ranks + min(at + j * LP_WG * 4, groups * LP_WG - 4));
+            for (int j = 0; j < 8; j++) r[j] = *reinterpret_cast<const kv_u32x4*>(ranks + min(at + j * LP_WG * 4, groups * LP_WG - 4));
 #pragma unroll
-                for (int j = 0; j < 8; j++)
+            for (int j = 0; j < 8; j++)
 #pragma unroll
-                    for (int e = 0; e < 4; e++) most = max(most, at + j * LP_WG * 4 < groups * LP_WG ? r[j][e] : 0u);
-            }
-            lp_tops<T, true>(sh, R, groups, ranks, most, A.top);
+                for (int e = 0; e < 4; e++) most = max(most, at + j * LP_WG * 4 < groups * LP_WG ? r[j][e] : 0u);
         }
-        if (last) {
-            const float m = lp_wave_max(mine.m);
-            lp_scale(mine.m, mine.s, mine.t, m, A.scale);
-            const double s = __shfl(lp_wave_sum(mine.s), 63, 64);
-            const double z = lp_finish(A, row, m, s, lp_last(lp_wave_sum(mine.t)), token, given);
-            if (lane == 0) { rowMax = m; logz = z; }
-        }
-        if (TOP) {
-            __syncthreads();
-            lp_finish_top(A, row, rowMax, logz, sh.best);
-            if (row + (int)gridDim.x < A.rows) __syncthreads();
-        }
+        lp_tops<T, true>(sh, R, groups, ranks, most, A.top);
+    }
+    if (last) {
+        const float m = lp_wave_max(mine.m);
+        lp_scale(mine.m, mine.s, mine.t, m, A.scale);
+        const double s = __shfl(lp_wave_sum(mine.s), 63, 64);
+        const double z = lp_finish(A, row, m, s, lp_last(lp_wave_sum(mine.t)), token, given);
+        if (lane == 0) { rowMax = m; logz = z; }
+    }
+    if (TOP) {
+        __syncthreads();
+        lp_finish_top(A, row, rowMax, logz, sh.best);
     }
 }
 
@@ -559,7 +556,7 @@ extern "C" uint64_t mlh_logprobs_work_bytes(const mlh_logprobs* a) {
 }
 
 template <typename T> static int lp_go(const LpArgs& A, bool join, void* stream) {
-    const dim3 grid((unsigned)std::min<long long>((long long)A.rows * A.parts, 1 << 22)), rows((unsigned)std::min(A.rows, 1 << 22));
+    const dim3 grid((unsigned)std::min<long long>((long long)A.rows * A.parts, 1 << 22)), rows((unsigned)A.rows);
     const int rc = kv_launch(!A.top ? &k_logprobs<T, LP_SUMS> : join ? &k_logprobs<T, LP_PARTLY> : &k_logprobs<T, LP_WHOLE>, grid, LP_WG, 0, stream, A);
     if (rc || !join) return rc;
     return kv_launch(A.top ? &k_logprobs_join<T, true> : &k_logprobs_join<T, false>, rows, LP_WG, 0, stream, A);

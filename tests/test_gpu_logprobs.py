@@ -230,3 +230,34 @@ def test_two_calls_at_once(pkg, rows, vocab):
             pkg.logprobs(c.args, s.cuda_stream)
     for c in calls:
         c.check()
+
+
+def test_more_rows_than_workgroups(pkg):
+    rows = (1 << 22) + 77
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.randn(rows, 2, device="cuda", generator=gen) * 3
+    tok = torch.randint(0, 2, (rows, 1), device="cuda", dtype=torch.int32, generator=gen)
+    lp, ent, ids, tlp = torch.zeros(rows, 1, device="cuda"), torch.zeros(rows, device="cuda"), torch.zeros(rows, 1, dtype=torch.int32, device="cuda"), torch.zeros(rows, 1, device="cuda")
+    pkg.logprobs(pkg.LogProbs(logits=x.data_ptr(), stride=2, tokens=tok.data_ptr(), logProb=lp.data_ptr(), entropy=ent.data_ptr(), topIds=ids.data_ptr(), topLogProb=tlp.data_ptr(), rows=rows,
+                              vocab=2, type=pkg.DTYPE_F32, given=1, top=1))
+    torch.cuda.synchronize()
+    d = (x[:, 1] - x[:, 0]).double()
+    p = torch.stack([-torch.nn.functional.softplus(d, threshold=100), -torch.nn.functional.softplus(-d, threshold=100)], 1)
+    close = lambda got, want: float(((got.double() - want).abs() / (1e-3 + want.abs())).max()) < 1e-6  # (the exponent and the exponential: a few 2^-24 of them)
+    assert close(lp[:, 0], p.gather(1, tok.long())[:, 0]) and close(ent, -(p.exp() * p).sum(1))
+    assert torch.equal(ids[:, 0], (x[:, 1] > x[:, 0]).int()) and close(tlp[:, 0], p.max(1).values)
+
+
+@pytest.mark.parametrize("vocab,top", [(1000, 5), (140003, 20)])
+def test_far_offsets(pkg, vocab, top):
+    """Rows 2^25 + 1 elements apart: the last one behind 2^31 elements."""
+    if torch.cuda.mem_get_info()[0] < 24 << 30:
+        pytest.skip("needs 24 GiB")
+    rows, stride = 70, (1 << 25) + 1
+    x, gen = logits("bf16", rows, vocab, 77)
+    c = Call(pkg, x, torch.randint(0, vocab, (rows, 2), generator=gen), top)
+    buf = torch.empty(rows * stride, dtype=torch.bfloat16, device="cuda")
+    buf.view(rows, stride)[:, :vocab] = x.cuda()
+    c.args.logits, c.args.stride = buf.data_ptr(), stride
+    pkg.logprobs(c.args)
+    c.check()

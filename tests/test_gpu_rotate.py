@@ -141,3 +141,27 @@ def test_on_a_stream_and_in_a_graph(pkg):
         other = Call(pkg, "f16", 3, 1, 1, 64, 64, False, [1, 2, 3], pkg.rope_frequencies(64), seed=i)
         pkg.rotate(other.args)
         other.check("between")
+
+
+def test_more_rows_than_workgroups_and_far_offsets(pkg):
+    """2^20 + 3 rows of which each fills a workgroup, 2^32 elements from the first to the last; two elements of 512 are turned."""
+    rows, hd, stride = (1 << 20) + 3, 512, 4096
+    free = torch.cuda.mem_get_info()[0]
+    if free < 24 << 30:
+        pytest.skip("needs 24 GiB")
+    buf = torch.empty(rows * stride, dtype=torch.bfloat16, device="cuda").view(rows, stride)
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    buf[:, :hd + 1] = torch.randn(rows, hd + 1, generator=gen, device="cuda").to(torch.bfloat16)
+    out = torch.zeros(rows, hd, dtype=torch.bfloat16, device="cuda")
+    pos = torch.randint(0, 1000, (rows,), generator=gen, device="cuda", dtype=torch.int32)
+    freq = torch.tensor([0.37], dtype=torch.float64, device="cuda")
+    pkg.rotate(pkg.Rotate(q=buf.data_ptr(), qStride=stride, qOut=out.data_ptr(), qOutStride=hd, pos=pos.data_ptr(), freq=freq.data_ptr(), rows=rows, type=pkg.DTYPE_BF16, heads=1,
+                          headDim=hd, rotated=2, layout=pkg.ROTATE_PAIRS))
+    torch.cuda.synchronize()
+    assert torch.equal(out[:, 2:], buf[:, 2:hd])
+    some = torch.cat([torch.arange(0, 3000), torch.arange(rows - 3000, rows), torch.arange(0, rows, 4001)])
+    want, bound = so.turned(buf[some.cuda(), :hd].cpu().double()[:, None], pos[some.cuda()].cpu(), freq.cpu(), 2, False, 1.0, "bf16")
+    so.close(out[some.cuda()].cpu()[:, None], want, bound, "rows far apart")
+    angle = pos.double() * 0.37
+    a, b = buf[:, 0].double(), buf[:, 1].double()
+    assert float((out[:, 0].double() - (angle.cos() * a - angle.sin() * b)).abs().max()) < 2.0 ** -8 * float((a * a + b * b).sqrt().max()) + 1e-5

@@ -253,3 +253,30 @@ def test_laid_out_and_read_at_large_sizes(pkg, n, k, group):
     pkg.weights4_read(again, pkg.DTYPE_F32, out.data_ptr(), k)
     torch.cuda.synchronize()
     assert torch.equal(out[:n].cpu(), so.values4(c2, p2, group).float()) and bool((other[-64:] == 255).all())
+
+
+def test_a_matrix_beyond_32_bit_offsets(pkg):
+    """3.6 GB of codes: laid out, multiplied, read back; rows from all over it against the definition."""
+    if torch.cuda.mem_get_info()[0] < 24 << 30:
+        pytest.skip("needs 24 GiB")
+    n, k, group, m = 110000, 1 << 16, 128, 3
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    codes = torch.randint(0, 256, (n, k // 2), dtype=torch.uint8, device="cuda", generator=gen)
+    params = (torch.rand(n, k // group, 2, device="cuda", generator=gen) * 0.02 - 0.01).half()
+    params[..., 1] = params[..., 1].abs()
+    w, data = matrix(pkg, n, k, group)
+    assert pkg.weights4_bytes(n, k, group) > 1 << 31
+    pkg.weights4_set(w, codes.data_ptr(), params.data_ptr())
+    some = torch.cat([torch.arange(0, 40), torch.arange(60000, 60020), torch.arange(n - 40, n)])
+    packed = codes[some.cuda()].cpu().to(torch.int32)
+    c = torch.stack([packed & 15, packed >> 4], -1).flatten(1)
+    p = params[some.cuda()].cpu()
+    for kind, rows in (("bf16", m), ("f16", 20), ("f32", 5)):
+        t = so.TORCH[kind]
+        a = torch.randn(rows, k, device="cuda", generator=gen).to(t)
+        out = torch.zeros(rows, n, dtype=t, device="cuda")
+        pkg.gemm4(w, pkg.Gemm4(a=a.data_ptr(), aStride=k, c=out.data_ptr(), cStride=n, M=rows, type=so.code_of(pkg, kind)))
+        torch.cuda.synchronize()
+        want, bound = so.product4(a.cpu().double(), c, p, group, kind)
+        so.close(out[:, some.cuda()].cpu(), want, bound, kind)
+    assert bool((data[-64:] == 255).all())
