@@ -635,10 +635,11 @@ template <typename T, int G, int MT, int WN, int WK, int NT, int TPW, int AHEAD,
     return kv_launch(&k_gemm4_many<T, G, MT, WN, WK, NT, TPW, AHEAD, LOADERS>, dim3(grid, (A.M + rows - 1) / rows), (W4_WAVES + LOADERS) * 64, lds, stream, A);
 }
 
-// A workgroup's share of a product of more than eight rows: rows of A times 16-row bands of W, and what a round of such workgroups, one a compute unit, takes (tenths of a us at N 2048, K 8192, fp32 or
-// fp16, groups of 64).  Large shares read A and W less often, small ones fill the chip when there are few: taken is the share whose rounds take least, the fastest or within 6 % of it for 9 to 64
+// A workgroup's share of a product of more than four rows: rows of A times 16-row bands of W, and what a round of such workgroups, one a compute unit, takes (tenths of a us at N 2048, K 8192, fp32 or
+// fp16, groups of 64).  Large shares read A and W less often, small ones fill the chip when there are few: taken is the share whose rounds take least, the fastest or within 6 % of it for 5 to 64
 // rows of 48 to 2000 bands.  For instance, us with the share taken / the next ones, fp16, K 4096: 64 rows, 256 bands 16 x 4 8.8 / 32 x 4 10.9, 16 x 8 11.8; 1024 bands 32 x 8 18.6 / 32 x 4 25.4, 64 x 8 26.8;
-// 1280 bands 64 x 8 27.4 / 32 x 8 31.9; 32 rows, 1024 bands 32 x 4 14.9 / 16 x 8 15.2, 32 x 8 18.0; 16 rows, 256 bands 16 x 1 5.6 / 16 x 2 7.0, 16 x 4 8.1; fp32: 64 rows, 256 bands 16 x 4 13.4 / 16 x 8 17.5,
+// 1280 bands 64 x 8 27.4 / 32 x 8 31.9; 32 rows, 1024 bands 32 x 4 14.9 / 16 x 8 15.2, 32 x 8 18.0; 16 rows, 256 bands 16 x 1 5.6 / 16 x 2 7.0, 16 x 4 8.1; fp32: 8 rows, 256 bands 8 x 1 7.7 / 8 x 2 9.1,
+// 16 x 2 10.7; 64 rows, 256 bands 16 x 4 13.4 / 16 x 8 17.5,
 // 16 x 2 20.0, 32 x 8 26.3.  (64 x 4 takes longer than 32 x 8 everywhere: 21.1 for 18.6.)
 struct W4Share { int rows, bands, us; };
 static int w4_share(const W4Share* s, int n, int M, int bands) {
@@ -651,32 +652,34 @@ static int w4_share(const W4Share* s, int n, int M, int bands) {
     return best;
 }
 
-// Up to eight rows all of A is a wave's; with many bands of W a workgroup takes several, for fewer starts.  Microseconds by events around graph replays, fp16, groups of 64 unless said:
-//   M 1:  256 bands, K 4096 4.5 with eight waves a band, 7.6 with four of two and two; 1792, K 8192, groups of 32 27.6 / 30.1; 2000, K 2048 11.9 / 10.3; fp32 the same three 6.0 / 11.3, 43.6 / 38.4, 18.7 / 11.8
-//   M 8:  256 bands, K 4096 5.2 with eight waves of a band, 6.2 of two; M 5, 512, K 28672 37 / 32; 1792, K 8192 37.7 / 31.2, four of two and two 31.8
+// Up to four rows a band is a workgroup's eight waves; four bands where there are many and their last round over the compute units is not mostly empty: fewer starts, but fewer codes on their way, which
+// counts with long K of 16-bit types.  Us, one band / four, fp16, groups of 32: 1024 bands, K 4096 10.6 / 10.8; 1280, K 4096 13.2 / 15.5; 1792, K 8192 29.8 / 30.7; 2000, K 2048 11.2 / 10.5; 256, K 4096
+// 4.7 / 8.1; fp32 the same five 15.6 / 14.2, 19.0 / 20.0, 44.7 / 39.7, 19.2 / 13.5, 6.2 / 11.8.
 template <typename T, int G> static int gemm4_go(const Gemm4Args& A, void* stream) {
     constexpr bool f32 = sizeof(T) == 4;
     const int bands = (A.N + W4_ROWS - 1) / W4_ROWS;
-    if (A.M <= 4) return bands >= 1024 && (f32 || A.K <= 4096) ? gemm4_few<T, G, 1, 2, 4, 2, 2>(A, stream) : gemm4_few<T, G, 1, 1, 8, 1, 2>(A, stream);
-    if (A.M <= 8) return bands >= 1024 ? gemm4_few<T, G, 2, 2, 4, 2, 2>(A, stream) : bands >= 512 ? gemm4_few<T, G, 2, 1, 8, 2, 2>(A, stream) : gemm4_few<T, G, 2, 1, 8, 1, 2>(A, stream);
+    if (A.M <= 4) return bands >= 1024 && bands >= (bands + 1023) / 1024 * 768 && (f32 || A.K <= 4096) ? gemm4_few<T, G, 1, 2, 4, 2, 2>(A, stream) : gemm4_few<T, G, 1, 1, 8, 1, 2>(A, stream);
     if constexpr (f32) {
-        static const W4Share shares[] = {{8, 1, 127}, {16, 2, 174}, {16, 4, 209}, {16, 8, 304}, {32, 8, 488}};
-        switch (w4_share(shares, 5, A.M, bands)) {
+        static const W4Share shares[] = {{8, 1, 120}, {8, 2, 141}, {16, 2, 174}, {16, 4, 209}, {16, 8, 304}, {32, 8, 488}};
+        switch (w4_share(shares, 6, A.M, bands)) {
         case 0: return gemm4_few<T, G, 2, 1, 8, 1, 2>(A, stream);
-        case 1: return gemm4_many<T, G, 1, 2, 4, 1, 1, 2, 8>(A, stream);
-        case 2: return gemm4_many<T, G, 1, 2, 4, 2, 1, 2, 8>(A, stream);
-        case 3: return gemm4_many<T, G, 1, 4, 2, 2, 2, 1, 4>(A, stream);
+        case 1: return gemm4_few<T, G, 2, 1, 8, 2, 2>(A, stream);
+        case 2: return gemm4_many<T, G, 1, 2, 4, 1, 1, 2, 8>(A, stream);
+        case 3: return gemm4_many<T, G, 1, 2, 4, 2, 1, 2, 8>(A, stream);
+        case 4: return gemm4_many<T, G, 1, 4, 2, 2, 2, 1, 4>(A, stream);
         default: return gemm4_many<T, G, 2, 4, 2, 2, 1, 1, 8>(A, stream);
         }
     } else {
-        static const W4Share shares[] = {{16, 1, 80}, {16, 2, 103}, {16, 4, 124}, {16, 8, 192}, {32, 4, 171}, {32, 8, 264}, {64, 8, 406}};
-        switch (w4_share(shares, 7, A.M, bands)) {
-        case 0: return gemm4_few<T, G, 4, 1, 8, 1, 2>(A, stream);
-        case 1: return gemm4_few<T, G, 4, 1, 8, 2, 2>(A, stream);
-        case 2: return gemm4_many<T, G, 1, 2, 4, 2, 2, 1, 8>(A, stream);
-        case 3: return gemm4_many<T, G, 1, 4, 2, 2, 2, 2, G == 64 ? 8 : 4>(A, stream);
-        case 4: return gemm4_many<T, G, 2, 2, 4, 2, 2, 1, 8>(A, stream);
-        case 5: return gemm4_many<T, G, 2, 4, 2, 2, 2, 1, 4>(A, stream);
+        static const W4Share shares[] = {{8, 1, 77}, {8, 2, 94}, {16, 1, 80}, {16, 2, 103}, {16, 4, 124}, {16, 8, 192}, {32, 4, 171}, {32, 8, 264}, {64, 8, 406}};
+        switch (w4_share(shares, 9, A.M, bands)) {
+        case 0: return gemm4_few<T, G, 2, 1, 8, 1, 2>(A, stream);
+        case 1: return gemm4_few<T, G, 2, 1, 8, 2, 2>(A, stream);
+        case 2: return gemm4_few<T, G, 4, 1, 8, 1, 2>(A, stream);
+        case 3: return gemm4_few<T, G, 4, 1, 8, 2, 2>(A, stream);
+        case 4: return gemm4_many<T, G, 1, 2, 4, 2, 2, 1, 8>(A, stream);
+        case 5: return gemm4_many<T, G, 1, 4, 2, 2, 2, 2, G == 64 ? 8 : 4>(A, stream);
+        case 6: return gemm4_many<T, G, 2, 2, 4, 2, 2, 1, 8>(A, stream);
+        case 7: return gemm4_many<T, G, 2, 4, 2, 2, 2, 1, 4>(A, stream);
         default: return gemm4_many<T, G, 4, 4, 2, 2, 2, 1, 4>(A, stream);
         }
     }

@@ -216,7 +216,7 @@ def test_on_a_stream_and_in_a_graph(pkg, m, kind):
 
 
 @pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
-@pytest.mark.parametrize("n,k,group", [(4500, 416, 64), (6201, 1056, 32), (8190, 160, 128), (8193, 736, 64), (16383, 1184, 128), (16400, 288, 32), (20481, 416, 64)])
+@pytest.mark.parametrize("n,k,group", [(3001, 736, 128), (1030, 544, 32), (4500, 416, 64), (6201, 1056, 32), (8190, 160, 128), (8193, 736, 64), (16383, 1184, 128), (16400, 288, 32), (20481, 416, 64)])
 def test_every_way_that_waves_are_dealt(pkg, kind, n, k, group):
     """Rows of A and bands of W on both sides of every bound that chooses a kernel or its shape."""
     weights = set_from(pkg, n, k, group, n)
