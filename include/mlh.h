@@ -528,8 +528,9 @@ int mlh_gemm4_device(const mlh_weights4* w, const mlh_gemm4* args, void* stream)
 
 /* What rows of logits say: with p = softmax(logits / temperature) of a row, logProb = log p of `given` tokens of the caller's, entropy = -sum p log p (an element of p = 0 adds 0),
  * and the `top` most likely tokens, most likely first and of equal logits the lower id first, with their log p (inference_orchestrator.cu:68-84 sorts the probabilities of a row on the host).
- * Sums of exponentials are in 64 bits, the largest logit is their 1, so that log p of a token that is nearly certain keeps its digits down to 2^-40; results are rounded to fp32.  A masked token is a logit of -infinity: its
- * log p is -infinity.  A row with NaN or +infinity in it, or with nothing but -infinity, has no distribution: all its log probabilities and its entropy are NaN (its top tokens are those of
+ * An exponential is fp32, off by (3 |d| + 4) 2^-24 of itself at d = (x - largest) / temperature; sixteen of a thread's are added up in fp32 and those sums in 64 bits (the entropy's, sum p d, in 64 bits after at
+ * most 512 elements of a thread in fp32), whatever the length of a row.  The largest logit is the sums' 1, so that log p of a token that is nearly certain keeps its digits down to 2^-40; results are rounded to fp32.
+ * A masked token is a logit of -infinity: its log p is -infinity.  A row with NaN or +infinity in it, or with nothing but -infinity, has no distribution: all its log probabilities and its entropy are NaN (its top tokens are those of
  * the largest logits, NaN as -infinity).  A given token below 0 asks for nothing: its log p is 0; one of vocab or more is NaN.
  * Rows `stride` elements apart, aligned to their elements (odd vocabularies; 16-byte aligned rows are read faster).  tokens and logProb [rows, given], entropy [rows] (may be null), topIds and topLogProb [rows, top].
  * work: mlh_logprobs_work_bytes() bytes (of the same structure; 0: none), 16-byte aligned, undefined before and after, not shared by calls that may overlap.  As the

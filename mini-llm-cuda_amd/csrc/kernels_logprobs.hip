@@ -14,6 +14,7 @@
 #define LP_WG 256
 #define LP_WAVES (LP_WG / 64)
 #define LP_CHUNK 16                            // elements a thread takes at once
+#define LP_FLUSH 8                             // chunks whose share of the entropy's sum is one in fp32
 #define LP_GROUP 32                            // ... and whose largest it notes
 #define LP_UNIT (LP_WG * LP_GROUP)             // elements of which every thread has a group; parts are whole units
 #define LP_GROUPS 16                           // groups of a thread, at most, where one workgroup has a row
@@ -64,14 +65,14 @@ __device__ __forceinline__ float lp_value(uint64_t key) {
     return __uint_as_float((r & 0x80000000u) ? r & 0x7fffffffu : ~r);
 }
 
-// (m, s, t) as seen from a maximum `to` that is not smaller.  Nothing seen: m is -infinity and s and t are 0.
-__device__ __forceinline__ void lp_scale(float& m, double& s, float& t, float to, float scale) {
-    if (m < to) {
-        const float d = fmaxf((m - to) * scale, -1e4f), f = __builtin_amdgcn_exp2f(d); // (2^-1e4 is 0; an infinity would make NaN of 0)
-        t = f * fmaf((float)s, d, t);
-        s *= f;
-        m = to;
-    }
+// (m, s, t) as seen from a maximum `to` that is not smaller; the factor.  Nothing seen: m is -infinity and s and t are 0.
+template <typename E> __device__ __forceinline__ float lp_scale(float& m, double& s, E& t, float to, float scale) {
+    if (!(m < to)) return 1.f;
+    const float d = fmaxf((m - to) * scale, -1e4f), f = __builtin_amdgcn_exp2f(d); // (2^-1e4 is 0; an infinity would make NaN of 0)
+    t = f * fma((E)s, (E)d, t);
+    s *= f;
+    m = to;
+    return f;
 }
 
 // A row's granules of 16 bytes; the first and the last may hold elements of other rows.
@@ -374,7 +375,8 @@ __global__ void __launch_bounds__(LP_WG, sizeof(T) == 4 ? 5 : 6) k_logprobs(LpAr
         }
         uint32_t* const ranks = KIND == LP_PARTLY ? lp_ranks(A, row) + first / (LP_UNIT / V) * LP_WG + t : nullptr;
         float m = -INFINITY, ent = 0.f; // m: the wave's
-        double s = 0.0;
+        // ent's sum of the chunks before the last LP_FLUSH, where there can be more (up to 1024: of equal logits all would be rounded the same way)
+        double s = 0.0, before = 0.0;
         uint32_t mine = 0;
         float grp = -INFINITY; // a group's largest, and whether it has any
         bool some = false;
@@ -418,7 +420,10 @@ __global__ void __launch_bounds__(LP_WG, sizeof(T) == 4 ? 5 : 6) k_logprobs(LpAr
             const bool less = __ballot(c >= m) == 0; // (most often)
             if (!less) {
                 const float cw = lp_wave_max(c);
-                if (cw > m) lp_scale(m, s, ent, cw, A.scale);
+                if (cw > m) {
+                    if (KIND == LP_WHOLE) lp_scale(m, s, ent, cw, A.scale);
+                    else ent *= lp_scale(m, s, before, cw, A.scale);
+                }
             }
             const float from = m > -INFINITY ? m : 0.f;
             if (less) {
@@ -439,9 +444,13 @@ __global__ void __launch_bounds__(LP_WG, sizeof(T) == 4 ? 5 : 6) k_logprobs(LpAr
                     ent = fmaf(e, fmaxf(d, -1e4f), ent);
                 }
             }
+            if (KIND != LP_WHOLE && j % LP_FLUSH == LP_FLUSH - 1) {
+                before += (double)ent;
+                ent = 0.f;
+            }
         }
         s = lp_wave_sum(s);
-        ent = lp_wave_sum(ent);
+        ent = lp_wave_sum(KIND == LP_WHOLE ? ent : (float)(before + (double)ent));
         if (lane == 63) of[wave] = LpSums{s, m, ent};
         if (KIND == LP_WHOLE) lp_tops<T, false>(sh, R, (chunks + 1) / 2, &sh.group[0][0], mine, A.top); // (with the barrier that the sums need)
         else __syncthreads();

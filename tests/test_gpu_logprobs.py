@@ -261,3 +261,34 @@ def test_far_offsets(pkg, vocab, top):
     c.args.logits, c.args.stride = buf.data_ptr(), stride
     pkg.logprobs(c.args)
     c.check()
+
+
+@pytest.mark.parametrize("kind,rows,top", [("bf16", 129, 0), ("f32", 129, 0), ("f16", 129, 0), ("bf16", 1030, 1)])
+def test_entropy_of_equal_logits_does_not_drift(pkg, kind, rows, top):
+    """Rows of 2^22 tokens that one workgroup has alone: eight tokens at 0, of which each wave meets one at its start, every other one at a distance below them
+    that differs from row to row (8 to 16; such sums are all rounded the same way).
+
+    Bound, with p the share of the others and d their logarithm: an exponential is off by (3 |d| + 4) 2^-24 of itself (as in the oracle), a product with its exponent by 3 more, the sums of
+    sixteen by 9, of eight of those (the entropy's) by 8, and what is joined behind them in pairs (the threads of a wave) by 6; the entropy's own rounding."""
+    vocab = 1 << 22
+    if torch.cuda.mem_get_info()[0] < 2 * rows * vocab * 4:
+        pytest.skip("needs twice the logits' memory")
+    d = -(128 + torch.arange(rows, dtype=torch.float64) % 129) / 16  # (exact in every type)
+    x = d.to(so.TORCH[kind]).cuda()[:, None].repeat(1, vocab)
+    x[:, :2048:256] = 0
+    ent, ids, tlp = torch.full((rows,), 55.0, device="cuda"), torch.zeros(rows, 1, dtype=torch.int32, device="cuda"), torch.zeros(rows, 1, device="cuda")
+    a = pkg.LogProbs(logits=x.data_ptr(), stride=vocab, entropy=ent.data_ptr(), rows=rows, vocab=vocab, type=so.code_of(pkg, kind), top=top, topIds=ids.data_ptr(), topLogProb=tlp.data_ptr())
+    size = pkg.logprobs_work_bytes(a)
+    work = torch.zeros(max(size, 16), dtype=torch.uint8, device="cuda")
+    a.work, a.workBytes = work.data_ptr(), size
+    pkg.logprobs(a)
+    torch.cuda.synchronize()
+    others = (vocab - 8) * torch.exp(d)
+    logz, p = torch.log(8 + others), others / (8 + others)
+    want = logz - p * d
+    dz = p * (3 * d.abs() + 4 + 9 + 6) * 2.0 ** -24
+    bound = 2.0 ** -24 * want + dz * (1 + want) + p * d.abs() * (3 * d.abs() + 4 + 3 + 9 + 8 + 6) * 2.0 ** -24
+    so.close(ent.cpu(), want, bound, "entropy")
+    if top:
+        assert not bool(ids.any())
+        so.close(tlp[:, 0].cpu(), -logz, 2.0 ** -24 * logz + dz, "top")
