@@ -165,7 +165,7 @@ int mlh_forward_full(mlh_ctx* ctx, int seq, const int32_t* ids, int n, float* lo
 /* The same forward for callers that want to know how likely a text is: per position i of the n tokens, logProb[i] = log p(ids[i + 1] | everything up to ids[i]) (0 for the last one, which has
  * no next token here), the entropy of that distribution, and its `top` (0 to 64) most likely tokens with their log p, [n, top], as mlh_logprobs_device defines them; temperature 0: 1.  logProb
  * and entropy may be null.  The logits stay on the device: of a text of 517 tokens and 20160 words 42 MB that mlh_forward_full would bring to the host.  Its work buffers
- * are that call's.  (The reference copies the probabilities of all columns to the host and sorts the last one there, inference_orchestrator.cu:68-84.) */
+ * are that call's.  Vocabularies up to 2^22 tokens; a refused call (-1) leaves the sequence as it was.  (The reference copies the probabilities of all columns to the host and sorts the last one there, inference_orchestrator.cu:68-84.) */
 int mlh_score(mlh_ctx* ctx, int seq, const int32_t* ids, int n, int top, float temperature, float* logProb, float* entropy, int32_t* topIds, float* topLogProb);
 
 /* 0 (default): MFMA products when the call has two or more tokens and dim, ffnDim,

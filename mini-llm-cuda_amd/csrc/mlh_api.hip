@@ -580,8 +580,6 @@ extern "C" int mlh_prefill(mlh_ctx* c, int seq, const int32_t* ids, int n) {
     return mlh_prefill_batch(c, 1, &seq, ids, &n);
 }
 
-// Teacher-forced forward over n tokens appended to `seq`: what runInference(L) leaves in vocabScores_DEVICE and
-// vocabScores_postSoftmax_DEVICE for all L columns (inference.cu:723-749), plus the mean next-token cross-entropy.
 // What mlh_forward_full and mlh_score ask of their input
 static int check_full(mlh_ctx* c, int seq, const int32_t* ids, int n) {
     int rc = check_ready(c);
@@ -628,6 +626,8 @@ static int full_logits(mlh_ctx* c, int seq, const int32_t* ids, int n, float* dL
     return rc;
 }
 
+// Teacher-forced forward over n tokens appended to `seq`: what runInference(L) leaves in vocabScores_DEVICE and
+// vocabScores_postSoftmax_DEVICE for all L columns (inference.cu:723-749), plus the mean next-token cross-entropy.
 extern "C" int mlh_forward_full(mlh_ctx* c, int seq, const int32_t* ids, int n, float* logitsOut, float* probsOut, float* meanNll) {
     int rc = check_full(c, seq, ids, n);
     if (rc) return rc;
@@ -666,9 +666,11 @@ extern "C" int mlh_forward_full(mlh_ctx* c, int seq, const int32_t* ids, int n, 
     return rc;
 }
 
+// The same forward with mlh_logprobs_device behind it.  What that would refuse is refused before the sequence grows.
 extern "C" int mlh_score(mlh_ctx* c, int seq, const int32_t* ids, int n, int top, float temperature, float* logProb, float* entropy, int32_t* topIds, float* topLogProb) {
     if (c && (top < 0 || top > 64 || (c->hp.vocabSize < top) || (top && (!topIds || !topLogProb)))) { c->err = "top must be 0 to 64, at most the vocabulary, with room for its results"; return -1; }
     if (c && temperature != 0.f && !(temperature >= 1e-4f && temperature <= 1e4f)) { c->err = "temperature must be 0 or 1e-4 to 1e4"; return -1; }
+    if (c && (c->hp.vocabSize > (1 << 22) || n > (1 << 24))) { c->err = "a vocabulary of more than 2^22 tokens, or more than 2^24 tokens at once"; return -1; }
     int rc = check_full(c, seq, ids, n);
     if (rc) return rc;
     // device results: logits, then per row its next token, log probability, entropy, best tokens and theirs; the operator's workspace

@@ -248,3 +248,13 @@ def test_score_refuses(pkg):
     assert pkg.dev.mlh_score(None, 0, ids.ctypes.data, 4, 0, 0.0, None, None, None, None) == -1
     assert pkg.dev.mlh_score(d._h, 0, ids.ctypes.data, 4, 0, 0.0, None, None, None, None) == 0 and d.seq_len(0) == 4
     d.close()
+
+
+def test_score_refuses_a_vocabulary_that_is_too_large_before_anything_else(pkg):
+    """Before the sequence is looked at, let alone appended to: also from a context that has no weights yet."""
+    hp = pkg.config(1, vocabSize=(1 << 22) + 1, dim=64, attnHeads=1, ffnDim=64, transformers=1, maxL=32)
+    d = pkg.Device(hp, 0)
+    with pytest.raises(pkg.MlhError, match="2\\^22"):
+        d.score(0, np.array([1, 2, 3], dtype=np.int32), 2)
+    assert d.seq_len(0) == 0
+    d.close()
