@@ -467,7 +467,7 @@ int mlh_attention_device(const mlh_kv_cache* cache, const mlh_kv_batch* batch, c
  * mlh_kv_append_device does not cover (inference.cu:113-134 has adjacent pairs of whole heads).  The first `rotated` elements of every head are pairs,
  * (2t, 2t + 1) with MLH_ROTATE_PAIRS and (t, t + rotated / 2) with MLH_ROTATE_HALVES; pair t of a row at position p becomes
  * amplitude * (c a - s b, s a + c b), c and s the cosine and sine of p * freq[t].  Elements behind them stay as they are.  Positions may be negative, which turns back:
- * rows read from a cache (mlh_kv_read_device) move to another place by the difference.  The angle is in 64 bits (off by 2^-52 of itself) and reduced there; with fp32 rows the
+ * rows read from a cache (mlh_kv_read_device) move to another place by the difference.  The angle is in 64 bits (off by less than 2^-52 of itself) and reduced there; with fp32 rows the
  * products are in 64 bits too, with rows of 16 bits cosine, sine and products are fp32.  Infinities and NaN stay in their pair.  freq: see mll_rope_frequencies.
  * Pointers 16-byte aligned (pos 4, freq 8), rows `stride` elements apart, strides multiples of 16 bytes.  qOut may be q with the same stride, kOut k likewise; rows must not overlap in any
  * other way.  k may be null (with kOut; kvHeads is not looked at then).  As the operators above: one launch on `stream`, no allocation, recordable, 0 / -1 / -2. */

@@ -46,7 +46,7 @@ template <bool NT, int V, typename T> __device__ __forceinline__ void rot_store(
     }
 }
 
-// A workgroup takes a few rows at a time: their cosines and sines once, into LDS, for all heads, then the heads.  The angle is counted in half turns, whose whole ones are taken off in 64 bits.
+// A workgroup takes a few rows at a time: their cosines and sines once, into LDS, for all heads, then the heads.  The angle is counted in half turns, of which sincospi takes the whole ones off exactly.
 // A piece is V elements of a head: with halves the two times V that are V pairs, with pairs V neighbours, or V elements behind the turned ones.
 // Bound by memory: 16384 rows of 32 + 8 heads of 128 in bf16, 336 MB read and written, 58 us (5.8 TB/s; a copy of 1 GiB 5.2), fp32 rows 63 us for as many bytes (5.3).  A single token 2.6 us, the latency
 // of position, angle and LDS in turn.  Rows at once: about as many as give every thread a piece; of 40 heads one, two and four 58, 62 and 65 us, of 3 heads one, four and eight 18, 11 and 9.5.
@@ -61,9 +61,10 @@ __global__ void __launch_bounds__(ROT_WG) k_rotate(RotateArgs A) {
         if (row0 != (int)blockIdx.x * A.rowsAtOnce) __syncthreads();
         for (int u = threadIdx.x; u < rows * half; u += ROT_WG) {
             const int t = u % half;
-            const double turns = (double)A.pos[row0 + u / half] * (A.freq[t] * 0.31830988618379067154);
+            // pos freq / pi, off by 0.78 2^-52 of itself: what freq / pi loses when it is rounded goes with it, 1 / pi as a double is off by 0.28 2^-52, the last rounding is half of 2^-52
+            const double pos = (double)A.pos[row0 + u / half], freq = A.freq[t], f = freq * 0.31830988618379067154, turns = fma(pos, f, pos * fma(freq, 0.31830988618379067154, -f));
             double s, c;
-            sincospi(turns - 2.0 * rint(turns * 0.5), &s, &c);
+            sincospi(turns, &s, &c);
             cs[2 * u] = (C)(c * A.amplitude);
             cs[2 * u + 1] = (C)(s * A.amplitude);
         }

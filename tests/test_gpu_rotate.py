@@ -1,5 +1,6 @@
 """mlh_rotate_device against its formula in 64 bits."""
 import math
+from decimal import Decimal, localcontext
 
 import numpy as np
 import pytest
@@ -165,3 +166,25 @@ def test_more_rows_than_workgroups_and_far_offsets(pkg):
     angle = pos.double() * 0.37
     a, b = buf[:, 0].double(), buf[:, 1].double()
     assert float((out[:, 0].double() - (angle.cos() * a - angle.sin() * b)).abs().max()) < 2.0 ** -8 * float((a * a + b * b).sqrt().max()) + 1e-5
+
+
+@pytest.mark.parametrize("fast", [1.0, 1e6])
+def test_how_far_off_a_far_angle_is(pkg, fast):
+    """Pairs (1, 0) become (cos, sin) of position times frequency as they stand, reduced with 60 digits; positions of 32 bits, frequencies up to `fast` times the usual ones.
+
+    Bound: 2^-52 of the angle, the rounding to fp32, and 2^-51 for cosine and sine in 64 bits and the oracle's own."""
+    pos = np.concatenate([[2 ** 31 - 1, -2 ** 31, 16777217, 1000003, -65537, 3], np.random.default_rng(5).integers(-2 ** 31, 2 ** 31, 1500)])
+    freq = pkg.rope_frequencies(64) * fast
+    c = Call(pkg, "f32", len(pos), 1, 0, 64, 64, True, pos, freq)
+    row = torch.zeros(len(pos), 64)
+    row[:, :32] = 1
+    c.buf["q"][:len(pos), :64] = row.cuda()
+    pkg.rotate(c.args)
+    torch.cuda.synchronize()
+    with localcontext() as digits:
+        digits.prec = 60
+        turn = 2 * Decimal("3.14159265358979323846264338327950288419716939937510582097494459")
+        angle = np.array([[float((Decimal(int(p)) * Decimal(float(f))).remainder_near(turn)) for f in freq] for p in pos])
+    want = torch.from_numpy(np.concatenate([np.cos(angle), np.sin(angle)], 1))
+    size = torch.from_numpy(np.tile(np.abs(pos[:, None] * freq), 2))
+    so.close(c.out["q"].cpu()[:len(pos), :64], want, 2.0 ** -52 * size + 2.0 ** -24 * want.abs() + 2.0 ** -51, "cosine and sine")
