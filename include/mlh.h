@@ -533,7 +533,8 @@ int mlh_gemm4_device(const mlh_weights4* w, const mlh_gemm4* args, void* stream)
  * A masked token is a logit of -infinity: its log p is -infinity.  A row with NaN or +infinity in it, or with nothing but -infinity, has no distribution: all its log probabilities and its entropy are NaN (its top tokens are those of
  * the largest logits, NaN as -infinity).  A given token below 0 asks for nothing: its log p is 0; one of vocab or more is NaN.
  * Rows `stride` elements apart, aligned to their elements (odd vocabularies; 16-byte aligned rows are read faster).  tokens and logProb [rows, given], entropy [rows] (may be null), topIds and topLogProb [rows, top].
- * work: mlh_logprobs_work_bytes() bytes (of the same structure; 0: none), 16-byte aligned, undefined before and after, not shared by calls that may overlap.  As the
+ * work: mlh_logprobs_work_bytes() bytes (of the same structure, whose pointers and temperature are not looked at, so that it can be asked before there are any; 0: none, or sizes that the call refuses),
+ * 16-byte aligned, undefined before and after, not shared by calls that may overlap.  As the
  * operators above: launches on `stream`, no allocation, recordable, 0 / -1 / -2. */
 typedef struct {
     const void* logits;

@@ -528,13 +528,18 @@ __global__ void __launch_bounds__(LP_WG) k_logprobs_join(LpArgs A) {
 // ----------------------------------------------------------------------------
 // host side
 // ----------------------------------------------------------------------------
-static std::string lp_check(const mlh_logprobs* a) {
+static std::string lp_check_sizes(const mlh_logprobs* a) { // what the workspace goes by
     if (!a) return "null arguments";
     if (a->type != MLH_DTYPE_F32 && a->type != MLH_DTYPE_BF16 && a->type != MLH_DTYPE_F16) return "unknown type of logits";
     if (a->rows < 0 || a->rows > (1 << 24)) return "rows must be 0 to 2^24";
     if (a->vocab < 1 || a->vocab > (1 << 22)) return "vocab must be 1 to 2^22";
     if (a->stride < a->vocab || a->stride > (1ll << 32)) return "stride smaller than vocab, or beyond 2^32";
     if (a->given < 0 || a->given > 64 || a->top < 0 || a->top > 64 || a->top > a->vocab) return "given and top must be 0 to 64, top at most vocab";
+    return "";
+}
+static std::string lp_check(const mlh_logprobs* a) {
+    const std::string bad = lp_check_sizes(a);
+    if (!bad.empty()) return bad;
     if (!a->logits || (a->given && (!a->tokens || !a->logProb)) || (a->top && (!a->topIds || !a->topLogProb))) return "null pointer";
     if ((uintptr_t)a->logits % kv_elem_bytes(a->type)) return "logits must be aligned to their elements";
     if (((a->given ? (uintptr_t)a->tokens | (uintptr_t)a->logProb : 0) | (uintptr_t)a->entropy | (a->top ? (uintptr_t)a->topIds | (uintptr_t)a->topLogProb : 0)) % 4) return "tokens and results must be 4-byte aligned";
@@ -559,7 +564,7 @@ static LpCut lp_cut(const mlh_logprobs* a) {
 }
 
 extern "C" uint64_t mlh_logprobs_work_bytes(const mlh_logprobs* a) {
-    if (!lp_check(a).empty()) return 0;
+    if (!lp_check_sizes(a).empty()) return 0;
     const LpCut c = lp_cut(a);
     return c.join ? (uint64_t)a->rows * (c.parts * sizeof(LpSums) + (a->top ? (uint64_t)c.units * LP_WG * 4 : 0)) : 0;
 }

@@ -676,9 +676,6 @@ extern "C" int mlh_score(mlh_ctx* c, int seq, const int32_t* ids, int n, int top
     // device results: logits, then per row its next token, log probability, entropy, best tokens and theirs; the operator's workspace
     const size_t V = c->hp.vocabSize, rows = n, words = rows * (3 + 2 * (size_t)top), at = (rows * V + 3) / 4 * 4;
     mlh_logprobs a = {nullptr, (int64_t)V, nullptr, nullptr, nullptr, nullptr, nullptr, n, (int32_t)V, MLH_DTYPE_F32, 1, top, temperature, nullptr, 0};
-    a.logits = a.tokens = (const int32_t*)16; // (what the workspace takes does not go by them)
-    a.logProb = a.entropy = a.topLogProb = (float*)16;
-    a.topIds = (int32_t*)16;
     a.workBytes = mlh_logprobs_work_bytes(&a);
     const size_t workAt = (at + words + 3) / 4 * 4, need = workAt * 4 + a.workBytes;
     if ((rc = full_buffer(c, need)) || (rc = mlh_pin(c, c->pinIo, words * 4))) return rc;

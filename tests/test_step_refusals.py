@@ -115,6 +115,14 @@ def test_logprobs_of_rows_in_parts_want_their_work(pkg, kw):
         pkg.logprobs(_logprobs(pkg, **long, **kw))
 
 
+@pytest.mark.parametrize("kw", [dict(), dict(rows=1, vocab=1 << 22, stride=1 << 22), dict(rows=500, vocab=150001, stride=150016), dict(top=0, given=0), dict(rows=300, vocab=5000, stride=5000)])
+def test_the_work_of_logprobs_can_be_asked_before_there_are_pointers(pkg, kw):
+    kw = {**dict(rows=2, vocab=200000, stride=200000), **kw}
+    none = dict.fromkeys(("logits", "tokens", "logProb", "entropy", "topIds", "topLogProb", "work"))
+    assert pkg.logprobs_work_bytes(_logprobs(pkg, **kw, **none)) == pkg.logprobs_work_bytes(_logprobs(pkg, **kw))
+    assert (pkg.logprobs_work_bytes(_logprobs(pkg, **kw)) > 0) == (kw["vocab"] > 5000)
+
+
 def test_null_structures(pkg):
     assert pkg.dev.mlh_rotate_device(None, None) == -1 and b"null" in pkg.dev.mlh_last_error(None)
     assert pkg.dev.mlh_logprobs_device(None, None) == -1 and b"null" in pkg.dev.mlh_last_error(None)
