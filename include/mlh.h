@@ -508,10 +508,12 @@ int mlh_weights4_read_device(const mlh_weights4* w, int type, void* dst, int64_t
 
 /* C[M,N] = A[M,K] . W^T (+ R[M,N]) for few rows, as mlh_gemm_device with W in 4 bits; or, with swiglu, rows 2j and 2j + 1 of W are gate and up of unit j (N even,
  * no R) and C is [M, N/2], silu(gate) * up (inference.cu:262-281).  A, R and C are of one type, C is rounded to it once.  The codes are multiplied as whole numbers and
- * minimum and scale applied to the sums of a group, in fp32: products are exact (fp32 activations as three bf16 planes) and sums fp32, so no weight is rounded.  Rows of A with an infinity or NaN, and rows
- * of W with one among their minima and scales, give infinities or NaN, not always the ones that products with the values would give; fp32 elements of 3.3962e38 or more count as such, and sums may pass fp32's range where elements of fp32 or bf16 pass 8e34 (a group's 128 elements times 31 do).  What a row gives does not depend on what the other rows hold.
- * rStride may be 0: one row for all (a bias).  c may be r with the same stride.  Pointers 16-byte aligned, rows a multiple of 16 bytes apart, except those of R and C: aligned to their elements.
- * work: mlh_gemm4_work_bytes() bytes (of the same structures; 0: none), 16-byte aligned, undefined before and after, not shared by calls that may overlap.  As the
+ * minimum and scale applied to the sums of a group, in fp32.  fp16 rows meet the codes themselves.  bf16 and fp32 rows (those as three bf16 planes, which hold elements down to 2^-110; smaller ones are off by 2^-134)
+ * meet 16 + code, and minimum - 16 scale is one fp32 number: a single product is off by up to 2^-19 (bf16) or 2^-17 (fp32) of its element times its group's scale, also where the weight itself is tiny beside
+ * the scale, and sums are fp32 sums of such terms.  Rows of A with an infinity or NaN, and rows of W with one among their minima and scales, give infinities or NaN, not always the ones that products with the values would give; fp32 elements of 3.3962e38 or more count as such, and sums may pass fp32's range where elements of fp32 or bf16 pass 8e34 (a group's 128 elements times 31 do).  What a row gives does not depend on what the other rows hold, but its last bits
+ * may on M, which chooses the kernel.
+ * rStride may be 0: one row for all (a bias).  c may be r with the same stride; c's rows must not overlap those of a, nor those of r in any other way.  Pointers 16-byte aligned, rows a multiple of 16 bytes apart, except those of R and C: aligned to their elements.
+ * work, workBytes: reserved.  No product needs work as yet, mlh_gemm4_work_bytes() is 0 and neither is looked at; a caller who gives what that call says is ready for one that does.  As the
  * operators above: launches on `stream`, no allocation, recordable, 0 / -1 / -2. */
 typedef struct {
     const void *a, *r; /* r may be null */

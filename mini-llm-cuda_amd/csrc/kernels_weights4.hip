@@ -143,7 +143,7 @@ struct Gemm4Args {
 // Columns 2j and 2j + 1 of a word of codes, each in bits 3 to 6 of a half
 template <int J> __device__ __forceinline__ uint32_t w4_turn(uint32_t x) { return J == 0 ? x : J == 3 ? __builtin_amdgcn_alignbit(x, x, 12) : x >> (4 * J); }
 
-// How codes and activations meet on the matrix cores, exactly.  PLANES: of an activation.  codes(x): a word of eight codes as an operand that stands for UNIT * (code + SHIFT); unit(): one of UNIT.
+// How codes and activations meet on the matrix cores; every product there is exact.  PLANES: of an activation.  codes(x): a word of eight codes as an operand that stands for UNIT * (code + SHIFT); unit(): one of UNIT.
 template <typename T> struct W4Mul;
 template <> struct W4Mul<f16_t> { // codes as halves below 2^-14, code * 2^-21
     static constexpr int PLANES = 1;
@@ -229,7 +229,9 @@ template <typename T, int ROWS> __device__ __forceinline__ void w4_rows(Gemm4Arg
 }
 
 // Products with minimum and scale behind the sums: the sum over a group of a (min + scale code) is (scale D + (min - scale SHIFT) S) / UNIT, D the sum of a UNIT (code + SHIFT) and S that of
-// a UNIT; both come from the matrix cores, S as a product with UNIT.  Lane l of a result holds column l % 16 (a row of W) and the instruction's rows 4 (l / 16) + i, i = 0 .. 3.
+// a UNIT; both come from the matrix cores, S as a product with UNIT.  All of it is fp32.  With SHIFT 16 the roundings of min - 16 scale and of its product
+// with S are up to 2^-19 of the scale in a weight, those of D (fp32 rows: a (16 + code) has up to 29 bits) and its product with the scale 62 2^-24, where quantising leaves half the scale; codes that
+// stand for themselves would take another instruction a pair, min and 16 scale applied apart another matrix instruction of 32 cycles for every 128 of 16-bit products.  Lane l of a result holds column l % 16 (a row of W) and the instruction's rows 4 (l / 16) + i, i = 0 .. 3.
 //
 // Few rows, four in an operand: the instruction's row 4 m + s is row m of A in the s-th 32 columns of a tile, so that one load brings a tile's share of A to the lanes that multiply it and the product with
 // the s-th step's codes has that step's sums, of row m, in element s of lanes 16 m to 16 m + 15.  (The other elements are of rows and codes that do not belong together.)  One product with UNIT gives the S of

@@ -280,3 +280,56 @@ def test_a_matrix_beyond_32_bit_offsets(pkg):
         want, bound = so.product4(a.cpu().double(), c, p, group, kind)
         so.close(out[:, some.cuda()].cpu(), want, bound, kind)
     assert bool((data[-64:] == 255).all())
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("low", [0.0, 0.001, -7.5])
+def test_how_far_off_a_single_product_is(pkg, kind, group, low):
+    """Rows of A with one element in them, groups of scale 8 whose minimum is tiny beside it (or, -7.5 scales, an ordinary one): every kernel.
+
+    Bound, in |a| 2^-24.  fp16: roundings of scale * code, of the minimum's product and of their sum, 3 (|min| + 15 scale).  bf16 and fp32 rows: the minimum - 16 scale is rounded to fp32, and so
+    may be its product with a, each half a step of up to |min| + 16 scale; fp32 rows: the sum of a's planes by 16 + code and its product with the scale are rounded too, each by up to 31 scale.
+    Then the result's own, in fp32 and in the type."""
+    n, k, scale = 70, 384, 8.0
+    codes, params = codes_and_params(n, k, group, 11)
+    params[..., 0] = low * (scale if low < 0 else 1)
+    params[..., 1] = scale
+    w, data = matrix(pkg, n, k, group)
+    dc, dp = so.packed4(codes).cuda(), params.cuda()
+    pkg.weights4_set(w, dc.data_ptr(), dp.data_ptr())
+    values = so.values4(codes, params, group)
+    size = float(params[0, 0, 0].abs())
+    roundings = {"f16": 3 * (size + 15 * scale), "bf16": 2 * (size + 16 * scale), "f32": 2 * (size + 16 * scale) + 2 * 31 * scale}[kind]
+    for m in (1, 4, 8, 16, 32, 64):
+        p = Product(pkg, kind, m, n, k, group, weights=(w, data, codes, params), seed=m)
+        at, x = torch.arange(m) * 55 % k, p.a[:, 0].clone()
+        p.a = torch.zeros(m, k, dtype=so.TORCH[kind])
+        p.a[torch.arange(m), at] = x
+        p.da.copy_(p.a)
+        p.run()
+        torch.cuda.synchronize()
+        x = x.double()[:, None]
+        want = x * values[:, at].T
+        bound = x.abs() * roundings * 2.0 ** -24 + (2.0 ** -24 + so.U[kind]) * want.abs()
+        so.close(p.c[:m, :n].cpu(), want, bound * (1 + so.U[kind]) + so.TINY[kind], f"M {m}")
+
+
+@pytest.mark.parametrize("exponent", [-96, -109, -116, -126, -140])
+def test_how_small_fp32_elements_may_be(pkg, exponent):
+    """Elements of all 24 bits: three planes hold them down to 2^-110, below that what is left of them is off by half of a step of the smallest bf16, 2^-134, times 16 + code."""
+    n, k, group = 70, 256, 64
+    codes, params = codes_and_params(n, k, group, 12)
+    params[..., 0], params[..., 1] = -7.5 * 1024, 1024
+    w, data = matrix(pkg, n, k, group)
+    dc, dp = so.packed4(codes).cuda(), params.cuda()
+    pkg.weights4_set(w, dc.data_ptr(), dp.data_ptr())
+    values = so.values4(codes, params, group)
+    for m in (1, 8, 16, 64):
+        p = Product(pkg, "f32", m, n, k, group, weights=(w, data, codes, params), seed=m)
+        p.a = torch.ldexp(1 + p.a.abs().remainder(1), torch.tensor(exponent))
+        p.da.copy_(p.a)
+        p.run()
+        torch.cuda.synchronize()
+        want, bound = so.product4(p.a.double(), codes, params, group, "f32")
+        so.close(p.c[:m, :n].cpu(), want, bound + (2.0 ** -134 * 31 * 1024 * k if exponent < -110 else 0), f"M {m}")
