@@ -340,9 +340,9 @@ __device__ __forceinline__ void lp_finish_top(const LpArgs& A, int row, float m,
     }
 }
 
-// What bounds it: many rows memory (8192 of 50257 in bf16, 823 MB: 155 us, 5.3 TB/s), with the instructions for 16 exponentials a chunk close behind (162 with a maximum over the wave for every chunk); few rows the latencies of one workgroup (a row
+// What bounds it: many rows memory (8192 of 50257 in bf16, 823 MB: 148 to 153 us, 5.4 to 5.6 TB/s), with the instructions for 16 exponentials a chunk close behind (162 with a maximum over the wave for every chunk); few rows the latencies of one workgroup (a row
 // of 8192 in fp32, five tokens: 6 us, of which the launch is 2).  Workgroups of 512 and 1024 threads were no faster: a compute unit takes 0.1 us for 1000 elements however they are dealt.
-// Rows in parts: 64 of 131075 in bf16 16 us, of which the parts take 7.5 and the join 8.4, a row alone 3.8 and 6.9: the join waits for memory three times (ranks, groups, given tokens' logits) and for
+// Rows in parts: 64 of 131075 in bf16 15.0 to 15.5 us, of which the parts take 8.0 and the join 7.5, a row alone 3.8 and 6.9: the join waits for memory three times (ranks, groups, given tokens' logits) and for
 // its own code.  Parts that picked their own top tokens took 14 + 5 us; joined by the last part to end, counted by atomics, 25 to 52.
 enum { LP_SUMS, LP_WHOLE, LP_PARTLY }; // no top tokens; with them, of rows that are one workgroup's; the groups left in work
 template <typename T, int KIND>
@@ -547,8 +547,8 @@ static std::string lp_check(const mlh_logprobs* a) {
     return "";
 }
 
-// How rows are cut.  A row is one workgroup's where it can be (LP_GROUPS): a second launch costs about 4 us, and many rows fill the chip.  Few and long rows are cut into as many parts as make 1024
-// workgroups of whole units (512: up to 1 us more), since one compute unit takes 0.1 us for 1000 elements.  bf16 with the 20 most likely, us whole / cut: 1 row of 32768 10.5 / 10.7, 40000 11.9 / 10.6,
+// How rows are cut.  A row is one workgroup's where it can be (LP_GROUPS): a second launch costs about 4 us, and many rows fill the chip.  Few and long rows are cut into parts of as many whole
+// units as keep them within 1024 workgroups (512: up to 1 us more; 64 rows of 131075 are 17 units each, two a part: 576 workgroups), since one compute unit takes 0.1 us for 1000 elements.  bf16 with the 20 most likely, us whole / cut: 1 row of 32768 10.5 / 10.7, 40000 11.9 / 10.6,
 // 100000 20.6 / 11.2; 64 rows 11.2 / 11.9, 12.3 / 12.2, 21.3 / 14.3; 128 rows of 32768 11.3 / 13.1, 50000 14.4 / 13.8, 100000 21.8 / 17.1; 256 rows of 50000 14.5 / 16.9, 100000 22.8 / 23.3.
 struct LpCut { int units, parts, per; bool join; }; // units: of a row; per: of a part
 static LpCut lp_cut(const mlh_logprobs* a) {

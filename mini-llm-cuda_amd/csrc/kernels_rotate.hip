@@ -48,7 +48,8 @@ template <bool NT, int V, typename T> __device__ __forceinline__ void rot_store(
 
 // A workgroup takes a few rows at a time: their cosines and sines once, into LDS, for all heads, then the heads.  The angle is counted in half turns, of which sincospi takes the whole ones off exactly.
 // A piece is V elements of a head: with halves the two times V that are V pairs, with pairs V neighbours, or V elements behind the turned ones.
-// Bound by memory: 16384 rows of 32 + 8 heads of 128 in bf16, 336 MB read and written, 58 us (5.8 TB/s; a copy of 1 GiB 5.2), fp32 rows 63 us for as many bytes (5.3).  A single token 2.6 us, the latency
+// Bound by memory: 16384 rows of 32 + 8 heads of 128 in bf16, 336 MB read and written, 58 us (5.8 TB/s; a copy of 1 GiB 5.2), fp32 rows 63 us for as many bytes (5.3).  Narrower pieces take longer: 8192 rows of the same heads in bf16, halves, 20 turned
+// of 80 (two elements a piece) 50 us, 2.1 TB/s, 24 of 96 (four) 41, 3.1, 62 of 128 (one) 104, 1.6.  A single token 2.6 us, the latency
 // of position, angle and LDS in turn.  Rows at once: about as many as give every thread a piece; of 40 heads one, two and four 58, 62 and 65 us, of 3 heads one, four and eight 18, 11 and 9.5.
 template <typename T, bool HALVES, int V, bool NT>
 __global__ void __launch_bounds__(ROT_WG) k_rotate(RotateArgs A) {

@@ -28,7 +28,7 @@ struct W4Args {
 };
 
 // A wave: a tile, as the lanes of a product hold it: lane l row l % 16, eight columns of each of the four steps.  The columns of a group are those of 1, 2 or 4 steps in the four lanes of a row.
-// Bound by memory.  28672 columns of 8192 rows, groups of 32: codes laid out in 74 us, 3.6 TB/s (read four bytes at a time 99, and written so, 64 apart, 142), packed from bf16 in 153, read back in 171.
+// Bound by memory.  28672 columns of 8192 rows, groups of 32: codes laid out in 70 to 75 us, 3.9 to 4.2 TB/s (read four bytes at a time 99 us, and written so, 64 apart, 142), packed from bf16 in 153, 4.0 TB/s, read back in 170, 3.6.
 struct W4Place { int n, k, lane; }; // row and first column of step 0
 __device__ __forceinline__ W4Place w4_place(const W4Args& A, size_t tile) {
     const int perBand = w4_tiles(A.K), lane = threadIdx.x & 63;
@@ -337,7 +337,7 @@ __global__ void __launch_bounds__(W4_WAVES * 64) k_gemm4_few(Gemm4Args A) {
 // S does not depend on W: the loaders take it, with UNIT in the four rows of the instruction that belong to a group and zeros in the others, so that four groups add up in one result and stand where
 // v_mfma_f32_16x16x4_f32 wants them, which multiplies four groups' S with their minima at once, in fp32.  (With S and its products in every multiplying wave fp32 took 5 to 12 % longer, groups of 32 up to 15 %.)
 // Groups of 128 are two of 64 here, for fewer registers.  Eight loaders where the registers of 16 waves hold the shape (S and A in time: fp32, 16 rows, 7.8 us for 8.8 at 128 bands), four elsewhere.
-// 64 rows, N 28672, K 8192, groups of 64, fp16 take 55 us, 550 TFLOP/s, twice what the matrix cores alone need.  Left out in turn (before the loaders took S), the loads of W saved 13 us, A's out of LDS 6,
+// 64 rows, N 28672, K 8192, groups of 64, fp16 take 50 us, 600 TFLOP/s, twice what the matrix cores alone need.  Left out in turn (before the loaders took S, of 55 to 60 us), the loads of W saved 13 us, A's out of LDS 6,
 // the loaders 2, and all three half the time: the three wait for each other; two and three blocks of codes ahead, other waves and shares were no faster.
 // In LDS piece q (eight columns) of step s (32 columns) of row m stands at [m][s ^ (m / 4 % 4)][q ^ (m % 4)], so that neither the lanes of a store, which share a row, nor those of a load, which share
 // step and piece, meet in a bank.
@@ -638,8 +638,9 @@ template <typename T, int G, int MT, int WN, int WK, int NT, int TPW, int AHEAD,
 }
 
 // A workgroup's share of a product of more than four rows: rows of A times 16-row bands of W, and what a round of such workgroups, one a compute unit, takes (tenths of a us at N 2048, K 8192, fp32 or
-// fp16, groups of 64).  Large shares read A and W less often, small ones fill the chip when there are few: taken is the share whose rounds take least, the fastest or within 6 % of it for 5 to 64
-// rows of 48 to 2000 bands.  For instance, us with the share taken / the next ones, fp16, K 4096: 64 rows, 256 bands 16 x 4 8.8 / 32 x 4 10.9, 16 x 8 11.8; 1024 bands 32 x 8 18.6 / 32 x 4 25.4, 64 x 8 26.8;
+// fp16, groups of 64).  Large shares read A and W less often, small ones fill the chip when there are few: taken is the share whose rounds take least.  With every share
+// forced in turn, 5 to 64 rows of 48 to 1792 bands, fp16 and fp32, groups of 32 to 128, the one taken was within 7 % of the fastest at K 2048 and 4096, 10 % at 8192 and 16384, 15 % at 32768; where K is shorter
+// than 2048, starts count for more than these times say: up to 18 % at K 1024, 30 % at 512, half more at 256 (fp32, 64 rows, 1280 bands 14.6 for 9.8).  For instance, us with the share taken / the next ones, fp16, K 4096: 64 rows, 256 bands 16 x 4 8.8 / 32 x 4 10.9, 16 x 8 11.8; 1024 bands 32 x 8 18.6 / 32 x 4 25.4, 64 x 8 26.8;
 // 1280 bands 64 x 8 27.4 / 32 x 8 31.9; 32 rows, 1024 bands 32 x 4 14.9 / 16 x 8 15.2, 32 x 8 18.0; 16 rows, 256 bands 16 x 1 5.6 / 16 x 2 7.0, 16 x 4 8.1; fp32: 8 rows, 256 bands 8 x 1 7.7 / 8 x 2 9.1,
 // 16 x 2 10.7; 64 rows, 256 bands 16 x 4 13.4 / 16 x 8 17.5,
 // 16 x 2 20.0, 32 x 8 26.3.  (64 x 4 takes longer than 32 x 8 everywhere: 21.1 for 18.6.)
